@@ -357,6 +357,160 @@ int spb_gemv_bf16(const uint16_t* W, const uint16_t* x, float* y, int rows, int 
  * (src/main.cpp:194-200). */
 int spb_argmax_f32(const float* x, int n, int* out_index, spb_stream_t stream);
 
+/* ---- batches of tokens over a paged key / value cache ------------------------
+ * No reference counterpart: the batched, paged forms of rope_gpu,
+ * scatter_kv_gpu and the attention wrappers above (one token, one contiguous
+ * cache per sequence), for callers that serve several sequences of different
+ * lengths from one pool of pages.
+ *
+ * New tokens of all sequences stand packed one after the other.  A token's
+ * heads are contiguous ([heads][head_dim]); tokens are `*_stride` elements
+ * apart (the q, k and v parts of a stacked projection are three pointers with
+ * one stride).  Each entry point exists for fp16 (_f16) and bf16 (_bf16);
+ * arithmetic is float32, outputs are rounded once.
+ *
+ * Arrays on the device are not read by the host: numbers in them that fall
+ * outside the batch, the table or the pool are clamped or skipped on the
+ * device as described, so they never lead outside the given buffers. */
+
+/* Rotary positions.  inv_freq: device float64 [rotary_dim / 2], radians per
+ * position of each pair.  Pair i of a head is elements (2i, 2i + 1) when
+ * interleaved (rope_gpu's layout), else (i, i + rotary_dim / 2); it turns by
+ * position * inv_freq[i], and the turned pair is multiplied by `scale`.
+ * Elements from rotary_dim on stay as they are.  The angle is reduced to a
+ * turn in float64, so far positions are as exact as near ones.
+ * rotary_dim even, 2 <= rotary_dim <= head_dim. */
+typedef struct spb_rope {
+    const double* inv_freq;
+    int rotary_dim;
+    int interleaved;
+    float scale;
+} spb_rope;
+
+/* Fills inv_freq (HOST, rotary_dim / 2 doubles) and *scale (nullable) for
+ * spb_rope.  With f = theta^(-2i / rotary_dim):
+ *   SPB_ROPE_PLAIN   f
+ *   SPB_ROPE_LINEAR  f / factor (position interpolation)
+ *   SPB_ROPE_NTK     f with theta * factor^(rotary_dim / (rotary_dim - 2))
+ *   SPB_ROPE_YARN    between f (pairs with more than beta_fast turns over
+ *                    original_positions) and f / factor (fewer than
+ *                    beta_slow), linear in the pair's index between; scale
+ *                    0.1 ln(factor) + 1 (1 for factor <= 1)
+ * scale is 1 for the others.  beta_fast, beta_slow and original_positions are
+ * read for SPB_ROPE_YARN only. */
+enum { SPB_ROPE_PLAIN = 0, SPB_ROPE_LINEAR = 1, SPB_ROPE_NTK = 2, SPB_ROPE_YARN = 3 };
+int spb_rope_inv_freq(double* inv_freq, float* scale, int rotary_dim, double theta, int scaling,
+                      double factor, int original_positions, double beta_fast, double beta_slow);
+
+/* output[t] = x[t] with every head rotated to positions[t] (device int32).
+ * A token with a negative position is padding: its output is not written.
+ * output == x rotates in place; other overlaps are not allowed.
+ * head_dim even, at most 256. */
+int spb_rope_tokens_f16(const uint16_t* x, uint16_t* output, const int* positions,
+                        const spb_rope* rope, int num_tokens, int num_heads, int head_dim,
+                        long x_stride, long output_stride, spb_stream_t stream);
+int spb_rope_tokens_bf16(const uint16_t* x, uint16_t* output, const int* positions,
+                         const spb_rope* rope, int num_tokens, int num_heads, int head_dim,
+                         long x_stride, long output_stride, spb_stream_t stream);
+
+/* RMSNorm of every query and key head, then the rotation, in one pass:
+ * y = rotate((x / sqrt(mean(x^2) + eps)) * w), mean over the head's head_dim
+ * elements, w float32 [head_dim] (q_weight for q, k_weight for k).  rope may
+ * be NULL (norms only; positions is then not read and may be NULL).  Padding
+ * tokens, aliasing and head_dim as in spb_rope_tokens. */
+int spb_qk_norm_rope_f16(const uint16_t* q, const uint16_t* k, uint16_t* q_output,
+                         uint16_t* k_output, const float* q_weight, const float* k_weight,
+                         const int* positions, const spb_rope* rope, int num_tokens,
+                         int num_heads, int num_kv_heads, int head_dim, long q_stride,
+                         long k_stride, long q_output_stride, long k_output_stride, float eps,
+                         spb_stream_t stream);
+int spb_qk_norm_rope_bf16(const uint16_t* q, const uint16_t* k, uint16_t* q_output,
+                          uint16_t* k_output, const float* q_weight, const float* k_weight,
+                          const int* positions, const spb_rope* rope, int num_tokens,
+                          int num_heads, int num_kv_heads, int head_dim, long q_stride,
+                          long k_stride, long q_output_stride, long k_output_stride, float eps,
+                          spb_stream_t stream);
+
+/* A pool of pages for K and one for V.  Element d of slot i of kv head h of
+ * page p is at p * page_stride + h * head_stride + i * slot_stride + d in
+ * both (elements; multiples of 8), so a page may be [num_kv_heads][page_size]
+ * [head_dim] (scatter_kv_gpu's cache of page_size positions) or [page_size]
+ * [num_kv_heads][head_dim].  k and v 16-byte aligned; head_dim a multiple of
+ * 8, at most 256; any page_size >= 1. */
+typedef struct spb_paged_cache {
+    uint16_t* k;
+    uint16_t* v;
+    long page_stride, head_stride, slot_stride;
+    int num_pages, page_size, num_kv_heads, head_dim;
+} spb_paged_cache;
+
+/* A batch of new tokens (device int32 arrays).  Sequence s has the tokens
+ * token_starts[s] .. token_starts[s + 1] - 1 (none is allowed), which are the
+ * LAST of its kv_lens[s] cached positions: token i of n is at position
+ * kv_lens[s] - n + i.  Position j is slot j % page_size of page
+ * page_table[s * table_width + j / page_size].  token_starts [num_seqs + 1]
+ * does not decrease; tokens from token_starts[num_seqs] on belong to no
+ * sequence, and their rows of every output stay as they were.  Positions past
+ * table_width * page_size do not exist (kv_lens is clamped to them; append
+ * skips them).  max_new: the most tokens a sequence has, or 0 if not known
+ * (it selects a kernel; a wrong one costs time only).  num_seqs <= 65536. */
+typedef struct spb_paged_batch {
+    const int* token_starts;
+    const int* kv_lens;
+    const int* page_table;
+    int num_seqs, table_width, num_tokens, max_new;
+} spb_paged_batch;
+
+/* Writes the batch's keys and values into their pages, the keys rotated to
+ * their positions on the way (rope NULL: as they are).  q (nullable): the
+ * batch's queries, rotated to q_output in the same launch.  q_weight and
+ * k_weight (nullable): RMSNorm before the rotation, as spb_qk_norm_rope
+ * (q_weight needs q).  k NULL and v NULL together: no cache write (queries
+ * only).  A token whose position is negative (kv_lens[s] smaller than its
+ * sequence's tokens) is skipped altogether; where its page id is outside
+ * [0, num_pages) or past the table, its key and value are dropped.  Two tokens
+ * must not have the same slot. */
+int spb_paged_append_f16(const spb_paged_cache* cache, const spb_paged_batch* batch,
+                         const uint16_t* k, const uint16_t* v, const uint16_t* q,
+                         uint16_t* q_output, long k_stride, long v_stride, long q_stride,
+                         long q_output_stride, int num_heads, const float* q_weight,
+                         const float* k_weight, float eps, const spb_rope* rope,
+                         spb_stream_t stream);
+int spb_paged_append_bf16(const spb_paged_cache* cache, const spb_paged_batch* batch,
+                          const uint16_t* k, const uint16_t* v, const uint16_t* q,
+                          uint16_t* q_output, long k_stride, long v_stride, long q_stride,
+                          long q_output_stride, int num_heads, const float* q_weight,
+                          const float* k_weight, float eps, const spb_rope* rope,
+                          spb_stream_t stream);
+
+/* Attention of the batch's new tokens over their sequences' pages (which
+ * already hold the new tokens' keys and values).  The query of position p,
+ * head h attends positions j of kv head h / (num_heads / num_kv_heads) with
+ *   j < kv_lens[s],  j <= p when causal,  j > p - window when window > 0:
+ * output[t][h] = sum_j softmax_j(scale * q . k_j) v_j.  A query that sees no
+ * position gives zeros.  Positions in pages whose id is outside [0, num_pages)
+ * count as not there.  What is not seen has no effect, whatever it holds (inf
+ * and NaN too).  num_heads a multiple of num_kv_heads; scale > 0; q and output
+ * 16-byte aligned with strides that are multiples of 8; q == output is
+ * allowed (same stride), other overlaps are not.
+ * workspace: at least spb_paged_attention_workspace_size bytes, 16-byte
+ * aligned, contents irrelevant; calls that share one must be ordered (same
+ * stream).  The size depends on the head counts, head_dim and the device
+ * only (the arguments are rejected as the call would: 0 is returned).  Runs
+ * on the bf16 / fp16 matrix cores; probabilities are rounded to the storage
+ * type before their product with V, sums and statistics are float32. */
+size_t spb_paged_attention_workspace_size(int num_heads, int num_kv_heads, int head_dim);
+int spb_paged_attention_f16(const spb_paged_cache* cache, const spb_paged_batch* batch,
+                            const uint16_t* q, uint16_t* output, long q_stride,
+                            long output_stride, int num_heads, float scale, int causal,
+                            int window, void* workspace, size_t workspace_size,
+                            spb_stream_t stream);
+int spb_paged_attention_bf16(const spb_paged_cache* cache, const spb_paged_batch* batch,
+                             const uint16_t* q, uint16_t* output, long q_stride,
+                             long output_stride, int num_heads, float scale, int causal,
+                             int window, void* workspace, size_t workspace_size,
+                             spb_stream_t stream);
+
 /* ---- decode engine --------------------------------------------------------
  * bs=1 greedy decode of a BitNet b1.58 transformer whose linear layers are
  * 2:4 sparse-ternary, with bf16 activations, bf16 KV cache and a bf16 tied or

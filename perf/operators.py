@@ -232,8 +232,7 @@ def _plan(st):
         st["batch"] = K.PagedBatch(st["starts"], st["lens"], st["table"], st["n"],
                                    max_new=st["new_max"])
     if st["case"]["kind"] == "attention":
-        size = K.paged_attention_workspace_size(st["n"], st["case"]["seqs"], st["nh"], st["kvh"],
-                                                st["hd"])
+        size = K.paged_attention_workspace_size(st["nh"], st["kvh"], st["hd"])
         st["workspace"] = torch.empty(size, dtype=torch.uint8, device=DEV)
 
 
