@@ -489,8 +489,8 @@ int spb_paged_append_bf16(const spb_paged_cache* cache, const spb_paged_batch* b
  *   j < kv_lens[s],  j <= p when causal,  j > p - window when window > 0:
  * output[t][h] = sum_j softmax_j(scale * q . k_j) v_j.  A query that sees no
  * position gives zeros.  Positions in pages whose id is outside [0, num_pages)
- * count as not there.  What is not seen has no effect, whatever it holds (inf
- * and NaN too).  num_heads a multiple of num_kv_heads; scale > 0; q and output
+ * are left out (a query with no others gives NaN).  What is not seen has no
+ * effect, whatever it holds (inf and NaN too).  num_heads a multiple of num_kv_heads; scale > 0; q and output
  * 16-byte aligned with strides that are multiples of 8; q == output is
  * allowed (same stride), other overlaps are not.
  * workspace: at least spb_paged_attention_workspace_size bytes, 16-byte

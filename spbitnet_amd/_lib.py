@@ -17,6 +17,8 @@ LIB_PATH = os.path.join(PKG, "libspbitnet_amd.so")
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
+_D = ctypes.c_double
+_L = ctypes.c_long
 
 # name -> argtypes (restype int unless listed in _RESTYPES)
 SIGNATURES = {
@@ -72,6 +74,17 @@ SIGNATURES = {
     "spb_gemv_f16": [_P, _P, _P, _I, _I, _P],
     "spb_gemv_bf16": [_P, _P, _P, _I, _I, _P],
     "spb_argmax_f32": [_P, _I, _P, _P],
+    # batches of tokens over a paged cache (descriptors passed by pointer)
+    "spb_rope_inv_freq": [_P, _P, _I, _D, _I, _D, _I, _D, _D],
+    "spb_rope_tokens_f16": [_P, _P, _P, _P, _I, _I, _I, _L, _L, _P],
+    "spb_rope_tokens_bf16": [_P, _P, _P, _P, _I, _I, _I, _L, _L, _P],
+    "spb_qk_norm_rope_f16": [_P] * 8 + [_I] * 4 + [_L] * 4 + [_F, _P],
+    "spb_qk_norm_rope_bf16": [_P] * 8 + [_I] * 4 + [_L] * 4 + [_F, _P],
+    "spb_paged_append_f16": [_P] * 6 + [_L] * 4 + [_I, _P, _P, _F, _P, _P],
+    "spb_paged_append_bf16": [_P] * 6 + [_L] * 4 + [_I, _P, _P, _F, _P, _P],
+    "spb_paged_attention_workspace_size": [_I, _I, _I],
+    "spb_paged_attention_f16": [_P] * 4 + [_L, _L, _I, _F, _I, _I, _P, ctypes.c_size_t, _P],
+    "spb_paged_attention_bf16": [_P] * 4 + [_L, _L, _I, _F, _I, _I, _P, ctypes.c_size_t, _P],
     # decode engine (structs passed by pointer)
     "spb_engine_create": [_P, _P, _P, _P, _P, _I, _P],
     "spb_engine_destroy": [_P],
@@ -105,6 +118,7 @@ SIGNATURES = {
 }
 _RESTYPES = {"spb_last_error_string": ctypes.c_char_p,
              "spb_bitlinear_workspace_size": ctypes.c_size_t,
+             "spb_paged_attention_workspace_size": ctypes.c_size_t,
              "spb_sparse_i8_compressed_size": ctypes.c_long}
 
 
@@ -129,6 +143,25 @@ class ModelConfigC(ctypes.Structure):
                                   "max_position_embeddings", "head_dim")] + \
                [("rms_norm_eps", _F), ("rope_theta", _F), ("bos_token_id", _I),
                 ("eos_token_id", _I)]
+
+
+class RopeC(ctypes.Structure):
+    """spb_rope (include/spbitnet_amd.h)."""
+    _fields_ = [("inv_freq", _P), ("rotary_dim", _I), ("interleaved", _I), ("scale", _F)]
+
+
+class PagedCacheC(ctypes.Structure):
+    """spb_paged_cache (include/spbitnet_amd.h)."""
+    _fields_ = [("k", _P), ("v", _P), ("page_stride", _L), ("head_stride", _L),
+                ("slot_stride", _L), ("num_pages", _I), ("page_size", _I), ("num_kv_heads", _I),
+                ("head_dim", _I)]
+
+
+class PagedBatchC(ctypes.Structure):
+    """spb_paged_batch (include/spbitnet_amd.h)."""
+    _fields_ = [("token_starts", _P), ("kv_lens", _P), ("page_table", _P), ("num_seqs", _I),
+                ("table_width", _I), ("num_tokens", _I), ("max_new", _I)]
+
 
 _lib = None
 

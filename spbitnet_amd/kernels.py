@@ -11,7 +11,8 @@ cols == 0 is a no-op, as in the reference.
 """
 from __future__ import annotations
 
-from typing import Optional
+import ctypes
+from typing import Optional, Tuple
 
 import torch
 
@@ -333,3 +334,255 @@ def bitlinear_gpu(meta, values, x, output, gamma, rows, cols, meta_row_stride,
     fn = getattr(_lib.load(), f"spb_bitlinear_{kind}")
     _lib.check(fn(pm, pv, px, po, float(gamma), rows, cols, meta_row_stride, values_row_stride,
                   pw, workspace.numel(), _stream_ptr(stream)), "bitlinear_gpu")
+
+
+# ---- batches of tokens over a paged cache (no reference counterpart) ---------
+
+_ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+
+
+def _here(t: torch.Tensor, name: str) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a GPU tensor")
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
+
+
+def _half(t: torch.Tensor, name: str) -> str:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    kind = _HALF_KIND.get(t.dtype)
+    if kind is None:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected float16 or bfloat16")
+    return kind
+
+
+def _heads(t, name: str, dtype, tokens: int, heads: int, head_dim: int) -> Tuple[int, int]:
+    """Pointer and token stride of a [tokens][heads][head_dim] tensor whose
+    tokens' heads are contiguous (a part of a stacked projection may be one)."""
+    _here(t, name)
+    if t.dtype != dtype:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
+    if t.shape != (tokens, heads, head_dim):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected "
+                         f"({tokens}, {heads}, {head_dim})")
+    st = t.stride()
+    if st[2] != 1 or (heads > 1 and st[1] != head_dim):
+        raise ValueError(f"{name}: a token's heads must be contiguous")
+    return t.data_ptr(), st[0] if tokens > 1 else heads * head_dim
+
+
+def _ints(t, name: str, *shape: int) -> int:
+    """Pointer of a contiguous int32 GPU tensor of this shape."""
+    _here(t, name)
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected torch.int32")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _weight(t, name: str, head_dim: int) -> Optional[int]:
+    if t is None:
+        return None
+    _here(t, name)
+    if t.dtype != torch.float32:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected torch.float32")
+    if t.shape != (head_dim,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous vector of {head_dim} elements")
+    return t.data_ptr()
+
+
+def rope_inv_freq(rotary_dim: int, theta: float = 10000.0, scaling: str = "none",
+                  factor: float = 1.0, original_positions: int = 0, beta_fast: float = 32.0,
+                  beta_slow: float = 1.0) -> Tuple[torch.Tensor, float]:
+    """Radians per position of each pair (float64, on the host) and the factor of
+    the rotated pairs, for scaling "none", "linear", "ntk" or "yarn"
+    (spb_rope_inv_freq)."""
+    if scaling not in _ROPE_SCALING:
+        raise ValueError(f"scaling must be one of {sorted(_ROPE_SCALING)}, not {scaling!r}")
+    out = torch.empty(max(rotary_dim // 2, 1), dtype=torch.float64)
+    scale = ctypes.c_float()
+    _lib.check(_lib.load().spb_rope_inv_freq(out.data_ptr(), ctypes.addressof(scale),
+                                             int(rotary_dim), float(theta),
+                                             _ROPE_SCALING[scaling], float(factor),
+                                             int(original_positions), float(beta_fast),
+                                             float(beta_slow)), "rope_inv_freq")
+    return out, scale.value
+
+
+class Rope:
+    """A rotation (spb_rope): inv_freq, float64 radians per position of each pair
+    (rotary_dim / 2 of them, moved to the GPU if they are not there), the factor
+    of the rotated pairs and their layout: pairs (2i, 2i + 1) when interleaved,
+    else (i, i + rotary_dim / 2)."""
+
+    def __init__(self, inv_freq: torch.Tensor, scale: float = 1.0, interleaved: bool = True):
+        if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.numel() < 1:
+            raise ValueError("inv_freq must be a float64 vector")
+        if not inv_freq.is_cuda:
+            inv_freq = inv_freq.to(torch.device("cuda", torch.cuda.current_device()))
+        self.inv_freq = inv_freq.contiguous()
+        _here(self.inv_freq, "inv_freq")
+        self.rotary_dim = 2 * inv_freq.numel()
+        self.scale, self.interleaved = float(scale), bool(interleaved)
+        self._c = _lib.RopeC(self.inv_freq.data_ptr(), self.rotary_dim, int(self.interleaved),
+                             self.scale)
+        self._ptr = ctypes.addressof(self._c)
+
+    @staticmethod
+    def scaled(rotary_dim: int, theta: float = 10000.0, interleaved: bool = True,
+               **scaling) -> "Rope":
+        """The rotation of rope_inv_freq(rotary_dim, theta, **scaling)."""
+        f, scale = rope_inv_freq(rotary_dim, theta, **scaling)
+        return Rope(f, scale, interleaved)
+
+
+def rope_tokens_gpu(x, output, positions, rope: Rope, stream=None):
+    """Rotates the heads of x [tokens][heads][head_dim] to positions (int32
+    [tokens]; a negative one is padding, its output stays as it was) into output,
+    which may be x (spb_rope_tokens_*)."""
+    kind = _half(x, "x")
+    if x.dim() != 3:
+        raise ValueError("x must be [tokens][heads][head_dim]")
+    n, heads, hd = x.shape
+    px, sx = _heads(x, "x", x.dtype, n, heads, hd)
+    py, sy = _heads(output, "output", x.dtype, n, heads, hd)
+    fn = getattr(_lib.load(), f"spb_rope_tokens_{kind}")
+    _lib.check(fn(px, py, _ints(positions, "positions", n), rope._ptr, n, heads, hd, sx, sy,
+                  _stream_ptr(stream)), "rope_tokens_gpu")
+
+
+def qk_norm_rope_gpu(q, k, q_output, k_output, q_weight, k_weight, positions,
+                     rope: Optional[Rope], eps: float = 1e-5, stream=None):
+    """RMSNorm of every head of q [tokens][heads][head_dim] and k
+    [tokens][kv heads][head_dim] with the weights (float32 [head_dim]), then the
+    rotation to positions, in one pass (spb_qk_norm_rope_*).  rope None: norms
+    only.  The outputs may be q and k."""
+    kind = _half(q, "q")
+    if q.dim() != 3 or not isinstance(k, torch.Tensor) or k.dim() != 3:
+        raise ValueError("q and k must be [tokens][heads][head_dim]")
+    n, nh, hd = q.shape
+    nkv = k.shape[1]
+    pq, sq = _heads(q, "q", q.dtype, n, nh, hd)
+    pk, sk = _heads(k, "k", q.dtype, n, nkv, hd)
+    pqo, sqo = _heads(q_output, "q_output", q.dtype, n, nh, hd)
+    pko, sko = _heads(k_output, "k_output", q.dtype, n, nkv, hd)
+    pp = _ints(positions, "positions", n) if rope is not None else None
+    fn = getattr(_lib.load(), f"spb_qk_norm_rope_{kind}")
+    _lib.check(fn(pq, pk, pqo, pko, _weight(q_weight, "q_weight", hd),
+                  _weight(k_weight, "k_weight", hd), pp, rope._ptr if rope is not None else None,
+                  n, nh, nkv, hd, sq, sk, sqo, sko, eps, _stream_ptr(stream)),
+               "qk_norm_rope_gpu")
+
+
+class PagedKVCache:
+    """A pool of pages (spb_paged_cache) in two tensors k and v
+    [pages][kv heads][page_size][head_dim] (fp16 or bf16) of equal strides; the
+    last dimension is contiguous, so pages laid out [page_size][kv heads][head_dim]
+    come as a transposed view.  Keeps the tensors alive."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor):
+        self.kind = _half(k, "k")
+        _here(k, "k")
+        _here(v, "v")
+        if v.dtype != k.dtype:
+            raise TypeError(f"v has dtype {v.dtype}, expected {k.dtype}")
+        if k.dim() != 4 or v.shape != k.shape:
+            raise ValueError("k and v must be [pages][kv heads][page_size][head_dim]")
+        if k.stride() != v.stride() or k.stride(3) != 1:
+            raise ValueError("k and v must have the same strides and a contiguous last dimension")
+        self.k, self.v, self.dtype = k, v, k.dtype
+        self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k.shape
+        st = k.stride()
+        self._c = _lib.PagedCacheC(k.data_ptr(), v.data_ptr(), st[0], st[1], st[2],
+                                   self.num_pages, self.page_size, self.num_kv_heads,
+                                   self.head_dim)
+        self._ptr = ctypes.addressof(self._c)
+
+
+class PagedBatch:
+    """A batch of new tokens (spb_paged_batch): int32 GPU tensors token_starts
+    [sequences + 1], kv_lens [sequences] and page_table [sequences][width];
+    num_tokens rows in the token tensors (those past token_starts' last entry are
+    padding); max_new, the most new tokens of a sequence, if the program knows it.
+    The tensors are read by the calls, so a program may refill them between
+    calls (and between replays of a captured one)."""
+
+    def __init__(self, token_starts, kv_lens, page_table, num_tokens: int, max_new: int = 0):
+        if not isinstance(kv_lens, torch.Tensor) or kv_lens.dim() != 1:
+            raise ValueError("kv_lens must be a vector")
+        if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
+            raise ValueError("page_table must be [sequences][width]")
+        n, width = kv_lens.numel(), page_table.shape[1]
+        if num_tokens < 0 or max_new < 0:
+            raise ValueError("negative number of tokens")
+        self.token_starts, self.kv_lens, self.page_table = token_starts, kv_lens, page_table
+        self.num_seqs, self.num_tokens, self.max_new = n, int(num_tokens), int(max_new)
+        self._c = _lib.PagedBatchC(_ints(token_starts, "token_starts", n + 1),
+                                   _ints(kv_lens, "kv_lens", n),
+                                   _ints(page_table, "page_table", n, width), n, width,
+                                   self.num_tokens, self.max_new)
+        self._ptr = ctypes.addressof(self._c)
+
+
+def paged_append_gpu(cache: PagedKVCache, batch: PagedBatch, k, v, rope: Optional[Rope] = None,
+                     q=None, q_output=None, q_weight=None, k_weight=None, eps: float = 1e-5,
+                     stream=None):
+    """Writes the batch's k and v [tokens][kv heads][head_dim] into their pages, the
+    keys rotated to their positions on the way (rope None: as they are), and, if q
+    [tokens][heads][head_dim] is given, rotates it into q_output (which may be q) in the same launch.
+    q_weight / k_weight (float32 [head_dim]): RMSNorm before the rotation
+    (spb_paged_append_*)."""
+    n, hd, nkv, dt = batch.num_tokens, cache.head_dim, cache.num_kv_heads, cache.dtype
+    pk = pv = pq = pqo = None
+    sk = sv = sq = sqo = nh = 0
+    if k is not None or v is not None:
+        pk, sk = _heads(k, "k", dt, n, nkv, hd)
+        pv, sv = _heads(v, "v", dt, n, nkv, hd)
+    if q is not None or q_output is not None:
+        _half(q, "q")
+        nh = q.shape[1] if q.dim() == 3 else 0
+        pq, sq = _heads(q, "q", dt, n, nh, hd)
+        pqo, sqo = _heads(q_output, "q_output", dt, n, nh, hd)
+    fn = getattr(_lib.load(), f"spb_paged_append_{cache.kind}")
+    _lib.check(fn(cache._ptr, batch._ptr, pk, pv, pq, pqo, sk, sv, sq, sqo, nh,
+                  _weight(q_weight, "q_weight", hd), _weight(k_weight, "k_weight", hd), eps,
+                  rope._ptr if rope is not None else None, _stream_ptr(stream)),
+               "paged_append_gpu")
+
+
+def paged_attention_workspace_size(num_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    """Bytes of the workspace that paged_attention_gpu needs for these heads."""
+    n = int(_lib.load().spb_paged_attention_workspace_size(num_heads, num_kv_heads, head_dim))
+    if n == 0:
+        _lib.check(1, "paged_attention_workspace_size")
+    return n
+
+
+def paged_attention_gpu(cache: PagedKVCache, batch: PagedBatch, q, output, workspace,
+                        scale: Optional[float] = None, causal: bool = True, window: int = 0,
+                        stream=None):
+    """Attention of the batch's queries q [tokens][heads][head_dim] over their
+    sequences' pages into output (which may be q): position p sees positions j <= p
+    when causal, j > p - window when window > 0, and the whole cached length
+    otherwise.  scale None: head_dim ** -0.5.  workspace: a uint8 GPU tensor of
+    paged_attention_workspace_size bytes (spb_paged_attention_*)."""
+    n, hd, dt = batch.num_tokens, cache.head_dim, cache.dtype
+    _half(q, "q")
+    nh = q.shape[1] if q.dim() == 3 else 0
+    pq, sq = _heads(q, "q", dt, n, nh, hd)
+    po, so = _heads(output, "output", dt, n, nh, hd)
+    _here(workspace, "workspace")
+    if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise TypeError("workspace must be a contiguous uint8 tensor")
+    fn = getattr(_lib.load(), f"spb_paged_attention_{cache.kind}")
+    _lib.check(fn(cache._ptr, batch._ptr, pq, po, sq, so, nh,
+                  hd ** -0.5 if scale is None else scale, 1 if causal else 0, window,
+                  workspace.data_ptr(), workspace.numel(), _stream_ptr(stream)),
+               "paged_attention_gpu")
