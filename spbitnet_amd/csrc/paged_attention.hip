@@ -11,14 +11,14 @@
 // permuted), and V^T's operand is read from LDS in the same permuted order by
 // the transposing LDS read (4 keys of one column per lane).
 #include <algorithm>
-#include <atomic>
+#include <type_traits>
 
 #include "paged.hpp"
 
 namespace spb {
 namespace {
 
-constexpr int kAttnBlock = 256;
+constexpr int kJoinBlock = 256;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -61,6 +61,12 @@ template <> struct Prob<BF16> {
     }
 };
 
+// What a worker leaves to the join: the tile that begins in its part and goes on in
+// others' (pieces of the tile; 0 if there is none).
+struct Split {
+    int pieces, first, count, len, qt, kvh;
+};
+
 struct AttnArgs {
     BatchArgs b;
     const uint16_t *q, *k, *v;
@@ -70,136 +76,218 @@ struct AttnArgs {
     FastDiv group;  // query heads of a kv head
     float c;        // scale * log2(e)
     int causal, window;
-    int target;   // pieces of work to aim at
-    int slots;    // partial results that the workspace holds
-    float* ws;
+    // keys that a tile with a window sees at most: the window and its tokens, (BM -
+    // 1) / group + 1 of them and one more where it begins inside a token
+    double reach;
+    double per_worker;  // 1 / the least cost worth a worker
+    uint32_t workers;   // at most, = blocks launched
+    Split* splits;     // [workers]
+    float* ws;         // partial results, 2 per worker
 };
 
-// A tile's shape: RG groups of 32 rows times KG groups of NS * 32 keys over the
-// four waves.  One group of rows (decoding): the waves take different keys and
-// their results are joined at the end; four: all waves read the same keys.
+// A tile's shape: RG waves of 32 rows each, which all walk over the same keys; a
+// single wave of rows (decoding) gets a second one, and the two take turns at 32
+// keys and join their results at the end.
 template <int RG>
 struct Shape {
-    static constexpr int KG = 4 / RG, NS = RG == 1 ? 1 : 2;
+    static constexpr int KG = RG == 1 ? 2 : 1, NS = RG == 1 ? 1 : 2;  // groups of 32 NS keys
+    static constexpr int kWaves = RG * KG, kThreads = kWave * kWaves;
     static constexpr int BM = 32 * RG, BN = 32 * KG * NS;
+    static_assert(BN == kWave, "a lane per key of a tile");
+    // Fewest keys worth a worker of their own.
+    static constexpr int kMinKeys = RG == 4 ? 256 : 64;
 };
 
-// One piece of work: keys [kb, ke) for the tile `qt` of a sequence and kv head.
-struct Piece {
-    int seq, first, count, len;
-    int qt, kvh, lo, hi;  // keys that any row of the tile sees
-    int kb, ke;
-    int nsplit;  // pieces of this tile
-    int slot;    // the tile's first partial result
-    int split;
+// How a batch's work is shared out.  Its tiles stand in one line, ordered by
+// sequence, kv head and row tile, each as long as its cost (keys seen times the
+// group / 32, and a block for what a tile costs besides); the line is cut into
+// equal parts, one per worker, and every worker walks over its part.  So the work
+// per worker is the same whatever the mix of lengths, and a tile is split only where
+// a cut falls into it.  Every wave computes the cuts by itself from the batch's
+// arrays, a lane per sequence.  Places are whole numbers in float64, exact below
+// 2^53 (rows times keys times the group / 1024: 2^46 for a million tokens of 64
+// heads over a million keys); a 64-bit integer division took a microsecond of the
+// 10 that a small call has.  A cost need not be exact: it decides only who does
+// what.
+struct Plan {
+    double part, total;  // of the line
+    uint32_t workers;    // those with work
+    __device__ __forceinline__ double cut(uint32_t w) const {
+        return w >= workers ? total : floor(part * w);
+    }
+    // The worker in whose part lies the last of the line before `end` > 0.
+    __device__ __forceinline__ uint32_t last_before(double end) const {
+        uint32_t w = min(static_cast<uint32_t>(end / part), workers - 1);
+        while (w > 0 && cut(w) >= end) --w;
+        while (w + 1 < workers && cut(w + 1) < end) ++w;
+        return w;
+    }
 };
+
+// A sequence in the line: tile j of each kv head costs c0 + c1 j.
+struct SeqCost {
+    double c0, c1, head;  // head: all tiles of one kv head
+    int tiles;
+};
+
+// Cost of the tiles before tile j.
+__device__ __forceinline__ double cost_before(double c0, double c1, int j) {
+    const double n = j;
+    return n * c0 + c1 * (n * (n - 1.0) * 0.5);
+}
+
+template <int BM, int BN>
+__device__ __forceinline__ SeqCost seq_cost(const AttnArgs& a, const SeqSpan& q) {
+    const int group = a.group.d;
+    const uint32_t rows = static_cast<uint32_t>(q.count) * group;
+    SeqCost r;
+    r.tiles = static_cast<int>((rows + BM - 1) / BM);
+    const bool grows = a.causal && (a.window == 0 || a.reach >= q.len);
+    const double keys = grows ? max(q.len - q.count, 0) : (a.causal ? a.reach : q.len);
+    r.c0 = floor((keys + BN) * group * (1.0 / 32)) + (grows ? BM / 32 : 0) + 1.0;
+    r.c1 = grows ? BM / 32 : 0.0;
+    r.head = cost_before(r.c0, r.c1, r.tiles);
+    return r;
+}
 
 __device__ __forceinline__ int lane_int(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+__device__ __forceinline__ double lane_f64(double v, int l) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = lane_int(static_cast<int>(u), l), hi = lane_int(static_cast<int>(u >> 32), l);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+// A value that all lanes have, in scalar registers.
+__device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ double scalar(double v) { return lane_f64(v, 0); }
 
-// Positions that the tile's rows see: [lo, hi).
+// Sums over the lanes up to each lane, by lane shifts inside rows of 16 and two
+// broadcasts across them.
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), kCtrl, kRowMask, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), kCtrl, kRowMask, 0xF, false);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double prefix_sum(double v) {
+    v += dpp_f64<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+    v += dpp_f64<0x112, 0xF>(v);
+    v += dpp_f64<0x114, 0xF>(v);
+    v += dpp_f64<0x118, 0xF>(v);
+    v += dpp_f64<0x142, 0xA>(v);  // lane 15 of each even row into the next
+    v += dpp_f64<0x143, 0xC>(v);  // lane 31 into the upper half
+    return v;
+}
+
+// 64 sequences, a lane each: what they cost, and the places where they end in the
+// line if the first begins at 0.
+struct Lanes {
+    SeqSpan q;
+    SeqCost c;
+    double end;
+};
+
+template <int BM, int BN>
+__device__ __forceinline__ Lanes look(const AttnArgs& a, int base) {
+    Lanes r;
+    const int s = base + (threadIdx.x & (kWave - 1));
+    r.q = {0, 0, 0};
+    if (s < a.b.seqs) r.q = seq_span(a.b, s);
+    r.c = seq_cost<BM, BN>(a, r.q);
+    r.end = prefix_sum(r.c.head * a.kv_heads);
+    return r;
+}
+
+template <int BM, int BN>
+__device__ __forceinline__ Plan make_plan(const AttnArgs& a, const Lanes& first) {
+    Plan p;
+    p.total = lane_f64(first.end, kWave - 1);
+    for (int base = kWave; base < a.b.seqs; base += kWave)
+        p.total += lane_f64(look<BM, BN>(a, base).end, kWave - 1);
+    const double most = p.total * a.per_worker + 1.0;
+    p.workers = p.total == 0.0 ? 0 : scalar(static_cast<int>(fmin(most, a.workers)));
+    p.part = scalar(p.total / p.workers);
+    return p;
+}
+
+// The tile at a place of the line.
+struct Tile {
+    double begin, end;  // in the line
+    double c0, c1;      // of its sequence
+    int tiles, seq, first, count, len;
+    int qt, kvh;
+};
+
+template <int BM, int BN>
+__device__ __forceinline__ Tile find_tile(const AttnArgs& a, Lanes x, double at) {
+    double before = 0.0;
+    Tile r = {};
+    for (int base = 0; base < a.b.seqs; base += kWave) {
+        if (base) x = look<BM, BN>(a, base);
+        const uint64_t hit = __ballot(at < before + x.end);
+        if (hit) {
+            const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+            r.seq = base + l;
+            r.first = lane_int(x.q.first, l);
+            r.count = lane_int(x.q.count, l);
+            r.len = lane_int(x.q.len, l);
+            r.c0 = lane_f64(x.c.c0, l);
+            r.c1 = lane_f64(x.c.c1, l);
+            r.tiles = lane_int(x.c.tiles, l);
+            const double head = lane_f64(x.c.head, l);
+            // the place in the sequence
+            double in = at - (before + lane_f64(x.end, l) - head * a.kv_heads);
+            r.kvh = scalar(static_cast<int>(in / head));
+            if (r.kvh * head > in) --r.kvh;  // a quotient that was rounded up
+            in -= r.kvh * head;
+            r.qt = 0;
+            if (r.tiles > 1) {  // cost_before(j) = in, solved in float32, then put right
+                const float h = static_cast<float>(r.c0 - 0.5 * r.c1), y = static_cast<float>(in);
+                const float c1 = static_cast<float>(r.c1);
+                const float j = c1 == 0.0f ? y / h : (sqrtf(h * h + 2.0f * c1 * y) - h) / c1;
+                r.qt = min(max(scalar(static_cast<int>(j)), 0), r.tiles - 1);
+                while (r.qt > 0 && cost_before(r.c0, r.c1, r.qt) > in) --r.qt;
+                while (r.qt + 1 < r.tiles && cost_before(r.c0, r.c1, r.qt + 1) <= in) ++r.qt;
+            }
+            r.begin = scalar(at - in + cost_before(r.c0, r.c1, r.qt));
+            r.end = scalar(r.begin + (r.c0 + r.c1 * r.qt));
+            return r;
+        }
+        before += lane_f64(x.end, kWave - 1);
+    }
+    return r;
+}
+
+template <int BM, int BN>
+__device__ __forceinline__ void next_tile(const AttnArgs& a, Tile& t) {
+    if (++t.qt == t.tiles) {
+        t.qt = 0;
+        if (++t.kvh == a.kv_heads) {
+            t = find_tile<BM, BN>(a, look<BM, BN>(a, 0), t.end);
+            return;
+        }
+    }
+    t.begin = t.end;
+    t.end = scalar(t.end + (t.c0 + t.c1 * t.qt));
+}
+
+// Keys that the tile's rows see: [lo, hi).
 template <int BM>
-__device__ __forceinline__ void tile_range(const AttnArgs& a, int count, int len, int qt, int& lo,
-                                           int& hi) {
-    const int rows = count * static_cast<int>(a.group.d);
-    const int i0 = a.group.div(qt * BM), i1 = a.group.div(min(qt * BM + BM, rows) - 1);
-    const int p0 = len - count + i0, p1 = len - count + i1;
-    hi = a.causal ? min(p1 + 1, len) : len;
+__device__ __forceinline__ void tile_range(const AttnArgs& a, const Tile& t, int& lo, int& hi) {
+    const int rows = t.count * static_cast<int>(a.group.d);
+    const int i0 = a.group.div(t.qt * BM), i1 = a.group.div(min(t.qt * BM + BM, rows) - 1);
+    const int p0 = t.len - t.count + i0, p1 = t.len - t.count + i1;
+    hi = a.causal ? min(p1 + 1, t.len) : t.len;
     lo = a.window ? max(p0 - a.window + 1, 0) : 0;
     if (hi < lo) hi = lo;
 }
 
-// Work item -> piece.  Every wave finds its own, a lane per sequence and 64
-// sequences at a time: the total work W (tiles times blocks of BN keys) gives
-// the blocks per piece C = ceil(W / target), so long sequences are split and
-// short ones are not, whatever the mix; then a prefix sum over the sequences'
-// pieces finds the item's.  kTiles: items are (tile, kv head), without splits.
-template <int BM, int BN, bool kTiles>
-__device__ __forceinline__ bool find_piece(const AttnArgs& a, unsigned item, Piece& r) {
-    const int lane = threadIdx.x & (kWave - 1);
-    const int group = a.group.d;
-    // tokens of a tile: (BM - 1) / group + 1, one more where it begins inside a token
-    const int reach = a.window > 0 && a.causal && a.window < 0x3FFFFFFF
-                          ? a.window + (BM - 1) / group + 2 : 0x7FFFFFFF;
-    SeqSpan q0 = {0, 0, 0};
-    if (lane < a.b.seqs) q0 = seq_span(a.b, lane);
-    uint64_t work = 0;
-    for (int base = 0; base < a.b.seqs; base += kWave) {
-        SeqSpan q = q0;
-        if (base) {
-            q = {0, 0, 0};
-            if (base + lane < a.b.seqs) q = seq_span(a.b, base + lane);
-        }
-        const uint32_t tiles = (static_cast<uint32_t>(q.count) * group + BM - 1) / BM;
-        // a window's keys need not begin at a block's
-        const uint32_t blocks = min((q.len + BN - 1) / BN, reach / BN + 2);
-        uint64_t w = static_cast<uint64_t>(tiles) * blocks;
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1)
-            w += static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(w), off, kWave));
-        work += w;
-    }
-    work *= a.kv_heads;
-    const uint64_t per64 = (work + a.target - 1) / a.target;
-    const int per = static_cast<int>(min(max(per64, uint64_t{1}), uint64_t{0x7FFFFFFF}));
-    unsigned seen = 0;
-    int slot = 0;
-    for (int base = 0; base < a.b.seqs; base += kWave) {
-        SeqSpan q = q0;
-        if (base) {
-            q = {0, 0, 0};
-            if (base + lane < a.b.seqs) q = seq_span(a.b, base + lane);
-        }
-        const unsigned tiles = (static_cast<unsigned>(q.count) * group + BM - 1) / BM;
-        const int blocks = min((q.len + BN - 1) / BN, reach / BN + 2);
-        const int split = max(1, (blocks + per - 1) / per);
-        const unsigned all = tiles * a.kv_heads * split;
-        const unsigned mine = kTiles ? tiles * a.kv_heads : all;
-        const unsigned kept = split > 1 ? all : 0;
-        unsigned sum = mine, ksum = kept;
-#pragma unroll
-        for (int off = 1; off < kWave; off <<= 1) {
-            const unsigned x = __shfl_up(sum, off, kWave), y = __shfl_up(ksum, off, kWave);
-            if (lane >= off) {
-                sum += x;
-                ksum += y;
-            }
-        }
-        const uint64_t hit = __ballot(item < seen + sum && mine > 0);
-        if (hit) {
-            const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
-            r.seq = base + l;
-            r.first = lane_int(q.first, l);
-            r.count = lane_int(q.count, l);
-            r.len = lane_int(q.len, l);
-            const int ns = lane_int(split, l);
-            unsigned local = item - (seen + lane_int(static_cast<int>(sum - mine), l));
-            const int seq_slot = slot + lane_int(static_cast<int>(ksum - kept), l);
-            int sp = 0;
-            if (!kTiles) {
-                sp = local % ns;
-                local /= ns;
-            }
-            const int unit = local;
-            r.kvh = unit % a.kv_heads;
-            const int ntiles = lane_int(static_cast<int>(tiles), l);
-            r.qt = ntiles - 1 - unit / a.kv_heads;  // the tiles that see most first
-            r.slot = seq_slot + unit * ns;
-            tile_range<BM>(a, r.count, r.len, r.qt, r.lo, r.hi);
-            const int b0 = r.lo / BN, nb = r.hi > r.lo ? (r.hi + BN - 1) / BN - b0 : 0;
-            // even pieces of the tile's own blocks
-            r.nsplit = min(ns, max(1, (nb + per - 1) / per));
-            const int each = max(1, (nb + r.nsplit - 1) / r.nsplit);
-            r.nsplit = max(1, (nb + each - 1) / each);
-            r.split = sp;
-            r.kb = (b0 + sp * each) * BN;
-            r.ke = static_cast<int>(min(static_cast<long>(r.hi),
-                                        static_cast<long>(b0 + sp * each + each) * BN));
-            return kTiles || sp < r.nsplit;
-        }
-        seen += lane_int(static_cast<int>(sum), kWave - 1);
-        slot += lane_int(static_cast<int>(ksum), kWave - 1);
-    }
-    return false;
+// The blocks of BN keys of a tile that lie before a place of the line: the share of
+// the tile's cost, so neighbours that compute it for their common cut agree.
+__device__ __forceinline__ int blocks_before(const Tile& t, double at, int blocks) {
+    if (at <= t.begin) return 0;
+    if (at >= t.end) return blocks;
+    return scalar(static_cast<int>((at - t.begin) * blocks / (t.end - t.begin)));
 }
 
 // Bytes of an LDS row of K or V, and the swizzle of its 16-byte units: lanes
@@ -210,14 +298,34 @@ struct Row {
     static constexpr int kPitch = HD <= 64 ? 128 : (HD <= 128 ? 256 : 512);
     static constexpr int kUnits = kPitch / 16;
     static constexpr int kMask = kUnits < 16 ? kUnits - 1 : 15;
+    static __device__ __forceinline__ int k_unit(int key, int unit) { return unit ^ (key & kMask); }
+    static __device__ __forceinline__ int v_unit(int key, int unit) {
+        return unit ^ (kPitch >= 256 ? (key & 3) << 2 : (key & 2) << 1);
+    }
     static __device__ __forceinline__ int k_at(int key, int unit) {
-        return key * kPitch + ((unit ^ (key & kMask)) << 4);
+        return key * kPitch + (k_unit(key, unit) << 4);
     }
     static __device__ __forceinline__ int v_at(int key, int unit) {
-        const int x = kPitch >= 256 ? (key & 3) << 2 : (key & 2) << 1;
-        return key * kPitch + ((unit ^ x) << 4);
+        return key * kPitch + (v_unit(key, unit) << 4);
     }
 };
+
+// 16 bytes of each active lane from memory to LDS, at lds + 16 lane.
+template <bool kOnce>  // non-temporal
+__device__ __forceinline__ void load_to_lds(const uint16_t* from, uint8_t* lds) {
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) void*)from,
+        (__attribute__((address_space(3))) void*)lds, 16, 0, kOnce ? 2 : 0);
+}
+// All of this wave's loads have arrived.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
+// Whether token i of a sequence sees any position.
+__device__ __forceinline__ bool row_sees(const AttnArgs& a, int count, int len, int i) {
+    const int pos = len - count + i;
+    const int hi = a.causal ? min(pos + 1, len) : len;
+    return hi > (a.window ? max(pos - a.window + 1, 0) : 0);
+}
 
 // x of the lower and of the upper half of the wave, in all lanes.
 __device__ __forceinline__ float2 halves(float x) {
@@ -250,335 +358,540 @@ __device__ __forceinline__ void store4(uint16_t* p, float x, float y, float z, f
     *reinterpret_cast<uint2*>(p) = r;
 }
 
-// Inf and NaN of a packed pair replaced by 0; `bad` notes that there was one.
+// Not 0 where a packed pair holds an inf or NaN: an exponent of all ones carries
+// into the bit above it, and no field into another.
 template <class T>
-__device__ __forceinline__ uint32_t finite_pair(uint32_t x, bool& bad) {
-    constexpr uint32_t e = Prob<T>::kExp;
-    const bool lo = (x & e) == e, hi = (x & (e << 16)) == (e << 16);
-    bad = bad || lo || hi;
-    return x & (lo ? 0xFFFF0000u : 0xFFFFFFFFu) & (hi ? 0x0000FFFFu : 0xFFFFFFFFu);
+__device__ __forceinline__ uint32_t non_finite(uint32_t x) {
+    constexpr uint32_t e = Prob<T>::kExp, one = e & (0u - e);
+    return ((x & (e << 16 | e)) + (one << 16 | one)) & 0x80008000u;
 }
 
+// One tile's state in a wave: 32 rows, their sums and statistics.
 template <class T, int HD, int RG>
-__global__ __launch_bounds__(kAttnBlock, HD <= 128 ? 2 : 1) void paged_attention_kernel(
-    const AttnArgs a) {
-    typedef Shape<RG> S;
+struct RowState {
+    u32x4 q[HD / 16];       // Q^T operand: row lane % 32, elements 16 step + 8 half ..
+    f32x16 o[HD / 32];      // O^T
+    float m, l;             // reference and (this half wave's) sum of the lane's row
+    int see_lo, see_hi;     // keys that the lane's row sees, of this piece
+    int all_lo, all_hi;     // ... that all rows of the wave see
+    int any_lo, any_hi;     // ... that any sees
+};
+
+// One tile of keys t .. t + BN in LDS (K, then V) against the wave's rows.
+template <class T, int HD, int RG>
+__device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, RG>& r,
+                                       const uint8_t* buf, int t, int kg, uint64_t there) {
     typedef Row<HD> R;
     typedef Prob<T> P;
-    constexpr int KG = S::KG, NS = S::NS, BM = S::BM, BN = S::BN;
-    constexpr int kSteps = HD / 16, kCols = HD / 32, kUnits = HD / 8;
-    constexpr int kLoads = BN * kUnits / kAttnBlock;  // 16-byte units of a thread, K and V each
-    extern __shared__ __align__(16) uint8_t attn_smem[];
-    uint8_t* const k_lds = attn_smem;
-    uint8_t* const v_lds = attn_smem + BN * R::kPitch;
-    float* const ml_lds = reinterpret_cast<float*>(attn_smem + 2 * BN * R::kPitch);  // [KG][BM][2]
-    int* const bad_lds = reinterpret_cast<int*>(ml_lds + KG * BM * 2);
+    constexpr int NS = Shape<RG>::NS, kSteps = HD / 16, kCols = HD / 32, kKeys = 32 * NS;
+    const int j0 = t + kKeys * kg;
+    if (j0 >= r.any_hi || j0 + kKeys <= r.any_lo) return;
+    const uint8_t* const kw = buf + kKeys * kg * R::kPitch;
+    const uint8_t* const vw = kw + Shape<RG>::BN * R::kPitch;
+    const int lane = threadIdx.x & (kWave - 1), half = lane >> 5;
+    // Reads of LDS go out a group ahead of the products that use them: left to itself
+    // the compiler puts each right before its use, whose wait then shows.
+    f32x16 s[NS];
+    constexpr int kGroup = 2, kGroups = kSteps / kGroup;  // steps
+    u32x4 k[2][kGroup][NS];
+    auto load_k = [&](int g) {
+#pragma unroll
+        for (int st = 0; st < kGroup; ++st)
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+                k[g & 1][st][n] = *reinterpret_cast<const u32x4*>(
+                    kw + R::k_at(32 * n + (lane & 31), 2 * (g * kGroup + st) + half));
+    };
+    static_assert(kSteps % kGroup == 0, "whole groups");
+    load_k(0);
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        if (g + 1 < kGroups) load_k(g + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int st = 0; st < kGroup; ++st)
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+                s[n] = P::mfma(k[g & 1][st][n], r.q[g * kGroup + st],
+                               g + st == 0 ? f32x16{} : s[n]);
+    }
+    // V^T operands of 16 keys; lane: column 32 c + lane % 32, keys 4 half .. and 8 + 4 half ..
+    const int l16 = lane & 15;
+    auto load_v = [&](int g, u32x4 (&v)[kCols]) {
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+            const int key = 16 * g + 4 * half + (l16 >> 2);
+            const int unit = 4 * c + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+            const int off = (l16 & 1) << 3;
+            union {
+                s16x4 h[2];
+                u32x4 v;
+            } x;
+            x.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s16x4*)(vw + R::v_at(key, unit) + off));
+            x.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s16x4*)(vw + R::v_at(key + 8, unit) + off));
+            v[c] = x.v;
+        }
+    };
+    u32x4 v[2][kCols];
+    if (j0 < r.all_lo || j0 + kKeys > r.all_hi || there != ~uint64_t{0}) {  // not all rows see all
+        const int lo = r.see_lo - j0 - 4 * half, hi = r.see_hi - j0 - 4 * half;
+        const uint64_t mine = there >> (kKeys * kg + 4 * half);
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int j = 32 * n + 8 * (i / 4) + i % 4;
+                if (j < lo || j >= hi || !(mine >> j & 1)) s[n][i] = -INFINITY;
+            }
+    }
+    // the row's largest score, and its reference
+    float top = s[0][0];
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
+    top = half_max(top) * a.c - P::kBias;
+    const bool move = top > r.m + P::kSlack;  // also from m = -inf
+    if (__any(move)) {
+        const float f = move ? __builtin_amdgcn_exp2f(r.m - top) : 1.0f;
+        if (move) r.m = top;
+        r.l *= f;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r.o[c][i] *= f;
+    }
+    const float ref = r.m == -INFINITY ? 0.0f : r.m;  // a row that has seen nothing yet
+    load_v(0, v[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4 pf[2 * NS];
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], a.c, -ref));
+            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i + 1], a.c, -ref));
+            sum[i % 4] += x;
+            sum[i % 4 + 1] += y;
+            pf[2 * n + i / 8][(i % 8) / 2] = P::pack(x, y);
+        }
+    r.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    // O^T += V^T P^T
+#pragma unroll
+    for (int g = 0; g < 2 * NS; ++g) {
+        if (g + 1 < 2 * NS) load_v(g + 1, v[(g + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) r.o[c] = P::mfma(v[g & 1][c], pf[g], r.o[c]);
+    }
+}
 
-    Piece w;
-    if (!find_piece<BM, BN, false>(a, blockIdx.x, w)) return;
+// Keys that some rows of a tile see and others do not must not have inf or NaN in V:
+// the product of a probability of 0 with them would reach the rows that do not see
+// them.  Replaces them by 0 in LDS and says whether there were any (here or in an
+// earlier tile).  All threads call it.
+template <class T, int HD, int RG>
+__device__ __forceinline__ bool take_out(uint8_t* buf, int* found) {
+    typedef Shape<RG> S;
+    constexpr int kAll = S::BN * Row<HD>::kUnits;
+    u32x4* const v = reinterpret_cast<u32x4*>(buf + S::BN * Row<HD>::kPitch);
+    for (int i = threadIdx.x; i < kAll; i += S::kThreads) {
+        u32x4 x = v[i];
+        if (non_finite<T>(x[0]) | non_finite<T>(x[1]) | non_finite<T>(x[2]) | non_finite<T>(x[3])) {
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t bad = non_finite<T>(x[e]);
+                x[e] &= (bad & 0x8000u ? 0u : 0x0000FFFFu) | (bad >> 31 ? 0u : 0xFFFF0000u);
+            }
+            v[i] = x;
+            *found = 1;
+        }
+    }
+    __syncthreads();
+    return *found != 0;
+}
 
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+// Adds what take_out took out of the tile to the rows that see it, from memory.
+template <class T, int HD, int RG>
+__device__ __forceinline__ void put_back(const AttnArgs& a, RowState<T, HD, RG>& r, int t, int end,
+                                         int kg, const int* table, const uint16_t* vbase) {
+    constexpr int kKeys = 32 * Shape<RG>::NS;
+    const int half = (threadIdx.x & (kWave - 1)) >> 5;
+    for (int j = t + kKeys * kg; j < min(t + kKeys * (kg + 1), end); ++j) {
+        const int p = a.b.page.div(j), id = table[p];
+        if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.b.pages)) continue;
+        const uint16_t* const v = vbase + id * a.page_stride +
+                                  (j - p * static_cast<int>(a.b.page.d)) * a.slot_stride + 4 * half;
+        const bool mine = j >= r.see_lo && j < r.see_hi;
+        int hd = a.head_dim;
+        asm volatile("" : "+v"(hd));  // else the comparisons below are kept over all tiles
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                if (32 * c + 2 * i >= hd) continue;
+                const uint2 x = *reinterpret_cast<const uint2*>(v + 32 * c + 2 * i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t y = (e < 2 ? x.x : x.y) >> (e % 2 * 16) & 0xFFFFu;
+                    if (mine && (y & Prob<T>::kExp) == Prob<T>::kExp)
+                        r.o[c][i + e] += T::to_float(static_cast<uint16_t>(y));
+                }
+            }
+    }
+}
+
+// What lanes load for keys and columns that are not there.
+__device__ __align__(16) const uint32_t kZeros[4] = {0, 0, 0, 0};
+
+// Blocks of a CU that LDS and registers hold.
+template <int HD, int RG>
+constexpr int resident() { return HD > 128 ? 1 : (RG <= 2 && HD <= 64 ? 4 : 2); }
+
+template <int HD, int RG>
+constexpr int waves_per_simd() { return Shape<RG>::kWaves * resident<HD, RG>() >= 8 ? 2 : 1; }
+
+template <class T, int HD, int RG>
+__global__ __launch_bounds__((Shape<RG>::kThreads), (waves_per_simd<HD, RG>()))
+void paged_attention_kernel(const AttnArgs a) {
+    typedef Shape<RG> S;
+    typedef Row<HD> R;
+    constexpr int KG = S::KG, BM = S::BM, BN = S::BN;
+    constexpr int kSteps = HD / 16, kCols = HD / 32;
+    constexpr int kRows = kWave / R::kUnits;                // rows of K that a wave's load fills
+    constexpr int kLoads = BN / (kRows * S::kWaves);        // loads of a wave, K and V each
+    // Two tiles of keys: one is filled while the other is read.  Two arrays, so that
+    // the compiler sees that reads of one need not wait for loads into the other.
+    __shared__ __align__(16) uint8_t buf0[2 * BN * R::kPitch];
+    __shared__ __align__(16) uint8_t buf1[2 * BN * R::kPitch];
+    __shared__ float ml_lds[KG][BM][2];
+    __shared__ int found_lds;  // take_out's
+
+    const Lanes lanes = look<BM, BN>(a, 0);
+    const Plan plan = make_plan<BM, BN>(a, lanes);
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = scalar(tid / kWave);
+    if (blockIdx.x >= plan.workers) {
+        if (tid == 0) a.splits[blockIdx.x].pieces = 0;
+        return;
+    }
+    // Blocks go to the 8 dies in turn, each with its own L2: a die gets a run of the
+    // line, whose neighbouring tiles read the same keys.
+    const uint32_t die = blockIdx.x & 7, of_die = plan.workers >> 3, more = plan.workers & 7;
+    const uint32_t worker = die * of_die + min(die, more) + (blockIdx.x >> 3);
+    const double from = scalar(plan.cut(worker)), to = scalar(plan.cut(worker + 1));
     const int rg = wave % RG, kg = wave / RG, half = lane >> 5;
-    const int group = a.group.d, rows = w.count * group;
-    const int row0 = w.qt * BM + 32 * rg, row = row0 + (lane & 31);
-    const int tok = a.group.div(min(row, rows - 1)), head = w.kvh * group + min(row, rows - 1) - tok * group;
-    const bool live = row0 < rows;  // the wave has a row
+    const int group = a.group.d;
+    if (tid == 0) found_lds = 0;  // the next barrier is before the first tile's
+    Split left_over = {0, 0, 0, 0, 0, 0};
 
-    // the keys that this lane's row sees, of this piece
-    int see_lo = 0, see_hi = 0;
-    bool none = true;
-    if (row < rows) {
-        const int pos = w.len - w.count + tok;
-        see_hi = a.causal ? min(pos + 1, w.len) : w.len;
-        see_lo = a.window ? max(pos - a.window + 1, 0) : 0;
-        none = see_hi <= see_lo;
-    }
-    // ... and all rows of the wave: keys [all_lo, all_hi) need no mask
-    int all_lo = 0, all_hi = 0, any_lo = 0, any_hi = 0;
-    if (live) {
-        const int t0 = a.group.div(row0), t1 = a.group.div(min(row0 + 31, rows - 1));
-        const int p0 = w.len - w.count + t0, p1 = w.len - w.count + t1;
-        all_hi = a.causal ? min(p0 + 1, w.len) : w.len;
-        any_hi = a.causal ? min(p1 + 1, w.len) : w.len;
-        all_lo = a.window ? max(p1 - a.window + 1, 0) : 0;
-        any_lo = a.window ? max(p0 - a.window + 1, 0) : 0;
-    }
-    see_lo = max(see_lo, w.kb);
-    see_hi = min(see_hi, w.ke);
-    all_lo = max(all_lo, w.kb);
-    all_hi = min(all_hi, w.ke);
-    any_lo = max(any_lo, w.kb);
-    any_hi = min(any_hi, w.ke);
+    for (Tile w = find_tile<BM, BN>(a, lanes, from);; next_tile<BM, BN>(a, w)) {
+        const int rows = w.count * group;
+        const bool whole = w.begin >= from && w.end <= to;
+        int kb, ke;  // this worker's keys of the tile
+        {
+            int lo, hi;
+            tile_range<BM>(a, w, lo, hi);
+            const int b0 = lo / BN, blocks = hi > lo ? (hi + BN - 1) / BN - b0 : 0;
+            const int k0 = blocks_before(w, from, blocks), k1 = blocks_before(w, to, blocks);
+            kb = (b0 + k0) * BN;
+            ke = k0 == k1 ? kb : (k1 == blocks ? hi : (b0 + k1) * BN);
+        }
+        const int row0 = w.qt * BM + 32 * rg, row = row0 + (lane & 31);
+        const int tok = a.group.div(min(row, rows - 1));
+        const int head = w.kvh * group + min(row, rows - 1) - tok * group;
 
-    // Q^T operand: row lane % 32, elements 16 step + 8 half ..
-    u32x4 qf[kSteps];
-    {
-        const uint16_t* qp = a.q + static_cast<long>(w.first + tok) * a.q_stride +
-                             static_cast<long>(head) * a.head_dim + 8 * half;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            qf[s] = u32x4{0, 0, 0, 0};
-            if (row < rows && 16 * s + 8 * half < a.head_dim)
-                qf[s] = *reinterpret_cast<const u32x4*>(qp + 16 * s);
+        RowState<T, HD, RG> r;
+        r.see_lo = r.see_hi = r.all_lo = r.all_hi = r.any_lo = r.any_hi = 0;
+        bool none = true;
+        if (row < rows) {
+            const int pos = w.len - w.count + tok;
+            r.see_hi = a.causal ? min(pos + 1, w.len) : w.len;
+            r.see_lo = a.window ? max(pos - a.window + 1, 0) : 0;
+            none = r.see_hi <= r.see_lo;
         }
-    }
+        if (row0 < rows) {
+            const int t0 = a.group.div(row0), t1 = a.group.div(min(row0 + 31, rows - 1));
+            const int p0 = w.len - w.count + t0, p1 = w.len - w.count + t1;
+            r.all_hi = a.causal ? min(p0 + 1, w.len) : w.len;
+            r.any_hi = a.causal ? min(p1 + 1, w.len) : w.len;
+            r.all_lo = a.window ? max(p1 - a.window + 1, 0) : 0;
+            r.any_lo = a.window ? max(p0 - a.window + 1, 0) : 0;
+        }
+        r.see_lo = max(r.see_lo, kb);
+        r.see_hi = min(r.see_hi, ke);
+        r.all_lo = max(r.all_lo, kb);
+        r.all_hi = min(r.all_hi, ke);
+        r.any_lo = max(r.any_lo, kb);
+        r.any_hi = min(r.any_hi, ke);
 
-    // Loads of a tile of keys: thread unit i is row (tid + 256 i) / kUnits, unit
-    // (tid + 256 i) % kUnits.  Page ids are fetched a tile ahead of their pages.
-    const int* const table = a.b.table + static_cast<long>(w.seq) * a.b.width;
-    const uint16_t* const kbase = a.k + w.kvh * a.head_stride;
-    const uint16_t* const vbase = a.v + w.kvh * a.head_stride;
-    u32x4 kreg[kLoads], vreg[kLoads];
-    int page[kLoads];
-    auto fetch_pages = [&](int t) {
+        // Loads go from memory straight to LDS, 16 bytes a lane and a wave's lanes side
+        // by side; the swizzle is in which unit of its row a lane fetches.  Lane i of a
+        // wave finds the place of key t + i, its page a tile ahead of its use; a load's
+        // lanes get their rows' places from it.  Keys past the piece's end, those of bad
+        // pages and columns past head_dim are zeros.
+        const int* const table = a.b.table + static_cast<long>(w.seq) * a.b.width;
+        const uint16_t* const kbase = a.k + w.kvh * a.head_stride;
+        const uint16_t* const vbase = a.v + w.kvh * a.head_stride;
+        const int units = a.head_dim / 8;
+        int page = 0;
+        auto fetch_page = [&](int t) {
+            if (t < ke) page = table[a.b.page.div(min(t + lane, ke - 1))];
+        };
+        auto load_tile = [&](int t, uint8_t* buf) {  // -> which of its keys are there
+            const int j = min(t + lane, ke - 1);
+            const int slot = j - static_cast<int>(a.b.page.div(j) * a.b.page.d);
+            const bool in_pool = static_cast<unsigned>(page) < static_cast<unsigned>(a.b.pages);
+            const uint64_t there = __ballot(in_pool);
+            const bool here = in_pool && t + lane < ke;
+            const long at = here ? page * a.page_stride + slot * a.slot_stride : -1;
+            const int at_lo = static_cast<int>(at), at_hi = static_cast<int>(at >> 32);
+            const bool full = units == R::kUnits && __ballot(here) == ~uint64_t{0};
+            auto loads = [&](auto whole) {
+                int ln = lane;
+                // the rarer form computes its lane's numbers where it needs them, in place
+                // of registers held through all tiles
+                if (!decltype(whole)::value) asm volatile("" : "+v"(ln));
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int j = t + (tid + kAttnBlock * i) / kUnits;
-            page[i] = -1;
-            if (j < w.ke) page[i] = table[a.b.page.div(j)];
-        }
-    };
-    bool saw_bad = false;
-    auto load_tile = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int idx = tid + kAttnBlock * i, j = t + idx / kUnits, u = idx % kUnits;
-            kreg[i] = u32x4{0, 0, 0, 0};
-            vreg[i] = u32x4{0, 0, 0, 0};
-            const bool there = static_cast<unsigned>(page[i]) < static_cast<unsigned>(a.b.pages);
-            saw_bad = saw_bad || (j < w.ke && !there);
-            if (j < w.ke && there && 8 * u < a.head_dim) {
-                const int slot = j - static_cast<int>(a.b.page.div(j) * a.b.page.d);
-                const long at = page[i] * a.page_stride + slot * a.slot_stride + 8 * u;
-                kreg[i] = *reinterpret_cast<const u32x4*>(kbase + at);
-                vreg[i] = *reinterpret_cast<const u32x4*>(vbase + at);
-            }
-        }
-    };
-    auto store_tile = [&]() {
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int idx = tid + kAttnBlock * i, r = idx / kUnits, u = idx % kUnits;
-            *reinterpret_cast<u32x4*>(k_lds + R::k_at(r, u)) = kreg[i];
-            *reinterpret_cast<u32x4*>(v_lds + R::v_at(r, u)) = vreg[i];
-        }
-        if (saw_bad) *bad_lds = 1;
-    };
-
-    f32x16 o[kCols];
-#pragma unroll
-    for (int c = 0; c < kCols; ++c)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-
-    if (tid == 0) *bad_lds = 0;
-    fetch_pages(w.kb);
-    load_tile(w.kb);
-    fetch_pages(w.kb + BN);
-    for (int t = w.kb; t < w.ke; t += BN) {
-        __syncthreads();
-        store_tile();
-        __syncthreads();
-        if (t + BN < w.ke) {
-            load_tile(t + BN);
-            fetch_pages(t + 2 * BN);
-        }
-        const int j0 = t + 32 * NS * kg;  // this wave's keys
-        if (!live || j0 >= any_hi || j0 + 32 * NS <= any_lo) continue;
-        const uint8_t* const kw = k_lds + 32 * NS * kg * R::kPitch;
-        f32x16 s[NS];
-#pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
-#pragma unroll
-        for (int st = 0; st < kSteps; ++st)
-#pragma unroll
-            for (int n = 0; n < NS; ++n)
-                s[n] = P::mfma(*reinterpret_cast<const u32x4*>(
-                                   kw + R::k_at(32 * n + (lane & 31), 2 * st + half)),
-                               qf[st], s[n]);
-        const bool bad_page = *bad_lds != 0;
-        const bool masked = j0 < all_lo || j0 + 32 * NS > all_hi || bad_page;
-        if (masked) {
-#pragma unroll
-            for (int n = 0; n < NS; ++n)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int j = j0 + 32 * n + 8 * (i / 4) + 4 * half + i % 4;
-                    if (j < see_lo || j >= see_hi) s[n][i] = -INFINITY;
-                }
-            if (bad_page) {
-#pragma unroll
-                for (int n = 0; n < NS; ++n)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int j = j0 + 32 * n + 8 * (i / 4) + 4 * half + i % 4;
-                        if (j >= see_lo && j < see_hi &&
-                            static_cast<unsigned>(table[a.b.page.div(j)]) >=
-                                static_cast<unsigned>(a.b.pages))
-                            s[n][i] = -INFINITY;
+                for (int i = 0; i < kLoads; ++i) {
+                    const int row = (i * S::kWaves + wave) * kRows;  // of the wave's first lane
+                    const int key = row + ln / R::kUnits;
+                    const uint32_t lo = __shfl(at_lo, key, kWave), hi = __shfl(at_hi, key, kWave);
+                    const long off = static_cast<long>(static_cast<uint64_t>(hi) << 32 | lo);
+                    const int ku = R::k_unit(key, ln % R::kUnits);
+                    const int vu = R::v_unit(key, ln % R::kUnits);
+                    const uint16_t* kp = kbase + off + 8 * ku;
+                    const uint16_t* vp = vbase + off + 8 * vu;
+                    if (!decltype(whole)::value) {
+                        const uint16_t* const zeros = reinterpret_cast<const uint16_t*>(kZeros);
+                        if (off < 0 || ku >= units) kp = zeros;
+                        if (off < 0 || vu >= units) vp = zeros;
                     }
-            }
-        }
-        // the row's largest score, and its reference
-        float top = s[0][0];
-#pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
-        top = half_max(top) * a.c - P::kBias;
-        const bool move = top > m + P::kSlack;  // also from m = -inf
-        if (__any(move)) {
-            const float f = move ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
-            if (move) m = top;
-            l *= f;
-#pragma unroll
-            for (int c = 0; c < kCols; ++c)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[c][i] *= f;
-        }
-        const float ref = m == -INFINITY ? 0.0f : m;  // a row that has seen nothing yet
-        u32x4 pf[NS][2];
-#pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], a.c, -ref));
-                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i + 1], a.c, -ref));
-                l += x;
-                l += y;
-                pf[n][i / 8][(i % 8) / 2] = P::pack(x, y);
-            }
-        // O^T += V^T P^T; lane: column 32 c + lane % 32, keys 4 half .. and 8 + 4 half ..
-        const int l16 = lane & 15;
-        const uint8_t* const vw = v_lds + 32 * NS * kg * R::kPitch;
-        bool bad = false;
-#pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-                for (int c = 0; c < kCols; ++c) {
-                    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-                    const int key = 32 * n + 16 * g + 4 * half + (l16 >> 2);
-                    const int unit = 4 * c + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
-                    const int off = (l16 & 1) << 3;
-                    union {
-                        s16x4 h[2];
-                        u32x4 v;
-                    } x;
-                    x.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_s16x4*)(vw + R::v_at(key, unit) + off));
-                    x.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_s16x4*)(vw + R::v_at(key + 8, unit) + off));
-                    if (masked) {  // 0 * inf would reach rows that do not see the key
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x.v[e] = finite_pair<T>(x.v[e], bad);
-                    }
-                    o[c] = P::mfma(x.v, pf[n][g], o[c]);
+                    load_to_lds<RG <= 2>(kp, buf + row * R::kPitch);
+                    load_to_lds<RG <= 2>(vp, buf + (BN + row) * R::kPitch);
                 }
-        if (__any(bad)) {  // add what was taken out to the rows that see it
-            for (int j = 0; j < 32 * NS; ++j) {
-                const bool seen = j0 + j >= see_lo && j0 + j < see_hi;
+            };
+            if (full) loads(std::true_type());
+            else loads(std::false_type());
+            return there;
+        };
+
+        fetch_page(kb);
+        uint64_t there = ~uint64_t{0};
+        if (kb < ke) there = load_tile(kb, buf0);
+        fetch_page(kb + BN);
+        {
+            const uint16_t* qp = a.q + static_cast<long>(w.first + tok) * a.q_stride +
+                                 static_cast<long>(head) * a.head_dim + 8 * half;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                r.q[s] = u32x4{0, 0, 0, 0};
+                if (row < rows && 16 * s + 8 * half < a.head_dim)
+                    r.q[s] = *reinterpret_cast<const u32x4*>(qp + 16 * s);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r.o[c][i] = 0.0f;
+        r.m = -INFINITY;
+        r.l = 0.0f;
+        // keys that some rows of the tile see and others do not: [lo0, lo1) and [hi0, hi1)
+        int lo0, lo1, hi0, hi1;
+        {
+            const int t0 = a.group.div(w.qt * BM), t1 = a.group.div(min(w.qt * BM + BM, rows) - 1);
+            const int p0 = w.len - w.count + t0, p1 = w.len - w.count + t1;
+            hi0 = a.causal ? p0 + 1 : w.len;
+            hi1 = a.causal ? p1 + 1 : w.len;
+            lo0 = a.window ? p0 - a.window + 1 : 0;
+            lo1 = a.window ? p1 - a.window + 1 : 0;
+        }
+        auto step = [&](int t, uint8_t* buf, uint8_t* other) {
+            wait_loads();
+            __syncthreads();
+            uint64_t next = ~uint64_t{0};
+            if (t + BN < ke) next = load_tile(t + BN, other);
+            fetch_page(t + 2 * BN);
+            bool taken = false;
+            if ((t < hi1 && t + BN > hi0 && hi0 < hi1) || (t < lo1 && t + BN > lo0 && lo0 < lo1))
+                taken = take_out<T, HD, RG>(buf, &found_lds);
+            attend<T, HD, RG>(a, r, buf, t, kg, there);
+            if (taken) put_back<T, HD, RG>(a, r, t, ke, kg, table, vbase);
+            there = next;
+        };
+        for (int t = kb; t < ke; t += 2 * BN) {
+            step(t, buf0, buf1);
+            if (t + BN >= ke) break;
+            step(t + BN, buf1, buf0);
+        }
+
+        r.l = half_sum(r.l);
+        float* const part = partial<HD, BM>(a, 2 * worker + (w.begin >= from ? 1 : 0));
+        if (KG == 1) {
+            const int rt = 32 * rg + (lane & 31);
+            if (row >= rows) {
+            } else if (!whole) {
+                if (half == 0) {
+                    part[BM * HD + 2 * rt] = r.m;
+                    part[BM * HD + 2 * rt + 1] = r.l;
+                }
 #pragma unroll
                 for (int c = 0; c < kCols; ++c)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int d = 32 * c + 8 * (i / 4) + 4 * half + i % 4;
-                        const uint16_t x = *reinterpret_cast<const uint16_t*>(
-                            vw + R::v_at(j, d >> 3) + 2 * (d & 7));
-                        if (seen && (x & P::kExp) == P::kExp) o[c][i] += T::to_float(x);
+                    for (int i = 0; i < 16; i += 4)
+                        *reinterpret_cast<float4*>(part + rt * HD + 32 * c + 8 * (i / 4) + 4 * half) =
+                            make_float4(r.o[c][i], r.o[c][i + 1], r.o[c][i + 2], r.o[c][i + 3]);
+            } else {
+                const float inv = none ? 0.0f : 1.0f / r.l;
+                uint16_t* const op = a.out + static_cast<long>(w.first + tok) * a.out_stride +
+                                     static_cast<long>(head) * a.head_dim;
+#pragma unroll
+                for (int c = 0; c < kCols; ++c)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const int d = 32 * c + 8 * (i / 4) + 4 * half;
+                        if (d < a.head_dim)
+                            store4<T>(op + d, r.o[c][i] * inv, r.o[c][i + 1] * inv,
+                                      r.o[c][i + 2] * inv, r.o[c][i + 3] * inv);
                     }
             }
-        }
-    }
-
-    l = half_sum(l);
-    float* const part = partial<HD, BM>(a, w.slot + w.split);
-    if (KG == 1) {
-        if (row >= rows) return;
-        const int r = 32 * rg + (lane & 31);
-        if (w.nsplit > 1) {
+        } else {
+            // join the key groups: the references first, then the scaled sums through LDS
+            const int rt = 32 * rg + (lane & 31);
             if (half == 0) {
-                part[BM * HD + 2 * r] = m;
-                part[BM * HD + 2 * r + 1] = l;
+                ml_lds[kg][rt][0] = r.m;
+                ml_lds[kg][rt][1] = r.l;
             }
+            __syncthreads();  // also: every wave has read its last keys
+            float top = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < kCols; ++c)
+            for (int k = 0; k < KG; ++k) top = fmaxf(top, ml_lds[k][rt][0]);
+            const float f = r.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(r.m - top);
+            float* const obuf = reinterpret_cast<float*>(buf0);  // [KG][BM][HD]
+            const int left = min(rows - w.qt * BM, BM);
+            if (row < rows)
 #pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                    *reinterpret_cast<float4*>(part + r * HD + 32 * c + 8 * (i / 4) + 4 * half) =
-                        make_float4(o[c][i], o[c][i + 1], o[c][i + 2], o[c][i + 3]);
-            return;
+                for (int c = 0; c < kCols; ++c)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const int d = 32 * c + 8 * (i / 4) + 4 * half;
+                        *reinterpret_cast<float4*>(obuf + (kg * BM + rt) * HD + d) = make_float4(
+                            r.o[c][i] * f, r.o[c][i + 1] * f, r.o[c][i + 2] * f, r.o[c][i + 3] * f);
+                    }
+            __syncthreads();
+            for (int idx = tid; idx < left * (HD / 4); idx += S::kThreads) {
+                const int y = idx / (HD / 4), d = 4 * (idx % (HD / 4));
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                float tm = -INFINITY, tl = 0.0f;
+#pragma unroll
+                for (int k = 0; k < KG; ++k) tm = fmaxf(tm, ml_lds[k][y][0]);
+#pragma unroll
+                for (int k = 0; k < KG; ++k) {
+                    const float4 z = *reinterpret_cast<const float4*>(obuf + (k * BM + y) * HD + d);
+                    const float km = ml_lds[k][y][0], kl = ml_lds[k][y][1];
+                    tl += km == -INFINITY ? kl : kl * __builtin_amdgcn_exp2f(km - tm);
+                    x.x += z.x;
+                    x.y += z.y;
+                    x.z += z.z;
+                    x.w += z.w;
+                }
+                if (!whole) {
+                    *reinterpret_cast<float4*>(part + y * HD + d) = x;
+                    if (d == 0) {
+                        part[BM * HD + 2 * y] = tm;
+                        part[BM * HD + 2 * y + 1] = tl;
+                    }
+                } else if (d < a.head_dim) {
+                    const int gr = w.qt * BM + y, tk = a.group.div(gr);
+                    const float inv = row_sees(a, w.count, w.len, tk) ? 1.0f / tl : 0.0f;
+                    store4<T>(a.out + static_cast<long>(w.first + tk) * a.out_stride +
+                                  static_cast<long>(w.kvh * group + gr - tk * group) * a.head_dim + d,
+                              x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+                }
+            }
         }
-        const float inv = none ? 0.0f : 1.0f / l;
-        uint16_t* const op = a.out + static_cast<long>(w.first + tok) * a.out_stride +
-                             static_cast<long>(head) * a.head_dim;
-#pragma unroll
-        for (int c = 0; c < kCols; ++c)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int d = 32 * c + 8 * (i / 4) + 4 * half;
-                if (d < a.head_dim)
-                    store4<T>(op + d, o[c][i] * inv, o[c][i + 1] * inv, o[c][i + 2] * inv,
-                              o[c][i + 3] * inv);
-            }
-        return;
+        if (w.end >= to || w.end <= w.begin) {
+            if (w.begin >= from && w.end > to)  // who else has a part of it
+                left_over = {static_cast<int>(plan.last_before(w.end) - worker) + 1, w.first, w.count,
+                             w.len, w.qt, w.kvh};
+            break;
+        }
+        __syncthreads();  // the next tile's loads overwrite what this one's waves read
     }
-    // join the key groups: the references first, then the scaled sums through LDS
-    const int r32 = 32 * rg + (lane & 31);
-    if (half == 0) {
-        ml_lds[(kg * BM + r32) * 2] = m;
-        ml_lds[(kg * BM + r32) * 2 + 1] = l;
-    }
-    __syncthreads();  // also: every wave has read its last keys
-    float top = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < KG; ++k) top = fmaxf(top, ml_lds[(k * BM + r32) * 2]);
-    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-    float* const obuf = reinterpret_cast<float*>(attn_smem);  // [KG][BM][HD]
+    if (tid == 0) a.splits[worker] = left_over;
+}
+
+// Joins the pieces of split tiles: block (worker in which the tile begins, rows).
+// HD / 4 threads take a row, 4 columns each; kSpread: they take every kGroups-th
+// piece of the block's one row, else all pieces of a row of their own.
+template <class T, int HD, int RG, bool kSpread>
+__global__ __launch_bounds__(kJoinBlock) void paged_attention_join_kernel(const AttnArgs a) {
+    constexpr int BM = Shape<RG>::BM;
+    constexpr int kLanes = HD / 4, kGroups = kJoinBlock / kLanes;
+    __shared__ float acc[kSpread ? kGroups : 1][HD + 2];
+    const Split w = a.splits[blockIdx.x];
+    if (w.pieces == 0) return;
+    const int tid = threadIdx.x, g = tid / kLanes, d = 4 * (tid % kLanes);
+    const int group = a.group.d, rows = w.count * group;
     const int left = min(rows - w.qt * BM, BM);
-    if (row < rows)
-#pragma unroll
-        for (int c = 0; c < kCols; ++c)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int d = 32 * c + 8 * (i / 4) + 4 * half;
-                *reinterpret_cast<float4*>(obuf + (kg * BM + r32) * HD + d) = make_float4(
-                    o[c][i] * f, o[c][i + 1] * f, o[c][i + 2] * f, o[c][i + 3] * f);
-            }
-    __syncthreads();
-    for (int idx = tid; idx < left * (HD / 4); idx += kAttnBlock) {
-        const int r = idx / (HD / 4), d = 4 * (idx % (HD / 4));
+    const int per_block = kSpread ? 1 : kGroups;
+    // on by the grid's rows if the batch has more than the caller told
+    for (int r0 = blockIdx.y * per_block; r0 < left; r0 += gridDim.y * per_block) {
+        const int r = kSpread ? r0 : r0 + g;
         float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float tm = -INFINITY, tl = 0.0f;
-#pragma unroll
-        for (int k = 0; k < KG; ++k) tm = fmaxf(tm, ml_lds[(k * BM + r) * 2]);
-#pragma unroll
-        for (int k = 0; k < KG; ++k) {
-            const float4 y = *reinterpret_cast<const float4*>(obuf + (k * BM + r) * HD + d);
-            const float km = ml_lds[(k * BM + r) * 2];
-            tl += km == -INFINITY ? ml_lds[(k * BM + r) * 2 + 1]
-                                  : ml_lds[(k * BM + r) * 2 + 1] * __builtin_amdgcn_exp2f(km - tm);
-            x.x += y.x;
-            x.y += y.y;
-            x.z += y.z;
-            x.w += y.w;
-        }
-        if (w.nsplit > 1) {
-            *reinterpret_cast<float4*>(part + r * HD + d) = x;
-            if (d == 0) {
-                part[BM * HD + 2 * r] = tm;
-                part[BM * HD + 2 * r + 1] = tl;
+        float m = -INFINITY, l = 0.0f;
+        if (g < kGroups && r < left) {
+#pragma unroll 4
+            for (int s = kSpread ? g : 0; s < w.pieces; s += kSpread ? kGroups : 1) {
+                // the piece where the tile begins is its worker's second, the others' first
+                const float* const p = partial<HD, BM>(a, 2 * (blockIdx.x + s) + (s == 0 ? 1 : 0));
+                const float2 ml = *reinterpret_cast<const float2*>(p + BM * HD + 2 * r);
+                const float4 y = *reinterpret_cast<const float4*>(p + r * HD + d);
+                const float top = fmaxf(m, ml.x);
+                const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+                const float h = ml.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml.x - top);
+                x.x = __builtin_fmaf(x.x, f, y.x * h);
+                x.y = __builtin_fmaf(x.y, f, y.y * h);
+                x.z = __builtin_fmaf(x.z, f, y.z * h);
+                x.w = __builtin_fmaf(x.w, f, y.w * h);
+                l = __builtin_fmaf(l, f, ml.y * h);
+                m = top;
             }
-        } else if (d < a.head_dim) {
+        }
+        if (kSpread) {
+            if (g < kGroups) {
+                acc[g][d] = x.x;
+                acc[g][d + 1] = x.y;
+                acc[g][d + 2] = x.z;
+                acc[g][d + 3] = x.w;
+                if (d == 0) {
+                    acc[g][HD] = m;
+                    acc[g][HD + 1] = l;
+                }
+            }
+            __syncthreads();
+            if (g == 0) {
+                float top = -INFINITY;
+                for (int k = 0; k < kGroups; ++k) top = fmaxf(top, acc[k][HD]);
+                x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                l = 0.0f;
+                for (int k = 0; k < kGroups; ++k) {
+                    const float h = acc[k][HD] == -INFINITY
+                                        ? 1.0f : __builtin_amdgcn_exp2f(acc[k][HD] - top);
+                    x.x = __builtin_fmaf(acc[k][d], h, x.x);
+                    x.y = __builtin_fmaf(acc[k][d + 1], h, x.y);
+                    x.z = __builtin_fmaf(acc[k][d + 2], h, x.z);
+                    x.w = __builtin_fmaf(acc[k][d + 3], h, x.w);
+                    l = __builtin_fmaf(acc[k][HD + 1], h, l);
+                }
+            }
+            __syncthreads();  // before the next row's
+        }
+        if ((kSpread ? g == 0 : g < kGroups && r < left) && d < a.head_dim) {
             const int gr = w.qt * BM + r, tk = a.group.div(gr);
-            const int pos = w.len - w.count + tk;
-            const int hi = a.causal ? min(pos + 1, w.len) : w.len;
-            const int lo = a.window ? max(pos - a.window + 1, 0) : 0;
-            const float inv = hi <= lo ? 0.0f : 1.0f / tl;
+            const float inv = row_sees(a, w.count, w.len, tk) ? 1.0f / l : 0.0f;
             store4<T>(a.out + static_cast<long>(w.first + tk) * a.out_stride +
                           static_cast<long>(w.kvh * group + gr - tk * group) * a.head_dim + d,
                       x.x * inv, x.y * inv, x.z * inv, x.w * inv);
@@ -586,130 +899,63 @@ __global__ __launch_bounds__(kAttnBlock, HD <= 128 ? 2 : 1) void paged_attention
     }
 }
 
-// Joins the pieces of split tiles: block (tile and kv head, rows), a group of
-// head_dim / 4 threads per piece.
-template <class T, int HD, int RG>
-__global__ __launch_bounds__(kAttnBlock) void paged_attention_join_kernel(const AttnArgs a,
-                                                                          const int per_block) {
-    constexpr int BM = Shape<RG>::BM, BN = Shape<RG>::BN;
-    constexpr int kLanes = HD / 4, kGroups = kAttnBlock / kLanes;
-    __shared__ float acc[kGroups][HD + 2];
-    Piece w;
-    if (!find_piece<BM, BN, true>(a, blockIdx.x, w) || w.nsplit <= 1) return;
-    const int tid = threadIdx.x, g = tid / kLanes, d = 4 * (tid % kLanes);
-    const int group = a.group.d, rows = w.count * group;
-    const int left = min(rows - w.qt * BM, BM);
-    for (int i = 0;; ++i) {  // per_block rows, and on by the grid's if the batch has more than told
-        const int r = (i / per_block * gridDim.y + blockIdx.y) * per_block + i % per_block;
-        if (r >= left) break;
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float m = -INFINITY, l = 0.0f;
-        if (g < kGroups)
-            for (int s = g; s < w.nsplit; s += kGroups) {
-                const float* const p = partial<HD, BM>(a, w.slot + s);
-                const float sm = p[BM * HD + 2 * r], sl = p[BM * HD + 2 * r + 1];
-                const float4 y = *reinterpret_cast<const float4*>(p + r * HD + d);
-                const float top = fmaxf(m, sm);
-                const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-                const float h = sm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sm - top);
-                x.x = __builtin_fmaf(x.x, f, y.x * h);
-                x.y = __builtin_fmaf(x.y, f, y.y * h);
-                x.z = __builtin_fmaf(x.z, f, y.z * h);
-                x.w = __builtin_fmaf(x.w, f, y.w * h);
-                l = __builtin_fmaf(l, f, sl * h);
-                m = top;
-            }
-        if (g < kGroups) {
-            acc[g][d] = x.x;
-            acc[g][d + 1] = x.y;
-            acc[g][d + 2] = x.z;
-            acc[g][d + 3] = x.w;
-            if (d == 0) {
-                acc[g][HD] = m;
-                acc[g][HD + 1] = l;
-            }
-        }
-        __syncthreads();
-        if (tid < kLanes && 4 * tid < a.head_dim) {
-            float top = -INFINITY, total = 0.0f;
-            for (int k = 0; k < kGroups; ++k) top = fmaxf(top, acc[k][HD]);
-            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int k = 0; k < kGroups; ++k) {
-                const float h = acc[k][HD] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(acc[k][HD] - top);
-                y.x = __builtin_fmaf(acc[k][d], h, y.x);
-                y.y = __builtin_fmaf(acc[k][d + 1], h, y.y);
-                y.z = __builtin_fmaf(acc[k][d + 2], h, y.z);
-                y.w = __builtin_fmaf(acc[k][d + 3], h, y.w);
-                total = __builtin_fmaf(acc[k][HD + 1], h, total);
-            }
-            const int gr = w.qt * BM + r, tk = a.group.div(gr);
-            const int pos = w.len - w.count + tk;
-            const int hi = a.causal ? min(pos + 1, w.len) : w.len;
-            const int lo = a.window ? max(pos - a.window + 1, 0) : 0;
-            const float inv = hi <= lo ? 0.0f : 1.0f / total;
-            store4<T>(a.out + static_cast<long>(w.first + tk) * a.out_stride +
-                          static_cast<long>(w.kvh * group + gr - tk * group) * a.head_dim + d,
-                      y.x * inv, y.y * inv, y.z * inv, y.w * inv);
-        }
-        __syncthreads();
-    }
-}
-
 // ---- host -------------------------------------------------------------------
 
 int padded_dim(int hd) { return hd <= 64 ? 64 : (hd <= 96 ? 96 : (hd <= 128 ? 128 : (hd <= 192 ? 192 : 256))); }
 
-// Two blocks per CU are resident; pieces that fill them once.
-int target_pieces() { return 2 * device_cu_count(); }
+size_t splits_bytes(int workers) { return (workers * sizeof(Split) + 255) / 256 * 256; }
 
-// Split tiles have at most 2 target pieces together: one of a sequence with
-// more than C blocks is ceil(blocks / C) < 2 blocks / C pieces, and all tiles'
-// blocks / C together are at most the target.
-size_t workspace_bytes(int hd) {
-    return static_cast<size_t>(2 * target_pieces()) * Shape<4>::BM * (padded_dim(hd) + 2) *
-           sizeof(float);
+// A worker per resident block.
+template <int HD, int RG>
+int worker_count() { return device_cu_count() * resident<HD, RG>(); }
+
+// A worker has at most two tiles that it shares with others: its first and its last.
+template <int HD, int RG>
+size_t workspace_of() {
+    const size_t workers = worker_count<HD, RG>();
+    return splits_bytes(workers) + 2 * workers * Shape<RG>::BM * (HD + 2) * sizeof(float);
 }
 
-constexpr int kMaxAttnDevices = 64;
+template <int HD>
+size_t workspace_of_any() {
+    return std::max(workspace_of<HD, 1>(), std::max(workspace_of<HD, 2>(), workspace_of<HD, 4>()));
+}
 
-// Raises a kernel's LDS limit on the current device, once.
-template <class F>
-int raise_lds(const char* fn, F* kernel, size_t bytes, std::atomic<bool>* done) {
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxAttnDevices) dev = -1;
-    if (dev >= 0 && done[dev].load(std::memory_order_acquire)) return 0;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(bytes));
-    if (e != hipSuccess) return failed(fn, e);
-    if (dev >= 0) done[dev].store(true, std::memory_order_release);
-    return 0;
+size_t workspace_bytes(int hd) {
+    switch (padded_dim(hd)) {
+    case 64: return workspace_of_any<64>();
+    case 96: return workspace_of_any<96>();
+    case 128: return workspace_of_any<128>();
+    case 192: return workspace_of_any<192>();
+    default: return workspace_of_any<256>();
+    }
 }
 
 template <class T, int HD, int RG>
-int launch_attention(const char* fn, const AttnArgs& a, int max_rows, hipStream_t st) {
+int launch_attention(const char* fn, AttnArgs a, void* ws, int max_rows, hipStream_t st) {
     typedef Shape<RG> S;
-    constexpr size_t lds = 2 * S::BN * Row<HD>::kPitch + S::KG * S::BM * 2 * sizeof(float) + 16;
-    static std::atomic<bool> done[kMaxAttnDevices];
-    if (int e = raise_lds(fn, paged_attention_kernel<T, HD, RG>, lds, done)) return e;
-    const long rows = static_cast<long>(a.b.tokens) * a.group.d;
-    const long tiles = std::min(rows, a.b.seqs + rows / S::BM) * a.kv_heads;
-    hipLaunchKernelGGL((paged_attention_kernel<T, HD, RG>), dim3(a.target + tiles),
-                       dim3(kAttnBlock), lds, st, a);
+    a.workers = worker_count<HD, RG>();
+    a.reach = static_cast<double>(a.window) + ((S::BM - 1) / a.group.d + 2);
+    a.per_worker = 32.0 / (static_cast<double>(S::kMinKeys) * a.group.d);
+    a.splits = static_cast<Split*>(ws);
+    a.ws = reinterpret_cast<float*>(static_cast<char*>(ws) + splits_bytes(a.workers));
+    hipLaunchKernelGGL((paged_attention_kernel<T, HD, RG>), dim3(a.workers), dim3(S::kThreads), 0,
+                       st, a);
     if (int e = launch_status(fn)) return e;
-    // a row a block where the rows are few
-    const int per = RG == 1 ? 1 : 16;
+    // few rows may have many pieces: a row a block, its pieces side by side
+    constexpr bool kSpread = RG == 1;
+    constexpr int per = kSpread ? 1 : kJoinBlock / (HD / 4);
     const int most = std::min(max_rows, S::BM);
-    hipLaunchKernelGGL((paged_attention_join_kernel<T, HD, RG>),
-                       dim3(tiles, (most + per - 1) / per), dim3(kAttnBlock), 0, st, a, per);
+    hipLaunchKernelGGL((paged_attention_join_kernel<T, HD, RG, kSpread>),
+                       dim3(a.workers, (most + per - 1) / per), dim3(kJoinBlock), 0, st, a);
     return launch_status(fn);
 }
 
 template <class T, int HD>
-int pick_rows(const char* fn, const AttnArgs& a, int max_rows, hipStream_t st) {
-    if (max_rows <= 32) return launch_attention<T, HD, 1>(fn, a, max_rows, st);
-    if (max_rows <= 64) return launch_attention<T, HD, 2>(fn, a, max_rows, st);
-    return launch_attention<T, HD, 4>(fn, a, max_rows, st);
+int pick_rows(const char* fn, const AttnArgs& a, void* ws, int max_rows, hipStream_t st) {
+    if (max_rows <= 32) return launch_attention<T, HD, 1>(fn, a, ws, max_rows, st);
+    if (max_rows <= 64) return launch_attention<T, HD, 2>(fn, a, ws, max_rows, st);
+    return launch_attention<T, HD, 4>(fn, a, ws, max_rows, st);
 }
 
 int check_heads(const char* fn, int nh, int nkv, int hd) {
@@ -760,19 +1006,16 @@ int paged_attention(const char* fn, const spb_paged_cache* c, const spb_paged_ba
     a.c = scale * kLog2e;
     a.causal = causal != 0;
     a.window = window;
-    a.target = target_pieces();
-    a.slots = 2 * a.target;
-    a.ws = static_cast<float*>(ws);
     const int most_new = b->max_new ? std::min(b->max_new, b->num_tokens) : b->num_tokens;
     const int max_rows = static_cast<int>(std::min<long>(
         static_cast<long>(most_new) * a.group.d, 0x7FFFFFFFL));
     const hipStream_t st = as_stream(stream);
     switch (padded_dim(c->head_dim)) {
-    case 64: return pick_rows<T, 64>(fn, a, max_rows, st);
-    case 96: return pick_rows<T, 96>(fn, a, max_rows, st);
-    case 128: return pick_rows<T, 128>(fn, a, max_rows, st);
-    case 192: return pick_rows<T, 192>(fn, a, max_rows, st);
-    default: return pick_rows<T, 256>(fn, a, max_rows, st);
+    case 64: return pick_rows<T, 64>(fn, a, ws, max_rows, st);
+    case 96: return pick_rows<T, 96>(fn, a, ws, max_rows, st);
+    case 128: return pick_rows<T, 128>(fn, a, ws, max_rows, st);
+    case 192: return pick_rows<T, 192>(fn, a, ws, max_rows, st);
+    default: return pick_rows<T, 256>(fn, a, ws, max_rows, st);
     }
 }
 
