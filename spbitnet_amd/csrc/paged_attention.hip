@@ -312,7 +312,7 @@ struct Row {
 
 // 16 bytes of each active lane from memory to LDS, at lds + 16 lane.
 template <bool kOnce>  // non-temporal
-__device__ __forceinline__ void load_to_lds(const uint16_t* from, uint8_t* lds) {
+__device__ __forceinline__ void load_to_lds(const void* from, uint8_t* lds) {
     __builtin_amdgcn_global_load_lds(
         (const __attribute__((address_space(1))) void*)from,
         (__attribute__((address_space(3))) void*)lds, 16, 0, kOnce ? 2 : 0);
@@ -377,15 +377,21 @@ struct RowState {
     int any_lo, any_hi;     // ... that any sees
 };
 
-// One tile of keys t .. t + BN in LDS (K, then V) against the wave's rows.
-template <class T, int HD, int RG>
+// One tile of keys t .. t + BN in LDS (K, then V) against the wave's rows.  `between`
+// is called kBetween times among the matrix products, whose time hides what it issues.
+constexpr int kBetween = 4;
+template <class T, int HD, int RG, class F>
 __device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, RG>& r,
-                                       const uint8_t* buf, int t, int kg, uint64_t there) {
+                                       const uint8_t* buf, int t, int kg, uint64_t there,
+                                       F between) {
     typedef Row<HD> R;
     typedef Prob<T> P;
     constexpr int NS = Shape<RG>::NS, kSteps = HD / 16, kCols = HD / 32, kKeys = 32 * NS;
     const int j0 = t + kKeys * kg;
-    if (j0 >= r.any_hi || j0 + kKeys <= r.any_lo) return;
+    if (j0 >= r.any_hi || j0 + kKeys <= r.any_lo) {
+        for (int i = 0; i < kBetween; ++i) between(i);
+        return;
+    }
     const uint8_t* const kw = buf + kKeys * kg * R::kPitch;
     const uint8_t* const vw = kw + Shape<RG>::BN * R::kPitch;
     const int lane = threadIdx.x & (kWave - 1), half = lane >> 5;
@@ -407,6 +413,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, RG>& r
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
         if (g + 1 < kGroups) load_k(g + 1);
+        if (g < kBetween) between(g);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int st = 0; st < kGroup; ++st)
@@ -415,6 +422,8 @@ __device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, RG>& r
                 s[n] = P::mfma(k[g & 1][st][n], r.q[g * kGroup + st],
                                g + st == 0 ? f32x16{} : s[n]);
     }
+#pragma unroll
+    for (int g = kGroups; g < kBetween; ++g) between(g);
     // V^T operands of 16 keys; lane: column 32 c + lane % 32, keys 4 half .. and 8 + 4 half ..
     const int l16 = lane & 15;
     auto load_v = [&](int g, u32x4 (&v)[kCols]) {
@@ -640,47 +649,59 @@ void paged_attention_kernel(const AttnArgs a) {
         auto fetch_page = [&](int t) {
             if (t < ke) page = table[a.b.page.div(min(t + lane, ke - 1))];
         };
-        auto load_tile = [&](int t, uint8_t* buf) {  // -> which of its keys are there
+        // Where a page's slots come in whole runs of a load's rows, all rows of a load
+        // have one place: a scalar base and a lane offset that stays the same.
+        const bool runs = a.b.page.d % kRows == 0 && units == R::kUnits;
+        const uint32_t lane_row = (lane / R::kUnits) * static_cast<uint32_t>(a.slot_stride) * 2;
+        uint64_t there = ~uint64_t{0}, next = ~uint64_t{0};
+        long at = 0;
+        bool easy = true;
+        auto place_tile = [&](int t) {  // of the next tile's keys, and which are there
             const int j = min(t + lane, ke - 1);
             const int slot = j - static_cast<int>(a.b.page.div(j) * a.b.page.d);
             const bool in_pool = static_cast<unsigned>(page) < static_cast<unsigned>(a.b.pages);
-            const uint64_t there = __ballot(in_pool);
+            next = __ballot(in_pool);
             const bool here = in_pool && t + lane < ke;
-            const long at = here ? page * a.page_stride + slot * a.slot_stride : -1;
+            at = here ? page * a.page_stride + slot * a.slot_stride : -1;
+            easy = runs && __ballot(here) == ~uint64_t{0};
+        };
+        auto load_part = [&](int i, uint8_t* buf) {  // load i of kLoads, easy
+            const int row = (i * S::kWaves + wave) * kRows;  // of the wave's first lane
+            const uint32_t lo = lane_int(static_cast<int>(at), row);
+            const uint32_t hi = lane_int(static_cast<int>(at >> 32), row);
+            const long off = static_cast<long>(static_cast<uint64_t>(hi) << 32 | lo);
+            const int key = row + lane / R::kUnits;
+            const uint32_t ku = lane_row + 16 * R::k_unit(key, lane % R::kUnits);
+            const uint32_t vu = lane_row + 16 * R::v_unit(key, lane % R::kUnits);
+            load_to_lds<RG <= 2>(reinterpret_cast<const char*>(kbase + off) + ku, buf + row * R::kPitch);
+            load_to_lds<RG <= 2>(reinterpret_cast<const char*>(vbase + off) + vu,
+                                 buf + (BN + row) * R::kPitch);
+        };
+        auto load_any = [&](uint8_t* buf) {  // the tile, any lengths, pages and head_dim
+            int ln = lane;
+            asm volatile("" : "+v"(ln));  // its numbers are not held in registers meanwhile
             const int at_lo = static_cast<int>(at), at_hi = static_cast<int>(at >> 32);
-            const bool full = units == R::kUnits && __ballot(here) == ~uint64_t{0};
-            auto loads = [&](auto whole) {
-                int ln = lane;
-                // the rarer form computes its lane's numbers where it needs them, in place
-                // of registers held through all tiles
-                if (!decltype(whole)::value) asm volatile("" : "+v"(ln));
 #pragma unroll
-                for (int i = 0; i < kLoads; ++i) {
-                    const int row = (i * S::kWaves + wave) * kRows;  // of the wave's first lane
-                    const int key = row + ln / R::kUnits;
-                    const uint32_t lo = __shfl(at_lo, key, kWave), hi = __shfl(at_hi, key, kWave);
-                    const long off = static_cast<long>(static_cast<uint64_t>(hi) << 32 | lo);
-                    const int ku = R::k_unit(key, ln % R::kUnits);
-                    const int vu = R::v_unit(key, ln % R::kUnits);
-                    const uint16_t* kp = kbase + off + 8 * ku;
-                    const uint16_t* vp = vbase + off + 8 * vu;
-                    if (!decltype(whole)::value) {
-                        const uint16_t* const zeros = reinterpret_cast<const uint16_t*>(kZeros);
-                        if (off < 0 || ku >= units) kp = zeros;
-                        if (off < 0 || vu >= units) vp = zeros;
-                    }
-                    load_to_lds<RG <= 2>(kp, buf + row * R::kPitch);
-                    load_to_lds<RG <= 2>(vp, buf + (BN + row) * R::kPitch);
-                }
-            };
-            if (full) loads(std::true_type());
-            else loads(std::false_type());
-            return there;
+            for (int i = 0; i < kLoads; ++i) {
+                const int row = (i * S::kWaves + wave) * kRows;
+                const int key = row + ln / R::kUnits;
+                const uint32_t lo = __shfl(at_lo, key, kWave), hi = __shfl(at_hi, key, kWave);
+                const long off = static_cast<long>(static_cast<uint64_t>(hi) << 32 | lo);
+                const int ku = R::k_unit(key, ln % R::kUnits), vu = R::v_unit(key, ln % R::kUnits);
+                const uint16_t* const zeros = reinterpret_cast<const uint16_t*>(kZeros);
+                load_to_lds<RG <= 2>(off < 0 || ku >= units ? zeros : kbase + off + 8 * ku,
+                                     buf + row * R::kPitch);
+                load_to_lds<RG <= 2>(off < 0 || vu >= units ? zeros : vbase + off + 8 * vu,
+                                     buf + (BN + row) * R::kPitch);
+            }
         };
 
         fetch_page(kb);
-        uint64_t there = ~uint64_t{0};
-        if (kb < ke) there = load_tile(kb, buf0);
+        if (kb < ke) {
+            place_tile(kb);
+            load_any(buf0);
+            there = next;
+        }
         fetch_page(kb + BN);
         {
             const uint16_t* qp = a.q + static_cast<long>(w.first + tok) * a.q_stride +
@@ -711,14 +732,24 @@ void paged_attention_kernel(const AttnArgs a) {
         auto step = [&](int t, uint8_t* buf, uint8_t* other) {
             wait_loads();
             __syncthreads();
-            uint64_t next = ~uint64_t{0};
-            if (t + BN < ke) next = load_tile(t + BN, other);
-            fetch_page(t + 2 * BN);
+            const bool more = t + BN < ke;
+            bool spread = false;
+            if (more) {
+                place_tile(t + BN);
+                spread = easy;
+                if (!easy) load_any(other);
+            }
             bool taken = false;
             if ((t < hi1 && t + BN > hi0 && hi0 < hi1) || (t < lo1 && t + BN > lo0 && lo0 < lo1))
                 taken = take_out<T, HD, RG>(buf, &found_lds);
-            attend<T, HD, RG>(a, r, buf, t, kg, there);
+            attend<T, HD, RG>(a, r, buf, t, kg, there, [&](int i) {
+                if (spread)
+#pragma unroll
+                    for (int k = 0; k < kLoads; ++k)
+                        if (k * kBetween / kLoads == i) load_part(k, other);
+            });
             if (taken) put_back<T, HD, RG>(a, r, t, ke, kg, table, vbase);
+            fetch_page(t + 2 * BN);
             there = next;
         };
         for (int t = kb; t < ke; t += 2 * BN) {
