@@ -341,18 +341,28 @@ def bitlinear_gpu(meta, values, x, output, gamma, rows, cols, meta_row_stride,
 _ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 
 
-def _here(t: torch.Tensor, name: str) -> None:
-    if not isinstance(t, torch.Tensor):
+# These calls are short (a decode step's rotation runs 2.6 us), so their checks
+# are: one condition per tensor, and the reason is looked for when it fails.
+
+_Tensor = torch.Tensor
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _device(t, name: str) -> int:
+    """The index of the GPU that a call runs on: t's, which must be the current one."""
+    if not isinstance(t, _Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
+    dev = t.get_device()
+    if dev < 0:
         raise ValueError(f"{name} must be a GPU tensor")
-    if t.get_device() != torch.cuda.current_device():
+    if dev != torch._C._cuda_getDevice():
         raise ValueError(f"{name} is on {t.device}, the current device is "
                          f"cuda:{torch.cuda.current_device()}")
+    return dev
 
 
-def _half(t: torch.Tensor, name: str) -> str:
-    if not isinstance(t, torch.Tensor):
+def _kind(t, name: str) -> str:
+    if not isinstance(t, _Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     kind = _HALF_KIND.get(t.dtype)
     if kind is None:
@@ -360,42 +370,40 @@ def _half(t: torch.Tensor, name: str) -> str:
     return kind
 
 
-def _heads(t, name: str, dtype, tokens: int, heads: int, head_dim: int) -> Tuple[int, int]:
-    """Pointer and token stride of a [tokens][heads][head_dim] tensor whose
-    tokens' heads are contiguous (a part of a stacked projection may be one)."""
-    _here(t, name)
+def _refuse(t, name: str, dtype, shape, dev: int):
+    """Raises what is wrong with a tensor; returns if its layout is."""
+    if _device(t, name) != dev:
+        raise ValueError(f"{name} is on {t.device}, others are on cuda:{dev}")
     if t.dtype != dtype:
         raise TypeError(f"{name} has dtype {t.dtype}, expected {dtype}")
-    if t.shape != (tokens, heads, head_dim):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected "
-                         f"({tokens}, {heads}, {head_dim})")
-    st = t.stride()
-    if st[2] != 1 or (heads > 1 and st[1] != head_dim):
-        raise ValueError(f"{name}: a token's heads must be contiguous")
-    return t.data_ptr(), st[0] if tokens > 1 else heads * head_dim
-
-
-def _ints(t, name: str, *shape: int) -> int:
-    """Pointer of a contiguous int32 GPU tensor of this shape."""
-    _here(t, name)
-    if t.dtype != torch.int32:
-        raise TypeError(f"{name} has dtype {t.dtype}, expected torch.int32")
     if t.shape != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+
+
+def _heads(t, name: str, dtype, shape, dev: int) -> Tuple[int, int]:
+    """Pointer and token stride of a [tokens][heads][head_dim] tensor whose
+    tokens' heads are contiguous (a part of a stacked projection may be one)."""
+    if (not isinstance(t, _Tensor) or t.get_device() != dev or t.dtype != dtype
+            or t.shape != shape):
+        _refuse(t, name, dtype, shape, dev)
+    st, (n, heads, hd) = t.stride(), shape
+    if st[2] != 1 or (heads > 1 and st[1] != hd):
+        raise ValueError(f"{name}: a token's heads must be contiguous")
+    return t.data_ptr(), st[0] if n > 1 else heads * hd
+
+
+def _flat(t, name: str, dtype, shape, dev: int) -> int:
+    """Pointer of a contiguous tensor."""
+    if (not isinstance(t, _Tensor) or t.get_device() != dev or t.dtype != dtype
+            or t.shape != shape):
+        _refuse(t, name, dtype, shape, dev)
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t.data_ptr()
 
 
-def _weight(t, name: str, head_dim: int) -> Optional[int]:
-    if t is None:
-        return None
-    _here(t, name)
-    if t.dtype != torch.float32:
-        raise TypeError(f"{name} has dtype {t.dtype}, expected torch.float32")
-    if t.shape != (head_dim,) or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous vector of {head_dim} elements")
-    return t.data_ptr()
+def _on(stream, dev: int):
+    return (_raw_stream(dev) or None) if stream is None else _stream_ptr(stream)
 
 
 def rope_inv_freq(rotary_dim: int, theta: float = 10000.0, scaling: str = "none",
@@ -428,7 +436,7 @@ class Rope:
         if not inv_freq.is_cuda:
             inv_freq = inv_freq.to(torch.device("cuda", torch.cuda.current_device()))
         self.inv_freq = inv_freq.contiguous()
-        _here(self.inv_freq, "inv_freq")
+        self._dev = _device(self.inv_freq, "inv_freq")
         self.rotary_dim = 2 * inv_freq.numel()
         self.scale, self.interleaved = float(scale), bool(interleaved)
         self._c = _lib.RopeC(self.inv_freq.data_ptr(), self.rotary_dim, int(self.interleaved),
@@ -443,19 +451,29 @@ class Rope:
         return Rope(f, scale, interleaved)
 
 
+def _same_device(x, name: str, dev: int) -> None:
+    if x._dev != dev:
+        raise ValueError(f"{name} is on cuda:{x._dev}, the tensors are on cuda:{dev}")
+
+
 def rope_tokens_gpu(x, output, positions, rope: Rope, stream=None):
     """Rotates the heads of x [tokens][heads][head_dim] to positions (int32
     [tokens]; a negative one is padding, its output stays as it was) into output,
     which may be x (spb_rope_tokens_*)."""
-    kind = _half(x, "x")
-    if x.dim() != 3:
+    kind = _kind(x, "x")
+    shape, dt = x.shape, x.dtype
+    if len(shape) != 3:
         raise ValueError("x must be [tokens][heads][head_dim]")
-    n, heads, hd = x.shape
-    px, sx = _heads(x, "x", x.dtype, n, heads, hd)
-    py, sy = _heads(output, "output", x.dtype, n, heads, hd)
-    fn = getattr(_lib.load(), f"spb_rope_tokens_{kind}")
-    _lib.check(fn(px, py, _ints(positions, "positions", n), rope._ptr, n, heads, hd, sx, sy,
-                  _stream_ptr(stream)), "rope_tokens_gpu")
+    dev = _device(x, "x")
+    px, sx = _heads(x, "x", dt, shape, dev)
+    py, sy = _heads(output, "output", dt, shape, dev)
+    n, heads, hd = shape
+    pp = _flat(positions, "positions", torch.int32, (n,), dev)
+    _same_device(rope, "rope", dev)
+    L = _lib.load()
+    fn = L.spb_rope_tokens_f16 if kind == "f16" else L.spb_rope_tokens_bf16
+    _lib.check(fn(px, py, pp, rope._ptr, n, heads, hd, sx, sy, _on(stream, dev)),
+               "rope_tokens_gpu")
 
 
 def qk_norm_rope_gpu(q, k, q_output, k_output, q_weight, k_weight, positions,
@@ -464,21 +482,28 @@ def qk_norm_rope_gpu(q, k, q_output, k_output, q_weight, k_weight, positions,
     [tokens][kv heads][head_dim] with the weights (float32 [head_dim]), then the
     rotation to positions, in one pass (spb_qk_norm_rope_*).  rope None: norms
     only.  The outputs may be q and k."""
-    kind = _half(q, "q")
-    if q.dim() != 3 or not isinstance(k, torch.Tensor) or k.dim() != 3:
-        raise ValueError("q and k must be [tokens][heads][head_dim]")
-    n, nh, hd = q.shape
-    nkv = k.shape[1]
-    pq, sq = _heads(q, "q", q.dtype, n, nh, hd)
-    pk, sk = _heads(k, "k", q.dtype, n, nkv, hd)
-    pqo, sqo = _heads(q_output, "q_output", q.dtype, n, nh, hd)
-    pko, sko = _heads(k_output, "k_output", q.dtype, n, nkv, hd)
-    pp = _ints(positions, "positions", n) if rope is not None else None
-    fn = getattr(_lib.load(), f"spb_qk_norm_rope_{kind}")
-    _lib.check(fn(pq, pk, pqo, pko, _weight(q_weight, "q_weight", hd),
-                  _weight(k_weight, "k_weight", hd), pp, rope._ptr if rope is not None else None,
-                  n, nh, nkv, hd, sq, sk, sqo, sko, eps, _stream_ptr(stream)),
-               "qk_norm_rope_gpu")
+    kind = _kind(q, "q")
+    _kind(k, "k")
+    qs, ks, dt, dev = q.shape, k.shape, q.dtype, _device(q, "q")
+    if len(qs) != 3 or len(ks) != 3 or ks[0] != qs[0] or ks[2] != qs[2]:
+        raise ValueError("q and k must be [tokens][heads][head_dim] with the same tokens and "
+                         "head_dim")
+    n, nh, hd = qs
+    pq, sq = _heads(q, "q", dt, qs, dev)
+    pk, sk = _heads(k, "k", dt, ks, dev)
+    pqo, sqo = _heads(q_output, "q_output", dt, qs, dev)
+    pko, sko = _heads(k_output, "k_output", dt, ks, dev)
+    pqw = _flat(q_weight, "q_weight", torch.float32, (hd,), dev)
+    pkw = _flat(k_weight, "k_weight", torch.float32, (hd,), dev)
+    pp = pr = None
+    if rope is not None:
+        pp = _flat(positions, "positions", torch.int32, (n,), dev)
+        _same_device(rope, "rope", dev)
+        pr = rope._ptr
+    L = _lib.load()
+    fn = L.spb_qk_norm_rope_f16 if kind == "f16" else L.spb_qk_norm_rope_bf16
+    _lib.check(fn(pq, pk, pqo, pko, pqw, pkw, pp, pr, n, nh, ks[1], hd, sq, sk, sqo, sko, eps,
+                  _on(stream, dev)), "qk_norm_rope_gpu")
 
 
 class PagedKVCache:
@@ -488,11 +513,10 @@ class PagedKVCache:
     come as a transposed view.  Keeps the tensors alive."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor):
-        self.kind = _half(k, "k")
-        _here(k, "k")
-        _here(v, "v")
-        if v.dtype != k.dtype:
-            raise TypeError(f"v has dtype {v.dtype}, expected {k.dtype}")
+        self.kind = _kind(k, "k")
+        self._dev = _device(k, "k")
+        if _device(v, "v") != self._dev or v.dtype != k.dtype:
+            raise TypeError(f"v is {v.dtype} on {v.device}, expected {k.dtype} on {k.device}")
         if k.dim() != 4 or v.shape != k.shape:
             raise ValueError("k and v must be [pages][kv heads][page_size][head_dim]")
         if k.stride() != v.stride() or k.stride(3) != 1:
@@ -522,12 +546,13 @@ class PagedBatch:
         n, width = kv_lens.numel(), page_table.shape[1]
         if num_tokens < 0 or max_new < 0:
             raise ValueError("negative number of tokens")
+        self._dev = dev = _device(kv_lens, "kv_lens")
         self.token_starts, self.kv_lens, self.page_table = token_starts, kv_lens, page_table
         self.num_seqs, self.num_tokens, self.max_new = n, int(num_tokens), int(max_new)
-        self._c = _lib.PagedBatchC(_ints(token_starts, "token_starts", n + 1),
-                                   _ints(kv_lens, "kv_lens", n),
-                                   _ints(page_table, "page_table", n, width), n, width,
-                                   self.num_tokens, self.max_new)
+        self._c = _lib.PagedBatchC(_flat(token_starts, "token_starts", torch.int32, (n + 1,), dev),
+                                   _flat(kv_lens, "kv_lens", torch.int32, (n,), dev),
+                                   _flat(page_table, "page_table", torch.int32, (n, width), dev),
+                                   n, width, self.num_tokens, self.max_new)
         self._ptr = ctypes.addressof(self._c)
 
 
@@ -536,25 +561,35 @@ def paged_append_gpu(cache: PagedKVCache, batch: PagedBatch, k, v, rope: Optiona
                      stream=None):
     """Writes the batch's k and v [tokens][kv heads][head_dim] into their pages, the
     keys rotated to their positions on the way (rope None: as they are), and, if q
-    [tokens][heads][head_dim] is given, rotates it into q_output (which may be q) in the same launch.
-    q_weight / k_weight (float32 [head_dim]): RMSNorm before the rotation
-    (spb_paged_append_*)."""
-    n, hd, nkv, dt = batch.num_tokens, cache.head_dim, cache.num_kv_heads, cache.dtype
-    pk = pv = pq = pqo = None
+    [tokens][heads][head_dim] is given, rotates it into q_output (which may be q)
+    in the same launch.  q_weight / k_weight (float32 [head_dim]): RMSNorm before
+    the rotation (spb_paged_append_*)."""
+    n, hd, dt = batch.num_tokens, cache.head_dim, cache.dtype
+    dev = _device(cache.k, "the cache")
+    _same_device(batch, "batch", dev)
+    pk = pv = pq = pqo = pqw = pkw = pr = None
     sk = sv = sq = sqo = nh = 0
     if k is not None or v is not None:
-        pk, sk = _heads(k, "k", dt, n, nkv, hd)
-        pv, sv = _heads(v, "v", dt, n, nkv, hd)
+        shape = (n, cache.num_kv_heads, hd)
+        pk, sk = _heads(k, "k", dt, shape, dev)
+        pv, sv = _heads(v, "v", dt, shape, dev)
     if q is not None or q_output is not None:
-        _half(q, "q")
+        _kind(q, "q")
         nh = q.shape[1] if q.dim() == 3 else 0
-        pq, sq = _heads(q, "q", dt, n, nh, hd)
-        pqo, sqo = _heads(q_output, "q_output", dt, n, nh, hd)
-    fn = getattr(_lib.load(), f"spb_paged_append_{cache.kind}")
-    _lib.check(fn(cache._ptr, batch._ptr, pk, pv, pq, pqo, sk, sv, sq, sqo, nh,
-                  _weight(q_weight, "q_weight", hd), _weight(k_weight, "k_weight", hd), eps,
-                  rope._ptr if rope is not None else None, _stream_ptr(stream)),
-               "paged_append_gpu")
+        shape = (n, nh, hd)
+        pq, sq = _heads(q, "q", dt, shape, dev)
+        pqo, sqo = _heads(q_output, "q_output", dt, shape, dev)
+    if q_weight is not None:
+        pqw = _flat(q_weight, "q_weight", torch.float32, (hd,), dev)
+    if k_weight is not None:
+        pkw = _flat(k_weight, "k_weight", torch.float32, (hd,), dev)
+    if rope is not None:
+        _same_device(rope, "rope", dev)
+        pr = rope._ptr
+    L = _lib.load()
+    fn = L.spb_paged_append_f16 if cache.kind == "f16" else L.spb_paged_append_bf16
+    _lib.check(fn(cache._ptr, batch._ptr, pk, pv, pq, pqo, sk, sv, sq, sqo, nh, pqw, pkw, eps, pr,
+                  _on(stream, dev)), "paged_append_gpu")
 
 
 def paged_attention_workspace_size(num_heads: int, num_kv_heads: int, head_dim: int) -> int:
@@ -571,18 +606,20 @@ def paged_attention_gpu(cache: PagedKVCache, batch: PagedBatch, q, output, works
     """Attention of the batch's queries q [tokens][heads][head_dim] over their
     sequences' pages into output (which may be q): position p sees positions j <= p
     when causal, j > p - window when window > 0, and the whole cached length
-    otherwise.  scale None: head_dim ** -0.5.  workspace: a uint8 GPU tensor of
-    paged_attention_workspace_size bytes (spb_paged_attention_*)."""
-    n, hd, dt = batch.num_tokens, cache.head_dim, cache.dtype
-    _half(q, "q")
+    otherwise.  scale None: head_dim ** -0.5.  workspace: a contiguous uint8 GPU
+    tensor of paged_attention_workspace_size bytes (spb_paged_attention_*)."""
+    hd, dt = cache.head_dim, cache.dtype
+    dev = _device(cache.k, "the cache")
+    _same_device(batch, "batch", dev)
+    _kind(q, "q")
     nh = q.shape[1] if q.dim() == 3 else 0
-    pq, sq = _heads(q, "q", dt, n, nh, hd)
-    po, so = _heads(output, "output", dt, n, nh, hd)
-    _here(workspace, "workspace")
-    if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-        raise TypeError("workspace must be a contiguous uint8 tensor")
-    fn = getattr(_lib.load(), f"spb_paged_attention_{cache.kind}")
+    shape = (batch.num_tokens, nh, hd)
+    pq, sq = _heads(q, "q", dt, shape, dev)
+    po, so = _heads(output, "output", dt, shape, dev)
+    size = workspace.numel() if isinstance(workspace, _Tensor) else 0
+    pw = _flat(workspace, "workspace", torch.uint8, (size,), dev)
+    L = _lib.load()
+    fn = L.spb_paged_attention_f16 if cache.kind == "f16" else L.spb_paged_attention_bf16
     _lib.check(fn(cache._ptr, batch._ptr, pq, po, sq, so, nh,
-                  hd ** -0.5 if scale is None else scale, 1 if causal else 0, window,
-                  workspace.data_ptr(), workspace.numel(), _stream_ptr(stream)),
-               "paged_attention_gpu")
+                  hd ** -0.5 if scale is None else scale, 1 if causal else 0, window, pw, size,
+                  _on(stream, dev)), "paged_attention_gpu")
