@@ -18,7 +18,7 @@ namespace spb {
 namespace {
 
 constexpr int kHeadBlock = 256;
-constexpr int kMaxTile = 4;      // tokens of a block
+constexpr int kMaxTile = 2;      // tokens of a block
 constexpr int kMaxHalf = 128;    // pairs of the widest head
 
 // A run of heads of the batch's tokens: head h of token t at
@@ -34,7 +34,8 @@ struct HeadSpan {
 
 struct HeadsArgs {
     HeadSpan span[3];  // q, k, v (a single span of any heads for spb_rope_tokens)
-    int all_heads, head_dim, tokens;
+    int head_dim, tokens;
+    FastDiv all_heads;
     int units;      // lanes' shares of a head: head_dim / (2 V)
     int rot_units;  // those that are rotated: rotary / (2 V)
     int lanes_log;  // lanes of a head, 2^lanes_log >= units / kUnits
@@ -85,55 +86,128 @@ __device__ __forceinline__ Place find_place(const HeadsArgs& a, int t) {
     return r;
 }
 
-template <class T, int V>
-__device__ __forceinline__ void load_part(const uint16_t* p, float (&f)[V]) {
+template <int V>
+struct Part {  // V 16-bit values that are loaded and stored at once
     uint16_t w[V];
-    __builtin_memcpy(w, __builtin_assume_aligned(p, 2 * V), 2 * V);
-#pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = T::to_float(w[e]);
+};
+template <int V>
+__device__ __forceinline__ Part<V> load_part(const uint16_t* p) {
+    Part<V> r;
+    __builtin_memcpy(r.w, __builtin_assume_aligned(p, 2 * V), 2 * V);
+    return r;
 }
-
-template <class T, int V>
+template <class T, int V, bool kStream>
 __device__ __forceinline__ void store_part(uint16_t* p, const float (&f)[V]) {
-    uint16_t w[V];
+    Part<V> r;
 #pragma unroll
-    for (int e = 0; e < V; ++e) w[e] = T::from_float(f[e]);
-    __builtin_memcpy(__builtin_assume_aligned(p, 2 * V), w, 2 * V);
+    for (int e = 0; e < V; ++e) r.w[e] = T::from_float(f[e]);
+    if (V > 1 && kStream) {
+        typedef uint32_t words __attribute__((ext_vector_type(V > 1 ? V / 2 : 2)));
+        words x;
+        __builtin_memcpy(&x, r.w, V > 1 ? 2 * V : 0);
+        __builtin_nontemporal_store(x, reinterpret_cast<words*>(p));
+    } else {
+        __builtin_memcpy(__builtin_assume_aligned(p, 2 * V), r.w, 2 * V);
+    }
+}
+// V floats of a lane in LDS: four at a time, lane after lane, so that neighbouring
+// lanes read neighbouring 16 bytes.  Value i of `units` lanes' V values each:
+template <int V>
+__device__ __forceinline__ int lds_at(int i, int units) {
+    if (V == 1) return i;
+    return (i % V / 4 * units + i / V) * 4 + i % 4;
+}
+template <int V>
+__device__ __forceinline__ void load_lds(const float* p, int u, int units, float (&f)[V]) {
+    if (V == 1) {
+        f[0] = p[u];
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            const float4 x = reinterpret_cast<const float4*>(p)[j / 4 * units + u];
+            f[j] = x.x;
+            f[(j + 1) % V] = x.y;
+            f[(j + 2) % V] = x.z;
+            f[(j + 3) % V] = x.w;
+        }
+    }
 }
 
 // A block takes `tile` tokens.  2^lanes_log lanes take a head and each lane V
 // pairs of it (unit u): elements [V u, V u + V) and the same past half in the
 // half layout, [2 V u, 2 V u + 2 V) in the interleaved one and past the rotary
-// part.  kUnits: units of a lane (2 only where a head has more than 64).
-template <class T, int V, int kUnits, bool kNorm, bool kPaged>
+// part.  kUnits: units of a lane (2 only where a head has more than 64).  A head
+// is loaded while the one before it is worked on, the first while the angles are.
+// 8192 tokens of 25 heads of 128, half of each rotated: 20.1 us, 5.2 TB/s (a large
+// copy reaches 4.9); 2049 tokens with norms 9.6 us, 2.7 TB/s; one token 2.6 us.
+// kStream: non-temporal stores (a template's, as the compiler joins the two stores of
+// a branch into a plain one).
+template <class T, int V, int kUnits, bool kNorm, bool kPaged, bool kStream>
 __global__ __launch_bounds__(kHeadBlock) void heads_kernel(const HeadsArgs a, const int tile) {
-    __shared__ float cs[2][kMaxTile * kMaxHalf];
+    __shared__ __align__(16) float cs[2][kMaxTile * kMaxHalf];
+    __shared__ __align__(16) float wt[kNorm ? 2 : 1][kNorm ? 2 * kMaxHalf : 1];
     __shared__ Place place[kMaxTile];
     const int tid = threadIdx.x, t0 = blockIdx.x * tile;
     const int n = min(tile, a.tokens - t0);
+    const int lanes = 1 << a.lanes_log, u0 = tid & (lanes - 1);
+    const int heads = a.all_heads.d, items = n * heads, step = kHeadBlock >> a.lanes_log;
+
+    int item = tid >> a.lanes_log;
+    Part<V> raw[kUnits][2], ahead[kUnits][2];
+    int at[kUnits][2];
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+        const int u = u0 + (k << a.lanes_log);
+        const bool split = u < a.rot_units && !a.interleaved;
+        at[k][0] = split ? V * u : 2 * V * u;
+        at[k][1] = split ? V * u + a.half : 2 * V * u + V;
+    }
+    auto fetch = [&](int it, Part<V> (&to)[kUnits][2]) {
+        const int tt = a.all_heads.div(it);
+        int h = it - tt * heads;
+        const int n0 = a.span[0].heads, n1 = n0 + a.span[1].heads;
+        const uint16_t* src = h < n0 ? a.span[0].src : (h < n1 ? a.span[1].src : a.span[2].src);
+        const long stride = h < n0 ? a.span[0].src_stride
+                                   : (h < n1 ? a.span[1].src_stride : a.span[2].src_stride);
+        h -= h < n0 ? 0 : (h < n1 ? n0 : n1);
+        src += (t0 + tt) * stride + static_cast<long>(h) * a.head_dim;
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k)
+            if (u0 + (k << a.lanes_log) < a.units) {
+                to[k][0] = load_part<V>(src + at[k][0]);
+                to[k][1] = load_part<V>(src + at[k][1]);
+            }
+    };
+    if (item < items) fetch(item, raw);
+
     if (kPaged) {
-        const int wave = tid / kWave;
-        if (wave < n) {
-            const Place p = find_place(a, t0 + wave);
-            if ((tid & (kWave - 1)) == 0) place[wave] = p;
+        for (int w = tid / kWave; w < n; w += kHeadBlock / kWave) {
+            const Place p = find_place(a, t0 + w);
+            if ((tid & (kWave - 1)) == 0) place[w] = p;
         }
         __syncthreads();
     }
+    if (kNorm)
+        for (int i = tid; i < 2 * a.head_dim; i += kHeadBlock) {
+            const int which = i >= a.head_dim, d = i - which * a.head_dim;
+            const float* const w = which ? a.span[1].weight : a.span[0].weight;
+            if (w) wt[which][d] = w[d];
+        }
     for (int i = tid; i < n * a.half; i += kHeadBlock) {
         const int tt = i / a.half, pair = i - tt * a.half;
         const int pos = kPaged ? place[tt].pos : a.positions[t0 + tt];
         double turns = static_cast<double>(pos) * (a.inv_freq[pair] * 0.15915494309189533577);
         turns -= rint(turns);
         const float x = static_cast<float>(turns);
-        cs[0][i] = __builtin_amdgcn_cosf(x) * a.scale;
-        cs[1][i] = __builtin_amdgcn_sinf(x) * a.scale;
+        const int to = tt * a.half + lds_at<V>(pair, a.rot_units);
+        cs[0][to] = __builtin_amdgcn_cosf(x) * a.scale;
+        cs[1][to] = __builtin_amdgcn_sinf(x) * a.scale;
     }
     __syncthreads();
-    const int lanes = 1 << a.lanes_log, u0 = tid & (lanes - 1);
-    const int items = n * a.all_heads;
-    for (int item = tid >> a.lanes_log; item < items; item += kHeadBlock >> a.lanes_log) {
-        const int tt = item / a.all_heads;
-        int h = item - tt * a.all_heads, which = 0;
+    for (; item < items; item += step) {
+        if (item + step < items) fetch(item + step, ahead);
+        const int tt = a.all_heads.div(item);
+        int h = item - tt * heads, which = 0;
         if (h >= a.span[0].heads) {
             h -= a.span[0].heads;
             which = 1;
@@ -145,80 +219,81 @@ __global__ __launch_bounds__(kHeadBlock) void heads_kernel(const HeadsArgs a, co
         // selects, not an index: indexed kernel arguments are copied to scratch memory
         const HeadSpan sp = which == 0 ? a.span[0] : (which == 1 ? a.span[1] : a.span[2]);
         const int pos = kPaged ? place[tt].pos : (a.positions ? a.positions[t0 + tt] : 0);
-        if (pos < 0) continue;  // padding; all lanes of a head agree
         const long t = t0 + tt;
-        const uint16_t* src = sp.src + t * sp.src_stride + static_cast<long>(h) * a.head_dim;
-        uint16_t* dst;
-        if (kPaged && sp.dst == nullptr) {
-            if (place[tt].slot < 0) continue;
-            dst = (which == 1 ? a.k_pages : a.v_pages) + place[tt].slot + h * a.head_stride;
-        } else {
-            dst = sp.dst + t * sp.dst_stride + static_cast<long>(h) * a.head_dim;
+        uint16_t* dst = nullptr;
+        if (pos >= 0) {  // else padding; all lanes of a head agree
+            if (!kPaged || sp.dst)
+                dst = sp.dst + t * sp.dst_stride + static_cast<long>(h) * a.head_dim;
+            else if (place[tt].slot >= 0)
+                dst = (which == 1 ? a.k_pages : a.v_pages) + place[tt].slot + h * a.head_stride;
         }
-        float x[kUnits][2][V];
-        int at[kUnits][2];
-#pragma unroll
-        for (int k = 0; k < kUnits; ++k) {
-            const int u = u0 + (k << a.lanes_log);
-            const bool split = u < a.rot_units && !a.interleaved;
-            at[k][0] = split ? V * u : 2 * V * u;
-            at[k][1] = split ? V * u + a.half : 2 * V * u + V;
-            if (u < a.units) {
-                load_part<T, V>(src + at[k][0], x[k][0]);
-                load_part<T, V>(src + at[k][1], x[k][1]);
-            }
-        }
-        if (kNorm && sp.weight) {
-            float ss = 0.0f;
+        if (dst) {
+            float x[kUnits][2][V];
 #pragma unroll
             for (int k = 0; k < kUnits; ++k)
-                if (u0 + (k << a.lanes_log) < a.units)
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const bool have = u0 + (k << a.lanes_log) < a.units;
+                    x[k][0][e] = have ? T::to_float(raw[k][0].w[e]) : 0.0f;
+                    x[k][1][e] = have ? T::to_float(raw[k][1].w[e]) : 0.0f;
+                }
+            if (kNorm && sp.weight) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int k = 0; k < kUnits; ++k)
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
                         ss = __builtin_fmaf(x[k][0][e], x[k][0][e], ss);
                         ss = __builtin_fmaf(x[k][1][e], x[k][1][e], ss);
                     }
-            for (int off = lanes >> 1; off > 0; off >>= 1) ss += __shfl_xor(ss, off, kWave);
-            const float inv = 1.0f / sqrtf(ss / static_cast<float>(a.head_dim) + a.eps);
+                for (int off = lanes >> 1; off > 0; off >>= 1) ss += __shfl_xor(ss, off, kWave);
+                const float inv = 1.0f / sqrtf(ss / static_cast<float>(a.head_dim) + a.eps);
 #pragma unroll
-            for (int k = 0; k < kUnits; ++k)
-                if (u0 + (k << a.lanes_log) < a.units)
+                for (int k = 0; k < kUnits; ++k)
+                    if (u0 + (k << a.lanes_log) < a.units)
 #pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        x[k][0][e] = (x[k][0][e] * inv) * sp.weight[at[k][0] + e];
-                        x[k][1][e] = (x[k][1][e] * inv) * sp.weight[at[k][1] + e];
+                        for (int j = 0; j < 2; ++j) {
+                            float w[V];
+                            __builtin_memcpy(w, __builtin_assume_aligned(
+                                &wt[which][at[k][j]], V == 1 ? 4 : 16), 4 * V);
+#pragma unroll
+                            for (int e = 0; e < V; ++e) x[k][j][e] = (x[k][j][e] * inv) * w[e];
+                        }
+            }
+#pragma unroll
+            for (int k = 0; k < kUnits; ++k) {
+                const int u = u0 + (k << a.lanes_log);
+                if (u >= a.units) continue;
+                if (sp.rotate && u < a.rot_units) {
+                    float c[V], s[V], y[2 * V];
+                    load_lds<V>(&cs[0][tt * a.half], u, a.rot_units, c);
+                    load_lds<V>(&cs[1][tt * a.half], u, a.rot_units, s);
+#pragma unroll
+                    for (int e = 0; e < 2 * V; ++e) y[e] = x[k][e / V][e % V];
+                    if (a.interleaved) {
+#pragma unroll
+                        for (int e = 0; e < V; ++e) {
+                            const float p = y[2 * e], q = y[2 * e + 1];
+                            x[k][2 * e / V][2 * e % V] = __builtin_fmaf(p, c[e], -(q * s[e]));
+                            x[k][(2 * e + 1) / V][(2 * e + 1) % V] = __builtin_fmaf(p, s[e], q * c[e]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < V; ++e) {
+                            const float p = y[e], q = y[V + e];
+                            x[k][0][e] = __builtin_fmaf(p, c[e], -(q * s[e]));
+                            x[k][1][e] = __builtin_fmaf(p, s[e], q * c[e]);
+                        }
                     }
+                }
+                store_part<T, V, kStream>(dst + at[k][0], x[k][0]);
+                store_part<T, V, kStream>(dst + at[k][1], x[k][1]);
+            }
         }
 #pragma unroll
         for (int k = 0; k < kUnits; ++k) {
-            const int u = u0 + (k << a.lanes_log);
-            if (u >= a.units) continue;
-            if (sp.rotate && u < a.rot_units) {
-                const float* c = &cs[0][tt * a.half + V * u];
-                const float* s = &cs[1][tt * a.half + V * u];
-                float y[2 * V];
-                if (a.interleaved) {
-#pragma unroll
-                    for (int e = 0; e < 2 * V; ++e) y[e] = x[k][e / V][e % V];
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        const float p = y[2 * e], q = y[2 * e + 1];
-                        const float r = __builtin_fmaf(p, c[e], -(q * s[e]));
-                        const float i = __builtin_fmaf(p, s[e], q * c[e]);
-                        x[k][(2 * e) / V][(2 * e) % V] = r;
-                        x[k][(2 * e + 1) / V][(2 * e + 1) % V] = i;
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        const float p = x[k][0][e], q = x[k][1][e];
-                        x[k][0][e] = __builtin_fmaf(p, c[e], -(q * s[e]));
-                        x[k][1][e] = __builtin_fmaf(p, s[e], q * c[e]);
-                    }
-                }
-            }
-            store_part<T, V>(dst + at[k][0], x[k][0]);
-            store_part<T, V>(dst + at[k][1], x[k][1]);
+            raw[k][0] = ahead[k][0];
+            raw[k][1] = ahead[k][1];
         }
     }
 }
@@ -254,16 +329,19 @@ int check_span(const char* fn, const char* what, const HeadSpan& s, int tokens, 
     return 0;
 }
 
-template <class T, int V, int kUnits>
-void launch_heads(const HeadsArgs& a, int tile, bool norm, bool paged, hipStream_t st) {
+template <class T, int V, int kUnits, bool kNorm, bool kPaged>
+void launch_heads(const HeadsArgs& a, int tile, bool past, hipStream_t st) {
     const dim3 grid((a.tokens + tile - 1) / tile), block(kHeadBlock);
-    if (paged) {
-        if (norm) hipLaunchKernelGGL((heads_kernel<T, V, kUnits, true, true>), grid, block, 0, st, a, tile);
-        else hipLaunchKernelGGL((heads_kernel<T, V, kUnits, false, true>), grid, block, 0, st, a, tile);
-    } else {
-        if (norm) hipLaunchKernelGGL((heads_kernel<T, V, kUnits, true, false>), grid, block, 0, st, a, tile);
-        else hipLaunchKernelGGL((heads_kernel<T, V, kUnits, false, false>), grid, block, 0, st, a, tile);
-    }
+    if (past) hipLaunchKernelGGL((heads_kernel<T, V, kUnits, kNorm, kPaged, V != 1>), grid, block, 0, st, a, tile);
+    else hipLaunchKernelGGL((heads_kernel<T, V, kUnits, kNorm, kPaged, false>), grid, block, 0, st, a, tile);
+}
+
+template <class T, int V, int kUnits>
+void pick_heads(const HeadsArgs& a, int tile, bool norm, bool paged, bool past, hipStream_t st) {
+    if (paged && norm) launch_heads<T, V, kUnits, true, true>(a, tile, past, st);
+    else if (paged) launch_heads<T, V, kUnits, false, true>(a, tile, past, st);
+    else if (norm) launch_heads<T, V, kUnits, true, false>(a, tile, past, st);
+    else launch_heads<T, V, kUnits, false, false>(a, tile, past, st);
 }
 
 // Launches over the filled spans; the widest pair count whose parts all lie
@@ -275,7 +353,7 @@ int run_heads(const char* fn, HeadsArgs& a, const spb_rope* rope, bool paged, sp
     a.interleaved = rope ? rope->interleaved != 0 : 1;
     a.scale = rope ? rope->scale : 1.0f;
     a.inv_freq = rope ? rope->inv_freq : nullptr;
-    a.all_heads = a.span[0].heads + a.span[1].heads + a.span[2].heads;
+    a.all_heads = FastDiv(a.span[0].heads + a.span[1].heads + a.span[2].heads);
     bool norm = false;
     auto fits = [&](int v) {
         if (hd % (2 * v) || rot % (2 * v)) return false;
@@ -291,12 +369,18 @@ int run_heads(const char* fn, HeadsArgs& a, const spb_rope* rope, bool paged, sp
     a.rot_units = rot / (2 * v);
     a.lanes_log = 0;
     while ((1 << a.lanes_log) < a.units && a.lanes_log < 6) ++a.lanes_log;
-    // Several tokens a block once one a block fills the chip.
+    // Two tokens a block once one a block fills the chip.  us for 1 / 2 / 3 / 5 / 8:
+    // 8192 tokens of 25 heads of 128 27.2 / 25.8 / 26.8 / 28.1 / 27.4, 2049 normed
+    // tokens 10.4 / 10.4 / 11.1 / 12.3 / 15.6, 3540 tokens appended 20.7 / 19.9 /
+    // 21.3 / 21.3 / 24.9 (plain stores).
     const int tile = a.tokens >= 4 * device_cu_count() ? kMaxTile : 1;
+    // What is larger than a die's L2 is written past it: 25.8 -> 20.1, 10.4 -> 9.6
+    // and 19.9 -> 17.8 us for the same three (non-temporal loads lose as much).
+    const bool past = static_cast<long>(a.tokens) * static_cast<long>(a.all_heads.d) * hd * 2 > (4L << 20);
     const hipStream_t st = as_stream(stream);
-    if (v == 8) launch_heads<T, 8, 1>(a, tile, norm, paged, st);
-    else if (v == 4) launch_heads<T, 4, 1>(a, tile, norm, paged, st);
-    else launch_heads<T, 1, 2>(a, tile, norm, paged, st);
+    if (v == 8) pick_heads<T, 8, 1>(a, tile, norm, paged, past, st);
+    else if (v == 4) pick_heads<T, 4, 1>(a, tile, norm, paged, past, st);
+    else pick_heads<T, 1, 2>(a, tile, norm, paged, past, st);
     return launch_status(fn);
 }
 
