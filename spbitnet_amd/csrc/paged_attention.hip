@@ -2,8 +2,10 @@
 //
 // The rows of a tile are (token, query head) pairs of one sequence and one kv
 // head, so K and V are read once for all query heads of a kv head.  A wave holds
-// 32 rows and walks over keys 32 at a time on the 32x32x16 matrix instructions:
-//   S^T = K Q^T   lane l has row l % 32 and keys 8 (i / 4) + 4 (l / 32) + i % 4
+// W = 32 (or 16) rows and walks over the keys with the matrix instructions that
+// take W x W results:
+//   S^T = K Q^T   lane l has row l % W and, of each W keys, those
+//                 4 (64 / W) (i / 4) + 4 (l / W) + i % 4
 //   p = 2^(s c - m), c = scale log2(e), m a running reference of the row
 //   O^T += V^T P^T
 // The sum over keys of the second product may run in any order, so P goes from
@@ -22,6 +24,7 @@ constexpr int kJoinBlock = 256;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
@@ -42,6 +45,10 @@ template <> struct Prob<F16> {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(frag, a),
                                                       __builtin_bit_cast(frag, b), c, 0, 0, 0);
     }
+    static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(frag, a),
+                                                      __builtin_bit_cast(frag, b), c, 0, 0, 0);
+    }
     static __device__ __forceinline__ uint32_t pack(float x, float y) {
         typedef _Float16 h2 __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, h2{static_cast<_Float16>(x), static_cast<_Float16>(y)});
@@ -53,6 +60,10 @@ template <> struct Prob<BF16> {
     typedef b16x8 frag;
     static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(frag, a),
+                                                       __builtin_bit_cast(frag, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(frag, a),
                                                        __builtin_bit_cast(frag, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ uint32_t pack(float x, float y) {
@@ -85,27 +96,37 @@ struct AttnArgs {
     float* ws;         // partial results, 2 per worker
 };
 
-// A tile's shape: RG waves of 32 rows each, which all walk over the same keys; a
-// single wave of rows (decoding) gets a second one, and the two take turns at 32
-// keys and join their results at the end.
-template <int RG>
+// A tile of BM rows: a wave takes W of them, 32, or 16 where the tile has no more (a
+// decoding step: half the arithmetic and registers).  The waves of 64 and 128 rows
+// walk over the same keys; a single wave of rows gets a second one, and the two take
+// turns at 32 keys and join their results at the end.
+template <int BM>
 struct Shape {
-    static constexpr int KG = RG == 1 ? 2 : 1, NS = RG == 1 ? 1 : 2;  // groups of 32 NS keys
+    static constexpr int W = BM < 32 ? BM : 32;
+    static constexpr int RG = BM / W, KG = RG == 1 ? 2 : 1;  // waves by rows and by keys
+    static constexpr int kKeys = RG == 1 ? 32 : 64;          // of a wave
     static constexpr int kWaves = RG * KG, kThreads = kWave * kWaves;
-    static constexpr int BM = 32 * RG, BN = 32 * KG * NS;
+    static constexpr int BN = kKeys * KG;
     static_assert(BN == kWave, "a lane per key of a tile");
     // Fewest keys worth a worker of their own.
     static constexpr int kMinKeys = RG == 4 ? 256 : 64;
+    static constexpr bool kOnce = RG <= 2;  // keys are read once: not kept in L2
 };
+
+// A product's result in a wave: W x W, element i of lane l is column l % W and row
+// 4 (64 / W) (i / 4) + 4 (l / W) + i % 4.
+template <int W> struct Acc;
+template <> struct Acc<32> { typedef f32x16 type; };
+template <> struct Acc<16> { typedef f32x4 type; };
 
 // How a batch's work is shared out.  Its tiles stand in one line, ordered by
 // sequence, kv head and row tile, each as long as its cost (keys seen times the
-// group / 32, and a block for what a tile costs besides); the line is cut into
+// group / 16, and a block for what a tile costs besides); the line is cut into
 // equal parts, one per worker, and every worker walks over its part.  So the work
 // per worker is the same whatever the mix of lengths, and a tile is split only where
 // a cut falls into it.  Every wave computes the cuts by itself from the batch's
 // arrays, a lane per sequence.  Places are whole numbers in float64, exact below
-// 2^53 (rows times keys times the group / 1024: 2^46 for a million tokens of 64
+// 2^53 (rows times keys times the group / 256: 2^48 for a million tokens of 64
 // heads over a million keys); a 64-bit integer division took a microsecond of the
 // 10 that a small call has.  A cost need not be exact: it decides only who does
 // what.
@@ -144,8 +165,8 @@ __device__ __forceinline__ SeqCost seq_cost(const AttnArgs& a, const SeqSpan& q)
     r.tiles = static_cast<int>((rows + BM - 1) / BM);
     const bool grows = a.causal && (a.window == 0 || a.reach >= q.len);
     const double keys = grows ? max(q.len - q.count, 0) : (a.causal ? a.reach : q.len);
-    r.c0 = floor((keys + BN) * group * (1.0 / 32)) + (grows ? BM / 32 : 0) + 1.0;
-    r.c1 = grows ? BM / 32 : 0.0;
+    r.c0 = floor((keys + BN) * group * (1.0 / 16)) + (grows ? BM / 16 : 0) + 1.0;
+    r.c1 = grows ? BM / 16 : 0.0;
     r.head = cost_before(r.c0, r.c1, r.tiles);
     return r;
 }
@@ -292,7 +313,7 @@ __device__ __forceinline__ int blocks_before(const Tile& t, double at, int block
 
 // Bytes of an LDS row of K or V, and the swizzle of its 16-byte units: lanes
 // that read K take one unit of 32 consecutive keys (spread over the units by the
-// key), those that read V take 64 bytes of 4 consecutive keys.
+// key), those that read V take 64 bytes of 4 consecutive keys or 32 of 8.
 template <int HD>
 struct Row {
     static constexpr int kPitch = HD <= 64 ? 128 : (HD <= 128 ? 256 : 512);
@@ -300,7 +321,7 @@ struct Row {
     static constexpr int kMask = kUnits < 16 ? kUnits - 1 : 15;
     static __device__ __forceinline__ int k_unit(int key, int unit) { return unit ^ (key & kMask); }
     static __device__ __forceinline__ int v_unit(int key, int unit) {
-        return unit ^ (kPitch >= 256 ? (key & 3) << 2 : (key & 2) << 1);
+        return unit ^ (kPitch >= 256 ? (key & 3) << 2 | (key & 4) >> 1 : (key & 2) << 1 | (key & 4) >> 1);
     }
     static __device__ __forceinline__ int k_at(int key, int unit) {
         return key * kPitch + (k_unit(key, unit) << 4);
@@ -327,20 +348,35 @@ __device__ __forceinline__ bool row_sees(const AttnArgs& a, int count, int len, 
     return hi > (a.window ? max(pos - a.window + 1, 0) : 0);
 }
 
-// x of the lower and of the upper half of the wave, in all lanes.
-__device__ __forceinline__ float2 halves(float x) {
+// Two exchanges of lanes l and l ^ 32, l and l ^ 16: both lanes' values in both.
+__device__ __forceinline__ float2 across32(float x) {
     const uint32_t a = __builtin_bit_cast(uint32_t, x);
     const auto s = __builtin_amdgcn_permlane32_swap(a, a, false, false);
     // copies: a bit cast of a vector's element itself reads element 0
     const uint32_t lower = s[0], upper = s[1];
     return make_float2(__builtin_bit_cast(float, lower), __builtin_bit_cast(float, upper));
 }
-__device__ __forceinline__ float half_max(float x) {
-    const float2 h = halves(x);
+__device__ __forceinline__ float2 across16(float x) {
+    const uint32_t a = __builtin_bit_cast(uint32_t, x);
+    const auto s = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    const uint32_t lower = s[0], upper = s[1];
+    return make_float2(__builtin_bit_cast(float, lower), __builtin_bit_cast(float, upper));
+}
+// Over the lanes that hold a row.
+template <int W>
+__device__ __forceinline__ float row_max(float x) {
+    float2 h = across32(x);
+    x = fmaxf(h.x, h.y);
+    if (W == 32) return x;
+    h = across16(x);
     return fmaxf(h.x, h.y);
 }
-__device__ __forceinline__ float half_sum(float x) {
-    const float2 h = halves(x);
+template <int W>
+__device__ __forceinline__ float row_sum(float x) {
+    float2 h = across32(x);
+    x = h.x + h.y;
+    if (W == 32) return x;
+    h = across16(x);
     return h.x + h.y;
 }
 
@@ -366,49 +402,57 @@ __device__ __forceinline__ uint32_t non_finite(uint32_t x) {
     return ((x & (e << 16 | e)) + (one << 16 | one)) & 0x80008000u;
 }
 
-// One tile's state in a wave: 32 rows, their sums and statistics.
-template <class T, int HD, int RG>
+// One tile's state in a wave: W rows, their sums and statistics.
+template <class T, int HD, int BM>
 struct RowState {
-    u32x4 q[HD / 16];       // Q^T operand: row lane % 32, elements 16 step + 8 half ..
-    f32x16 o[HD / 32];      // O^T
-    float m, l;             // reference and (this half wave's) sum of the lane's row
-    int see_lo, see_hi;     // keys that the lane's row sees, of this piece
-    int all_lo, all_hi;     // ... that all rows of the wave see
-    int any_lo, any_hi;     // ... that any sees
+    static constexpr int W = Shape<BM>::W;
+    u32x4 q[HD * W / 512];          // Q^T operand: row lane % W, elements 512 / W step + 8 (lane / W) ..
+    typename Acc<W>::type o[HD / W];  // O^T
+    float m, l;                     // reference and (these lanes' part of the) sum of the lane's row
+    int see_lo, see_hi;             // keys that the lane's row sees, of this piece
+    int all_lo, all_hi;             // ... that all rows of the wave see
+    int any_lo, any_hi;             // ... that any sees
+    // Column of O^T's element i of tile c, in this lane.
+    static __device__ __forceinline__ int column(int c, int i) {
+        const int lane = threadIdx.x & (kWave - 1);
+        return W * c + 256 / W * (i / 4) + 4 * (lane / W) + i % 4;
+    }
 };
 
 // One tile of keys t .. t + BN in LDS (K, then V) against the wave's rows.  `between`
 // is called kBetween times among the matrix products, whose time hides what it issues.
 constexpr int kBetween = 4;
-template <class T, int HD, int RG, class F>
-__device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, RG>& r,
+template <class T, int HD, int BM, class F>
+__device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, BM>& r,
                                        const uint8_t* buf, int t, int kg, uint64_t there,
                                        F between) {
     typedef Row<HD> R;
     typedef Prob<T> P;
-    constexpr int NS = Shape<RG>::NS, kSteps = HD / 16, kCols = HD / 32, kKeys = 32 * NS;
-    const int j0 = t + kKeys * kg;
+    constexpr int W = Shape<BM>::W, kKeys = Shape<BM>::kKeys;
+    constexpr int kDepth = 512 / W;                  // of a product
+    constexpr int kSteps = HD / kDepth, kTiles = kKeys / W, kCols = HD / W, kEach = W * W / kWave;
+    typedef typename Acc<W>::type acc;
+    const int j0 = t + kKeys * kg;  // this wave's keys
     if (j0 >= r.any_hi || j0 + kKeys <= r.any_lo) {
         for (int i = 0; i < kBetween; ++i) between(i);
         return;
     }
     const uint8_t* const kw = buf + kKeys * kg * R::kPitch;
-    const uint8_t* const vw = kw + Shape<RG>::BN * R::kPitch;
-    const int lane = threadIdx.x & (kWave - 1), half = lane >> 5;
+    const uint8_t* const vw = kw + Shape<BM>::BN * R::kPitch;
+    const int lane = threadIdx.x & (kWave - 1), part = lane / W;
     // Reads of LDS go out a group ahead of the products that use them: left to itself
     // the compiler puts each right before its use, whose wait then shows.
-    f32x16 s[NS];
-    constexpr int kGroup = 2, kGroups = kSteps / kGroup;  // steps
-    u32x4 k[2][kGroup][NS];
+    acc s[kTiles];
+    constexpr int kGroup = kSteps % 2 ? 1 : 2, kGroups = kSteps / kGroup;  // steps
+    u32x4 k[2][kGroup][kTiles];
     auto load_k = [&](int g) {
 #pragma unroll
         for (int st = 0; st < kGroup; ++st)
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
+            for (int n = 0; n < kTiles; ++n)
                 k[g & 1][st][n] = *reinterpret_cast<const u32x4*>(
-                    kw + R::k_at(32 * n + (lane & 31), 2 * (g * kGroup + st) + half));
+                    kw + R::k_at(W * n + lane % W, kDepth / 8 * (g * kGroup + st) + part));
     };
-    static_assert(kSteps % kGroup == 0, "whole groups");
     load_k(0);
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
@@ -418,20 +462,21 @@ __device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, RG>& r
 #pragma unroll
         for (int st = 0; st < kGroup; ++st)
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
+            for (int n = 0; n < kTiles; ++n)
                 s[n] = P::mfma(k[g & 1][st][n], r.q[g * kGroup + st],
-                               g + st == 0 ? f32x16{} : s[n]);
+                               g + st == 0 ? acc{} : s[n]);
     }
 #pragma unroll
     for (int g = kGroups; g < kBetween; ++g) between(g);
-    // V^T operands of 16 keys; lane: column 32 c + lane % 32, keys 4 half .. and 8 + 4 half ..
+    // V^T operands of kDepth keys; lane: column W c + lane % W, keys 4 part .. and
+    // kDepth / 2 + 4 part ..
     const int l16 = lane & 15;
     auto load_v = [&](int g, u32x4 (&v)[kCols]) {
 #pragma unroll
         for (int c = 0; c < kCols; ++c) {
             typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-            const int key = 16 * g + 4 * half + (l16 >> 2);
-            const int unit = 4 * c + 2 * ((lane >> 4) & 1) + ((l16 & 3) >> 1);
+            const int key = kDepth * g + 4 * part + (l16 >> 2);
+            const int unit = W / 8 * c + (W == 32 ? lane >> 3 & 2 : 0) + ((l16 & 3) >> 1);
             const int off = (l16 & 1) << 3;
             union {
                 s16x4 h[2];
@@ -440,29 +485,30 @@ __device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, RG>& r
             x.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (lds_s16x4*)(vw + R::v_at(key, unit) + off));
             x.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_s16x4*)(vw + R::v_at(key + 8, unit) + off));
+                (lds_s16x4*)(vw + R::v_at(key + kDepth / 2, unit) + off));
             v[c] = x.v;
         }
     };
+    auto key_of = [&](int n, int i) { return W * n + 256 / W * (i / 4) + i % 4; };  // + 4 part
     u32x4 v[2][kCols];
     if (j0 < r.all_lo || j0 + kKeys > r.all_hi || there != ~uint64_t{0}) {  // not all rows see all
-        const int lo = r.see_lo - j0 - 4 * half, hi = r.see_hi - j0 - 4 * half;
-        const uint64_t mine = there >> (kKeys * kg + 4 * half);
+        const int lo = r.see_lo - j0 - 4 * part, hi = r.see_hi - j0 - 4 * part;
+        const uint64_t mine = there >> (kKeys * kg + 4 * part);
 #pragma unroll
-        for (int n = 0; n < NS; ++n)
+        for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int j = 32 * n + 8 * (i / 4) + i % 4;
+            for (int i = 0; i < kEach; ++i) {
+                const int j = key_of(n, i);
                 if (j < lo || j >= hi || !(mine >> j & 1)) s[n][i] = -INFINITY;
             }
     }
     // the row's largest score, and its reference
     float top = s[0][0];
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
+    for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
-    top = half_max(top) * a.c - P::kBias;
+        for (int i = 0; i < kEach; ++i) top = fmaxf(top, s[n][i]);
+    top = row_max<W>(top) * a.c - P::kBias;
     const bool move = top > r.m + P::kSlack;  // also from m = -inf
     if (__any(move)) {
         const float f = move ? __builtin_amdgcn_exp2f(r.m - top) : 1.0f;
@@ -471,28 +517,28 @@ __device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, RG>& r
 #pragma unroll
         for (int c = 0; c < kCols; ++c)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) r.o[c][i] *= f;
+            for (int i = 0; i < kEach; ++i) r.o[c][i] *= f;
     }
     const float ref = r.m == -INFINITY ? 0.0f : r.m;  // a row that has seen nothing yet
     load_v(0, v[0]);
     __builtin_amdgcn_sched_barrier(0);
-    u32x4 pf[2 * NS];
+    constexpr int kParts = kKeys / kDepth;  // 8 probabilities of a lane each
+    u32x4 pf[kParts];
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], a.c, -ref));
-            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i + 1], a.c, -ref));
-            sum[i % 4] += x;
-            sum[i % 4 + 1] += y;
-            pf[2 * n + i / 8][(i % 8) / 2] = P::pack(x, y);
-        }
+    for (int e = 0; e < kTiles * kEach; e += 2) {
+        const acc& y = s[e / kEach];
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[e % kEach], a.c, -ref));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[e % kEach + 1], a.c, -ref));
+        sum[e % 4] += p0;
+        sum[e % 4 + 1] += p1;
+        pf[e / 8][e % 8 / 2] = P::pack(p0, p1);
+    }
     r.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     // O^T += V^T P^T
 #pragma unroll
-    for (int g = 0; g < 2 * NS; ++g) {
-        if (g + 1 < 2 * NS) load_v(g + 1, v[(g + 1) & 1]);
+    for (int g = 0; g < kParts; ++g) {
+        if (g + 1 < kParts) load_v(g + 1, v[(g + 1) & 1]);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < kCols; ++c) r.o[c] = P::mfma(v[g & 1][c], pf[g], r.o[c]);
@@ -503,9 +549,9 @@ __device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, RG>& r
 // the product of a probability of 0 with them would reach the rows that do not see
 // them.  Replaces them by 0 in LDS and says whether there were any (here or in an
 // earlier tile).  All threads call it.
-template <class T, int HD, int RG>
+template <class T, int HD, int BM>
 __device__ __forceinline__ bool take_out(uint8_t* buf, int* found) {
-    typedef Shape<RG> S;
+    typedef Shape<BM> S;
     constexpr int kAll = S::BN * Row<HD>::kUnits;
     u32x4* const v = reinterpret_cast<u32x4*>(buf + S::BN * Row<HD>::kPitch);
     for (int i = threadIdx.x; i < kAll; i += S::kThreads) {
@@ -524,25 +570,26 @@ __device__ __forceinline__ bool take_out(uint8_t* buf, int* found) {
 }
 
 // Adds what take_out took out of the tile to the rows that see it, from memory.
-template <class T, int HD, int RG>
-__device__ __forceinline__ void put_back(const AttnArgs& a, RowState<T, HD, RG>& r, int t, int end,
+template <class T, int HD, int BM>
+__device__ __forceinline__ void put_back(const AttnArgs& a, RowState<T, HD, BM>& r, int t, int end,
                                          int kg, const int* table, const uint16_t* vbase) {
-    constexpr int kKeys = 32 * Shape<RG>::NS;
-    const int half = (threadIdx.x & (kWave - 1)) >> 5;
+    constexpr int W = Shape<BM>::W, kKeys = Shape<BM>::kKeys, kEach = W * W / kWave;
+    const int part = (threadIdx.x & (kWave - 1)) / W;
     for (int j = t + kKeys * kg; j < min(t + kKeys * (kg + 1), end); ++j) {
         const int p = a.b.page.div(j), id = table[p];
         if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.b.pages)) continue;
         const uint16_t* const v = vbase + id * a.page_stride +
-                                  (j - p * static_cast<int>(a.b.page.d)) * a.slot_stride + 4 * half;
+                                  (j - p * static_cast<int>(a.b.page.d)) * a.slot_stride + 4 * part;
         const bool mine = j >= r.see_lo && j < r.see_hi;
-        int hd = a.head_dim;
+        int hd = a.head_dim - 4 * part;
         asm volatile("" : "+v"(hd));  // else the comparisons below are kept over all tiles
 #pragma unroll
-        for (int c = 0; c < HD / 32; ++c)
+        for (int c = 0; c < HD / W; ++c)
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                if (32 * c + 2 * i >= hd) continue;
-                const uint2 x = *reinterpret_cast<const uint2*>(v + 32 * c + 2 * i);
+            for (int i = 0; i < kEach; i += 4) {
+                const int d = W * c + 256 / W * (i / 4);
+                if (d >= hd) continue;
+                const uint2 x = *reinterpret_cast<const uint2*>(v + d);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint32_t y = (e < 2 ? x.x : x.y) >> (e % 2 * 16) & 0xFFFFu;
@@ -557,21 +604,22 @@ __device__ __forceinline__ void put_back(const AttnArgs& a, RowState<T, HD, RG>&
 __device__ __align__(16) const uint32_t kZeros[4] = {0, 0, 0, 0};
 
 // Blocks of a CU that LDS and registers hold.
-template <int HD, int RG>
-constexpr int resident() { return HD > 128 ? 1 : (RG <= 2 && HD <= 64 ? 4 : 2); }
+template <int HD, int BM>
+constexpr int resident() { return HD > 128 ? 1 : (BM <= 64 && HD <= 64 ? 4 : 2); }
+// Registers for two waves on a SIMD up to 128 columns, also where one is resident: with
+// more of them the compiler keeps O in accumulation registers, which costs moves.
+template <int HD, int BM>
+constexpr int waves_per_simd() { return HD <= 128 ? 2 : 1; }
 
-template <int HD, int RG>
-constexpr int waves_per_simd() { return Shape<RG>::kWaves * resident<HD, RG>() >= 8 ? 2 : 1; }
-
-template <class T, int HD, int RG>
-__global__ __launch_bounds__((Shape<RG>::kThreads), (waves_per_simd<HD, RG>()))
+template <class T, int HD, int BM>
+__global__ __launch_bounds__((Shape<BM>::kThreads), (waves_per_simd<HD, BM>()))
 void paged_attention_kernel(const AttnArgs a) {
-    typedef Shape<RG> S;
+    typedef Shape<BM> S;
     typedef Row<HD> R;
-    constexpr int KG = S::KG, BM = S::BM, BN = S::BN;
-    constexpr int kSteps = HD / 16, kCols = HD / 32;
-    constexpr int kRows = kWave / R::kUnits;                // rows of K that a wave's load fills
-    constexpr int kLoads = BN / (kRows * S::kWaves);        // loads of a wave, K and V each
+    constexpr int W = S::W, RG = S::RG, KG = S::KG, BN = S::BN;
+    constexpr int kDepth = 512 / W, kSteps = HD / kDepth, kCols = HD / W, kEach = W * W / kWave;
+    constexpr int kRows = kWave / R::kUnits;          // rows of K that a wave's load fills
+    constexpr int kLoads = BN / (kRows * S::kWaves);  // loads of a wave, K and V each
     // Two tiles of keys: one is filled while the other is read.  Two arrays, so that
     // the compiler sees that reads of one need not wait for loads into the other.
     __shared__ __align__(16) uint8_t buf0[2 * BN * R::kPitch];
@@ -579,24 +627,38 @@ void paged_attention_kernel(const AttnArgs a) {
     __shared__ float ml_lds[KG][BM][2];
     __shared__ int found_lds;  // take_out's
 
-    const Lanes lanes = look<BM, BN>(a, 0);
-    const Plan plan = make_plan<BM, BN>(a, lanes);
+    // The arguments' lines, fetched together: a small call has a microsecond for each
+    // that would be waited for by itself.
+    asm volatile("" ::"s"(a.b.starts), "s"(a.b.seqs), "s"(a.q), "s"(a.k), "s"(a.out), "s"(a.q_stride),
+                 "s"(a.slot_stride), "s"(a.c), "s"(a.reach), "s"(a.workers), "s"(a.ws));
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = scalar(tid / kWave);
-    if (blockIdx.x >= plan.workers) {
-        if (tid == 0) a.splits[blockIdx.x].pieces = 0;
-        return;
-    }
-    // Blocks go to the 8 dies in turn, each with its own L2: a die gets a run of the
-    // line, whose neighbouring tiles read the same keys.
-    const uint32_t die = blockIdx.x & 7, of_die = plan.workers >> 3, more = plan.workers & 7;
-    const uint32_t worker = die * of_die + min(die, more) + (blockIdx.x >> 3);
-    const double from = scalar(plan.cut(worker)), to = scalar(plan.cut(worker + 1));
-    const int rg = wave % RG, kg = wave / RG, half = lane >> 5;
+    const int rg = wave % RG, kg = wave / RG, part = lane / W;
     const int group = a.group.d;
     if (tid == 0) found_lds = 0;  // the next barrier is before the first tile's
     Split left_over = {0, 0, 0, 0, 0, 0};
+    Plan plan = {};
+    Tile w = {};
+    double from = 0.0, to = 0.0;
+    uint32_t worker = 0;
 
-    for (Tile w = find_tile<BM, BN>(a, lanes, from);; next_tile<BM, BN>(a, w)) {
+    for (bool first = true;; first = false) {
+        if (first) {  // in the loop: what the compiler takes out of it comes before these loads' wait
+            const Lanes lanes = look<BM, BN>(a, 0);
+            plan = make_plan<BM, BN>(a, lanes);
+            if (blockIdx.x >= plan.workers) {
+                if (tid == 0) a.splits[blockIdx.x].pieces = 0;
+                return;
+            }
+            // Blocks go to the 8 dies in turn, each with its own L2: a die gets a run of
+            // the line, whose neighbouring tiles read the same keys.
+            const uint32_t die = blockIdx.x & 7, of_die = plan.workers >> 3, more = plan.workers & 7;
+            worker = die * of_die + min(die, more) + (blockIdx.x >> 3);
+            from = scalar(plan.cut(worker));
+            to = scalar(plan.cut(worker + 1));
+            w = find_tile<BM, BN>(a, lanes, from);
+        } else {
+            next_tile<BM, BN>(a, w);
+        }
         const int rows = w.count * group;
         const bool whole = w.begin >= from && w.end <= to;
         int kb, ke;  // this worker's keys of the tile
@@ -608,11 +670,35 @@ void paged_attention_kernel(const AttnArgs a) {
             kb = (b0 + k0) * BN;
             ke = k0 == k1 ? kb : (k1 == blocks ? hi : (b0 + k1) * BN);
         }
-        const int row0 = w.qt * BM + 32 * rg, row = row0 + (lane & 31);
+        // Loads go from memory straight to LDS, 16 bytes a lane and a wave's lanes side
+        // by side; the swizzle is in which unit of its row a lane fetches.  Lane i of a
+        // wave finds the place of key t + i, its page a tile ahead of its use; a load's
+        // lanes get their rows' places from it.  Keys past the piece's end, those of bad
+        // pages and columns past head_dim are zeros.
+        const int* const table = a.b.table + static_cast<long>(w.seq) * a.b.width;
+        int page = 0;
+        auto fetch_page = [&](int t) {
+            if (t < ke) page = table[a.b.page.div(min(t + lane, ke - 1))];
+        };
+        fetch_page(kb);
+        const uint16_t* const kbase = a.k + w.kvh * a.head_stride;
+        const uint16_t* const vbase = a.v + w.kvh * a.head_stride;
+        const int units = a.head_dim / 8;
+
+        const int row0 = w.qt * BM + W * rg, row = row0 + lane % W;
         const int tok = a.group.div(min(row, rows - 1));
         const int head = w.kvh * group + min(row, rows - 1) - tok * group;
-
-        RowState<T, HD, RG> r;
+        RowState<T, HD, BM> r;
+        {
+            const uint16_t* qp = a.q + static_cast<long>(w.first + tok) * a.q_stride +
+                                 static_cast<long>(head) * a.head_dim + 8 * part;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                r.q[s] = u32x4{0, 0, 0, 0};
+                if (row < rows && kDepth * s + 8 * part < a.head_dim)
+                    r.q[s] = *reinterpret_cast<const u32x4*>(qp + kDepth * s);
+            }
+        }
         r.see_lo = r.see_hi = r.all_lo = r.all_hi = r.any_lo = r.any_hi = 0;
         bool none = true;
         if (row < rows) {
@@ -622,7 +708,7 @@ void paged_attention_kernel(const AttnArgs a) {
             none = r.see_hi <= r.see_lo;
         }
         if (row0 < rows) {
-            const int t0 = a.group.div(row0), t1 = a.group.div(min(row0 + 31, rows - 1));
+            const int t0 = a.group.div(row0), t1 = a.group.div(min(row0 + W, rows) - 1);
             const int p0 = w.len - w.count + t0, p1 = w.len - w.count + t1;
             r.all_hi = a.causal ? min(p0 + 1, w.len) : w.len;
             r.any_hi = a.causal ? min(p1 + 1, w.len) : w.len;
@@ -635,20 +721,23 @@ void paged_attention_kernel(const AttnArgs a) {
         r.all_hi = min(r.all_hi, ke);
         r.any_lo = max(r.any_lo, kb);
         r.any_hi = min(r.any_hi, ke);
+        // keys that some rows of the tile see and others do not: [lo0, lo1) and [hi0, hi1)
+        int lo0, lo1, hi0, hi1;
+        {
+            const int t0 = a.group.div(w.qt * BM), t1 = a.group.div(min(w.qt * BM + BM, rows) - 1);
+            const int p0 = w.len - w.count + t0, p1 = w.len - w.count + t1;
+            hi0 = a.causal ? p0 + 1 : w.len;
+            hi1 = a.causal ? p1 + 1 : w.len;
+            lo0 = a.window ? p0 - a.window + 1 : 0;
+            lo1 = a.window ? p1 - a.window + 1 : 0;
+        }
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) r.o[c][i] = 0.0f;
+        r.m = -INFINITY;
+        r.l = 0.0f;
 
-        // Loads go from memory straight to LDS, 16 bytes a lane and a wave's lanes side
-        // by side; the swizzle is in which unit of its row a lane fetches.  Lane i of a
-        // wave finds the place of key t + i, its page a tile ahead of its use; a load's
-        // lanes get their rows' places from it.  Keys past the piece's end, those of bad
-        // pages and columns past head_dim are zeros.
-        const int* const table = a.b.table + static_cast<long>(w.seq) * a.b.width;
-        const uint16_t* const kbase = a.k + w.kvh * a.head_stride;
-        const uint16_t* const vbase = a.v + w.kvh * a.head_stride;
-        const int units = a.head_dim / 8;
-        int page = 0;
-        auto fetch_page = [&](int t) {
-            if (t < ke) page = table[a.b.page.div(min(t + lane, ke - 1))];
-        };
         // Where a page's slots come in whole runs of a load's rows, all rows of a load
         // have one place: a scalar base and a lane offset that stays the same.
         const bool runs = a.b.page.d % kRows == 0 && units == R::kUnits;
@@ -673,15 +762,15 @@ void paged_attention_kernel(const AttnArgs a) {
             const int key = row + lane / R::kUnits;
             const uint32_t ku = lane_row + 16 * R::k_unit(key, lane % R::kUnits);
             const uint32_t vu = lane_row + 16 * R::v_unit(key, lane % R::kUnits);
-            load_to_lds<RG <= 2>(reinterpret_cast<const char*>(kbase + off) + ku, buf + row * R::kPitch);
-            load_to_lds<RG <= 2>(reinterpret_cast<const char*>(vbase + off) + vu,
-                                 buf + (BN + row) * R::kPitch);
+            load_to_lds<S::kOnce>(reinterpret_cast<const char*>(kbase + off) + ku, buf + row * R::kPitch);
+            load_to_lds<S::kOnce>(reinterpret_cast<const char*>(vbase + off) + vu,
+                                  buf + (BN + row) * R::kPitch);
         };
         auto load_any = [&](uint8_t* buf) {  // the tile, any lengths, pages and head_dim
             int ln = lane;
             asm volatile("" : "+v"(ln));  // its numbers are not held in registers meanwhile
             const int at_lo = static_cast<int>(at), at_hi = static_cast<int>(at >> 32);
-#pragma unroll
+#pragma unroll 1
             for (int i = 0; i < kLoads; ++i) {
                 const int row = (i * S::kWaves + wave) * kRows;
                 const int key = row + ln / R::kUnits;
@@ -689,66 +778,43 @@ void paged_attention_kernel(const AttnArgs a) {
                 const long off = static_cast<long>(static_cast<uint64_t>(hi) << 32 | lo);
                 const int ku = R::k_unit(key, ln % R::kUnits), vu = R::v_unit(key, ln % R::kUnits);
                 const uint16_t* const zeros = reinterpret_cast<const uint16_t*>(kZeros);
-                load_to_lds<RG <= 2>(off < 0 || ku >= units ? zeros : kbase + off + 8 * ku,
-                                     buf + row * R::kPitch);
-                load_to_lds<RG <= 2>(off < 0 || vu >= units ? zeros : vbase + off + 8 * vu,
-                                     buf + (BN + row) * R::kPitch);
+                load_to_lds<S::kOnce>(off < 0 || ku >= units ? zeros : kbase + off + 8 * ku,
+                                      buf + row * R::kPitch);
+                load_to_lds<S::kOnce>(off < 0 || vu >= units ? zeros : vbase + off + 8 * vu,
+                                      buf + (BN + row) * R::kPitch);
             }
         };
-
-        fetch_page(kb);
         if (kb < ke) {
             place_tile(kb);
-            load_any(buf0);
             there = next;
-        }
-        fetch_page(kb + BN);
-        {
-            const uint16_t* qp = a.q + static_cast<long>(w.first + tok) * a.q_stride +
-                                 static_cast<long>(head) * a.head_dim + 8 * half;
+            if (easy) {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                r.q[s] = u32x4{0, 0, 0, 0};
-                if (row < rows && 16 * s + 8 * half < a.head_dim)
-                    r.q[s] = *reinterpret_cast<const u32x4*>(qp + 16 * s);
+                for (int i = 0; i < kLoads; ++i) load_part(i, buf0);
+            } else {
+                load_any(buf0);
             }
         }
-#pragma unroll
-        for (int c = 0; c < kCols; ++c)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) r.o[c][i] = 0.0f;
-        r.m = -INFINITY;
-        r.l = 0.0f;
-        // keys that some rows of the tile see and others do not: [lo0, lo1) and [hi0, hi1)
-        int lo0, lo1, hi0, hi1;
-        {
-            const int t0 = a.group.div(w.qt * BM), t1 = a.group.div(min(w.qt * BM + BM, rows) - 1);
-            const int p0 = w.len - w.count + t0, p1 = w.len - w.count + t1;
-            hi0 = a.causal ? p0 + 1 : w.len;
-            hi1 = a.causal ? p1 + 1 : w.len;
-            lo0 = a.window ? p0 - a.window + 1 : 0;
-            lo1 = a.window ? p1 - a.window + 1 : 0;
-        }
+        fetch_page(kb + BN);
+
         auto step = [&](int t, uint8_t* buf, uint8_t* other) {
             wait_loads();
             __syncthreads();
-            const bool more = t + BN < ke;
             bool spread = false;
-            if (more) {
+            if (t + BN < ke) {
                 place_tile(t + BN);
                 spread = easy;
                 if (!easy) load_any(other);
             }
             bool taken = false;
             if ((t < hi1 && t + BN > hi0 && hi0 < hi1) || (t < lo1 && t + BN > lo0 && lo0 < lo1))
-                taken = take_out<T, HD, RG>(buf, &found_lds);
-            attend<T, HD, RG>(a, r, buf, t, kg, there, [&](int i) {
+                taken = take_out<T, HD, BM>(buf, &found_lds);
+            attend<T, HD, BM>(a, r, buf, t, kg, there, [&](int i) {
                 if (spread)
 #pragma unroll
                     for (int k = 0; k < kLoads; ++k)
                         if (k * kBetween / kLoads == i) load_part(k, other);
             });
-            if (taken) put_back<T, HD, RG>(a, r, t, ke, kg, table, vbase);
+            if (taken) put_back<T, HD, BM>(a, r, t, ke, kg, table, vbase);
             fetch_page(t + 2 * BN);
             there = next;
         };
@@ -758,21 +824,21 @@ void paged_attention_kernel(const AttnArgs a) {
             step(t + BN, buf1, buf0);
         }
 
-        r.l = half_sum(r.l);
-        float* const part = partial<HD, BM>(a, 2 * worker + (w.begin >= from ? 1 : 0));
+        r.l = row_sum<W>(r.l);
+        float* const piece = partial<HD, BM>(a, 2 * worker + (w.begin >= from ? 1 : 0));
+        const int rt = W * rg + lane % W;  // the lane's row of the tile
         if (KG == 1) {
-            const int rt = 32 * rg + (lane & 31);
             if (row >= rows) {
             } else if (!whole) {
-                if (half == 0) {
-                    part[BM * HD + 2 * rt] = r.m;
-                    part[BM * HD + 2 * rt + 1] = r.l;
+                if (part == 0) {
+                    piece[BM * HD + 2 * rt] = r.m;
+                    piece[BM * HD + 2 * rt + 1] = r.l;
                 }
 #pragma unroll
                 for (int c = 0; c < kCols; ++c)
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4)
-                        *reinterpret_cast<float4*>(part + rt * HD + 32 * c + 8 * (i / 4) + 4 * half) =
+                    for (int i = 0; i < kEach; i += 4)
+                        *reinterpret_cast<float4*>(piece + rt * HD + r.column(c, i)) =
                             make_float4(r.o[c][i], r.o[c][i + 1], r.o[c][i + 2], r.o[c][i + 3]);
             } else {
                 const float inv = none ? 0.0f : 1.0f / r.l;
@@ -781,17 +847,16 @@ void paged_attention_kernel(const AttnArgs a) {
 #pragma unroll
                 for (int c = 0; c < kCols; ++c)
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const int d = 32 * c + 8 * (i / 4) + 4 * half;
+                    for (int i = 0; i < kEach; i += 4) {
+                        const int d = r.column(c, i);
                         if (d < a.head_dim)
                             store4<T>(op + d, r.o[c][i] * inv, r.o[c][i + 1] * inv,
                                       r.o[c][i + 2] * inv, r.o[c][i + 3] * inv);
                     }
             }
         } else {
-            // join the key groups: the references first, then the scaled sums through LDS
-            const int rt = 32 * rg + (lane & 31);
-            if (half == 0) {
+            // join the waves' keys: the references first, then the scaled sums through LDS
+            if (part == 0) {
                 ml_lds[kg][rt][0] = r.m;
                 ml_lds[kg][rt][1] = r.l;
             }
@@ -806,11 +871,10 @@ void paged_attention_kernel(const AttnArgs a) {
 #pragma unroll
                 for (int c = 0; c < kCols; ++c)
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const int d = 32 * c + 8 * (i / 4) + 4 * half;
-                        *reinterpret_cast<float4*>(obuf + (kg * BM + rt) * HD + d) = make_float4(
-                            r.o[c][i] * f, r.o[c][i + 1] * f, r.o[c][i + 2] * f, r.o[c][i + 3] * f);
-                    }
+                    for (int i = 0; i < kEach; i += 4)
+                        *reinterpret_cast<float4*>(obuf + (kg * BM + rt) * HD + r.column(c, i)) =
+                            make_float4(r.o[c][i] * f, r.o[c][i + 1] * f, r.o[c][i + 2] * f,
+                                        r.o[c][i + 3] * f);
             __syncthreads();
             for (int idx = tid; idx < left * (HD / 4); idx += S::kThreads) {
                 const int y = idx / (HD / 4), d = 4 * (idx % (HD / 4));
@@ -829,10 +893,10 @@ void paged_attention_kernel(const AttnArgs a) {
                     x.w += z.w;
                 }
                 if (!whole) {
-                    *reinterpret_cast<float4*>(part + y * HD + d) = x;
+                    *reinterpret_cast<float4*>(piece + y * HD + d) = x;
                     if (d == 0) {
-                        part[BM * HD + 2 * y] = tm;
-                        part[BM * HD + 2 * y + 1] = tl;
+                        piece[BM * HD + 2 * y] = tm;
+                        piece[BM * HD + 2 * y + 1] = tl;
                     }
                 } else if (d < a.head_dim) {
                     const int gr = w.qt * BM + y, tk = a.group.div(gr);
@@ -857,9 +921,8 @@ void paged_attention_kernel(const AttnArgs a) {
 // Joins the pieces of split tiles: block (worker in which the tile begins, rows).
 // HD / 4 threads take a row, 4 columns each; kSpread: they take every kGroups-th
 // piece of the block's one row, else all pieces of a row of their own.
-template <class T, int HD, int RG, bool kSpread>
+template <class T, int HD, int BM, bool kSpread>
 __global__ __launch_bounds__(kJoinBlock) void paged_attention_join_kernel(const AttnArgs a) {
-    constexpr int BM = Shape<RG>::BM;
     constexpr int kLanes = HD / 4, kGroups = kJoinBlock / kLanes;
     __shared__ float acc[kSpread ? kGroups : 1][HD + 2];
     const Split w = a.splits[blockIdx.x];
@@ -937,19 +1000,20 @@ int padded_dim(int hd) { return hd <= 64 ? 64 : (hd <= 96 ? 96 : (hd <= 128 ? 12
 size_t splits_bytes(int workers) { return (workers * sizeof(Split) + 255) / 256 * 256; }
 
 // A worker per resident block.
-template <int HD, int RG>
-int worker_count() { return device_cu_count() * resident<HD, RG>(); }
+template <int HD, int BM>
+int worker_count() { return device_cu_count() * resident<HD, BM>(); }
 
 // A worker has at most two tiles that it shares with others: its first and its last.
-template <int HD, int RG>
+template <int HD, int BM>
 size_t workspace_of() {
-    const size_t workers = worker_count<HD, RG>();
-    return splits_bytes(workers) + 2 * workers * Shape<RG>::BM * (HD + 2) * sizeof(float);
+    const size_t workers = worker_count<HD, BM>();
+    return splits_bytes(workers) + 2 * workers * BM * (HD + 2) * sizeof(float);
 }
 
 template <int HD>
 size_t workspace_of_any() {
-    return std::max(workspace_of<HD, 1>(), std::max(workspace_of<HD, 2>(), workspace_of<HD, 4>()));
+    return std::max({workspace_of<HD, 16>(), workspace_of<HD, 32>(), workspace_of<HD, 64>(),
+                     workspace_of<HD, 128>()});
 }
 
 size_t workspace_bytes(int hd) {
@@ -962,31 +1026,32 @@ size_t workspace_bytes(int hd) {
     }
 }
 
-template <class T, int HD, int RG>
+template <class T, int HD, int BM>
 int launch_attention(const char* fn, AttnArgs a, void* ws, int max_rows, hipStream_t st) {
-    typedef Shape<RG> S;
-    a.workers = worker_count<HD, RG>();
-    a.reach = static_cast<double>(a.window) + ((S::BM - 1) / a.group.d + 2);
-    a.per_worker = 32.0 / (static_cast<double>(S::kMinKeys) * a.group.d);
+    typedef Shape<BM> S;
+    a.workers = worker_count<HD, BM>();
+    a.reach = static_cast<double>(a.window) + ((BM - 1) / a.group.d + 2);
+    a.per_worker = 16.0 / (static_cast<double>(S::kMinKeys) * a.group.d);
     a.splits = static_cast<Split*>(ws);
     a.ws = reinterpret_cast<float*>(static_cast<char*>(ws) + splits_bytes(a.workers));
-    hipLaunchKernelGGL((paged_attention_kernel<T, HD, RG>), dim3(a.workers), dim3(S::kThreads), 0,
+    hipLaunchKernelGGL((paged_attention_kernel<T, HD, BM>), dim3(a.workers), dim3(S::kThreads), 0,
                        st, a);
     if (int e = launch_status(fn)) return e;
     // few rows may have many pieces: a row a block, its pieces side by side
-    constexpr bool kSpread = RG == 1;
+    constexpr bool kSpread = BM <= 32;
     constexpr int per = kSpread ? 1 : kJoinBlock / (HD / 4);
-    const int most = std::min(max_rows, S::BM);
-    hipLaunchKernelGGL((paged_attention_join_kernel<T, HD, RG, kSpread>),
+    const int most = std::min(max_rows, BM);
+    hipLaunchKernelGGL((paged_attention_join_kernel<T, HD, BM, kSpread>),
                        dim3(a.workers, (most + per - 1) / per), dim3(kJoinBlock), 0, st, a);
     return launch_status(fn);
 }
 
 template <class T, int HD>
 int pick_rows(const char* fn, const AttnArgs& a, void* ws, int max_rows, hipStream_t st) {
-    if (max_rows <= 32) return launch_attention<T, HD, 1>(fn, a, ws, max_rows, st);
-    if (max_rows <= 64) return launch_attention<T, HD, 2>(fn, a, ws, max_rows, st);
-    return launch_attention<T, HD, 4>(fn, a, ws, max_rows, st);
+    if (max_rows <= 16) return launch_attention<T, HD, 16>(fn, a, ws, max_rows, st);
+    if (max_rows <= 32) return launch_attention<T, HD, 32>(fn, a, ws, max_rows, st);
+    if (max_rows <= 64) return launch_attention<T, HD, 64>(fn, a, ws, max_rows, st);
+    return launch_attention<T, HD, 128>(fn, a, ws, max_rows, st);
 }
 
 int check_heads(const char* fn, int nh, int nkv, int hd) {
