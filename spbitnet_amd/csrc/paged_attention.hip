@@ -109,7 +109,7 @@ struct Shape {
     static constexpr int BN = kKeys * KG;
     static_assert(BN == kWave, "a lane per key of a tile");
     // Fewest keys worth a worker of their own.
-    static constexpr int kMinKeys = RG == 4 ? 256 : 64;
+    static constexpr int kMinKeys = RG == 4 ? 128 : 64;
     static constexpr bool kOnce = RG <= 2;  // keys are read once: not kept in L2
 };
 
@@ -552,18 +552,28 @@ __device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, BM>& r
 template <class T, int HD, int BM>
 __device__ __forceinline__ bool take_out(uint8_t* buf, int* found) {
     typedef Shape<BM> S;
-    constexpr int kAll = S::BN * Row<HD>::kUnits;
-    u32x4* const v = reinterpret_cast<u32x4*>(buf + S::BN * Row<HD>::kPitch);
-    for (int i = threadIdx.x; i < kAll; i += S::kThreads) {
-        u32x4 x = v[i];
-        if (non_finite<T>(x[0]) | non_finite<T>(x[1]) | non_finite<T>(x[2]) | non_finite<T>(x[3])) {
+    constexpr int kEach = S::BN * Row<HD>::kUnits / S::kThreads;
+    u32x4* const v = reinterpret_cast<u32x4*>(buf + S::BN * Row<HD>::kPitch) + threadIdx.x;
+    u32x4 x[kEach];
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) x[i] = v[i * S::kThreads];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+        any |= non_finite<T>(x[i][0]) | non_finite<T>(x[i][1]) | non_finite<T>(x[i][2]) |
+               non_finite<T>(x[i][3]);
+    if (any) {
+#pragma unroll 1
+        for (int i = 0; i < kEach; ++i) {
+            u32x4 y = v[i * S::kThreads];
+#pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint32_t bad = non_finite<T>(x[e]);
-                x[e] &= (bad & 0x8000u ? 0u : 0x0000FFFFu) | (bad >> 31 ? 0u : 0xFFFF0000u);
+                const uint32_t bad = non_finite<T>(y[e]);
+                y[e] &= (bad & 0x8000u ? 0u : 0x0000FFFFu) | (bad >> 31 ? 0u : 0xFFFF0000u);
             }
-            v[i] = x;
-            *found = 1;
+            v[i * S::kThreads] = y;
         }
+        *found = 1;
     }
     __syncthreads();
     return *found != 0;
@@ -606,10 +616,8 @@ __device__ __align__(16) const uint32_t kZeros[4] = {0, 0, 0, 0};
 // Blocks of a CU that LDS and registers hold.
 template <int HD, int BM>
 constexpr int resident() { return HD > 128 ? 1 : (BM <= 64 && HD <= 64 ? 4 : 2); }
-// Registers for two waves on a SIMD up to 128 columns, also where one is resident: with
-// more of them the compiler keeps O in accumulation registers, which costs moves.
 template <int HD, int BM>
-constexpr int waves_per_simd() { return HD <= 128 ? 2 : 1; }
+constexpr int waves_per_simd() { return Shape<BM>::kWaves * resident<HD, BM>() >= 8 ? 2 : 1; }
 
 template <class T, int HD, int BM>
 __global__ __launch_bounds__((Shape<BM>::kThreads), (waves_per_simd<HD, BM>()))
@@ -627,10 +635,6 @@ void paged_attention_kernel(const AttnArgs a) {
     __shared__ float ml_lds[KG][BM][2];
     __shared__ int found_lds;  // take_out's
 
-    // The arguments' lines, fetched together: a small call has a microsecond for each
-    // that would be waited for by itself.
-    asm volatile("" ::"s"(a.b.starts), "s"(a.b.seqs), "s"(a.q), "s"(a.k), "s"(a.out), "s"(a.q_stride),
-                 "s"(a.slot_stride), "s"(a.c), "s"(a.reach), "s"(a.workers), "s"(a.ws));
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = scalar(tid / kWave);
     const int rg = wave % RG, kg = wave / RG, part = lane / W;
     const int group = a.group.d;
