@@ -453,7 +453,8 @@ typedef struct spb_paged_cache {
  * sequence, and their rows of every output stay as they were.  Positions past
  * table_width * page_size do not exist (kv_lens is clamped to them; append
  * skips them).  max_new: the most tokens a sequence has, or 0 if not known
- * (it selects a kernel; a wrong one costs time only).  num_seqs <= 65536. */
+ * (it selects among the attention's kernels, whose results differ by
+ * roundings; a wrong one costs time).  num_seqs <= 65536. */
 typedef struct spb_paged_batch {
     const int* token_starts;
     const int* kv_lens;

@@ -92,8 +92,8 @@ struct AttnArgs {
     double reach;
     double per_worker;  // 1 / the least cost worth a worker
     uint32_t workers;   // at most, = blocks launched
-    Split* splits;     // [workers]
-    float* ws;         // partial results, 2 per worker
+    Split* splits;      // [workers]
+    float* ws;          // partial results, 2 per worker
 };
 
 // A tile of BM rows: a wave takes W of them, 32, or 16 where the tile has no more (a
@@ -108,9 +108,14 @@ struct Shape {
     static constexpr int kWaves = RG * KG, kThreads = kWave * kWaves;
     static constexpr int BN = kKeys * KG;
     static_assert(BN == kWave, "a lane per key of a tile");
-    // Fewest keys worth a worker of their own.
+    // Fewest keys worth a worker of their own.  us with 32 / 64 / 128 / 256: one token
+    // behind 2048 15.7 / 14.2 / 15.6 / 17.5, 9 sequences of up to 5 tokens 23.1 / 19.2 /
+    // 22.3 / 26.3; at 128 rows, 128 / 256 / 512: 256 tokens 24.4 / 29.1 / 43.6, 2048
+    // behind 8192 242 / 239 / 241.
     static constexpr int kMinKeys = RG == 4 ? 128 : 64;
-    static constexpr bool kOnce = RG <= 2;  // keys are read once: not kept in L2
+    // Few tiles read the same keys: non-temporal, as they need not stay in L2 (32 ragged
+    // sequences of one token 75.8 -> 68.5 us; where many tiles do, 250 -> 313).
+    static constexpr bool kOnce = RG <= 2;
 };
 
 // A product's result in a wave: W x W, element i of lane l is column l % W and row
@@ -619,6 +624,19 @@ constexpr int resident() { return HD > 128 ? 1 : (BM <= 64 && HD <= 64 ? 4 : 2);
 template <int HD, int BM>
 constexpr int waves_per_simd() { return Shape<BM>::kWaves * resident<HD, BM>() >= 8 ? 2 : 1; }
 
+// What bounds it.  Decoding: memory, K and V being read once.  One sequence of 131,072
+// positions (336 MB) takes 65.6 us with the join, 5.1 TB/s, 32 ragged ones (363 MB)
+// 68.6, 5.3 TB/s; a large copy reaches 4.9.  Many rows: 2048 tokens behind 8192 (193
+// GFLOP) take 234 us, 0.83 PFLOP/s, where a large library product reaches 1.22.  By
+// counters the matrix units are busy 40 % of the time and the vector units 45 %, by
+// time stamps a wave's 64 keys take 1400 cycles for the scores, 900 for the softmax,
+// 1200 for the values and 1000 for the next keys' places, waits and barriers, and the
+// two waves of a SIMD overlap little.  Small calls: a chain of dependent steps, about
+// 14,000 cycles (lengths, the cut, pages, keys, one tile, the join of two waves).
+// Not kept: K and V staged in registers (spills, whose reloads wait in order behind
+// the loads: 444 us for the same 2048 tokens); two sets of 32 rows in a wave with K
+// and V read once for both (512 registers, 150 spilled: 609 us); raised priorities
+// around the products or the softmax (250.6 and 246 against 250).
 template <class T, int HD, int BM>
 __global__ __launch_bounds__((Shape<BM>::kThreads), (waves_per_simd<HD, BM>()))
 void paged_attention_kernel(const AttnArgs a) {
@@ -744,7 +762,8 @@ void paged_attention_kernel(const AttnArgs a) {
 
         // Where a page's slots come in whole runs of a load's rows, all rows of a load
         // have one place: a scalar base and a lane offset that stays the same.
-        const bool runs = a.b.page.d % kRows == 0 && units == R::kUnits;
+        const bool runs = a.b.page.d % kRows == 0 && units == R::kUnits &&
+                          a.slot_stride < (1L << 24);  // the offset is 32 bits
         const uint32_t lane_row = (lane / R::kUnits) * static_cast<uint32_t>(a.slot_stride) * 2;
         uint64_t there = ~uint64_t{0}, next = ~uint64_t{0};
         long at = 0;

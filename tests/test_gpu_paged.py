@@ -636,3 +636,69 @@ def test_two_streams_with_their_own_workspaces(gpu):
     torch.cuda.synchronize()
     for b, q, want, out, ws, st in parts:
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_mixed_batches(gpu, seed):
+    """Decoding sequences beside chunks, empty ones and ones shorter than their new
+    tokens, over head counts, widths, page sizes and windows."""
+    import random
+    r = random.Random(seed)
+    kind = r.choice(["f16", "bf16"])
+    nkv = r.choice([1, 2, 3, 5])
+    nh = nkv * r.choice([1, 2, 4, 7, 16, 17])
+    hd = r.choice([16, 64, 80, 96, 120, 128, 160, 192, 256])
+    page = r.choice([1, 4, 8, 16, 20, 33, 64, 512])
+    n = r.choice([1, 3, 10, 64, 65, 130])
+    if n >= 64:  # the float64 reference goes head by head
+        nh = nkv * r.choice([1, 2])
+    seqs = []
+    for _ in range(n):
+        new = r.choice([0, 1, 1, 1, 2, 5, r.randint(1, 60 if n < 20 else 9)])
+        seqs.append((new, r.choice([0, 1, new, new + r.randint(0, 100), r.randint(0, 1200)])))
+    if n < 20 and r.random() < 0.7:
+        seqs[r.randrange(n)] = (r.randint(50, 300), r.randint(300, 1500))
+    if sum(x for x, _ in seqs) == 0:
+        seqs[0] = (1, 5)
+    b = R.Batch(seqs, page, nkv, hd, HALF[kind], seed=seed, padding=r.choice([0, 2]),
+                extra_width=r.choice([0, 5]), token_major=r.random() < 0.3)
+    q = _randn(b.rows, nh, hd, dtype=HALF[kind], seed=seed, std=r.choice([0.5, 2.0]))
+    _attend(b, q, causal=r.random() < 0.8, window=r.choice([0, 0, 1, 37, 500]),
+            max_new=r.choice([0, max(x for x, _ in seqs)]), stale=math.nan)
+
+
+def test_more_sequences_than_a_wave_beside_a_chunk(gpu):
+    """150 sequences, a chunk among them, so that the search passes 64 and 128."""
+    seqs = [(1, 10 + 5 * s) for s in range(150)]
+    seqs[100] = (90, 700)
+    seqs[149] = (70, 70)
+    b = R.Batch(seqs, 16, 2, 128, torch.bfloat16, seed=3)
+    q = _randn(b.rows, 8, 128, dtype=torch.bfloat16, seed=4)
+    _attend(b, q, stale=math.nan)
+    _attend(b, q, window=64)
+
+
+def test_long_ragged_decode_splits(gpu):
+    """Lengths from one to tens of thousands in one call: pieces of every kind."""
+    seqs = [(1, n) for n in (1, 40000, 63, 64, 65, 30000, 2, 129, 12345, 7)]
+    for kind in ("f16", "bf16"):
+        b = R.Batch(seqs, 64, 2, 64, HALF[kind], seed=5)
+        q = _randn(b.rows, 8, 64, dtype=HALF[kind], seed=6)
+        _attend(b, q, max_new=1)
+        _attend(b, q, window=5000, max_new=1)
+
+
+def test_rows_of_a_load_far_apart(gpu):
+    """A slot stride past 2^24 elements: the rows of one load have 64-bit offsets."""
+    K = _k()
+    slot = (1 << 24) + 64
+    store = [torch.zeros(8 * slot + 64, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    k, v = (t.as_strided((3, 1, 8, 64), (64 * 8, 64 * 8 * 3, slot, 1)) for t in store)
+    b = R.Batch([(1, 20)], 8, 1, 64, torch.bfloat16, seed=5, spare=0)
+    k.copy_(b.k)
+    v.copy_(b.v)
+    q = _randn(1, 2, 64, dtype=torch.bfloat16, seed=6)
+    want, out = _attend(b, q), torch.empty_like(q)
+    K.paged_attention_gpu(K.PagedKVCache(k, v), K.PagedBatch(b.starts, b.lens, b.table, 1), q, out,
+                          _workspace(2, 1, 64))
+    assert torch.equal(out, want)
