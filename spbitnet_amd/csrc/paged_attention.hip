@@ -96,10 +96,13 @@ struct AttnArgs {
     float* ws;          // partial results, 2 per worker
 };
 
-// A tile of BM rows: a wave takes W of them, 32, or 16 where the tile has no more (a
-// decoding step: half the arithmetic and registers).  The waves of 64 and 128 rows
-// walk over the same keys; a single wave of rows gets a second one, and the two take
-// turns at 32 keys and join their results at the end.
+// A tile of BM = 16 or 128 rows.  Four waves of 32 rows walk over the same keys; the
+// 16 of a decoding step (half the arithmetic and registers of 32) are two waves' that
+// take turns at 32 keys and join their results at the end.  Tiles of 32 and 64 rows,
+// of two waves, were no faster than those of 128 (us, 4 sequences of 8 and 16 tokens,
+// 8 heads on 2, 2000 to 4000 positions: 64 wide 23.4 against 18.3 and 26.3 against
+// 23.1, 128 wide 27.1 against 25.5 and 39.3 against 29.2, 256 wide 63.3 against 48.9
+// and 77.6 against 52.9).
 template <int BM>
 struct Shape {
     static constexpr int W = BM < 32 ? BM : 32;
@@ -108,14 +111,6 @@ struct Shape {
     static constexpr int kWaves = RG * KG, kThreads = kWave * kWaves;
     static constexpr int BN = kKeys * KG;
     static_assert(BN == kWave, "a lane per key of a tile");
-    // Fewest keys worth a worker of their own.  us with 32 / 64 / 128 / 256: one token
-    // behind 2048 15.7 / 14.2 / 15.6 / 17.5, 9 sequences of up to 5 tokens 23.1 / 19.2 /
-    // 22.3 / 26.3; at 128 rows, 128 / 256 / 512: 256 tokens 24.4 / 29.1 / 43.6, 2048
-    // behind 8192 242 / 239 / 241.
-    static constexpr int kMinKeys = RG == 4 ? 128 : 64;
-    // Few tiles read the same keys: non-temporal, as they need not stay in L2 (32 ragged
-    // sequences of one token 75.8 -> 68.5 us; where many tiles do, 250 -> 313).
-    static constexpr bool kOnce = RG <= 2;
 };
 
 // A product's result in a wave: W x W, element i of lane l is column l % W and row
@@ -337,11 +332,11 @@ struct Row {
 };
 
 // 16 bytes of each active lane from memory to LDS, at lds + 16 lane.
-template <bool kOnce>  // non-temporal
+template <bool kStream>  // kStream: non-temporal
 __device__ __forceinline__ void load_to_lds(const void* from, uint8_t* lds) {
     __builtin_amdgcn_global_load_lds(
         (const __attribute__((address_space(1))) void*)from,
-        (__attribute__((address_space(3))) void*)lds, 16, 0, kOnce ? 2 : 0);
+        (__attribute__((address_space(3))) void*)lds, 16, 0, kStream ? 2 : 0);
 }
 // All of this wave's loads have arrived.
 __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }
@@ -445,7 +440,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, BM>& r
     const uint8_t* const kw = buf + kKeys * kg * R::kPitch;
     const uint8_t* const vw = kw + Shape<BM>::BN * R::kPitch;
     const int lane = threadIdx.x & (kWave - 1), part = lane / W;
-    // Reads of LDS go out a group ahead of the products that use them: left to itself
+    // Reads of LDS go out two groups ahead of the products that use them: left to itself
     // the compiler puts each right before its use, whose wait then shows.
     acc s[kTiles];
     constexpr int kGroup = kSteps % 2 ? 1 : 2, kGroups = kSteps / kGroup;  // steps
@@ -459,9 +454,9 @@ __device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, BM>& r
                     kw + R::k_at(W * n + lane % W, kDepth / 8 * (g * kGroup + st) + part));
     };
     load_k(0);
+    if (kGroups > 1) load_k(1);
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-        if (g + 1 < kGroups) load_k(g + 1);
         if (g < kBetween) between(g);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -470,6 +465,8 @@ __device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, BM>& r
             for (int n = 0; n < kTiles; ++n)
                 s[n] = P::mfma(k[g & 1][st][n], r.q[g * kGroup + st],
                                g + st == 0 ? acc{} : s[n]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (g + 2 < kGroups) load_k(g + 2);
     }
 #pragma unroll
     for (int g = kGroups; g < kBetween; ++g) between(g);
@@ -526,6 +523,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, BM>& r
     }
     const float ref = r.m == -INFINITY ? 0.0f : r.m;  // a row that has seen nothing yet
     load_v(0, v[0]);
+    if (kKeys > kDepth) load_v(1, v[1]);
     __builtin_amdgcn_sched_barrier(0);
     constexpr int kParts = kKeys / kDepth;  // 8 probabilities of a lane each
     u32x4 pf[kParts];
@@ -543,10 +541,10 @@ __device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, BM>& r
     // O^T += V^T P^T
 #pragma unroll
     for (int g = 0; g < kParts; ++g) {
-        if (g + 1 < kParts) load_v(g + 1, v[(g + 1) & 1]);
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < kCols; ++c) r.o[c] = P::mfma(v[g & 1][c], pf[g], r.o[c]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (g + 2 < kParts) load_v(g + 2, v[g & 1]);
     }
 }
 
@@ -620,15 +618,20 @@ __device__ __align__(16) const uint32_t kZeros[4] = {0, 0, 0, 0};
 
 // Blocks of a CU that LDS and registers hold.
 template <int HD, int BM>
-constexpr int resident() { return HD > 128 ? 1 : (BM <= 64 && HD <= 64 ? 4 : 2); }
+constexpr int resident() { return HD > 128 ? 1 : (BM == 16 && HD <= 64 ? 4 : 2); }
 template <int HD, int BM>
 constexpr int waves_per_simd() { return Shape<BM>::kWaves * resident<HD, BM>() >= 8 ? 2 : 1; }
 
+// Tiles of 16 rows are a sequence's only ones: no two read the same keys, which are
+// loaded non-temporal (32 ragged sequences of one token 75.8 -> 68.5 us).  With 128 rows
+// others may read them too (2048 tokens 250 -> 313 us), and one tile of 20 to 64 rows
+// gains nothing either (9 sequences of 5 tokens 18.1 against 17.9).
+//
 // What bounds it.  Decoding: memory, K and V being read once.  One sequence of 131,072
 // positions (336 MB) takes 65.6 us with the join, 5.1 TB/s, 32 ragged ones (363 MB)
 // 68.6, 5.3 TB/s; a large copy reaches 4.9.  Many rows: 2048 tokens behind 8192 (193
-// GFLOP) take 234 us, 0.83 PFLOP/s, where a large library product reaches 1.22.  By
-// counters the matrix units are busy 40 % of the time and the vector units 45 %, by
+// GFLOP) take 240 us, 0.80 PFLOP/s, where a large library product reaches 1.22.  By
+// counters the matrix units are busy 44 % of the time and the vector units 50 %, by
 // time stamps a wave's 64 keys take 1400 cycles for the scores, 900 for the softmax,
 // 1200 for the values and 1000 for the next keys' places, waits and barriers, and the
 // two waves of a SIMD overlap little.  Small calls: a chain of dependent steps, about
@@ -672,7 +675,8 @@ void paged_attention_kernel(const AttnArgs a) {
                 return;
             }
             // Blocks go to the 8 dies in turn, each with its own L2: a die gets a run of
-            // the line, whose neighbouring tiles read the same keys.
+            // the line, whose neighbouring tiles read the same keys (2048 tokens behind 8192
+            // 243 us; dies interleaved every 1, 4, 8, 16 or 32 workers 255, 250, 259, 254, 248).
             const uint32_t die = blockIdx.x & 7, of_die = plan.workers >> 3, more = plan.workers & 7;
             worker = die * of_die + min(die, more) + (blockIdx.x >> 3);
             from = scalar(plan.cut(worker));
@@ -785,8 +789,8 @@ void paged_attention_kernel(const AttnArgs a) {
             const int key = row + lane / R::kUnits;
             const uint32_t ku = lane_row + 16 * R::k_unit(key, lane % R::kUnits);
             const uint32_t vu = lane_row + 16 * R::v_unit(key, lane % R::kUnits);
-            load_to_lds<S::kOnce>(reinterpret_cast<const char*>(kbase + off) + ku, buf + row * R::kPitch);
-            load_to_lds<S::kOnce>(reinterpret_cast<const char*>(vbase + off) + vu,
+            load_to_lds<BM == 16>(reinterpret_cast<const char*>(kbase + off) + ku, buf + row * R::kPitch);
+            load_to_lds<BM == 16>(reinterpret_cast<const char*>(vbase + off) + vu,
                                   buf + (BN + row) * R::kPitch);
         };
         auto load_any = [&](uint8_t* buf) {  // the tile, any lengths, pages and head_dim
@@ -801,9 +805,9 @@ void paged_attention_kernel(const AttnArgs a) {
                 const long off = static_cast<long>(static_cast<uint64_t>(hi) << 32 | lo);
                 const int ku = R::k_unit(key, ln % R::kUnits), vu = R::v_unit(key, ln % R::kUnits);
                 const uint16_t* const zeros = reinterpret_cast<const uint16_t*>(kZeros);
-                load_to_lds<S::kOnce>(off < 0 || ku >= units ? zeros : kbase + off + 8 * ku,
+                load_to_lds<BM == 16>(off < 0 || ku >= units ? zeros : kbase + off + 8 * ku,
                                       buf + row * R::kPitch);
-                load_to_lds<S::kOnce>(off < 0 || vu >= units ? zeros : vbase + off + 8 * vu,
+                load_to_lds<BM == 16>(off < 0 || vu >= units ? zeros : vbase + off + 8 * vu,
                                       buf + (BN + row) * R::kPitch);
             }
         };
@@ -1035,8 +1039,7 @@ size_t workspace_of() {
 
 template <int HD>
 size_t workspace_of_any() {
-    return std::max({workspace_of<HD, 16>(), workspace_of<HD, 32>(), workspace_of<HD, 64>(),
-                     workspace_of<HD, 128>()});
+    return std::max(workspace_of<HD, 16>(), workspace_of<HD, 128>());
 }
 
 size_t workspace_bytes(int hd) {
@@ -1052,16 +1055,22 @@ size_t workspace_bytes(int hd) {
 template <class T, int HD, int BM>
 int launch_attention(const char* fn, AttnArgs a, void* ws, int max_rows, hipStream_t st) {
     typedef Shape<BM> S;
+    // Fewest keys worth a worker of their own.  us with 32 / 64 / 128 / 256 for one token
+    // behind 2048: 15.7 / 14.2 / 15.6 / 17.5.  For 128 rows with 64 / 128: 4 sequences of 8
+    // tokens (8 heads on 2, 2000 to 4000 positions) 33.7 / 26.6 at 128 wide, 22.8 / 18.7 at
+    // 64; 9 of 5 tokens in a window of 1000 16.2 / 18.2; with 128 / 256 / 512: 256 tokens
+    // 24.4 / 29.1 / 43.6, 2048 behind 8192 242 / 239 / 241.
+    constexpr int kMinKeys = BM == 16 ? 64 : 128;
     a.workers = worker_count<HD, BM>();
     a.reach = static_cast<double>(a.window) + ((BM - 1) / a.group.d + 2);
-    a.per_worker = 16.0 / (static_cast<double>(S::kMinKeys) * a.group.d);
+    a.per_worker = 16.0 / (static_cast<double>(kMinKeys) * a.group.d);
     a.splits = static_cast<Split*>(ws);
     a.ws = reinterpret_cast<float*>(static_cast<char*>(ws) + splits_bytes(a.workers));
-    hipLaunchKernelGGL((paged_attention_kernel<T, HD, BM>), dim3(a.workers), dim3(S::kThreads), 0,
-                       st, a);
+    hipLaunchKernelGGL((paged_attention_kernel<T, HD, BM>), dim3(a.workers),
+                       dim3(S::kThreads), 0, st, a);
     if (int e = launch_status(fn)) return e;
     // few rows may have many pieces: a row a block, its pieces side by side
-    constexpr bool kSpread = BM <= 32;
+    constexpr bool kSpread = BM == 16;
     constexpr int per = kSpread ? 1 : kJoinBlock / (HD / 4);
     const int most = std::min(max_rows, BM);
     hipLaunchKernelGGL((paged_attention_join_kernel<T, HD, BM, kSpread>),
@@ -1072,8 +1081,6 @@ int launch_attention(const char* fn, AttnArgs a, void* ws, int max_rows, hipStre
 template <class T, int HD>
 int pick_rows(const char* fn, const AttnArgs& a, void* ws, int max_rows, hipStream_t st) {
     if (max_rows <= 16) return launch_attention<T, HD, 16>(fn, a, ws, max_rows, st);
-    if (max_rows <= 32) return launch_attention<T, HD, 32>(fn, a, ws, max_rows, st);
-    if (max_rows <= 64) return launch_attention<T, HD, 64>(fn, a, ws, max_rows, st);
     return launch_attention<T, HD, 128>(fn, a, ws, max_rows, st);
 }
 
