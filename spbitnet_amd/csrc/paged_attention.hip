@@ -632,9 +632,9 @@ constexpr int waves_per_simd() { return Shape<BM>::kWaves * resident<HD, BM>() >
 // 68.6, 5.3 TB/s; a large copy reaches 4.9.  Many rows: 2048 tokens behind 8192 (193
 // GFLOP) take 240 us, 0.80 PFLOP/s, where a large library product reaches 1.22.  By
 // counters the matrix units are busy 44 % of the time and the vector units 50 %, by
-// time stamps (before LDS was read two groups ahead) a wave's 64 keys took 1400 cycles for the scores, 900 for the softmax,
-// 1200 for the values and 1000 for the next keys' places, waits and barriers, and the
-// two waves of a SIMD overlap little.  Small calls: a chain of dependent steps, about
+// time stamps (before LDS was read two groups ahead) a wave's 64 keys took 1400 cycles
+// for the scores, 900 for the softmax, 1200 for the values and 1000 for the next keys'
+// places, waits and barriers, and the two waves of a SIMD overlap little.  Small calls: a chain of dependent steps, about
 // 14,000 cycles (lengths, the cut, pages, keys, one tile, the join of two waves).
 // Not kept: K and V staged in registers (spills, whose reloads wait in order behind
 // the loads: 444 us for the same 2048 tokens); two sets of 32 rows in a wave with K
