@@ -548,10 +548,11 @@ __device__ __forceinline__ void attend(const AttnArgs& a, RowState<T, HD, BM>& r
     }
 }
 
-// Keys that some rows of a tile see and others do not must not have inf or NaN in V:
-// the product of a probability of 0 with them would reach the rows that do not see
-// them.  Replaces them by 0 in LDS and says whether there were any (here or in an
-// earlier tile).  All threads call it.
+// Keys of a loaded block that some rows of a tile do not see must not have inf or NaN
+// in V: the product of a probability of 0 with them would reach those rows.  So in the
+// blocks where the tile's rows differ, and in the one in which a window begins, whose
+// first keys no row may see.  Replaces them by 0 in LDS and says whether there were any
+// (here or in an earlier tile).  All threads call it.
 template <class T, int HD, int BM>
 __device__ __forceinline__ bool take_out(uint8_t* buf, int* found) {
     typedef Shape<BM> S;
@@ -747,7 +748,9 @@ void paged_attention_kernel(const AttnArgs a) {
         r.all_hi = min(r.all_hi, ke);
         r.any_lo = max(r.any_lo, kb);
         r.any_hi = min(r.any_hi, ke);
-        // keys that some rows of the tile see and others do not: [lo0, lo1) and [hi0, hi1)
+        // where the rows' keys begin and end: from lo0 (the tile's first row) to lo1 (its
+        // last), the same for a single token, and hi0 to hi1.  Keys from hi1 on are zeros
+        // (ke), those before lo0 are not: a tile's first block begins at a multiple of BN.
         int lo0, lo1, hi0, hi1;
         {
             const int t0 = a.group.div(w.qt * BM), t1 = a.group.div(min(w.qt * BM + BM, rows) - 1);
@@ -833,7 +836,7 @@ void paged_attention_kernel(const AttnArgs a) {
                 if (!easy) load_any(other);
             }
             bool taken = false;
-            if ((t < hi1 && t + BN > hi0 && hi0 < hi1) || (t < lo1 && t + BN > lo0 && lo0 < lo1))
+            if ((t < hi1 && t + BN > hi0 && hi0 < hi1) || (t < lo1 && t + BN > lo0))
                 taken = take_out<T, HD, BM>(buf, &found_lds);
             attend<T, HD, BM>(a, r, buf, t, kg, there, [&](int i) {
                 if (spread)

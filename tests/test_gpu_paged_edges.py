@@ -1,0 +1,54 @@
+"""GPU checks of the paged operators at the edges of what a call may hold: what
+lies before a window, and arguments at the ends of their ranges.  Tolerances are
+those of tests/paged64.py; everything else is compared bit for bit."""
+import math
+
+import pytest
+import torch
+
+from tests import paged64 as R
+from tests.test_gpu_paged import _attend, _k, _randn, _workspace
+
+pytestmark = pytest.mark.gpu
+
+HALF = R.HALF
+
+# seqs, heads, kv heads, window, max_new: every sequence's window begins inside a
+# block of 64 keys
+BEHIND = {
+    "decode": ([(1, 90), (1, 500), (1, 33)], 4, 2, 30, 1),
+    "decode, pieces": ([(1, 6000), (1, 5100)], 4, 2, 5000, 1),
+    "17 heads on one": ([(1, 500), (1, 2077)], 17, 1, 1000, 1),
+    "130 heads on one": ([(3, 300)], 130, 1, 70, 3),
+    "decode beside a chunk": ([(1, 1000), (40, 900), (1, 400)], 4, 2, 333, 0),
+    "chunk, pieces": ([(1, 4000), (150, 5000)], 2, 1, 3000, 0),
+    "drafts": ([(5, 700), (2, 400), (1, 260)], 8, 2, 100, 5),
+}
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 80, 128, 256])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("case", BEHIND)
+def test_what_lies_before_the_window_has_no_effect(gpu, kind, hd, causal, case):
+    """Positions that no row of a sequence sees hold inf and NaN: the same bits as
+    with finite ones, in tiles of one token and of several, whole and cut."""
+    K = _k()
+    seqs, nh, nkv, window, max_new = BEHIND[case]
+    assert all(0 < (n - new - window + 1) % 64 for new, n in seqs if n - new >= window)
+    b = R.Batch(seqs, 16, nkv, hd, HALF[kind], seed=hd)
+    q = _randn(b.rows, nh, hd, dtype=HALF[kind], seed=7)
+    clean = _attend(b, q, causal, window, max_new=max_new)
+    batch = K.PagedBatch(b.starts, b.lens, b.table, b.rows, max_new=max_new)
+    ws = _workspace(nh, nkv, hd)
+    for bad in (math.nan, math.inf, -math.inf):
+        for s, (new, n) in enumerate(seqs):
+            j = torch.arange(max(0, n - new - window + 1))
+            page = b.host_table[s].long()[j // 16].cuda()
+            b.k[page, :, (j % 16).cuda()] = bad
+            b.v[page, :, (j % 16).cuda()] = bad
+        out = torch.empty_like(q)
+        K.paged_attention_gpu(K.PagedKVCache(b.k, b.v), batch, q, out, ws, causal=causal,
+                              window=window)
+        same = torch.equal(out, clean)
+        assert same, bad
