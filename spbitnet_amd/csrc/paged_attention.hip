@@ -292,6 +292,13 @@ __device__ __forceinline__ void next_tile(const AttnArgs& a, Tile& t) {
     t.end = scalar(t.end + (t.c0 + t.c1 * t.qt));
 }
 
+// The first key that a query at a position sees, from 0 on.  A position may be negative
+// (fewer cached positions than new tokens) and the window anything up to 2^31 - 1, so
+// they are compared before one is taken from the other.
+__device__ __forceinline__ int first_seen(const AttnArgs& a, int pos) {
+    return a.window && pos >= a.window ? pos - a.window + 1 : 0;
+}
+
 // Keys that the tile's rows see: [lo, hi).
 template <int BM>
 __device__ __forceinline__ void tile_range(const AttnArgs& a, const Tile& t, int& lo, int& hi) {
@@ -299,7 +306,7 @@ __device__ __forceinline__ void tile_range(const AttnArgs& a, const Tile& t, int
     const int i0 = a.group.div(t.qt * BM), i1 = a.group.div(min(t.qt * BM + BM, rows) - 1);
     const int p0 = t.len - t.count + i0, p1 = t.len - t.count + i1;
     hi = a.causal ? min(p1 + 1, t.len) : t.len;
-    lo = a.window ? max(p0 - a.window + 1, 0) : 0;
+    lo = first_seen(a, p0);
     if (hi < lo) hi = lo;
 }
 
@@ -345,7 +352,7 @@ __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70
 __device__ __forceinline__ bool row_sees(const AttnArgs& a, int count, int len, int i) {
     const int pos = len - count + i;
     const int hi = a.causal ? min(pos + 1, len) : len;
-    return hi > (a.window ? max(pos - a.window + 1, 0) : 0);
+    return hi > first_seen(a, pos);
 }
 
 // Two exchanges of lanes l and l ^ 32, l and l ^ 16: both lanes' values in both.
@@ -731,7 +738,7 @@ void paged_attention_kernel(const AttnArgs a) {
         if (row < rows) {
             const int pos = w.len - w.count + tok;
             r.see_hi = a.causal ? min(pos + 1, w.len) : w.len;
-            r.see_lo = a.window ? max(pos - a.window + 1, 0) : 0;
+            r.see_lo = first_seen(a, pos);
             none = r.see_hi <= r.see_lo;
         }
         if (row0 < rows) {
@@ -739,8 +746,8 @@ void paged_attention_kernel(const AttnArgs a) {
             const int p0 = w.len - w.count + t0, p1 = w.len - w.count + t1;
             r.all_hi = a.causal ? min(p0 + 1, w.len) : w.len;
             r.any_hi = a.causal ? min(p1 + 1, w.len) : w.len;
-            r.all_lo = a.window ? max(p1 - a.window + 1, 0) : 0;
-            r.any_lo = a.window ? max(p0 - a.window + 1, 0) : 0;
+            r.all_lo = first_seen(a, p1);
+            r.any_lo = first_seen(a, p0);
         }
         r.see_lo = max(r.see_lo, kb);
         r.see_hi = min(r.see_hi, ke);
@@ -757,8 +764,8 @@ void paged_attention_kernel(const AttnArgs a) {
             const int p0 = w.len - w.count + t0, p1 = w.len - w.count + t1;
             hi0 = a.causal ? p0 + 1 : w.len;
             hi1 = a.causal ? p1 + 1 : w.len;
-            lo0 = a.window ? p0 - a.window + 1 : 0;
-            lo1 = a.window ? p1 - a.window + 1 : 0;
+            lo0 = first_seen(a, p0);
+            lo1 = first_seen(a, p1);
         }
 #pragma unroll
         for (int c = 0; c < kCols; ++c)

@@ -52,3 +52,17 @@ def test_what_lies_before_the_window_has_no_effect(gpu, kind, hd, causal, case):
                               window=window)
         same = torch.equal(out, clean)
         assert same, bad
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 25])
+@pytest.mark.parametrize("max_new", [0, 1])
+def test_windows_up_to_the_largest_int(gpu, kind, causal, window, max_new):
+    """No position is before them, also where a sequence has fewer positions than new
+    tokens (its first ones are negative: -23 - (2^31 - 1) + 1 does not fit in 32 bits)."""
+    b = R.Batch([(40, 17), (3, 0), (1, 90), (200, 150)], 16, 2, 64, HALF[kind], seed=3, padding=1)
+    q = _randn(b.rows, 4, 64, dtype=HALF[kind], seed=4)
+    out = _attend(b, q, causal, window, max_new=max_new)
+    same = torch.equal(out, _attend(b, q, causal, 0, max_new=max_new))
+    assert same
