@@ -71,8 +71,10 @@ __device__ __forceinline__ Place find_place(const HeadsArgs& a, int t) {
         if (hit == 0) continue;
         const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
         const int first = __shfl(q.first, l, kWave), count = __shfl(q.count, l, kWave);
-        // the position comes from the length as it is given: one past the table has no slot
-        const int pos = a.batch.lens[base + l] - count + (t - first);
+        // The position comes from the length as it is given: one past the table has no slot.
+        // A negative length is one of 0, whose tokens' positions are negative as well: near
+        // -2^31 the difference would not fit in 32 bits.
+        const int pos = max(a.batch.lens[base + l], 0) - count + (t - first);
         r.pos = pos;
         if (pos >= 0 && pos < a.batch.capacity) {
             const int p = a.batch.page.div(pos);

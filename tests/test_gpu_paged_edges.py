@@ -66,3 +66,25 @@ def test_windows_up_to_the_largest_int(gpu, kind, causal, window, max_new):
     out = _attend(b, q, causal, window, max_new=max_new)
     same = torch.equal(out, _attend(b, q, causal, 0, max_new=max_new))
     assert same
+
+
+@pytest.mark.parametrize("length", [-1, -2 ** 31 + 2, -2 ** 31])
+def test_append_skips_sequences_of_negative_length(gpu, length):
+    """Their positions are negative, however far the length is below 0: keys, values and
+    queries are left out.  (A length of 2^31 - 1 is past the table: the query is rotated,
+    key and value have no slot.)"""
+    K = _k()
+    b = R.Batch([(3, 20), (2, 9)], 16, 2, 64, torch.bfloat16, seed=6)
+    k, v = (_randn(5, 2, 64, dtype=torch.bfloat16, seed=s) for s in (1, 2))
+    q = _randn(5, 4, 64, dtype=torch.bfloat16, seed=3)
+    kp, vp = b.k.clone(), b.v.clone()
+    for n, first in ((length, 7.0), (2 ** 31 - 1, None)):
+        lens = torch.tensor([n, 9], dtype=torch.int32).cuda()
+        qo = torch.full_like(q, 7.0)
+        K.paged_append_gpu(K.PagedKVCache(b.k, b.v), K.PagedBatch(b.starts, lens, b.table, 5), k, v,
+                           q=q, q_output=qo)
+        page = int(b.host_table[1, 0])
+        kp[page, :, 7:9], vp[page, :, 7:9] = k[3:].transpose(0, 1), v[3:].transpose(0, 1)
+        assert torch.equal(b.k, kp) and torch.equal(b.v, vp)
+        assert torch.equal(qo[3:], q[3:])
+        assert torch.equal(qo[:3], q[:3] if first is None else torch.full_like(q[:3], first))
