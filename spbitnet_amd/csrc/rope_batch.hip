@@ -443,13 +443,14 @@ int paged_append(const char* fn, const spb_paged_cache* c, const spb_paged_batch
     if (int e = check_paged_batch(fn, b)) return e;
     if (int e = check_rope(fn, rope, c->head_dim)) return e;
     if (nh < 0) return invalid("%s: negative number of heads", fn);
+    if (!(eps >= 0.0f)) return invalid("%s: eps must not be negative", fn);
+    // before the pointers: those of empty tensors are null
+    if (b->num_tokens == 0 || b->num_seqs == 0) return 0;
     if ((k == nullptr) != (v == nullptr)) return invalid("%s: k and v come together", fn);
     if ((q == nullptr) != (qo == nullptr)) return invalid("%s: q and q_output come together", fn);
     if (!k && !q) return invalid("%s: neither keys nor queries", fn);
     if (q && nh < 1) return invalid("%s: queries need num_heads >= 1", fn);
     if ((qw && !q) || (kw && !k)) return invalid("%s: a weight without its heads", fn);
-    if (!(eps >= 0.0f)) return invalid("%s: eps must not be negative", fn);
-    if (b->num_tokens == 0 || b->num_seqs == 0) return 0;
     HeadsArgs a = {};
     const int nkv = c->num_kv_heads, hd = c->head_dim;
     if (q) a.span[0] = {q, qo, qs, qos, qw, nh, rope != nullptr};

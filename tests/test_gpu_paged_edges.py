@@ -88,3 +88,28 @@ def test_append_skips_sequences_of_negative_length(gpu, length):
         assert torch.equal(b.k, kp) and torch.equal(b.v, vp)
         assert torch.equal(qo[3:], q[3:])
         assert torch.equal(qo[:3], q[:3] if first is None else torch.full_like(q[:3], first))
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("seqs", [0, 3])
+def test_batches_without_tokens(gpu, kind, seqs):
+    """Every operator on a batch of no tokens, as a serving loop may have one."""
+    K = _k()
+    dt, nh, nkv, hd = HALF[kind], 4, 2, 64
+    k, v = (_randn(5, nkv, 16, hd, dtype=dt, seed=s) for s in (1, 2))
+    kp, vp = k.clone(), v.clone()
+    q, x = (torch.empty(0, h, hd, dtype=dt, device="cuda") for h in (nh, nkv))
+    w = torch.ones(hd, device="cuda")
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    rope = K.Rope.scaled(hd)
+    cache = K.PagedKVCache(k, v)
+    batch = K.PagedBatch(torch.zeros(seqs + 1, dtype=torch.int32, device="cuda"),
+                         torch.full((seqs,), 9, dtype=torch.int32, device="cuda"),
+                         torch.zeros(seqs, 1, dtype=torch.int32, device="cuda"), 0)
+    K.rope_tokens_gpu(q, q, none, rope)
+    K.qk_norm_rope_gpu(q, x, q, x, w, w, none, rope)
+    K.paged_append_gpu(cache, batch, x, x)
+    K.paged_append_gpu(cache, batch, x, x, rope=rope, q=q, q_output=q, q_weight=w, k_weight=w)
+    K.paged_append_gpu(cache, batch, None, None, rope=rope, q=q, q_output=q)
+    K.paged_attention_gpu(cache, batch, q, q, _workspace(nh, nkv, hd))
+    assert torch.equal(k, kp) and torch.equal(v, vp)

@@ -232,3 +232,17 @@ def test_python_refuses_host_tensors_and_wrong_types():
         K.PagedBatch(torch.zeros(3, dtype=torch.int32), i, i[:, None], 4)
     with pytest.raises(ValueError, match="vector"):
         K.PagedBatch(None, None, None, 4)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("size", [dict(num_tokens=0), dict(num_tokens=0, num_seqs=0)])
+def test_batches_without_tokens_have_no_pointers(lib, kind, size):
+    """An empty tensor's pointer is null: nothing to do, whatever else is asked for."""
+    fn = getattr(lib, f"spb_paged_append_{kind}")
+    batch = _batch(**size, token_starts=None, kv_lens=None, page_table=None)
+
+    def call(**rope):
+        return fn(ctypes.byref(_cache()), ctypes.byref(batch), None, None, None, None, 256, 256, 512,
+                  512, 4, A, A, ctypes.c_float(1e-5), ctypes.byref(_rope(**rope)), None)
+    assert call() == 0
+    _said(lib, call(rotary_dim=130), "rotary_dim")
