@@ -20,6 +20,9 @@ namespace {
 constexpr int kHeadBlock = 256;
 constexpr int kMaxTile = 2;      // tokens of a block
 constexpr int kMaxHalf = 128;    // pairs of the widest head
+// A launch holds less than 2^32 lanes, 2^24 blocks of them; a block's items (its
+// tokens' heads) and a step of them stay far below 2^31.
+constexpr int kMaxTokens = 1 << 24, kMaxHeads = 1 << 24;
 
 // A run of heads of the batch's tokens: head h of token t at
 // src + t * src_stride + h * head_dim.
@@ -351,6 +354,9 @@ void pick_heads(const HeadsArgs& a, int tile, bool norm, bool paged, bool past, 
 template <class T>
 int run_heads(const char* fn, HeadsArgs& a, const spb_rope* rope, bool paged, spb_stream_t stream) {
     const int rot = rope ? rope->rotary_dim : 0, hd = a.head_dim;
+    if (a.tokens > kMaxTokens) return invalid("%s: more than %d tokens", fn, kMaxTokens);
+    if (static_cast<long>(a.span[0].heads) + a.span[1].heads + a.span[2].heads > kMaxHeads)
+        return invalid("%s: more than %d heads", fn, kMaxHeads);
     a.half = rot / 2;
     a.interleaved = rope ? rope->interleaved != 0 : 1;
     a.scale = rope ? rope->scale : 1.0f;

@@ -113,3 +113,25 @@ def test_batches_without_tokens(gpu, kind, seqs):
     K.paged_append_gpu(cache, batch, None, None, rope=rope, q=q, q_output=q)
     K.paged_attention_gpu(cache, batch, q, q, _workspace(nh, nkv, hd))
     assert torch.equal(k, kp) and torch.equal(v, vp)
+
+
+def test_the_most_tokens_of_a_rotation(gpu):
+    """2^24 tokens (one head of 4), and that many heads of one token: the first and last
+    rows against a call of their own, all against float64."""
+    K = _k()
+    n, f = 1 << 24, K.rope_inv_freq(4)[0]
+    rope = K.Rope(f)
+    x = torch.randn(n, 1, 4, device="cuda").to(torch.float16)
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    y = torch.full_like(x, 7.0)
+    K.rope_tokens_gpu(x, y, pos, rope)
+    for rows in (slice(0, 5), slice(n - 5, n)):
+        z = torch.full_like(x[rows], 7.0)
+        K.rope_tokens_gpu(x[rows], z, pos[rows], rope)
+        assert torch.equal(z, y[rows])
+    R.check_rotated(y, x.double(), R.rotate(x.double(), pos, f.cuda(), 1.0, True), f.cuda(), 1.0, True)
+    heads = x.view(1, n, 4)
+    z = torch.full_like(heads, 7.0)
+    K.rope_tokens_gpu(heads, z, pos[3:4], rope)
+    R.check_rotated(z, heads.double(), R.rotate(heads.double(), pos[3:4], f.cuda(), 1.0, True),
+                    f.cuda(), 1.0, True)
