@@ -451,7 +451,13 @@ class Rope:
         return Rope(f, scale, interleaved)
 
 
-def _same_device(x, name: str, dev: int) -> None:
+def _check(x, kind, name: str) -> None:
+    if not isinstance(x, kind):
+        raise TypeError(f"{name} must be a {kind.__name__}, not {type(x).__name__}")
+
+
+def _same_device(x, kind, name: str, dev: int) -> None:
+    _check(x, kind, name)
     if x._dev != dev:
         raise ValueError(f"{name} is on cuda:{x._dev}, the tensors are on cuda:{dev}")
 
@@ -469,7 +475,7 @@ def rope_tokens_gpu(x, output, positions, rope: Rope, stream=None):
     py, sy = _heads(output, "output", dt, shape, dev)
     n, heads, hd = shape
     pp = _flat(positions, "positions", torch.int32, (n,), dev)
-    _same_device(rope, "rope", dev)
+    _same_device(rope, Rope, "rope", dev)
     L = _lib.load()
     fn = L.spb_rope_tokens_f16 if kind == "f16" else L.spb_rope_tokens_bf16
     _lib.check(fn(px, py, pp, rope._ptr, n, heads, hd, sx, sy, _on(stream, dev)),
@@ -498,7 +504,7 @@ def qk_norm_rope_gpu(q, k, q_output, k_output, q_weight, k_weight, positions,
     pp = pr = None
     if rope is not None:
         pp = _flat(positions, "positions", torch.int32, (n,), dev)
-        _same_device(rope, "rope", dev)
+        _same_device(rope, Rope, "rope", dev)
         pr = rope._ptr
     L = _lib.load()
     fn = L.spb_qk_norm_rope_f16 if kind == "f16" else L.spb_qk_norm_rope_bf16
@@ -564,9 +570,10 @@ def paged_append_gpu(cache: PagedKVCache, batch: PagedBatch, k, v, rope: Optiona
     [tokens][heads][head_dim] is given, rotates it into q_output (which may be q)
     in the same launch.  q_weight / k_weight (float32 [head_dim]): RMSNorm before
     the rotation (spb_paged_append_*)."""
-    n, hd, dt = batch.num_tokens, cache.head_dim, cache.dtype
+    _check(cache, PagedKVCache, "cache")
     dev = _device(cache.k, "the cache")
-    _same_device(batch, "batch", dev)
+    _same_device(batch, PagedBatch, "batch", dev)
+    n, hd, dt = batch.num_tokens, cache.head_dim, cache.dtype
     pk = pv = pq = pqo = pqw = pkw = pr = None
     sk = sv = sq = sqo = nh = 0
     if k is not None or v is not None:
@@ -584,7 +591,7 @@ def paged_append_gpu(cache: PagedKVCache, batch: PagedBatch, k, v, rope: Optiona
     if k_weight is not None:
         pkw = _flat(k_weight, "k_weight", torch.float32, (hd,), dev)
     if rope is not None:
-        _same_device(rope, "rope", dev)
+        _same_device(rope, Rope, "rope", dev)
         pr = rope._ptr
     L = _lib.load()
     fn = L.spb_paged_append_f16 if cache.kind == "f16" else L.spb_paged_append_bf16
@@ -608,9 +615,10 @@ def paged_attention_gpu(cache: PagedKVCache, batch: PagedBatch, q, output, works
     when causal, j > p - window when window > 0, and the whole cached length
     otherwise.  scale None: head_dim ** -0.5.  workspace: a contiguous uint8 GPU
     tensor of paged_attention_workspace_size bytes (spb_paged_attention_*)."""
-    hd, dt = cache.head_dim, cache.dtype
+    _check(cache, PagedKVCache, "cache")
     dev = _device(cache.k, "the cache")
-    _same_device(batch, "batch", dev)
+    _same_device(batch, PagedBatch, "batch", dev)
+    hd, dt = cache.head_dim, cache.dtype
     _kind(q, "q")
     nh = q.shape[1] if q.dim() == 3 else 0
     shape = (batch.num_tokens, nh, hd)

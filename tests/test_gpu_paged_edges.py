@@ -135,3 +135,28 @@ def test_the_most_tokens_of_a_rotation(gpu):
     K.rope_tokens_gpu(heads, z, pos[3:4], rope)
     R.check_rotated(z, heads.double(), R.rotate(heads.double(), pos[3:4], f.cuda(), 1.0, True),
                     f.cuda(), 1.0, True)
+
+
+def test_what_is_no_descriptor_is_refused(gpu):
+    K = _k()
+    b = R.Batch([(2, 9)], 16, 2, 64, torch.float16)
+    q, x = (_randn(2, h, 64, dtype=torch.float16, seed=h) for h in (4, 2))
+    w, pos = torch.ones(64, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    rope, cache = K.Rope.scaled(64), K.PagedKVCache(b.k, b.v)
+    batch, ws = K.PagedBatch(b.starts, b.lens, b.table, 2), _workspace(4, 2, 64)
+    for bad in (None, 1.0, cache):
+        with pytest.raises(TypeError, match="rope must be a Rope"):
+            K.rope_tokens_gpu(q, q, pos, bad)
+    with pytest.raises(TypeError, match="rope must be a Rope"):
+        K.qk_norm_rope_gpu(q, x, q, x, w, w, pos, batch)
+    with pytest.raises(TypeError, match="rope must be a Rope"):
+        K.paged_append_gpu(cache, batch, x, x, rope=rope.inv_freq)
+    for bad in (None, rope):
+        with pytest.raises(TypeError, match="batch must be a PagedBatch"):
+            K.paged_append_gpu(cache, bad, x, x)
+        with pytest.raises(TypeError, match="batch must be a PagedBatch"):
+            K.paged_attention_gpu(cache, bad, q, q, ws)
+        with pytest.raises(TypeError, match="cache must be a PagedKVCache"):
+            K.paged_append_gpu(bad, batch, x, x)
+        with pytest.raises(TypeError, match="cache must be a PagedKVCache"):
+            K.paged_attention_gpu(bad, batch, q, q, ws)

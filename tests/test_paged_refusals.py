@@ -278,3 +278,11 @@ def test_more_heads_than_a_block_counts(lib, kind, nh, nkv):
         _said(lib, getattr(lib, f"spb_paged_append_{kind}")(
             ctypes.byref(_cache(num_kv_heads=nkv)), ctypes.byref(_batch()), A, A, A, A, wide, wide,
             wide, wide, nh, None, None, ctypes.c_float(0), None, None), "heads")
+
+
+def test_python_refuses_what_is_no_cache():
+    for bad in (None, torch.zeros(1), {}):
+        with pytest.raises(TypeError, match="cache must be a PagedKVCache"):
+            K.paged_append_gpu(bad, None, None, None)
+        with pytest.raises(TypeError, match="cache must be a PagedKVCache"):
+            K.paged_attention_gpu(bad, None, None, None, None)
