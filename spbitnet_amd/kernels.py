@@ -346,6 +346,20 @@ _ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 
 _Tensor = torch.Tensor
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_INT_MAX = 2 ** 31 - 1
+
+
+# ctypes passes the low 32 bits of what is longer, so numbers are looked at before.
+
+def _int32(x, name: str):
+    if not -_INT_MAX <= x <= _INT_MAX:
+        raise ValueError(f"{name} {x} does not fit in 32 bits")
+    return x
+
+
+def _sizes(shape, name: str) -> None:
+    if max(shape, default=0) > _INT_MAX:
+        raise ValueError(f"{name} has shape {tuple(shape)}, which does not fit in 32 bits")
 
 
 def _device(t, name: str) -> int:
@@ -414,12 +428,14 @@ def rope_inv_freq(rotary_dim: int, theta: float = 10000.0, scaling: str = "none"
     (spb_rope_inv_freq)."""
     if scaling not in _ROPE_SCALING:
         raise ValueError(f"scaling must be one of {sorted(_ROPE_SCALING)}, not {scaling!r}")
+    rotary_dim = _int32(int(rotary_dim), "rotary_dim")
+    original_positions = _int32(int(original_positions), "original_positions")
     out = torch.empty(max(rotary_dim // 2, 1), dtype=torch.float64)
     scale = ctypes.c_float()
     _lib.check(_lib.load().spb_rope_inv_freq(out.data_ptr(), ctypes.addressof(scale),
-                                             int(rotary_dim), float(theta),
+                                             rotary_dim, float(theta),
                                              _ROPE_SCALING[scaling], float(factor),
-                                             int(original_positions), float(beta_fast),
+                                             original_positions, float(beta_fast),
                                              float(beta_slow)), "rope_inv_freq")
     return out, scale.value
 
@@ -470,6 +486,7 @@ def rope_tokens_gpu(x, output, positions, rope: Rope, stream=None):
     shape, dt = x.shape, x.dtype
     if len(shape) != 3:
         raise ValueError("x must be [tokens][heads][head_dim]")
+    _sizes(shape, "x")
     dev = _device(x, "x")
     px, sx = _heads(x, "x", dt, shape, dev)
     py, sy = _heads(output, "output", dt, shape, dev)
@@ -494,6 +511,8 @@ def qk_norm_rope_gpu(q, k, q_output, k_output, q_weight, k_weight, positions,
     if len(qs) != 3 or len(ks) != 3 or ks[0] != qs[0] or ks[2] != qs[2]:
         raise ValueError("q and k must be [tokens][heads][head_dim] with the same tokens and "
                          "head_dim")
+    _sizes(qs, "q")
+    _sizes(ks, "k")
     n, nh, hd = qs
     pq, sq = _heads(q, "q", dt, qs, dev)
     pk, sk = _heads(k, "k", dt, ks, dev)
@@ -525,6 +544,7 @@ class PagedKVCache:
             raise TypeError(f"v is {v.dtype} on {v.device}, expected {k.dtype} on {k.device}")
         if k.dim() != 4 or v.shape != k.shape:
             raise ValueError("k and v must be [pages][kv heads][page_size][head_dim]")
+        _sizes(k.shape, "each of k and v")
         if k.stride() != v.stride() or k.stride(3) != 1:
             raise ValueError("k and v must have the same strides and a contiguous last dimension")
         self.k, self.v, self.dtype = k, v, k.dtype
@@ -549,12 +569,15 @@ class PagedBatch:
             raise ValueError("kv_lens must be a vector")
         if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
             raise ValueError("page_table must be [sequences][width]")
+        _sizes(kv_lens.shape, "kv_lens")
+        _sizes(page_table.shape, "page_table")
         n, width = kv_lens.numel(), page_table.shape[1]
+        num_tokens, max_new = _int32(int(num_tokens), "num_tokens"), _int32(int(max_new), "max_new")
         if num_tokens < 0 or max_new < 0:
             raise ValueError("negative number of tokens")
         self._dev = dev = _device(kv_lens, "kv_lens")
         self.token_starts, self.kv_lens, self.page_table = token_starts, kv_lens, page_table
-        self.num_seqs, self.num_tokens, self.max_new = n, int(num_tokens), int(max_new)
+        self.num_seqs, self.num_tokens, self.max_new = n, num_tokens, max_new
         self._c = _lib.PagedBatchC(_flat(token_starts, "token_starts", torch.int32, (n + 1,), dev),
                                    _flat(kv_lens, "kv_lens", torch.int32, (n,), dev),
                                    _flat(page_table, "page_table", torch.int32, (n, width), dev),
@@ -582,6 +605,7 @@ def paged_append_gpu(cache: PagedKVCache, batch: PagedBatch, k, v, rope: Optiona
         pv, sv = _heads(v, "v", dt, shape, dev)
     if q is not None or q_output is not None:
         _kind(q, "q")
+        _sizes(q.shape, "q")
         nh = q.shape[1] if q.dim() == 3 else 0
         shape = (n, nh, hd)
         pq, sq = _heads(q, "q", dt, shape, dev)
@@ -601,7 +625,9 @@ def paged_append_gpu(cache: PagedKVCache, batch: PagedBatch, k, v, rope: Optiona
 
 def paged_attention_workspace_size(num_heads: int, num_kv_heads: int, head_dim: int) -> int:
     """Bytes of the workspace that paged_attention_gpu needs for these heads."""
-    n = int(_lib.load().spb_paged_attention_workspace_size(num_heads, num_kv_heads, head_dim))
+    n = int(_lib.load().spb_paged_attention_workspace_size(
+        _int32(num_heads, "num_heads"), _int32(num_kv_heads, "num_kv_heads"),
+        _int32(head_dim, "head_dim")))
     if n == 0:
         _lib.check(1, "paged_attention_workspace_size")
     return n
@@ -620,8 +646,10 @@ def paged_attention_gpu(cache: PagedKVCache, batch: PagedBatch, q, output, works
     _same_device(batch, PagedBatch, "batch", dev)
     hd, dt = cache.head_dim, cache.dtype
     _kind(q, "q")
+    _sizes(q.shape, "q")
     nh = q.shape[1] if q.dim() == 3 else 0
     shape = (batch.num_tokens, nh, hd)
+    window = _int32(window, "window")
     pq, sq = _heads(q, "q", dt, shape, dev)
     po, so = _heads(output, "output", dt, shape, dev)
     size = workspace.numel() if isinstance(workspace, _Tensor) else 0

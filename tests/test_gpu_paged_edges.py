@@ -1,6 +1,7 @@
 """GPU checks of the paged operators at the edges of what a call may hold: what
 lies before a window, and arguments at the ends of their ranges.  Tolerances are
 those of tests/paged64.py; everything else is compared bit for bit."""
+import ctypes
 import math
 
 import pytest
@@ -160,3 +161,54 @@ def test_what_is_no_descriptor_is_refused(gpu):
             K.paged_append_gpu(bad, batch, x, x)
         with pytest.raises(TypeError, match="cache must be a PagedKVCache"):
             K.paged_attention_gpu(bad, batch, q, q, ws)
+
+
+@pytest.mark.parametrize("far", [2 ** 32 + 5, 2 ** 31, -2 ** 32 + 5])
+def test_numbers_past_32_bits_are_refused(gpu, far):
+    """ctypes cuts them to 32 bits without a word: a window of 2^32 + 5 would be one of 5."""
+    K = _k()
+    b = R.Batch([(2, 9)], 16, 2, 64, torch.float16)
+    q = _randn(2, 4, 64, dtype=torch.float16, seed=1)
+    cache, batch, ws = K.PagedKVCache(b.k, b.v), K.PagedBatch(b.starts, b.lens, b.table, 2), _workspace(4, 2, 64)
+    with pytest.raises(ValueError, match="window"):
+        K.paged_attention_gpu(cache, batch, q, q, ws, window=far)
+    with pytest.raises(ctypes.ArgumentError):
+        K.paged_attention_gpu(cache, batch, q, q, ws, window=5.5)
+    with pytest.raises(ValueError, match="num_tokens"):
+        K.PagedBatch(b.starts, b.lens, b.table, far)
+    with pytest.raises(ValueError, match="max_new"):
+        K.PagedBatch(b.starts, b.lens, b.table, 2, max_new=far)
+
+
+def test_shapes_past_32_bits_are_refused(gpu):
+    """Views of one element: nothing is read or written."""
+    K = _k()
+    n = 2 ** 32 + 1
+    one = torch.zeros(1, 1, 64, dtype=torch.float16, device="cuda")
+    w, pos = torch.ones(64, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    rope = K.Rope.scaled(64)
+    for x in (one.expand(n, 1, 64), one.expand(1, n, 64)):
+        p = pos.expand(x.shape[0])
+        with pytest.raises(ValueError, match="x has shape"):
+            K.rope_tokens_gpu(x, x, p, rope)
+        with pytest.raises(ValueError, match="q has shape"):
+            K.qk_norm_rope_gpu(x, one.expand(x.shape[0], 1, 64), x, one, w, w, p, rope)
+    with pytest.raises(ValueError, match="k has shape"):
+        K.qk_norm_rope_gpu(one, one.expand(1, n, 64), one, one, w, w, pos, rope)
+    for at in range(3):
+        shape = [1, 1, 1, 64]
+        shape[at] = n
+        big = one.view(1, 1, 1, 64).expand(shape)
+        with pytest.raises(ValueError, match="k and v has shape"):
+            K.PagedKVCache(big, big)
+    b = R.Batch([(1, 9)], 16, 1, 64, torch.float16)
+    cache, batch, ws = K.PagedKVCache(b.k, b.v), K.PagedBatch(b.starts, b.lens, b.table, 1), _workspace(1, 1, 64)
+    q = one.expand(1, n, 64)
+    with pytest.raises(ValueError, match="q has shape"):
+        K.paged_append_gpu(cache, batch, one, one, q=q, q_output=q)
+    with pytest.raises(ValueError, match="q has shape"):
+        K.paged_attention_gpu(cache, batch, q, q, ws)
+    with pytest.raises(ValueError, match="page_table has shape"):
+        K.PagedBatch(b.starts, b.lens, b.table[:, :1].expand(1, n), 1)
+    with pytest.raises(ValueError, match="kv_lens has shape"):
+        K.PagedBatch(b.starts, b.lens.expand(n), b.table.expand(n, 1), 1)

@@ -286,3 +286,18 @@ def test_python_refuses_what_is_no_cache():
             K.paged_append_gpu(bad, None, None, None)
         with pytest.raises(TypeError, match="cache must be a PagedKVCache"):
             K.paged_attention_gpu(bad, None, None, None, None)
+
+
+@pytest.mark.parametrize("far", [2 ** 32 + 64, 2 ** 31, -2 ** 32 + 64, 2 ** 64 + 64])
+def test_python_refuses_numbers_past_32_bits(far):
+    """ctypes cuts them to 32 bits without a word: 2^32 + 64 would be 64."""
+    with pytest.raises(ValueError, match="rotary_dim"):
+        K.rope_inv_freq(far)
+    with pytest.raises(ValueError, match="original_positions"):
+        K.rope_inv_freq(64, scaling="yarn", factor=2.0, original_positions=far)
+    with pytest.raises(ValueError, match="num_heads"):
+        K.paged_attention_workspace_size(far, 1, 64)
+    with pytest.raises(ValueError, match="num_kv_heads"):
+        K.paged_attention_workspace_size(64, far, 64)
+    with pytest.raises(ValueError, match="head_dim"):
+        K.paged_attention_workspace_size(64, 1, far)
