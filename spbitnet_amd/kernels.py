@@ -440,7 +440,23 @@ def rope_inv_freq(rotary_dim: int, theta: float = 10000.0, scaling: str = "none"
     return out, scale.value
 
 
-class Rope:
+class _Descriptor:
+    """What a call passes on as a C struct of pointers and sizes, taken once.  Its
+    attributes hold the tensors and say the sizes that the calls check others against;
+    one set afterwards would free the memory behind a pointer or let a smaller tensor
+    pass, so that is refused."""
+
+    def __setattr__(self, name, value):
+        if "_ptr" in self.__dict__:  # set last
+            raise AttributeError(f"a {type(self).__name__} cannot be changed: make another "
+                                 "(the contents of its tensors may be)")
+        object.__setattr__(self, name, value)
+
+    def __delattr__(self, name):
+        raise AttributeError(f"a {type(self).__name__} cannot be changed")
+
+
+class Rope(_Descriptor):
     """A rotation (spb_rope): inv_freq, float64 radians per position of each pair
     (rotary_dim / 2 of them, moved to the GPU if they are not there), the factor
     of the rotated pairs and their layout: pairs (2i, 2i + 1) when interleaved,
@@ -531,7 +547,7 @@ def qk_norm_rope_gpu(q, k, q_output, k_output, q_weight, k_weight, positions,
                   _on(stream, dev)), "qk_norm_rope_gpu")
 
 
-class PagedKVCache:
+class PagedKVCache(_Descriptor):
     """A pool of pages (spb_paged_cache) in two tensors k and v
     [pages][kv heads][page_size][head_dim] (fp16 or bf16) of equal strides; the
     last dimension is contiguous, so pages laid out [page_size][kv heads][head_dim]
@@ -556,13 +572,14 @@ class PagedKVCache:
         self._ptr = ctypes.addressof(self._c)
 
 
-class PagedBatch:
+class PagedBatch(_Descriptor):
     """A batch of new tokens (spb_paged_batch): int32 GPU tensors token_starts
     [sequences + 1], kv_lens [sequences] and page_table [sequences][width];
     num_tokens rows in the token tensors (those past token_starts' last entry are
     padding); max_new, the most new tokens of a sequence, if the program knows it.
     The tensors are read by the calls, so a program may refill them between
-    calls (and between replays of a captured one)."""
+    calls (and between replays of a captured one); the object itself is fixed, as are
+    a Rope and a PagedKVCache."""
 
     def __init__(self, token_starts, kv_lens, page_table, num_tokens: int, max_new: int = 0):
         if not isinstance(kv_lens, torch.Tensor) or kv_lens.dim() != 1:

@@ -212,3 +212,20 @@ def test_shapes_past_32_bits_are_refused(gpu):
         K.PagedBatch(b.starts, b.lens, b.table[:, :1].expand(1, n), 1)
     with pytest.raises(ValueError, match="kv_lens has shape"):
         K.PagedBatch(b.starts, b.lens.expand(n), b.table.expand(n, 1), 1)
+
+
+def test_descriptors_are_fixed(gpu):
+    """Their C structs keep the first tensors' pointers and sizes."""
+    K = _k()
+    b = R.Batch([(2, 9)], 16, 2, 64, torch.float16)
+    for x, names in ((K.Rope.scaled(64), ("inv_freq", "scale", "interleaved", "rotary_dim")),
+                     (K.PagedKVCache(b.k, b.v), ("k", "v", "head_dim", "num_kv_heads", "dtype")),
+                     (K.PagedBatch(b.starts, b.lens, b.table, 2),
+                      ("token_starts", "kv_lens", "page_table", "num_tokens", "max_new", "other"))):
+        for name in names:
+            before = getattr(x, name, None)
+            with pytest.raises(AttributeError, match="cannot be changed"):
+                setattr(x, name, 1)
+            assert getattr(x, name, None) is before
+            with pytest.raises(AttributeError, match="cannot be changed"):
+                delattr(x, name)
