@@ -229,3 +229,66 @@ def test_descriptors_are_fixed(gpu):
             assert getattr(x, name, None) is before
             with pytest.raises(AttributeError, match="cannot be changed"):
                 delattr(x, name)
+
+
+def test_thousands_of_sequences(gpu):
+    """3000 short ones, empty ones among them, and a chunk near the end: every search
+    over them goes on past many groups of 64."""
+    K = _k()
+    seqs = [((1, 2, 0)[s % 3], 2 + s % 37) for s in range(3000)]
+    seqs[2900] = (150, 400)
+    b = R.Batch(seqs, 16, 1, 64, torch.float16, seed=8, padding=2)
+    q = _randn(b.rows, 2, 64, dtype=torch.float16, seed=9)
+    _attend(b, q, max_new=150)
+    _attend(b, q, window=5, max_new=2)
+    x = _randn(b.rows, 2, 64, dtype=torch.float16, seed=10)
+    kp, vp = b.k.clone(), b.v.clone()
+    K.paged_append_gpu(K.PagedKVCache(b.k, b.v), K.PagedBatch(b.starts, b.lens, b.table, b.rows),
+                       x[:, :1], x[:, 1:])
+    pos = torch.cat([torch.arange(n - new, n) for new, n in seqs])
+    page = torch.cat([b.host_table[s].long()[torch.arange(n - new, n) // 16]
+                      for s, (new, n) in enumerate(seqs)]).cuda()
+    slot = (pos % 16).cuda()
+    kp[page, :, slot], vp[page, :, slot] = x[:b.tokens, :1], x[:b.tokens, 1:]
+    assert torch.equal(b.k, kp) and torch.equal(b.v, vp)
+
+
+def test_two_graphs_share_a_workspace(gpu):
+    """Replayed in turn, with eager calls between: each finds its own results, whatever
+    the other left in the workspace."""
+    K = _k()
+    ws = _workspace(8, 2, 64)
+    parts = []
+    for seed, seqs, window in ((1, [(1, 6000), (1, 90)], 1000), (2, [(200, 700), (1, 3000)], 0)):
+        b = R.Batch(seqs, 16, 2, 64, torch.bfloat16, seed=seed)
+        q = _randn(b.rows, 8, 64, dtype=torch.bfloat16, seed=seed)
+        want, out = _attend(b, q, window=window), torch.zeros_like(q)
+        cache, batch = K.PagedKVCache(b.k, b.v), K.PagedBatch(b.starts, b.lens, b.table, b.rows)
+
+        def call(q=q, out=out, cache=cache, batch=batch, window=window):
+            K.paged_attention_gpu(cache, batch, q, out, ws, window=window)
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            call()
+        parts.append((b, graph, call, want, out))
+    for i in range(4):
+        for b, graph, call, want, out in parts:
+            out.fill_(7.0)
+            graph.replay()
+            assert torch.equal(out, want)
+            if i % 2:
+                out.fill_(7.0)
+                call()
+                assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_kernels_that_max_new_selects_agree(gpu, kind):
+    """What max_new says selects tiles of 16 or 128 rows: both results are within the
+    tolerance of float64, so they are within twice that of each other."""
+    b = R.Batch([(1, 700), (3, 90), (5, 2000)], 16, 2, 128, HALF[kind], seed=1)
+    q = _randn(b.rows, 8, 128, dtype=HALF[kind], seed=2)
+    _, tol = R.attention(b, q, 128 ** -0.5, True, 0, R.half_step(q.dtype))
+    one, other = _attend(b, q, max_new=1), _attend(b, q)
+    assert ((one.double() - other.double()).abs() <= 2 * tol).all()
