@@ -357,9 +357,13 @@ def _int32(x, name: str):
     return x
 
 
+def _too_long(shape, name: str):
+    raise ValueError(f"{name} has shape {tuple(shape)}, which does not fit in 32 bits")
+
+
 def _sizes(shape, name: str) -> None:
-    if max(shape, default=0) > _INT_MAX:
-        raise ValueError(f"{name} has shape {tuple(shape)}, which does not fit in 32 bits")
+    if max(shape) > _INT_MAX:
+        _too_long(shape, name)
 
 
 def _device(t, name: str) -> int:
@@ -483,13 +487,13 @@ class Rope(_Descriptor):
         return Rope(f, scale, interleaved)
 
 
-def _check(x, kind, name: str) -> None:
-    if not isinstance(x, kind):
-        raise TypeError(f"{name} must be a {kind.__name__}, not {type(x).__name__}")
+def _no(x, kind, name: str):
+    raise TypeError(f"{name} must be a {kind.__name__}, not {type(x).__name__}")
 
 
 def _same_device(x, kind, name: str, dev: int) -> None:
-    _check(x, kind, name)
+    if not isinstance(x, kind):
+        _no(x, kind, name)
     if x._dev != dev:
         raise ValueError(f"{name} is on cuda:{x._dev}, the tensors are on cuda:{dev}")
 
@@ -502,11 +506,12 @@ def rope_tokens_gpu(x, output, positions, rope: Rope, stream=None):
     shape, dt = x.shape, x.dtype
     if len(shape) != 3:
         raise ValueError("x must be [tokens][heads][head_dim]")
-    _sizes(shape, "x")
+    n, heads, hd = shape
+    if n > _INT_MAX or heads > _INT_MAX or hd > _INT_MAX:
+        _too_long(shape, "x")
     dev = _device(x, "x")
     px, sx = _heads(x, "x", dt, shape, dev)
     py, sy = _heads(output, "output", dt, shape, dev)
-    n, heads, hd = shape
     pp = _flat(positions, "positions", torch.int32, (n,), dev)
     _same_device(rope, Rope, "rope", dev)
     L = _lib.load()
@@ -527,9 +532,11 @@ def qk_norm_rope_gpu(q, k, q_output, k_output, q_weight, k_weight, positions,
     if len(qs) != 3 or len(ks) != 3 or ks[0] != qs[0] or ks[2] != qs[2]:
         raise ValueError("q and k must be [tokens][heads][head_dim] with the same tokens and "
                          "head_dim")
-    _sizes(qs, "q")
-    _sizes(ks, "k")
     n, nh, hd = qs
+    if n > _INT_MAX or nh > _INT_MAX or hd > _INT_MAX:
+        _too_long(qs, "q")
+    if ks[1] > _INT_MAX:
+        _too_long(ks, "k")
     pq, sq = _heads(q, "q", dt, qs, dev)
     pk, sk = _heads(k, "k", dt, ks, dev)
     pqo, sqo = _heads(q_output, "q_output", dt, qs, dev)
@@ -610,7 +617,8 @@ def paged_append_gpu(cache: PagedKVCache, batch: PagedBatch, k, v, rope: Optiona
     [tokens][heads][head_dim] is given, rotates it into q_output (which may be q)
     in the same launch.  q_weight / k_weight (float32 [head_dim]): RMSNorm before
     the rotation (spb_paged_append_*)."""
-    _check(cache, PagedKVCache, "cache")
+    if not isinstance(cache, PagedKVCache):
+        _no(cache, PagedKVCache, "cache")
     dev = _device(cache.k, "the cache")
     _same_device(batch, PagedBatch, "batch", dev)
     n, hd, dt = batch.num_tokens, cache.head_dim, cache.dtype
@@ -622,8 +630,9 @@ def paged_append_gpu(cache: PagedKVCache, batch: PagedBatch, k, v, rope: Optiona
         pv, sv = _heads(v, "v", dt, shape, dev)
     if q is not None or q_output is not None:
         _kind(q, "q")
-        _sizes(q.shape, "q")
         nh = q.shape[1] if q.dim() == 3 else 0
+        if nh > _INT_MAX:
+            _too_long(q.shape, "q")
         shape = (n, nh, hd)
         pq, sq = _heads(q, "q", dt, shape, dev)
         pqo, sqo = _heads(q_output, "q_output", dt, shape, dev)
@@ -658,13 +667,15 @@ def paged_attention_gpu(cache: PagedKVCache, batch: PagedBatch, q, output, works
     when causal, j > p - window when window > 0, and the whole cached length
     otherwise.  scale None: head_dim ** -0.5.  workspace: a contiguous uint8 GPU
     tensor of paged_attention_workspace_size bytes (spb_paged_attention_*)."""
-    _check(cache, PagedKVCache, "cache")
+    if not isinstance(cache, PagedKVCache):
+        _no(cache, PagedKVCache, "cache")
     dev = _device(cache.k, "the cache")
     _same_device(batch, PagedBatch, "batch", dev)
     hd, dt = cache.head_dim, cache.dtype
     _kind(q, "q")
-    _sizes(q.shape, "q")
     nh = q.shape[1] if q.dim() == 3 else 0
+    if nh > _INT_MAX:
+        _too_long(q.shape, "q")
     shape = (batch.num_tokens, nh, hd)
     window = _int32(window, "window")
     pq, sq = _heads(q, "q", dt, shape, dev)
