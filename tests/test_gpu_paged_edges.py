@@ -292,3 +292,37 @@ def test_kernels_that_max_new_selects_agree(gpu, kind):
     _, tol = R.attention(b, q, 128 ** -0.5, True, 0, R.half_step(q.dtype))
     one, other = _attend(b, q, max_new=1), _attend(b, q)
     assert ((one.double() - other.double()).abs() <= 2 * tol).all()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("window", [0, 1, 40, 130])
+@pytest.mark.parametrize("seqs,nh,hd,max_new", [
+    ([(150, 700)], 2, 128, 0), ([(7, 300)], 2, 80, 7), ([(1, 4000), (90, 90)], 3, 64, 0),
+    ([(40, 17), (33, 200)], 20, 64, 0)])
+def test_one_bad_value_reaches_the_rows_that_see_it(gpu, kind, window, seqs, nh, hd, max_new):
+    """NaN in V of one position of the last sequence: those rows are NaN, all others have
+    the bits that they have without it."""
+    K = _k()
+    b = R.Batch(seqs, 16, 1, hd, HALF[kind], seed=5)
+    q = _randn(b.rows, nh, hd, dtype=HALF[kind], seed=6)
+    clean = _attend(b, q, window=window, max_new=max_new)
+    cache = K.PagedKVCache(b.k, b.v)
+    batch = K.PagedBatch(b.starts, b.lens, b.table, b.rows, max_new=max_new)
+    ws, out = _workspace(nh, 1, hd), torch.empty_like(q)
+    s, (new, n) = len(seqs) - 1, seqs[-1]
+    pos = torch.arange(n - new, n)
+    g = torch.Generator().manual_seed(7)
+    places = torch.cat([torch.randint(max(0, n - new - window), n, (6,), generator=g),
+                        torch.tensor([0, n - 1, n - new, max(0, n - new - window)])])
+    for at in places.tolist():
+        page = int(b.host_table[s, at // 16])
+        before = b.v[page, 0, at % 16].clone()
+        b.v[page, 0, at % 16] = math.nan
+        K.paged_attention_gpu(cache, batch, q, out, ws, window=window)
+        b.v[page, 0, at % 16] = before
+        sees = (at <= pos) & ((at > pos - window) | (window == 0))
+        rows = torch.zeros(b.rows, dtype=torch.bool)
+        rows[b.host_starts[s]:b.host_starts[s + 1]] = sees
+        rows = rows.cuda()
+        same = torch.equal(out[~rows], clean[~rows])
+        assert same and out[rows].isnan().all(), at
