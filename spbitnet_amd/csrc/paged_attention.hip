@@ -636,14 +636,23 @@ constexpr int waves_per_simd() { return Shape<BM>::kWaves * resident<HD, BM>() >
 // gains nothing either (9 sequences of 5 tokens 18.1 against 17.9).
 //
 // What bounds it.  Decoding: memory, K and V being read once.  One sequence of 131,072
-// positions (336 MB) takes 65.6 us with the join, 5.1 TB/s, 32 ragged ones (363 MB)
-// 68.6, 5.3 TB/s; a large copy reaches 4.9.  Many rows: 2048 tokens behind 8192 (193
-// GFLOP) take 240 us, 0.80 PFLOP/s, where a large library product reaches 1.22.  By
-// counters the matrix units are busy 44 % of the time and the vector units 50 %, by
-// time stamps (before LDS was read two groups ahead) a wave's 64 keys took 1400 cycles
-// for the scores, 900 for the softmax, 1200 for the values and 1000 for the next keys'
-// places, waits and barriers, and the two waves of a SIMD overlap little.  Small calls: a chain of dependent steps, about
-// 14,000 cycles (lengths, the cut, pages, keys, one tile, the join of two waves).
+// positions (336 MB) takes 65.7 us with the join, 5.1 TB/s, 32 ragged ones (363 MB)
+// 68.2, 5.3 TB/s; a large copy reaches 4.9.  Heads whose padded row has columns to spare
+// go by load_any, and wait: one sequence of 131,072 takes 62.7 us 80 wide, 3.4 TB/s, and
+// 161.6 us 192 wide, 3.1, where 64, 128 and 256 reach 4.5, 5.2 and 5.5.
+// Many rows: 2048 tokens behind 8192 (193 GFLOP) take 233 to 251 us with the join, 0.77
+// to 0.83 PFLOP/s, where a large library product reaches 1.17 to 1.22.  The kernel's part
+// is 510,000 cycles, whose clock moves between 1.95 and 2.3 GHz.  By counters the matrix
+// units are busy 45 % of the time and the vector units 50 %, as each wave does scores,
+// softmax and values one after the other and the two waves of a SIMD overlap little.  10
+// of the 256 registers are spilled (36 bytes a lane).  256 wide, one wave a SIMD, it is
+// 69 of 512 (264 bytes): 2048 tokens behind 2048, 8 heads, 127 us, 0.41 PFLOP/s; 192 wide
+// 111 us, 0.35, without spills; 128 wide 61 us, 0.42.
+// Small calls: a chain of dependent steps.  One token behind 2048 positions: 14.6 us a
+// call, traces 11.8 of it here and 4.0 in the join.  By time stamps a block's first wave
+// takes 13,500 cycles, 5.4 us (lengths and the cut 4800, pages and Q until the first
+// keys' loads are out 3200, keys 3000, the end 2500), the slowest block 8.4 (two tiles),
+// and first start to last end 8.5; the rest of the trace is the launch's start and end.
 // Not kept: K and V staged in registers (spills, whose reloads wait in order behind
 // the loads: 444 us for the same 2048 tokens); two sets of 32 rows in a wave with K
 // and V read once for both (512 registers, 150 spilled: 609 us); raised priorities

@@ -143,8 +143,9 @@ __device__ __forceinline__ void load_lds(const float* p, int u, int units, float
 // half layout, [2 V u, 2 V u + 2 V) in the interleaved one and past the rotary
 // part.  kUnits: units of a lane (2 only where a head has more than 64).  A head
 // is loaded while the one before it is worked on, the first while the angles are.
-// 8192 tokens of 25 heads of 128, half of each rotated: 20.1 us, 5.2 TB/s (a large
-// copy reaches 4.9); 2049 tokens with norms 9.6 us, 2.7 TB/s; one token 2.6 us.
+// 8192 tokens of 25 heads of 128, half of each rotated: 20.2 us, 5.2 TB/s (a large
+// copy reaches 4.9); 2049 tokens with norms 8.2 us with calls in a row, 3.2 TB/s (9.1 in
+// a trace, which sets them apart); one token 2.8 us in a trace.
 // kStream: non-temporal stores (a template's, as the compiler joins the two stores of
 // a branch into a plain one).
 template <class T, int V, int kUnits, bool kNorm, bool kPaged, bool kStream>
@@ -380,10 +381,10 @@ int run_heads(const char* fn, HeadsArgs& a, const spb_rope* rope, bool paged, sp
     // Two tokens a block once one a block fills the chip.  us for 1 / 2 / 3 / 5 / 8:
     // 8192 tokens of 25 heads of 128 27.2 / 25.8 / 26.8 / 28.1 / 27.4, 2049 normed
     // tokens 10.4 / 10.4 / 11.1 / 12.3 / 15.6, 3540 tokens appended 20.7 / 19.9 /
-    // 21.3 / 21.3 / 24.9 (plain stores).
+    // 21.3 / 21.3 / 24.9 (in traces, with plain stores).
     const int tile = a.tokens >= 4 * device_cu_count() ? kMaxTile : 1;
     // What is larger than a die's L2 is written past it: 25.8 -> 20.1, 10.4 -> 9.6
-    // and 19.9 -> 17.8 us for the same three (non-temporal loads lose as much).
+    // and 19.9 -> 17.8 us in traces of the same three (non-temporal loads lose as much).
     const bool past = static_cast<long>(a.tokens) * static_cast<long>(a.all_heads.d) * hd * 2 > (4L << 20);
     const hipStream_t st = as_stream(stream);
     if (v == 8) pick_heads<T, 8, 1>(a, tile, norm, paged, past, st);
