@@ -367,8 +367,7 @@ int spb_argmax_f32(const float* x, int n, int* out_index, spb_stream_t stream);
  * heads are contiguous ([heads][head_dim]); tokens are `*_stride` elements
  * apart (the q, k and v parts of a stacked projection are three pointers with
  * one stride).  Each entry point exists for fp16 (_f16) and bf16 (_bf16);
- * arithmetic is float32, outputs are rounded once.  The rotation, the norms and
- * append take up to 2^24 tokens, of up to 2^24 heads (q, k and v together).
+ * arithmetic is float32, outputs are rounded once.
  *
  * Arrays on the device are not read by the host: numbers in them that fall
  * outside the batch, the table or the pool are clamped or skipped on the

@@ -10,6 +10,7 @@
 // cosine, which take turns, see a small number (v_sin_f32 and v_cos_f32 on
 // 65,536 turns of [-1/2, 1/2): at most 1.2e-7 off).  A token's sines and
 // cosines are computed once per block into LDS and used by all of its heads.
+#include <algorithm>
 #include <cmath>
 
 #include "paged.hpp"
@@ -20,9 +21,7 @@ namespace {
 constexpr int kHeadBlock = 256;
 constexpr int kMaxTile = 2;      // tokens of a block
 constexpr int kMaxHalf = 128;    // pairs of the widest head
-// A launch holds less than 2^32 lanes, 2^24 blocks of them; a block's items (its
-// tokens' heads) and a step of them stay far below 2^31.
-constexpr int kMaxTokens = 1 << 24, kMaxHeads = 1 << 24;
+constexpr int kMaxBlocks = 1 << 23;  // of a launch, which holds less than 2^32 lanes
 
 // A run of heads of the batch's tokens: head h of token t at
 // src + t * src_stride + h * head_dim.
@@ -38,6 +37,7 @@ struct HeadSpan {
 struct HeadsArgs {
     HeadSpan span[3];  // q, k, v (a single span of any heads for spb_rope_tokens)
     int head_dim, tokens;
+    int first;  // token of the launch's first block
     FastDiv all_heads;
     int units;      // lanes' shares of a head: head_dim / (2 V)
     int rot_units;  // those that are rotated: rotary / (2 V)
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(kHeadBlock) void heads_kernel(const HeadsArgs a, co
     __shared__ __align__(16) float cs[2][kMaxTile * kMaxHalf];
     __shared__ __align__(16) float wt[kNorm ? 2 : 1][kNorm ? 2 * kMaxHalf : 1];
     __shared__ Place place[kMaxTile];
-    const int tid = threadIdx.x, t0 = blockIdx.x * tile;
+    const int tid = threadIdx.x, t0 = a.first + blockIdx.x * tile;
     const int n = min(tile, a.tokens - t0);
     const int lanes = 1 << a.lanes_log, u0 = tid & (lanes - 1);
     const int heads = a.all_heads.d, items = n * heads, step = kHeadBlock >> a.lanes_log;
@@ -336,14 +336,19 @@ int check_span(const char* fn, const char* what, const HeadSpan& s, int tokens, 
 }
 
 template <class T, int V, int kUnits, bool kNorm, bool kPaged>
-void launch_heads(const HeadsArgs& a, int tile, bool past, hipStream_t st) {
-    const dim3 grid((a.tokens + tile - 1) / tile), block(kHeadBlock);
-    if (past) hipLaunchKernelGGL((heads_kernel<T, V, kUnits, kNorm, kPaged, V != 1>), grid, block, 0, st, a, tile);
-    else hipLaunchKernelGGL((heads_kernel<T, V, kUnits, kNorm, kPaged, false>), grid, block, 0, st, a, tile);
+void launch_heads(HeadsArgs& a, int tile, bool past, hipStream_t st) {
+    const dim3 block(kHeadBlock);
+    const long most = static_cast<long>(kMaxBlocks) * tile;
+    for (long first = 0; first < a.tokens; first += most) {
+        const dim3 grid(static_cast<unsigned>((std::min(most, a.tokens - first) + tile - 1) / tile));
+        a.first = static_cast<int>(first);
+        if (past) hipLaunchKernelGGL((heads_kernel<T, V, kUnits, kNorm, kPaged, V != 1>), grid, block, 0, st, a, tile);
+        else hipLaunchKernelGGL((heads_kernel<T, V, kUnits, kNorm, kPaged, false>), grid, block, 0, st, a, tile);
+    }
 }
 
 template <class T, int V, int kUnits>
-void pick_heads(const HeadsArgs& a, int tile, bool norm, bool paged, bool past, hipStream_t st) {
+void pick_heads(HeadsArgs& a, int tile, bool norm, bool paged, bool past, hipStream_t st) {
     if (paged && norm) launch_heads<T, V, kUnits, true, true>(a, tile, past, st);
     else if (paged) launch_heads<T, V, kUnits, false, true>(a, tile, past, st);
     else if (norm) launch_heads<T, V, kUnits, true, false>(a, tile, past, st);
@@ -355,14 +360,11 @@ void pick_heads(const HeadsArgs& a, int tile, bool norm, bool paged, bool past, 
 template <class T>
 int run_heads(const char* fn, HeadsArgs& a, const spb_rope* rope, bool paged, spb_stream_t stream) {
     const int rot = rope ? rope->rotary_dim : 0, hd = a.head_dim;
-    if (a.tokens > kMaxTokens) return invalid("%s: more than %d tokens", fn, kMaxTokens);
-    if (static_cast<long>(a.span[0].heads) + a.span[1].heads + a.span[2].heads > kMaxHeads)
-        return invalid("%s: more than %d heads", fn, kMaxHeads);
     a.half = rot / 2;
     a.interleaved = rope ? rope->interleaved != 0 : 1;
     a.scale = rope ? rope->scale : 1.0f;
     a.inv_freq = rope ? rope->inv_freq : nullptr;
-    a.all_heads = FastDiv(a.span[0].heads + a.span[1].heads + a.span[2].heads);
+    const long heads = static_cast<long>(a.span[0].heads) + a.span[1].heads + a.span[2].heads;
     bool norm = false;
     auto fits = [&](int v) {
         if (hd % (2 * v) || rot % (2 * v)) return false;
@@ -383,9 +385,12 @@ int run_heads(const char* fn, HeadsArgs& a, const spb_rope* rope, bool paged, sp
     // tokens 10.4 / 10.4 / 11.1 / 12.3 / 15.6, 3540 tokens appended 20.7 / 19.9 /
     // 21.3 / 21.3 / 24.9 (in traces, with plain stores).
     const int tile = a.tokens >= 4 * device_cu_count() ? kMaxTile : 1;
+    // a block counts its heads and one step further in 32 bits
+    if (heads * tile > 0x7FFFFFFFL - kHeadBlock) return invalid("%s: more than 2^31 heads", fn);
+    a.all_heads = FastDiv(static_cast<uint32_t>(heads));
     // What is larger than a die's L2 is written past it: 25.8 -> 20.1, 10.4 -> 9.6
     // and 19.9 -> 17.8 us in traces of the same three (non-temporal loads lose as much).
-    const bool past = static_cast<long>(a.tokens) * static_cast<long>(a.all_heads.d) * hd * 2 > (4L << 20);
+    const bool past = static_cast<long>(a.tokens) * heads * hd * 2 > (4L << 20);
     const hipStream_t st = as_stream(stream);
     if (v == 8) pick_heads<T, 8, 1>(a, tile, norm, paged, past, st);
     else if (v == 4) pick_heads<T, 4, 1>(a, tile, norm, paged, past, st);

@@ -116,26 +116,47 @@ def test_batches_without_tokens(gpu, kind, seqs):
     assert torch.equal(k, kp) and torch.equal(v, vp)
 
 
-def test_the_most_tokens_of_a_rotation(gpu):
-    """2^24 tokens (one head of 4), and that many heads of one token: the first and last
-    rows against a call of their own, all against float64."""
+def test_more_tokens_than_a_launch_holds(gpu):
+    """2^25 + 3 tokens of one head, and one token of that many heads, against float64."""
     K = _k()
-    n, f = 1 << 24, K.rope_inv_freq(4)[0]
-    rope = K.Rope(f)
-    x = torch.randn(n, 1, 4, device="cuda").to(torch.float16)
+    n, f = (1 << 25) + 3, K.rope_inv_freq(2)[0]
+    rope, none = K.Rope(f), torch.zeros(0, dtype=torch.float64, device="cuda")
+    x = torch.randn(n, 1, 2, device="cuda").to(torch.float16)
     pos = torch.arange(n, dtype=torch.int32, device="cuda")
     y = torch.full_like(x, 7.0)
     K.rope_tokens_gpu(x, y, pos, rope)
-    for rows in (slice(0, 5), slice(n - 5, n)):
+    R.check_rotated(y, x.double(), R.rotate(x.double(), pos, f.cuda(), 1.0, True), f.cuda(), 1.0, True)
+    for far in (0, 1 << 24, n):  # launches meet at 2^24: rows by a call of their own
+        rows = slice(max(0, far - 3), min(n, far + 3))
         z = torch.full_like(x[rows], 7.0)
         K.rope_tokens_gpu(x[rows], z, pos[rows], rope)
         assert torch.equal(z, y[rows])
-    R.check_rotated(y, x.double(), R.rotate(x.double(), pos, f.cuda(), 1.0, True), f.cuda(), 1.0, True)
-    heads = x.view(1, n, 4)
+    w = torch.ones(2, device="cuda")
+    y.fill_(7.0)
+    k, ko = x[:, :0], y[:, :0]
+    K.qk_norm_rope_gpu(x, k, y, ko, w, w, None, None)
+    want = R.norm(x.double(), w, 1e-5)
+    R.check_rotated(y, want, want, none, 1.0, True)
+    heads = x.view(1, n, 2)
     z = torch.full_like(heads, 7.0)
     K.rope_tokens_gpu(heads, z, pos[3:4], rope)
     R.check_rotated(z, heads.double(), R.rotate(heads.double(), pos[3:4], f.cuda(), 1.0, True),
                     f.cuda(), 1.0, True)
+
+
+def test_append_of_more_tokens_than_a_launch_holds(gpu):
+    K = _k()
+    n, page = (1 << 24) + 5, 1 << 12
+    held = -(-n // page)
+    k, v = (torch.randn(n, 1, 8, device="cuda").to(torch.bfloat16) for _ in range(2))
+    pools = [torch.zeros(held, 1, page, 8, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    batch = K.PagedBatch(torch.tensor([0, n], dtype=torch.int32).cuda(),
+                         torch.tensor([n], dtype=torch.int32).cuda(),
+                         torch.arange(held, dtype=torch.int32).cuda()[None], n)
+    K.paged_append_gpu(K.PagedKVCache(*pools), batch, k, v)
+    for got, want in zip(pools, (k, v)):
+        got = got.view(-1, 8)
+        assert torch.equal(got[:n], want.view(-1, 8)) and not got[n:].any()
 
 
 def test_what_is_no_descriptor_is_refused(gpu):

@@ -248,23 +248,8 @@ def test_batches_without_tokens_have_no_pointers(lib, kind, size):
     _said(lib, call(rotary_dim=130), "rotary_dim")
 
 
-MANY = (1 << 24) + 1
-
-
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
-@pytest.mark.parametrize("n", [MANY, 1 << 25, 2 ** 31 - 1])
-def test_more_tokens_than_a_launch_holds(lib, kind, n):
-    rope = ctypes.byref(_rope(rotary_dim=2))
-    _said(lib, getattr(lib, f"spb_rope_tokens_{kind}")(A, A, A, rope, n, 1, 2, 2, 2, None), "tokens")
-    _said(lib, getattr(lib, f"spb_qk_norm_rope_{kind}")(
-        A, A, A, A, A, A, A, rope, n, 1, 1, 2, 2, 2, 2, 2, ctypes.c_float(0), None), "tokens")
-    _said(lib, getattr(lib, f"spb_paged_append_{kind}")(
-        ctypes.byref(_cache(num_kv_heads=1)), ctypes.byref(_batch(num_tokens=n)), A, A, None, None,
-        128, 128, 0, 0, 0, None, None, ctypes.c_float(0), None, None), "tokens")
-
-
-@pytest.mark.parametrize("kind", ["f16", "bf16"])
-@pytest.mark.parametrize("nh,nkv", [(MANY, 0), (1 << 24, 1), (1 << 30, 1 << 30), (2 ** 31 - 1, 1)])
+@pytest.mark.parametrize("nh,nkv", [(2 ** 31 - 1, 0), (1 << 30, 1 << 30), (2 ** 31 - 1, 1)])
 def test_more_heads_than_a_block_counts(lib, kind, nh, nkv):
     rope = ctypes.byref(_rope(rotary_dim=2))
     wide = 1 << 33
