@@ -448,16 +448,24 @@ class _Descriptor:
     """What a call passes on as a C struct of pointers and sizes, taken once.  Its
     attributes hold the tensors and say the sizes that the calls check others against;
     one set afterwards would free the memory behind a pointer or let a smaller tensor
-    pass, so that is refused."""
+    pass, so that is refused.  A program may add attributes of its own."""
+
+    _fixed = ()  # names, once _ptr is set (last)
+
+    def _keep(self, name):
+        if name in self._fixed:
+            raise AttributeError(f"{name} of a {type(self).__name__} cannot be changed: make "
+                                 "another (the contents of its tensors may be)")
 
     def __setattr__(self, name, value):
-        if "_ptr" in self.__dict__:  # set last
-            raise AttributeError(f"a {type(self).__name__} cannot be changed: make another "
-                                 "(the contents of its tensors may be)")
+        self._keep(name)
         object.__setattr__(self, name, value)
+        if name == "_ptr":
+            object.__setattr__(self, "_fixed", frozenset(self.__dict__) | {"_fixed"})
 
     def __delattr__(self, name):
-        raise AttributeError(f"a {type(self).__name__} cannot be changed")
+        self._keep(name)
+        object.__delattr__(self, name)
 
 
 class Rope(_Descriptor):

@@ -242,7 +242,7 @@ def test_descriptors_are_fixed(gpu):
     for x, names in ((K.Rope.scaled(64), ("inv_freq", "scale", "interleaved", "rotary_dim")),
                      (K.PagedKVCache(b.k, b.v), ("k", "v", "head_dim", "num_kv_heads", "dtype")),
                      (K.PagedBatch(b.starts, b.lens, b.table, 2),
-                      ("token_starts", "kv_lens", "page_table", "num_tokens", "max_new", "other"))):
+                      ("token_starts", "kv_lens", "page_table", "num_tokens", "max_new", "_ptr", "_c", "_fixed"))):
         for name in names:
             before = getattr(x, name, None)
             with pytest.raises(AttributeError, match="cannot be changed"):
@@ -250,6 +250,10 @@ def test_descriptors_are_fixed(gpu):
             assert getattr(x, name, None) is before
             with pytest.raises(AttributeError, match="cannot be changed"):
                 delattr(x, name)
+        for value in (1, 2):  # a program's own
+            x.tag = value
+            assert x.tag == value
+        del x.tag
 
 
 def test_thousands_of_sequences(gpu):
