@@ -640,7 +640,7 @@ constexpr int waves_per_simd() { return Shape<BM>::kWaves * resident<HD, BM>() >
 // 68.2, 5.3 TB/s; a large copy reaches 4.9.  Heads whose padded row has columns to spare
 // go by load_any, and wait: one sequence of 131,072 takes 62.7 us 80 wide, 3.4 TB/s, and
 // 161.6 us 192 wide, 3.1, where 64, 128 and 256 reach 4.5, 5.2 and 5.5.
-// Many rows: 2048 tokens behind 8192 (193 GFLOP) take 233 to 251 us with the join, 0.77
+// Many rows: 2048 tokens behind 8192 (193 GFLOP) take 233 to 262 us with the join, 0.74
 // to 0.83 PFLOP/s, where a large library product reaches 1.17 to 1.22.  The kernel's part
 // is 510,000 cycles, whose clock moves between 1.95 and 2.3 GHz.  By counters the matrix
 // units are busy 45 % of the time and the vector units 50 %, as each wave does scores,
