@@ -512,6 +512,116 @@ int spb_paged_attention_bf16(const spb_paged_cache* cache, const spb_paged_batch
                              int window, void* workspace, size_t workspace_size,
                              spb_stream_t stream);
 
+/* ---- what each request of a shared batch brings of its own -------------------
+ * No reference counterpart: low-rank adapters beside the shared projections, and
+ * behind the logits the next token under each request's settings (spb_argmax_f32
+ * is the greedy pick of one row) and log-probabilities.  Adapter ids, settings and
+ * random numbers are device arrays that a captured graph reads anew at each
+ * replay.  Nothing allocates; a workspace's contents are irrelevant, and calls
+ * that share one must be ordered (same stream). */
+
+/* A pool of low-rank adapters of one projection [rows][cols].  A projection that is
+ * stacked of several (q|k|v, gate|up) has as many sections; section_rows sum up to
+ * rows.  Adapter i has
+ *   A: [num_sections * rank][cols] at a + i * a_adapter_stride, rows a_row_stride
+ *      apart; rows s * rank ... belong to section s,
+ *   B: [rows][rank] at b + i * b_adapter_stride, rows b_row_stride apart,
+ *   scales[i] (device float32) and its rank ranks[i] (device int32, clamped to
+ *   [0, rank]; ranks NULL: all of them have `rank`).  Rows of a section's A and
+ *   columns of B from an adapter's rank on are not used, whatever they hold.
+ * rank and cols multiples of 8, rank <= 256, cols and rows <= 2^20; a and b 16-byte
+ * aligned, strides multiples of 8. */
+enum { SPB_MAX_SECTIONS = 4 };
+typedef struct spb_adapters {
+    const uint16_t* a;
+    const uint16_t* b;
+    const float* scales;
+    const int* ranks;
+    long a_adapter_stride, a_row_stride, b_adapter_stride, b_row_stride;
+    int num_adapters, rank, cols, num_sections;
+    int section_rows[SPB_MAX_SECTIONS];
+} spb_adapters;
+
+/* output[t] = base[t] + scales[i] * B_i (A_i x[t]) with i = ids[t] (device int32):
+ * base is what the shared projection gave for x.  A token whose id is outside
+ * [0, num_adapters) has no adapter: its output is base.  Both products accumulate in
+ * float32; the inner one is kept in float32 or as two 16-bit numbers, and the output
+ * is rounded once.  base == output adds in place (same stride); other overlaps of
+ * output are not allowed.  x 16-byte aligned, x_stride a multiple of 8.
+ * num_tokens <= 2^20; the workspace of more tokens serves fewer. */
+size_t spb_adapters_workspace_size(const spb_adapters* adapters, int num_tokens);
+int spb_adapters_f16(const spb_adapters* adapters, const int* ids, const uint16_t* x,
+                     const uint16_t* base, uint16_t* output, int num_tokens, long x_stride,
+                     long base_stride, long output_stride, void* workspace, size_t workspace_size,
+                     spb_stream_t stream);
+int spb_adapters_bf16(const spb_adapters* adapters, const int* ids, const uint16_t* x,
+                      const uint16_t* base, uint16_t* output, int num_tokens, long x_stride,
+                      long base_stride, long output_stride, void* workspace,
+                      size_t workspace_size, spb_stream_t stream);
+
+/* Settings of sampling: of each a device vector [rows], or where that is NULL one
+ * value for all rows.
+ *   temperature  0: greedy (the first token of the order below)
+ *   top_k        keeps the k first tokens; 0, or more than there are: all
+ *   top_p        keeps tokens while those before them have less than top_p of the
+ *                weight of what top_k keeps; 1: all, 0: the first
+ *   min_p        keeps tokens with at least min_p of the first one's weight; 0: all
+ * The one value must be in range (temperature and top_k not negative, top_p and
+ * min_p in [0, 1]); in the vectors a temperature that is not above 0 is greedy, a NaN
+ * or a number past its range turns its filter off, and top_p below 0 is 0, min_p above
+ * 1 is 1. */
+typedef struct spb_sampling {
+    const float* temperatures;
+    const int* top_ks;
+    const float* top_ps;
+    const float* min_ps;
+    float temperature;
+    int top_k;
+    float top_p, min_p;
+} spb_sampling;
+
+/* The next token of each row of logits [rows][vocab] (rows logits_stride apart).  The
+ * tokens of a row stand in the order of falling logits, equal ones by index, with
+ * weights w = exp((logit - largest) / temperature); of what all filters keep, the
+ * first token is taken whose w with those before it is above u times the kept
+ * weight M.  u = uniforms[row] (device float32) in [0, 1): below and NaN count as 0,
+ * 1 and above as the largest number below 1.  logprobs (nullable): log(w / M).
+ * NaN logits count as minus infinity, which is never taken; of infinite ones the
+ * others have no weight.  A row of minus infinities gives token -1 and log-probability
+ * minus infinity.  Weights and their sums are exact to 2^-40 of the largest weight or
+ * better, and do not depend on the order of execution.  vocab <= 2^24, rows <= 2^20. */
+size_t spb_sample_workspace_size(int rows, int vocab);
+int spb_sample_f32(const float* logits, long logits_stride, const float* uniforms, int* tokens,
+                   float* logprobs, int rows, int vocab, const spb_sampling* sampling,
+                   void* workspace, size_t workspace_size, spb_stream_t stream);
+int spb_sample_f16(const uint16_t* logits, long logits_stride, const float* uniforms, int* tokens,
+                   float* logprobs, int rows, int vocab, const spb_sampling* sampling,
+                   void* workspace, size_t workspace_size, spb_stream_t stream);
+int spb_sample_bf16(const uint16_t* logits, long logits_stride, const float* uniforms, int* tokens,
+                    float* logprobs, int rows, int vocab, const spb_sampling* sampling,
+                    void* workspace, size_t workspace_size, spb_stream_t stream);
+
+/* Log-probabilities logit - log(sum of exp(logits)) of the token tokens[row] of each
+ * row (tokens and logprobs may be NULL together) and, for top > 0, of the `top`
+ * likeliest tokens, in the order of falling logits and equal ones by index: top_ids and
+ * top_logprobs are [rows][top].  A row whose token is outside [0, vocab) is padding:
+ * its outputs stay as they were.  NaN logits count as minus infinity; of infinite ones
+ * the others have no weight; in a row of minus infinities all log-probabilities are
+ * minus infinity.  top <= 64 and <= vocab; other limits as above. */
+size_t spb_token_logprobs_workspace_size(int rows, int vocab, int top);
+int spb_token_logprobs_f32(const float* logits, long logits_stride, const int* tokens,
+                           float* logprobs, int* top_ids, float* top_logprobs, int rows,
+                           int vocab, int top, void* workspace, size_t workspace_size,
+                           spb_stream_t stream);
+int spb_token_logprobs_f16(const uint16_t* logits, long logits_stride, const int* tokens,
+                           float* logprobs, int* top_ids, float* top_logprobs, int rows,
+                           int vocab, int top, void* workspace, size_t workspace_size,
+                           spb_stream_t stream);
+int spb_token_logprobs_bf16(const uint16_t* logits, long logits_stride, const int* tokens,
+                            float* logprobs, int* top_ids, float* top_logprobs, int rows,
+                            int vocab, int top, void* workspace, size_t workspace_size,
+                            spb_stream_t stream);
+
 /* ---- decode engine --------------------------------------------------------
  * bs=1 greedy decode of a BitNet b1.58 transformer whose linear layers are
  * 2:4 sparse-ternary, with bf16 activations, bf16 KV cache and a bf16 tied or

@@ -85,6 +85,18 @@ SIGNATURES = {
     "spb_paged_attention_workspace_size": [_I, _I, _I],
     "spb_paged_attention_f16": [_P] * 4 + [_L, _L, _I, _F, _I, _I, _P, ctypes.c_size_t, _P],
     "spb_paged_attention_bf16": [_P] * 4 + [_L, _L, _I, _F, _I, _I, _P, ctypes.c_size_t, _P],
+    # what each request of a shared batch brings of its own
+    "spb_adapters_workspace_size": [_P, _I],
+    "spb_adapters_f16": [_P] * 5 + [_I] + [_L] * 3 + [_P, ctypes.c_size_t, _P],
+    "spb_adapters_bf16": [_P] * 5 + [_I] + [_L] * 3 + [_P, ctypes.c_size_t, _P],
+    "spb_sample_workspace_size": [_I, _I],
+    "spb_sample_f32": [_P, _L, _P, _P, _P, _I, _I, _P, _P, ctypes.c_size_t, _P],
+    "spb_sample_f16": [_P, _L, _P, _P, _P, _I, _I, _P, _P, ctypes.c_size_t, _P],
+    "spb_sample_bf16": [_P, _L, _P, _P, _P, _I, _I, _P, _P, ctypes.c_size_t, _P],
+    "spb_token_logprobs_workspace_size": [_I, _I, _I],
+    "spb_token_logprobs_f32": [_P, _L] + [_P] * 4 + [_I] * 3 + [_P, ctypes.c_size_t, _P],
+    "spb_token_logprobs_f16": [_P, _L] + [_P] * 4 + [_I] * 3 + [_P, ctypes.c_size_t, _P],
+    "spb_token_logprobs_bf16": [_P, _L] + [_P] * 4 + [_I] * 3 + [_P, ctypes.c_size_t, _P],
     # decode engine (structs passed by pointer)
     "spb_engine_create": [_P, _P, _P, _P, _P, _I, _P],
     "spb_engine_destroy": [_P],
@@ -119,6 +131,9 @@ SIGNATURES = {
 _RESTYPES = {"spb_last_error_string": ctypes.c_char_p,
              "spb_bitlinear_workspace_size": ctypes.c_size_t,
              "spb_paged_attention_workspace_size": ctypes.c_size_t,
+             "spb_adapters_workspace_size": ctypes.c_size_t,
+             "spb_sample_workspace_size": ctypes.c_size_t,
+             "spb_token_logprobs_workspace_size": ctypes.c_size_t,
              "spb_sparse_i8_compressed_size": ctypes.c_long}
 
 
@@ -161,6 +176,20 @@ class PagedBatchC(ctypes.Structure):
     """spb_paged_batch (include/spbitnet_amd.h)."""
     _fields_ = [("token_starts", _P), ("kv_lens", _P), ("page_table", _P), ("num_seqs", _I),
                 ("table_width", _I), ("num_tokens", _I), ("max_new", _I)]
+
+
+class AdaptersC(ctypes.Structure):
+    """spb_adapters (include/spbitnet_amd.h)."""
+    _fields_ = [("a", _P), ("b", _P), ("scales", _P), ("ranks", _P), ("a_adapter_stride", _L),
+                ("a_row_stride", _L), ("b_adapter_stride", _L), ("b_row_stride", _L),
+                ("num_adapters", _I), ("rank", _I), ("cols", _I), ("num_sections", _I),
+                ("section_rows", _I * 4)]
+
+
+class SamplingC(ctypes.Structure):
+    """spb_sampling (include/spbitnet_amd.h)."""
+    _fields_ = [("temperatures", _P), ("top_ks", _P), ("top_ps", _P), ("min_ps", _P),
+                ("temperature", _F), ("top_k", _I), ("top_p", _F), ("min_p", _F)]
 
 
 _lib = None

@@ -695,3 +695,222 @@ def paged_attention_gpu(cache: PagedKVCache, batch: PagedBatch, q, output, works
     _lib.check(fn(cache._ptr, batch._ptr, pq, po, sq, so, nh,
                   hd ** -0.5 if scale is None else scale, 1 if causal else 0, window, pw, size,
                   _on(stream, dev)), "paged_attention_gpu")
+
+
+# ---- what each request of a shared batch brings of its own (no reference counterpart)
+
+_MAX_SECTIONS = 4
+_LOGITS_KIND = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
+
+
+class Adapters(_Descriptor):
+    """A pool of low-rank adapters of one projection (spb_adapters): a
+    [adapters][sections * rank][cols] and b [adapters][rows][rank] (fp16 or bf16, last
+    dimension contiguous, strides multiples of 8), scales float32 [adapters] and, where
+    adapters have fewer ranks than the pool, ranks int32 [adapters].  sections: the rows
+    of each part of a stacked projection, each with `rank` rows of a (None: one part).
+    Keeps the tensors alive; their contents may be changed between calls."""
+
+    def __init__(self, a, b, scales, ranks=None, sections=None):
+        self.kind = _kind(a, "a")
+        _kind(b, "b")
+        if a.dim() != 3 or b.dim() != 3 or b.shape[0] != a.shape[0]:
+            raise ValueError("a and b must be [adapters][sections * rank][cols] and "
+                             "[adapters][rows][rank]")
+        _sizes(a.shape, "a")
+        _sizes(b.shape, "b")
+        self._dev = dev = _device(a, "a")
+        if _device(b, "b") != dev or b.dtype != a.dtype:
+            raise TypeError(f"b is {b.dtype} on {b.device}, expected {a.dtype} on {a.device}")
+        num, rows, rank = b.shape
+        parts = (rows,) if sections is None else tuple(_int32(int(s), "a section")
+                                                       for s in sections)
+        if not 1 <= len(parts) <= _MAX_SECTIONS or min(parts) < 1 or sum(parts) != rows:
+            raise ValueError(f"sections {parts} must be 1 to {_MAX_SECTIONS} numbers that sum up "
+                             f"to the {rows} rows of b")
+        if a.shape[1] != len(parts) * rank:
+            raise ValueError(f"a has {a.shape[1]} rows, expected {len(parts)} sections of rank "
+                             f"{rank}")
+        for t, name in ((a, "a"), (b, "b")):
+            if t.shape[2] > 1 and t.stride(2) != 1:
+                raise ValueError(f"{name}: the last dimension must be contiguous")
+        self.a, self.b, self.scales, self.ranks = a, b, scales, ranks
+        self.dtype, self.num_adapters, self.rows, self.rank = a.dtype, num, rows, rank
+        self.cols, self.sections = a.shape[2], parts
+        ps = _flat(scales, "scales", torch.float32, (num,), dev)
+        pr = None if ranks is None else _flat(ranks, "ranks", torch.int32, (num,), dev)
+        self._c = _lib.AdaptersC(a.data_ptr(), b.data_ptr(), ps, pr, a.stride(0), a.stride(1),
+                                 b.stride(0), b.stride(1), num, rank, self.cols, len(parts),
+                                 (ctypes.c_int * _MAX_SECTIONS)(*parts))
+        self._ptr = ctypes.addressof(self._c)
+
+
+def _rows(t, name: str, dtype, shape, dev: int) -> Tuple[int, int]:
+    """Pointer and row stride of a matrix with contiguous rows."""
+    if (not isinstance(t, _Tensor) or t.get_device() != dev or t.dtype != dtype
+            or t.shape != shape):
+        _refuse(t, name, dtype, shape, dev)
+    st = t.stride()
+    if st[1] != 1 and shape[1] > 1:
+        raise ValueError(f"{name}: rows must be contiguous")
+    return t.data_ptr(), st[0] if shape[0] > 1 else shape[1]
+
+
+def adapters_workspace_size(adapters: Adapters, num_tokens: int) -> int:
+    """Bytes of the workspace that adapters_gpu needs for at most num_tokens tokens."""
+    if not isinstance(adapters, Adapters):
+        _no(adapters, Adapters, "adapters")
+    n = int(_lib.load().spb_adapters_workspace_size(adapters._ptr,
+                                                    _int32(num_tokens, "num_tokens")))
+    if n == 0:
+        _lib.check(1, "adapters_workspace_size")
+    return n
+
+
+def adapters_gpu(adapters: Adapters, ids, x, base, output, workspace, stream=None):
+    """output[t] = base[t] + scale * B (A x[t]) with the adapter ids[t] (int32 [tokens];
+    outside the pool: none, output[t] = base[t]).  x [tokens][cols]; base, what the
+    shared projection gave for x, and output, which may be base, [tokens][rows].
+    workspace: a contiguous uint8 GPU tensor of adapters_workspace_size bytes
+    (spb_adapters_*)."""
+    if not isinstance(adapters, Adapters):
+        _no(adapters, Adapters, "adapters")
+    dev, dt = _device(adapters.a, "adapters"), adapters.dtype
+    if not isinstance(ids, _Tensor) or ids.dim() != 1:
+        raise ValueError("ids must be a vector")
+    n = ids.shape[0]
+    if n > _INT_MAX:
+        _too_long(ids.shape, "ids")
+    pi = _flat(ids, "ids", torch.int32, (n,), dev)
+    px, sx = _rows(x, "x", dt, (n, adapters.cols), dev)
+    pb, sb = _rows(base, "base", dt, (n, adapters.rows), dev)
+    po, so = _rows(output, "output", dt, (n, adapters.rows), dev)
+    size = workspace.numel() if isinstance(workspace, _Tensor) else 0
+    pw = _flat(workspace, "workspace", torch.uint8, (size,), dev)
+    L = _lib.load()
+    fn = L.spb_adapters_f16 if adapters.kind == "f16" else L.spb_adapters_bf16
+    _lib.check(fn(adapters._ptr, pi, px, pb, po, n, sx, sb, so, pw, size, _on(stream, dev)),
+               "adapters_gpu")
+
+
+class Sampling(_Descriptor):
+    """Settings of sample_gpu (spb_sampling), each a number for all rows or a GPU vector
+    with one for each: temperature (float32; 0: greedy), top_k (int32; 0: all), top_p
+    (float32; 1: all) and min_p (float32; 0: all).  Vectors are read by the calls, so a
+    program may refill them between calls (and between replays of a captured one)."""
+
+    def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        self._dev, self.rows = None, None
+        ptrs, numbers = [], []
+        for name, x, dtype, off in (("temperature", temperature, torch.float32, 1.0),
+                                    ("top_k", top_k, torch.int32, 0),
+                                    ("top_p", top_p, torch.float32, 1.0),
+                                    ("min_p", min_p, torch.float32, 0.0)):
+            if isinstance(x, _Tensor):
+                if x.dim() != 1:
+                    raise ValueError(f"{name} must be a number or a vector")
+                _sizes((*x.shape, 0), name)
+                dev = _device(x, name)
+                if self._dev is not None and (dev, x.shape[0]) != (self._dev, self.rows):
+                    raise ValueError(f"{name} has {x.shape[0]} rows on cuda:{dev}, others "
+                                     f"{self.rows} on cuda:{self._dev}")
+                self._dev, self.rows = dev, x.shape[0]
+                ptrs.append(_flat(x, name, dtype, x.shape, dev))
+                numbers.append(off)
+            else:
+                ptrs.append(None)
+                numbers.append(_int32(int(x), name) if dtype is torch.int32 else float(x))
+        self.temperature, self.top_k, self.top_p, self.min_p = temperature, top_k, top_p, min_p
+        t, k, p, m = numbers
+        if not t >= 0 or k < 0 or not 0 <= p <= 1 or not 0 <= m <= 1:
+            raise ValueError(f"temperature {t} and top_k {k} must not be negative, top_p {p} and "
+                             f"min_p {m} must be in [0, 1]")
+        self._c = _lib.SamplingC(*ptrs, t, k, p, m)
+        self._ptr = ctypes.addressof(self._c)
+
+
+def _logits(t) -> str:
+    if not isinstance(t, _Tensor):
+        raise TypeError("logits must be a torch.Tensor")
+    kind = _LOGITS_KIND.get(t.dtype)
+    if kind is None:
+        raise TypeError(f"logits have dtype {t.dtype}, expected float32, float16 or bfloat16")
+    if t.dim() != 2:
+        raise ValueError("logits must be [rows][vocab]")
+    if max(t.shape) > _INT_MAX:
+        _too_long(t.shape, "logits")
+    return kind
+
+
+def sample_workspace_size(rows: int, vocab: int) -> int:
+    """Bytes of the workspace that sample_gpu needs for at most `rows` rows."""
+    n = int(_lib.load().spb_sample_workspace_size(_int32(rows, "rows"), _int32(vocab, "vocab")))
+    if n == 0:
+        _lib.check(1, "sample_workspace_size")
+    return n
+
+
+def sample_gpu(logits, uniforms, tokens, sampling: Sampling, workspace, logprobs=None,
+               stream=None):
+    """The next token of each row of logits [rows][vocab] (float32, fp16 or bf16) under
+    the settings, into tokens (int32 [rows]): in the order of falling logits, equal ones by
+    index, the first of the kept tokens whose weight with those before it passes
+    uniforms[row] (float32, in [0, 1)) times the kept weight; -1 where all logits are minus
+    infinity.  logprobs (float32 [rows]): the logarithm of its share of the kept weight.
+    workspace: a contiguous uint8 GPU tensor of sample_workspace_size bytes (spb_sample_*)."""
+    kind = _logits(logits)
+    dev, (n, vocab) = _device(logits, "logits"), logits.shape
+    pl, sl = _rows(logits, "logits", logits.dtype, logits.shape, dev)
+    pu = _flat(uniforms, "uniforms", torch.float32, (n,), dev)
+    pt = _flat(tokens, "tokens", torch.int32, (n,), dev)
+    pp = None if logprobs is None else _flat(logprobs, "logprobs", torch.float32, (n,), dev)
+    if not isinstance(sampling, Sampling):
+        _no(sampling, Sampling, "sampling")
+    if sampling._dev is not None and (sampling._dev != dev or sampling.rows != n):
+        raise ValueError(f"sampling has {sampling.rows} rows on cuda:{sampling._dev}, logits {n} "
+                         f"on cuda:{dev}")
+    size = workspace.numel() if isinstance(workspace, _Tensor) else 0
+    pw = _flat(workspace, "workspace", torch.uint8, (size,), dev)
+    fn = getattr(_lib.load(), "spb_sample_" + kind)
+    _lib.check(fn(pl, sl, pu, pt, pp, n, vocab, sampling._ptr, pw, size, _on(stream, dev)),
+               "sample_gpu")
+
+
+def token_logprobs_workspace_size(rows: int, vocab: int, top: int = 0) -> int:
+    """Bytes of the workspace that token_logprobs_gpu needs for at most `rows` rows."""
+    n = int(_lib.load().spb_token_logprobs_workspace_size(
+        _int32(rows, "rows"), _int32(vocab, "vocab"), _int32(top, "top")))
+    if n == 0:
+        _lib.check(1, "token_logprobs_workspace_size")
+    return n
+
+
+def token_logprobs_gpu(logits, tokens, logprobs, workspace, top_ids=None, top_logprobs=None,
+                       stream=None):
+    """Log-probabilities of tokens (int32 [rows]; outside the vocabulary: padding, the
+    row's outputs stay as they were) under logits [rows][vocab] (float32, fp16 or bf16), into
+    logprobs (float32 [rows]; both None: not asked for), and the likeliest tokens of each
+    row, the best first and equal ones by index, into top_ids (int32 [rows][top]) and
+    top_logprobs (float32 [rows][top]).  workspace: a contiguous uint8 GPU tensor of
+    token_logprobs_workspace_size bytes (spb_token_logprobs_*)."""
+    kind = _logits(logits)
+    dev, (n, vocab) = _device(logits, "logits"), logits.shape
+    pl, sl = _rows(logits, "logits", logits.dtype, logits.shape, dev)
+    pt = pp = pi = pv = None
+    top = 0
+    if tokens is not None or logprobs is not None:
+        pt = _flat(tokens, "tokens", torch.int32, (n,), dev)
+        pp = _flat(logprobs, "logprobs", torch.float32, (n,), dev)
+    if top_ids is not None or top_logprobs is not None:
+        if not isinstance(top_ids, _Tensor) or top_ids.dim() != 2:
+            raise ValueError("top_ids must be [rows][top]")
+        top = top_ids.shape[1]
+        if top > _INT_MAX:
+            _too_long(top_ids.shape, "top_ids")
+        pi = _flat(top_ids, "top_ids", torch.int32, (n, top), dev)
+        pv = _flat(top_logprobs, "top_logprobs", torch.float32, (n, top), dev)
+    size = workspace.numel() if isinstance(workspace, _Tensor) else 0
+    pw = _flat(workspace, "workspace", torch.uint8, (size,), dev)
+    fn = getattr(_lib.load(), "spb_token_logprobs_" + kind)
+    _lib.check(fn(pl, sl, pt, pp, pi, pv, n, vocab, top, pw, size, _on(stream, dev)),
+               "token_logprobs_gpu")
