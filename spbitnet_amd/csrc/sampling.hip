@@ -16,23 +16,41 @@
 #include "paged.hpp"
 #include "spbitnet_amd.h"
 
+#include <type_traits>
+
 namespace spb {
 namespace {
 
 constexpr int kMaxVocab = 1 << 24;
 constexpr int kMaxRows = 1 << 20;
 constexpr int kMaxTop = 64;
-constexpr int kRow = 1024;  // threads on one row
+constexpr int kRow = 512;  // threads on one row
 constexpr int kWaves = kRow / kWave;
 
 struct F32 {
     using Bits = float;
+    static constexpr int kVec = 4;  // logits of a 16-byte load
     static __device__ __forceinline__ float load(const Bits* p) { return *p; }
+    static __device__ __forceinline__ void unpack(const uint4& q, float* v) {
+        v[0] = __builtin_bit_cast(float, q.x);
+        v[1] = __builtin_bit_cast(float, q.y);
+        v[2] = __builtin_bit_cast(float, q.z);
+        v[3] = __builtin_bit_cast(float, q.w);
+    }
 };
 template <class T>
 struct Half {
     using Bits = uint16_t;
+    static constexpr int kVec = 8;
     static __device__ __forceinline__ float load(const Bits* p) { return T::to_float(*p); }
+    static __device__ __forceinline__ void unpack(const uint4& q, float* v) {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = T::to_float(static_cast<uint16_t>(w[i]));
+            v[2 * i + 1] = T::to_float(static_cast<uint16_t>(w[i] >> 16));
+        }
+    }
 };
 
 // A logit with NaN as minus infinity and one zero.
@@ -49,18 +67,143 @@ __device__ __forceinline__ float from_key(uint32_t k) {
     return __builtin_bit_cast(float, k >> 31 ? k & 0x7fffffffu : ~k);
 }
 
-// ---- reductions over a block of kRow threads; every thread gets the result ----
+// ---- over a wave and over a block of kRow threads -------------------------------------
+// Lane to lane moves (DPP) of 4- and 8-byte values: a step is an instruction or two, where
+// a shuffle goes through LDS.
 
+// The value of the lane that kCtrl names, or `none` where there is no such lane.
+template <int kCtrl, int kRowMask, class V>
+__device__ __forceinline__ V lane_move(V none, V v) {
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_bit_cast(
+            V, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v),
+                                           kCtrl, kRowMask, 0xf, false));
+    } else {
+        const auto n = __builtin_bit_cast(uint64_t, none), b = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = __builtin_amdgcn_update_dpp(static_cast<int>(n), static_cast<int>(b),
+                                                        kCtrl, kRowMask, 0xf, false);
+        const uint32_t hi =
+            __builtin_amdgcn_update_dpp(static_cast<int>(n >> 32), static_cast<int>(b >> 32),
+                                        kCtrl, kRowMask, 0xf, false);
+        return __builtin_bit_cast(V, static_cast<uint64_t>(hi) << 32 | lo);
+    }
+}
+
+// op over the lanes up to this one; none: op(none, v) = v.
 template <class V, class Op>
-__device__ __forceinline__ V block_reduce(V v, V* part, Op op) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = op(v, __shfl_xor(v, off, kWave));
+__device__ __forceinline__ V wave_scan(V v, V none, Op op) {
+    v = op(lane_move<0x111, 0xf>(none, v), v);  // 1, 2, 4, 8 lanes below, within 16
+    v = op(lane_move<0x112, 0xf>(none, v), v);
+    v = op(lane_move<0x114, 0xf>(none, v), v);
+    v = op(lane_move<0x118, 0xf>(none, v), v);
+    v = op(lane_move<0x142, 0xa>(none, v), v);  // lane 15 of the 16 below
+    v = op(lane_move<0x143, 0xc>(none, v), v);  // lane 31
+    return v;
+}
+
+struct Add {
+    template <class V>
+    __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
+};
+struct Min {
+    template <class V>
+    __device__ __forceinline__ V operator()(V a, V b) const { return b < a ? b : a; }
+};
+struct Max {
+    template <class V>
+    __device__ __forceinline__ V operator()(V a, V b) const { return b > a ? b : a; }
+};
+
+// The value of lane `from`, the same for all.
+template <class V>
+__device__ __forceinline__ V from_lane(V v, int from) {
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), from));
+    } else {
+        const auto b = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(b), from);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), from);
+        return __builtin_bit_cast(V, static_cast<uint64_t>(hi) << 32 | lo);
+    }
+}
+
+// op over the waves' results in part, by each wave (kWaves <= 16 lanes).
+template <class V, class Op>
+__device__ __forceinline__ V parts_scan(const V* part, V none, Op op) {
+    const int lane = threadIdx.x % kWave;
+    V v = lane < kWaves ? part[lane] : none;
+    v = op(lane_move<0x111, 0xf>(none, v), v);
+    v = op(lane_move<0x112, 0xf>(none, v), v);
+    v = op(lane_move<0x114, 0xf>(none, v), v);
+    if constexpr (kWaves > 8) v = op(lane_move<0x118, 0xf>(none, v), v);
+    return v;
+}
+
+// Every thread gets the result.  part: kWaves values.
+template <class V, class Op>
+__device__ __forceinline__ V block_reduce(V v, V none, V* part, Op op) {
+    v = wave_scan(v, none, op);
     __syncthreads();
-    if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = v;
+    if (threadIdx.x % kWave == kWave - 1) part[threadIdx.x / kWave] = v;
     __syncthreads();
-    V r = part[0];
-    for (int w = 1; w < kWaves; ++w) r = op(r, part[w]);
-    return r;
+    return from_lane(parts_scan(part, none, op), kWaves - 1);
+}
+
+// The sum of v over the threads before this one, and of all.  before() and after() are on
+// either side of a barrier.
+template <class V>
+struct BlockScan {
+    V upto;
+    __device__ __forceinline__ void before(V v, V* part) {
+        upto = wave_scan(v, V{0}, Add());
+        if (threadIdx.x % kWave == kWave - 1) part[threadIdx.x / kWave] = upto;
+    }
+    __device__ __forceinline__ V after(const V* part, V* total) {
+        const V below = lane_move<0x138, 0xf>(V{0}, upto);  // of the lane below
+        const V parts = parts_scan(part, V{0}, Add());
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+        *total = from_lane(parts, kWaves - 1);
+        return wave ? from_lane(parts, wave - 1) + below : below;
+    }
+};
+
+template <class V>
+__device__ __forceinline__ V block_scan(V v, V* part, V* total) {
+    BlockScan<V> s;
+    __syncthreads();
+    s.before(v, part);
+    __syncthreads();
+    return s.after(part, total);
+}
+
+// The value of lane ^ kLanes.
+template <int kLanes>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+    if constexpr (kLanes == 1) return __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, false);
+    if constexpr (kLanes == 2) return __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, false);
+    if constexpr (kLanes == 4) {  // the 8 mirrored (^ 7), then each 4 (^ 3)
+        const uint32_t m = __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false);
+        return __builtin_amdgcn_update_dpp(0, m, 0x1b, 0xf, 0xf, false);
+    }
+    if constexpr (kLanes == 8) return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false);
+    if constexpr (kLanes == 16) {
+        const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return threadIdx.x & 16 ? p[0] : p[1];
+    }
+    const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? p[0] : p[1];
+}
+__device__ __forceinline__ uint64_t lane_xor(uint64_t v, int lanes) {
+    const uint32_t lo = static_cast<uint32_t>(v), hi = static_cast<uint32_t>(v >> 32);
+    auto both = [](uint32_t h, uint32_t l) { return static_cast<uint64_t>(h) << 32 | l; };
+    switch (lanes) {
+        case 1: return both(lane_xor<1>(hi), lane_xor<1>(lo));
+        case 2: return both(lane_xor<2>(hi), lane_xor<2>(lo));
+        case 4: return both(lane_xor<4>(hi), lane_xor<4>(lo));
+        case 8: return both(lane_xor<8>(hi), lane_xor<8>(lo));
+        case 16: return both(lane_xor<16>(hi), lane_xor<16>(lo));
+        default: return both(lane_xor<32>(hi), lane_xor<32>(lo));
+    }
 }
 
 // ---- sampling -------------------------------------------------------------------
@@ -71,7 +214,7 @@ struct SampleArgs {
     const float* uniforms;
     int* tokens;
     float* logprobs;  // may be null
-    int rows, vocab;
+    int vocab;
     spb_sampling set;
 };
 
@@ -80,14 +223,17 @@ struct Settings {
     double inv_t, u;
     double top_p, min_p;  // 1 and 0: off
     int k;                // vocab: off
+    float bins;           // bins per unit of a logit
+    double unit, one;     // weights are added as whole numbers of 1 / unit, one = 2^52 / unit
 };
 
 __device__ __forceinline__ Settings settings_of(const SampleArgs& g, int row) {
     Settings s;
     float t = g.set.temperatures ? g.set.temperatures[row] : g.set.temperature;
     int k = g.set.top_ks ? g.set.top_ks[row] : g.set.top_k;
-    float p = g.set.top_ps ? g.set.top_ps[row] : g.set.top_p;
-    float m = g.set.min_ps ? g.set.min_ps[row] : g.set.min_p;
+    const float p = g.set.top_ps ? g.set.top_ps[row] : g.set.top_p;
+    const float m = g.set.min_ps ? g.set.min_ps[row] : g.set.min_p;
+    const float u = g.uniforms[row];
     if (k <= 0 || k > g.vocab) k = g.vocab;
     if (!(t > 0.0f)) {  // greedy: the first token of the order
         t = 1.0f;
@@ -98,32 +244,57 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs& g, int row) {
     s.min_p = m > 0.0f ? (m < 1.0f ? m : 1.0) : 0.0;
     s.k = k;
     s.inv_t = 1.0 / static_cast<double>(t);
-    const float u = g.uniforms[row];
     s.u = u > 0.0f ? (u < 1.0f ? u : 0x1.fffffep-1) : 0.0;
+    s.bins = static_cast<float>(__builtin_fmin(64.0 * __builtin_fmax(s.inv_t, 1.0), 0x1p40));
+    const int bits = 32 - __clz(g.vocab);  // vocab < 2^bits: a row of ones stays below 2^63
+    s.unit = __builtin_ldexp(1.0, min(49, 63 - bits));
+    s.one = __builtin_ldexp(1.0, max(3, bits - 11));
     return s;
 }
 
-// Weight of a logit (not minus infinity) below or at the maximum.
-__device__ __forceinline__ double weight_of(float l, float top, double inv_t) {
-    if (l == top) return 1.0;
-    const double d = (static_cast<double>(l) - static_cast<double>(top)) * inv_t;
-    return d > -64.0 ? exp(d) : 0.0;  // 2^24 weights below e^-64 are nothing beside the first, 1
+// exp(d) for d in (-64, 0]: 2^n times the exponential of the rest, at most ln(2) / 2, by its
+// series up to the 11th power: off by at most 7e-15 of itself (the 12th: 0.347^12 / 12!).
+// 18 instructions and no table: float64 runs at float32's rate here, and LDS is what the
+// histogram waits for.
+__device__ __forceinline__ double exp_of(double d) {
+    const double n = __builtin_rint(d * 0x1.71547652b82fep+0);      // 1 / ln 2
+    const double r = __builtin_fma(n, -0x1.62e42fefa39efp-1, d);    // ln 2
+    double p = __builtin_fma(r, 1.0 / 39916800, 1.0 / 3628800);
+    p = __builtin_fma(r, p, 1.0 / 362880);
+    p = __builtin_fma(r, p, 1.0 / 40320);
+    p = __builtin_fma(r, p, 1.0 / 5040);
+    p = __builtin_fma(r, p, 1.0 / 720);
+    p = __builtin_fma(r, p, 1.0 / 120);
+    p = __builtin_fma(r, p, 1.0 / 24);
+    p = __builtin_fma(r, p, 1.0 / 6);
+    p = __builtin_fma(r, p, 0.5);
+    p = __builtin_fma(r, p, 1.0);
+    p = __builtin_fma(r, p, 1.0);
+    return __builtin_ldexp(p, static_cast<int>(n));
 }
 
-// Where a sum of counts or weights along the order passes a bound: the logit there, how
-// many of that logit stand before the place, and the sums before it.
-struct Place {
-    uint32_t key;
-    int before_ties;    // tokens of that logit before the place
-    long long count;    // tokens before the place
-    double mass;        // weights before the place
-};
+// Weight of a logit (not minus infinity) at or below `top`.
+__device__ __forceinline__ double weight_of(float l, float top, double inv_t) {
+    const double d = (static_cast<double>(l) - static_cast<double>(top)) * inv_t;
+    if (l == top) return 1.0;
+    // 2^24 weights below e^-64 are nothing beside the first, 1
+    return d > -64.0 ? exp_of(d) : 0.0;
+}
+
+// A weight as a whole number of 1 / unit, one = 2^52 / unit.
+__device__ __forceinline__ unsigned long long fixed(double w, double one) {
+    return __builtin_bit_cast(unsigned long long, w + one) -
+           __builtin_bit_cast(unsigned long long, one);
+}
+
+// -- from the row itself, in up to a dozen readings: for rows whose borders fall among
+// -- thousands of nearly equal logits
 
 struct Hist {
     unsigned long long mass[256];
     int count[256];
     int digit;
-    long long before_count;
+    int before_count;
     unsigned long long before_mass;
 };
 
@@ -132,24 +303,26 @@ struct Row {
     const typename T::Bits* l;
     int vocab;
     float top;
-    double inv_t;
-    double one;   // 2^52 / unit: added to a weight, leaves it as a multiple of 1 / unit
-    double unit;  // weights are whole numbers of 1 / unit; a row of ones stays below 2^63
+    double inv_t, one, unit;
+
+    __device__ __forceinline__ double weight(float v) const { return weight_of(v, top, inv_t); }
 };
 
-__device__ __forceinline__ unsigned long long fixed(double w, double one) {
-    return __builtin_bit_cast(unsigned long long, w + one) -
-           __builtin_bit_cast(unsigned long long, one);
-}
+// A place in the order: the logit there, how many of that logit stand before it, and the
+// weights before it.
+struct Place {
+    uint32_t key;
+    int before_ties;
+    double mass;
+};
 
-// The first place of the order whose token ends past the bound: by count, the token of
-// rank `rank` (so the sums before it are those of the first `rank` tokens); by mass, the
-// first token whose weight with those before it is > bound.  Four digits of the key, each
-// a histogram of counts and weights of the tokens that share the digits before it.
+// By count, the token of rank `rank`; by mass, the first token whose weight with those
+// before it is above bound (at the end of all of them the last with a weight).  Four
+// digits of the key, each a histogram of the tokens that share the digits before it.
 template <bool kMass, class T>
-__device__ Place select(const Row<T>& r, long long rank, double bound, Hist& h) {
+__device__ Place select(const Row<T>& r, int rank, double bound, Hist& h) {
     uint32_t prefix = 0;
-    long long count = 0;
+    int count = 0;
     unsigned long long mass = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
         __syncthreads();
@@ -165,27 +338,48 @@ __device__ Place select(const Row<T>& r, long long rank, double bound, Hist& h) 
             if (shift < 24 && (key >> (shift + 8)) != (prefix >> (shift + 8))) continue;
             const int d = key >> shift & 255;
             atomicAdd(&h.count[d], 1);
-            atomicAdd(&h.mass[d], fixed(weight_of(l, r.top, r.inv_t), r.one));
+            atomicAdd(&h.mass[d], fixed(r.weight(l), r.one));
         }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            int last = -1, d = 255;
-            long long c = count, lc = 0;
-            unsigned long long m = mass, lm = 0;
-            for (; d >= 0; --d) {
-                if (!h.count[d]) continue;
-                if (!kMass || h.mass[d]) {  // past every weight: the last token that has one
-                    last = d;
-                    lc = c;
-                    lm = m;
-                }
-                c += h.count[d];
-                m += h.mass[d];
-                if (kMass ? static_cast<double>(m) > bound * r.unit : c > rank) break;
+        if (threadIdx.x < kWave) {  // a wave takes the digits from the highest on, 4 a lane
+            const int lane = threadIdx.x;
+            int c[4], sum_c = 0;
+            unsigned long long m[4], sum_m = 0;
+            for (int i = 0; i < 4; ++i) {
+                sum_c += c[i] = h.count[255 - 4 * lane - i];
+                sum_m += m[i] = h.mass[255 - 4 * lane - i];
             }
-            h.digit = last;
-            h.before_count = lc;
-            h.before_mass = lm;
+            int upto_c = sum_c;
+            unsigned long long upto_m = sum_m;
+            for (int off = 1; off < kWave; off <<= 1) {
+                const int oc = __shfl_up(upto_c, off, kWave);
+                const unsigned long long om = __shfl_up(upto_m, off, kWave);
+                if (lane >= off) {
+                    upto_c += oc;
+                    upto_m += om;
+                }
+            }
+            int bc = count + upto_c - sum_c, at_c = 0, first = -1, last = -1;
+            unsigned long long bm = mass + upto_m - sum_m, at_m = 0;
+            for (int i = 0; i < 4 && first < 0; ++i) {
+                if (kMass ? m[i] != 0 : c[i] != 0) {
+                    last = i;
+                    at_c = bc;
+                    at_m = bm;
+                }
+                bc += c[i];
+                bm += m[i];
+                if (last == i && (kMass ? static_cast<double>(bm) > bound * r.unit : bc > rank))
+                    first = i;
+            }
+            // the first digit that passes, or the last that has tokens
+            const unsigned long long passed = __ballot(first >= 0), some = __ballot(last >= 0);
+            const int to = passed ? __ffsll(passed) - 1 : some ? 63 - __clzll(some) : -1;
+            if (to < 0 ? lane == 0 : lane == to) {
+                h.digit = to < 0 ? -1 : 255 - 4 * lane - last;
+                h.before_count = at_c;
+                h.before_mass = at_m;
+            }
         }
         __syncthreads();
         if (h.digit < 0) break;
@@ -196,110 +390,660 @@ __device__ Place select(const Row<T>& r, long long rank, double bound, Hist& h) 
     Place p;
     p.key = prefix;
     const int ties = h.count[prefix & 255];
-    const double w = weight_of(from_key(prefix), r.top, r.inv_t);
+    const double w = r.weight(from_key(prefix));
     p.mass = static_cast<double>(mass) / r.unit;
-    long long in = kMass ? static_cast<long long>((bound - p.mass) / w) : rank - count;
-    in = in < 0 ? 0 : in >= ties ? ties - 1 : in;
-    p.before_ties = static_cast<int>(in);
-    p.count = count + in;
-    p.mass += in * w;
+    double in = kMass ? (bound - p.mass) / w : rank - count;
+    in = in < ties - 1 ? in : ties - 1;
+    p.before_ties = in > 0 ? static_cast<int>(in) : 0;
+    p.mass += p.before_ties * w;
     return p;
 }
 
-// One block a row, everything from the row itself: right for any row, at up to a dozen
-// readings of it.
 template <class T>
-__global__ __launch_bounds__(kRow) void sample_row_kernel(SampleArgs g) {
-    __shared__ Hist h;
+__device__ void sample_row(const SampleArgs& g, int row, const Settings& s, float top, Hist& h) {
     __shared__ union {
-        float f[kWaves];
         int i[kWaves];
         unsigned long long u[kWaves];
     } part;
-    const int row = blockIdx.x;
-    const Settings s = settings_of(g, row);
     Row<T> r;
     r.l = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
     r.vocab = g.vocab;
     r.inv_t = s.inv_t;
-    const int bits = 32 - __clz(g.vocab);  // vocab < 2^bits
-    r.unit = __builtin_ldexp(1.0, min(49, 63 - bits));
-    r.one = __builtin_ldexp(1.0, 52) / r.unit;
-    float top = -__builtin_inff();
+    r.top = top;
+    r.unit = s.unit;
+    r.one = s.one;
+    // the kept mass: the least of what each filter keeps
+    unsigned long long all = 0, high = 0;
     int live = 0;
     for (int i = threadIdx.x; i < g.vocab; i += kRow) {
         const float l = clean(T::load(r.l + i));
-        top = __builtin_fmaxf(top, l);
-        live += l != -__builtin_inff();
-    }
-    r.top = top = block_reduce(top, part.f, [](float a, float b) { return __builtin_fmaxf(a, b); });
-    live = block_reduce(live, part.i, [](int a, int b) { return a + b; });
-    if (live == 0) {
-        if (threadIdx.x == 0) {
-            g.tokens[row] = -1;
-            if (g.logprobs) g.logprobs[row] = -__builtin_inff();
-        }
-        return;
-    }
-    // the kept mass: the least of what each filter keeps
-    unsigned long long all = 0, high = 0;
-    for (int i = threadIdx.x; i < g.vocab; i += kRow) {
-        const float l = clean(T::load(r.l + i));
         if (l == -__builtin_inff()) continue;
-        const double w = weight_of(l, r.top, r.inv_t);
+        ++live;
+        const double w = r.weight(l);
         all += fixed(w, r.one);
         if (w >= s.min_p) high += fixed(w, r.one);
     }
-    auto add = [](unsigned long long a, unsigned long long b) { return a + b; };
-    double kept = static_cast<double>(block_reduce(all, part.u, add)) / r.unit;
-    const double over = static_cast<double>(block_reduce(high, part.u, add)) / r.unit;
+    live = block_reduce(live, 0, part.i, Add());
+    double kept = static_cast<double>(block_reduce(all, 0ull, part.u, Add())) / r.unit;
+    const double over = static_cast<double>(block_reduce(high, 0ull, part.u, Add())) / r.unit;
     if (s.k < live) kept = select<false>(r, s.k, 0.0, h).mass;
     if (s.top_p < 1.0) {
-        // tokens stay while the mass before them is below p * kept: the first one that
-        // reaches it is the last
+        // the token at the place passes the bound: it is the last that stays, unless the
+        // mass before it is the bound already
         const double bound = s.top_p * kept;
-        Place p = select<true>(r, 0, bound, h);
-        // the place's token passes the bound (mass with it > bound); it stays unless
-        // the mass before it is the bound already
-        const double with = p.mass + weight_of(from_key(p.key), r.top, r.inv_t);
-        const double cut = p.mass < bound ? with : p.mass;
+        const Place p = select<true>(r, 0, bound, h);
+        const double cut = p.mass < bound ? p.mass + r.weight(from_key(p.key)) : p.mass;
         kept = cut < kept ? cut : kept;
     }
     if (s.min_p > 0.0 && over < kept) kept = over;
     const Place p = select<true>(r, 0, s.u * kept, h);
     // the before_ties-th token of that logit, in the order of indices
-    int here = 0;
     const int each = (g.vocab + kRow - 1) / kRow;
     const int first = min(static_cast<int>(threadIdx.x) * each, g.vocab);
     const int end = min(first + each, g.vocab);
+    int here = 0;
     for (int i = first; i < end; ++i) here += key_of(clean(T::load(r.l + i))) == p.key;
-    int upto = here;
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-        const int o = __shfl_up(upto, off, kWave);
-        if (lane >= off) upto += o;
-    }
-    __syncthreads();
-    if (lane == kWave - 1) part.i[wave] = upto;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) upto += part.i[w];
-    int left = p.before_ties - (upto - here);
-    if (left >= 0 && left < here) {
-        for (int i = first; i < end; ++i) {
-            if (key_of(clean(T::load(r.l + i))) != p.key) continue;
-            if (left-- == 0) {
-                g.tokens[row] = i;
-                if (g.logprobs)
-                    g.logprobs[row] = static_cast<float>(
-                        log(weight_of(from_key(p.key), r.top, r.inv_t) / kept));
-                break;
-            }
-        }
+    int ties;
+    int left = p.before_ties - block_scan(here, part.i, &ties);
+    if (left < 0 || left >= here) return;
+    for (int i = first; i < end; ++i) {
+        if (key_of(clean(T::load(r.l + i))) != p.key) continue;
+        if (left-- > 0) continue;
+        g.tokens[row] = i;
+        if (g.logprobs)
+            g.logprobs[row] = static_cast<float>(log(r.weight(from_key(p.key)) / kept));
+        break;
     }
 }
 
-size_t sample_workspace(int rows, int vocab) { return 256; }
+// -- with a histogram: of 2048 bins of the logits, from the row's largest down, the weights
+// -- and, where top-k is on, the tokens.  Bins are 1/64 of the temperature wide, at most 1/64;
+// -- what is below the last is in the last.  The sums say which bins hold a border of a
+// -- filter or the place of u: their tokens (some hundreds, mostly) are taken from the row,
+// -- sorted, and decide.  Between the bins nothing needs an order.  So a row is read three
+// -- times: for its largest logit, for the bins, and for those tokens; parts whose largest
+// -- logit is below the bins in question are left out the third time.
+
+constexpr int kBins = 2048;
+constexpr int kOwn = kBins / kRow;  // bins of a thread
+constexpr int kList = 4096;         // tokens of the bins in question
+constexpr int kPeaks = 1024;        // units of a row whose largest logit is kept in LDS
+constexpr int kSplitBlock = 256;
+
+struct SampleWork {
+    float* peaks;              // [rows][units]: the largest logit of each
+    unsigned long long* mass;  // [rows][kBins]
+    int* count;                // [rows][kBins], where top-k is on
+    unsigned long long* list;  // [rows][kList]
+    int* listed;               // [rows]: tokens in the list, and blocks that are done
+    int* done;
+    int first, rows, units, parts;  // rows of this launch, blocks of a row in the last kernel
+};
+
+// A wave's part of a row: 4 loads of 16 bytes a lane, from 16-byte boundaries on, so unit u
+// begins up to 7 logits before u * kSize.
+template <class T>
+struct Unit {
+    static constexpr int kLoads = 4, kSize = kLoads * kWave * T::kVec;
+    uint4 bits[kLoads];
+
+    static __device__ __forceinline__ int start(const typename T::Bits* row, int unit) {
+        const int skew = (reinterpret_cast<uintptr_t>(row) & 15) / sizeof(typename T::Bits);
+        return unit * kSize - skew + static_cast<int>(threadIdx.x % kWave) * T::kVec;
+    }
+    __device__ __forceinline__ void load(const typename T::Bits* row, int vocab, int unit) {
+        const int first = start(row, unit);
+#pragma unroll
+        for (int n = 0; n < kLoads; ++n) {
+            const int i = first + n * kWave * T::kVec;
+            if (i >= 0 && i + T::kVec <= vocab)
+                bits[n] = *reinterpret_cast<const uint4*>(row + i);
+        }
+    }
+    // f(logit, index) of each loaded logit; minus infinity outside the row.
+    template <class F>
+    __device__ __forceinline__ void each(const typename T::Bits* row, int vocab, int unit, F f) const {
+        const int first = start(row, unit);
+#pragma unroll
+        for (int n = 0; n < kLoads; ++n) {
+            const int i = first + n * kWave * T::kVec;
+            float v[T::kVec];
+            if (i >= 0 && i + T::kVec <= vocab) {
+                T::unpack(bits[n], v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < T::kVec; ++e)
+                    v[e] = i + e >= 0 && i + e < vocab ? T::load(row + i + e) : -__builtin_inff();
+            }
+#pragma unroll
+            for (int e = 0; e < T::kVec; ++e) f(clean(v[e]), i + e);
+        }
+    }
+};
+
+template <class T>
+int units_of(int vocab) {
+    const int most_skew = 16 / static_cast<int>(sizeof(typename T::Bits)) - 1;
+    return (vocab + most_skew + Unit<T>::kSize - 1) / Unit<T>::kSize;
+}
+
+// Units `first`, first + step, ... of a row that `want` names, the next one's loads in flight.
+template <class T, class Want, class F>
+__device__ __forceinline__ void each_unit(const typename T::Bits* row, int vocab, int first, int step,
+                                          int units, Want want, F f) {
+    auto next = [&](int u) {
+        while (u < units && !want(u)) u += step;
+        return u;
+    };
+    Unit<T> now, ahead;
+    int u = next(first);
+    if (u < units) now.load(row, vocab, u);
+    while (u < units) {
+        const int v = next(u + step);
+        if (v < units) ahead.load(row, vocab, v);
+        f(now, u);
+        now = ahead;
+        u = v;
+    }
+}
+
+// A logit's bin below `top`.
+__device__ __forceinline__ int bin_of(float l, float top, float bins) {
+    return static_cast<int>(__builtin_fminf((top - l) * bins, kBins - 1.0f));
+}
+
+template <class T>
+__device__ __forceinline__ float unit_peak(const Unit<T>& x, const typename T::Bits* row, int vocab, int u) {
+    float peak = -__builtin_inff();
+    x.each(row, vocab, u, [&](float l, int) { peak = __builtin_fmaxf(peak, l); });
+    return from_lane(wave_scan(peak, -__builtin_inff(), Max()), kWave - 1);
+}
+
+// Adds a unit to a histogram in LDS.
+template <class T>
+__device__ __forceinline__ void add_unit(const Unit<T>& x, const typename T::Bits* row, int vocab, int u,
+                                         const Settings& s, float top, unsigned long long* mass, int* count) {
+    x.each(row, vocab, u, [&](float l, int) {
+        if (l == -__builtin_inff()) return;
+        const int b = bin_of(l, top, s.bins);
+        const unsigned long long m = fixed(weight_of(l, top, s.inv_t), s.one);
+        if (m) atomicAdd(&mass[b], m);
+        if (count) atomicAdd(&count[b], 1);
+    });
+}
+
+// Few rows: units over blocks.  First their largest logits ...
+template <class T>
+__global__ __launch_bounds__(kSplitBlock) void sample_peaks_kernel(SampleArgs g, SampleWork w) {
+    const int r = blockIdx.y, row = w.first + r, tid = threadIdx.x;
+    const int u = blockIdx.x * (kSplitBlock / kWave) + tid / kWave;
+    const typename T::Bits* logits = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
+    Unit<T> x;
+    if (u < w.units) x.load(logits, g.vocab, u);
+    for (int b = blockIdx.x * kSplitBlock + tid; b < kBins; b += gridDim.x * kSplitBlock) {
+        w.mass[static_cast<long>(r) * kBins + b] = 0;
+        w.count[static_cast<long>(r) * kBins + b] = 0;
+    }
+    if (blockIdx.x == 0 && tid == 0) {
+        w.listed[r] = 0;
+        w.done[r] = 0;
+    }
+    if (u >= w.units) return;
+    const float peak = unit_peak<T>(x, logits, g.vocab, u);
+    if (tid % kWave == 0) w.peaks[static_cast<long>(r) * w.units + u] = peak;
+}
+
+__device__ __forceinline__ float row_peak(const float* peaks, int units, int block, float* part, int parts) {
+    float top = -__builtin_inff();
+    for (int i = threadIdx.x; i < units; i += block) top = __builtin_fmaxf(top, peaks[i]);
+    top = wave_scan(top, -__builtin_inff(), Max());
+    if (threadIdx.x % kWave == kWave - 1) part[threadIdx.x / kWave] = top;
+    __syncthreads();
+    top = part[0];
+    for (int i = 1; i < parts; ++i) top = __builtin_fmaxf(top, part[i]);
+    return top;
+}
+
+// ... then the histogram, added up in LDS and from there in memory.
+template <class T>
+__global__ __launch_bounds__(kSplitBlock) void sample_bins_kernel(SampleArgs g, SampleWork w) {
+    __shared__ unsigned long long mass[kBins];
+    __shared__ int count[kBins];
+    __shared__ float part[kSplitBlock / kWave];
+    const int r = blockIdx.y, row = w.first + r, tid = threadIdx.x;
+    const int u = blockIdx.x * (kSplitBlock / kWave) + tid / kWave;
+    const typename T::Bits* logits = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
+    Unit<T> x;
+    if (u < w.units) x.load(logits, g.vocab, u);
+    const Settings s = settings_of(g, row);
+    const bool by_count = s.k < g.vocab;
+    for (int b = tid; b < kBins; b += kSplitBlock) {
+        mass[b] = 0;
+        if (by_count) count[b] = 0;
+    }
+    const float top = row_peak(w.peaks + static_cast<long>(r) * w.units, w.units, kSplitBlock, part,
+                               kSplitBlock / kWave);
+    if (__builtin_isinf(top)) return;
+    if (u < w.units) add_unit<T>(x, logits, g.vocab, u, s, top, mass, by_count ? count : nullptr);
+    __syncthreads();
+    for (int b = tid; b < kBins; b += kSplitBlock) {
+        if (mass[b])
+            __hip_atomic_fetch_add(&w.mass[static_cast<long>(r) * kBins + b], mass[b], __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_AGENT);
+        if (by_count && count[b])
+            __hip_atomic_fetch_add(&w.count[static_cast<long>(r) * kBins + b], count[b], __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_AGENT);
+    }
+}
+
+// Sorts list[0, n) ascending, n <= kRow * kEach; a thread holds kEach neighbours.  Pairs at
+// doubling distances: within a thread, within a wave by lane moves, and only pairs of
+// different waves through LDS.
+template <int kEach>
+__device__ __forceinline__ void sort_list(unsigned long long* list, int n) {
+    const int tid = threadIdx.x;
+    int size = 2 * kEach;
+    while (size < n) size *= 2;
+    const bool active = tid / kWave * kWave * kEach < size;  // whole waves
+    uint64_t v[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) v[e] = tid * kEach + e < n ? list[tid * kEach + e] : ~0ull;
+    auto keep = [](uint64_t& a, uint64_t o, bool smaller) { a = (o < a) == smaller ? o : a; };
+    for (int k = 2; k <= size; k *= 2) {
+        for (int d = k / 2; d >= kEach; d /= 2) {
+            const int lanes = d / kEach;
+            const bool smaller = ((tid * kEach & d) == 0) == ((tid * kEach & k) == 0);
+            if (lanes >= kWave) {
+                __syncthreads();
+                if (active)
+#pragma unroll
+                    for (int e = 0; e < kEach; ++e) list[tid * kEach + e] = v[e];
+                __syncthreads();
+                if (active)
+#pragma unroll
+                    for (int e = 0; e < kEach; ++e)
+                        keep(v[e], list[(tid ^ lanes) * kEach + e], smaller);
+            } else if (active) {
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) keep(v[e], lane_xor(v[e], lanes), smaller);
+            }
+        }
+        if constexpr (kEach > 1) {
+#pragma unroll
+            for (int d = kEach / 2; d > 0; d /= 2) {
+                if (d >= k) continue;
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    if (e & d) continue;
+                    const bool up = ((tid * kEach + e) & k) == 0;
+                    const uint64_t a = v[e], b = v[e + d];
+                    if ((b < a) == up) {
+                        v[e] = b;
+                        v[e + d] = a;
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+        if (tid * kEach + e < n) list[tid * kEach + e] = v[e];
+    __syncthreads();
+}
+
+// The token of a row.  kWhole: all of it by this block; else from the histogram in memory, the
+// tokens in question gathered by w.parts blocks.
+template <class T, bool kWhole>
+__global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, SampleWork w) {
+    __shared__ union {
+        unsigned long long fixed[kBins];
+        double before[kBins + 1];  // before each bin, and of all
+    } masses;
+    double* const mass = masses.before;
+    __shared__ int count[kBins + 1];
+    __shared__ union {
+        unsigned long long list[kList];  // ~key, index: ascending in the order
+        Hist hist;
+    } u;
+    __shared__ float own_peaks[kWhole ? kPeaks : 1];
+    __shared__ union {
+        float f[kWaves];
+        int i[kWaves];
+        double d[kWaves];
+    } part;
+    __shared__ struct {
+        double mass[kWaves];
+        int count[kWaves];
+    } sums;
+    __shared__ uint32_t marked[kBins / 32];
+    __shared__ int listed, found[5], heaviest_bin, base;
+    __shared__ double cut;
+    const int r = kWhole ? blockIdx.x : blockIdx.y, q = kWhole ? 0 : blockIdx.x;
+    const int row = w.first + r, tid = threadIdx.x;
+    const int lane = tid % kWave, wave = tid / kWave, own = tid * kOwn;
+    const typename T::Bits* logits = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
+    const float* peaks = kWhole ? own_peaks : w.peaks + static_cast<long>(r) * w.units;
+    const Settings s = settings_of(g, row);
+    const bool by_count = s.k < g.vocab;
+    if (tid < 5) found[tid] = kBins;
+    if (tid == 5) listed = 0;
+    if (tid == 6) heaviest_bin = 0;
+    if (tid < kBins / 32) marked[tid] = 0;
+    auto all_units = [](int) { return true; };
+    float top = -__builtin_inff();
+    if constexpr (kWhole) {
+        each_unit<T>(logits, g.vocab, wave, kWaves, w.units, all_units, [&](const Unit<T>& x, int u) {
+            const float peak = unit_peak<T>(x, logits, g.vocab, u);
+            if (lane == 0 && u < kPeaks) own_peaks[u] = peak;
+            top = __builtin_fmaxf(top, peak);
+        });
+    } else {
+        for (int i = tid; i < w.units; i += kRow) top = __builtin_fmaxf(top, peaks[i]);
+    }
+    top = block_reduce(top, -__builtin_inff(), part.f, Max());
+    if (top == -__builtin_inff()) {
+        if (q == 0 && tid == 0) {
+            g.tokens[row] = -1;
+            if (g.logprobs) g.logprobs[row] = top;
+        }
+        return;
+    }
+    if (top == __builtin_inff()) {  // bins below an infinite logit have no width
+        if (q == 0) sample_row<T>(g, row, s, top, u.hist);
+        return;
+    }
+    // kOwn neighbouring bins a thread
+    double mine[kOwn];
+    int mine_count[kOwn] = {};
+    if constexpr (kWhole) {
+        for (int b = tid; b < kBins; b += kRow) {
+            masses.fixed[b] = 0;
+            if (by_count) count[b] = 0;
+        }
+        __syncthreads();
+        each_unit<T>(logits, g.vocab, wave, kWaves, w.units, all_units, [&](const Unit<T>& x, int u) {
+            add_unit<T>(x, logits, g.vocab, u, s, top, masses.fixed, by_count ? count : nullptr);
+        });
+        __syncthreads();
+    }
+#pragma unroll
+    for (int h = 0; h < kOwn; ++h) {
+        const long at = static_cast<long>(r) * kBins + own + h;
+        mine[h] = static_cast<double>(kWhole ? masses.fixed[own + h] : w.mass[at]) / s.unit;
+        if (by_count) mine_count[h] = kWhole ? count[own + h] : w.count[at];
+    }
+    double total, sum = 0.0;
+    int total_count, sum_count = 0;
+#pragma unroll
+    for (int h = 0; h < kOwn; ++h) {
+        sum += mine[h];
+        sum_count += mine_count[h];
+    }
+    {
+        BlockScan<double> m;
+        BlockScan<int> c;
+        m.before(sum, sums.mass);
+        c.before(sum_count, sums.count);
+        __syncthreads();
+        sum = m.after(sums.mass, &total);
+        sum_count = c.after(sums.count, &total_count);
+    }
+#pragma unroll
+    for (int h = 0; h < kOwn; ++h) {
+        mass[own + h] = sum;
+        count[own + h] = sum_count;
+        sum += mine[h];
+        sum_count += mine_count[h];
+    }
+    if (tid == 0) {
+        mass[kBins] = total;
+        count[kBins] = total_count;
+    }
+    __syncthreads();
+    // bins in question.  The bounds of a sum that a bin leaves open give a first and a last
+    // bin, a little widened: sums over bins and over tokens round differently.
+    const double less = 1.0 - 0x1p-36, more = 1.0 + 0x1p-36;
+    double end[kOwn];
+    int heavy = -1;
+    auto find = [&](int which, auto holds) {  // the first bin of which it holds
+        int first = kBins;
+#pragma unroll
+        for (int h = kOwn - 1; h >= 0; --h)
+            if (holds(h)) first = own + h;
+        const unsigned long long set = __ballot(first < kBins);
+        if (set) {
+            first = from_lane(first, __ffsll(set) - 1);
+            if (lane == 0) atomicMin(&found[which], first);
+        }
+    };
+#pragma unroll
+    for (int h = 0; h < kOwn; ++h) {
+        end[h] = mass[own + h + 1];
+        if (mine[h] > 0.0) heavy = own + h;
+    }
+    const unsigned long long heavies = __ballot(heavy >= 0);
+    if (heavies) {
+        heavy = from_lane(heavy, 63 - __clzll(heavies));
+        if (lane == 0) atomicMax(&heaviest_bin, heavy);
+    }
+    if (by_count) find(0, [&](int h) { return count[own + h + 1] >= s.k; });
+    __syncthreads();
+    // bins behind the last one with a weight need no order: whatever is kept of them
+    const int heaviest = heaviest_bin;
+    int k_bin = kBins;
+    double low = total, upper = total;  // bounds of what top-k keeps
+    if (by_count && s.k < total_count && found[0] <= heaviest) {
+        k_bin = found[0];
+        low = upper = mass[k_bin + 1];
+        if (count[k_bin + 1] == s.k)
+            k_bin = kBins;  // ends with the bin
+        else
+            low = mass[k_bin];
+    }
+    const double k_mass = upper;  // of top-k, where no bin is in question
+    int first_marked = kBins, last_marked = -1;
+    auto mark = [&](int a, int b) {
+        a = max(a, 0);
+        b = min(b, heaviest);
+        if (a > b) return;
+        first_marked = min(first_marked, a);
+        last_marked = max(last_marked, b);
+        if (tid < kBins / 32 && tid >= a / 32 && tid <= b / 32) {
+            uint32_t bits = ~0u;
+            if (tid == a / 32) bits &= ~0u << (a % 32);
+            if (tid == b / 32) bits &= ~0u >> (31 - b % 32);
+            marked[tid] |= bits;  // its thread's own word
+        }
+    };
+    if (k_bin < kBins) mark(k_bin, k_bin);
+    if (s.top_p < 1.0) {
+        find(1, [&](int h) { return end[h] >= s.top_p * low * less; });
+        find(2, [&](int h) { return end[h] >= s.top_p * upper * more; });
+        __syncthreads();
+        const int a = min(found[1], heaviest), b = min(found[2], heaviest);
+        mark(a, b);
+        low = __builtin_fmin(low, s.top_p * low * less);
+        upper = __builtin_fmin(upper, mass[b + 1]);
+    }
+    int p_bin = kBins;  // the last bin that min-p may keep a part of
+    if (s.min_p > 0.0) {
+        const double x = -log(s.min_p) / s.inv_t * s.bins;
+        const double off = 1e-6 + 3e-7 * x;  // a logit's place among the bins is float32
+        const double a = x - off, b = x + off;
+        const int first = a > 0.0 ? (a < kBins - 1.0 ? static_cast<int>(a) : kBins - 1) : 0;
+        p_bin = b < kBins - 1.0 ? static_cast<int>(b) : kBins - 1;
+        mark(first, p_bin);
+        low = __builtin_fmin(low, mass[first]);
+        upper = __builtin_fmin(upper, mass[p_bin + 1]);
+    }
+    low = __builtin_fmax(low, 1.0);  // the first token stays
+    find(3, [&](int h) { return end[h] > s.u * low * less; });
+    find(4, [&](int h) { return end[h] > s.u * upper * more; });
+    __syncthreads();
+    mark(min(found[3], heaviest), min(found[4], heaviest));
+    const int from = first_marked, to = last_marked;
+    __syncthreads();
+    // their tokens
+    each_unit<T>(
+        logits, g.vocab, q * kWaves + wave, w.parts * kWaves, w.units,
+        [&](int u) { return (kWhole && u >= kPeaks) || bin_of(peaks[u], top, s.bins) <= to; },
+        [&](const Unit<T>& x, int unit) {
+            x.each(logits, g.vocab, unit, [&](float l, int i) {
+                const int b = bin_of(l, top, s.bins);
+                if (b < from || b > to || l == -__builtin_inff()) return;
+                if (!(marked[b / 32] >> (b % 32) & 1)) return;
+                const int place = atomicAdd(&listed, 1);
+                if (place < kList)
+                    u.list[place] = static_cast<unsigned long long>(~key_of(l)) << 32 |
+                                    static_cast<uint32_t>(i);
+            });
+        });
+    __syncthreads();
+    int n = listed;
+    if (!kWhole && w.parts > 1) {  // the block that is done last has all of them, and goes on
+        // Stores and loads past the per-XCD L2s (agent scope), each block's stores done
+        // (s_waitcnt) before it counts itself; a fence would write a whole L2 back: 90 us of
+        // 150 at 32 rows of 128256.
+        if (tid == 0)
+            base = __hip_atomic_fetch_add(&w.listed[r], n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        const int to = base;
+        for (int i = tid; i < min(n, kList); i += kRow)
+            if (to + i < kList)
+                __hip_atomic_store(&w.list[static_cast<long>(r) * kList + to + i], u.list[i],
+                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (tid == 0)
+            base = __hip_atomic_fetch_add(&w.done[r], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (base != w.parts - 1) return;
+        n = __hip_atomic_load(&w.listed[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int i = tid; i < min(n, kList); i += kRow)
+            u.list[i] = __hip_atomic_load(&w.list[static_cast<long>(r) * kList + i],
+                                          __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+    }
+    if (n > kList) {
+        sample_row<T>(g, row, s, top, u.hist);
+        return;
+    }
+    if (n <= kRow)
+        sort_list<1>(u.list, n);
+    else if (n <= 2 * kRow)
+        sort_list<2>(u.list, n);
+    else
+        sort_list<kList / kRow>(u.list, n);
+    // a thread's neighbours in the list: their weights, and those before them
+    constexpr int kEach = kList / kRow;
+    const int each = (n + kRow - 1) / kRow, at = tid * each;
+    double weight[kEach], before[kEach];
+    int bin[kEach];
+    sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        weight[e] = 0.0;
+        bin[e] = -1;
+        if (e >= each || at + e >= n) continue;
+        const float l = from_key(~static_cast<uint32_t>(u.list[at + e] >> 32));
+        weight[e] = weight_of(l, top, s.inv_t);
+        bin[e] = bin_of(l, top, s.bins);
+        before[e] = sum;
+        sum += weight[e];
+    }
+    double list_mass;
+    sum = block_scan(sum, part.d, &list_mass);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        if (bin[e] < 0) continue;
+        before[e] += sum;
+        const int i = at + e;
+        int previous = -1;
+        if (i > 0) {
+            const float l = from_key(~static_cast<uint32_t>(u.list[i - 1] >> 32));
+            previous = bin_of(l, top, s.bins);
+        }
+        if (previous != bin[e]) {  // sums before the bin, less those before it in the list
+            mass[bin[e]] -= before[e];
+            count[bin[e]] -= i;
+        }
+    }
+    if (tid == 0) cut = k_mass;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        if (bin[e] < 0) continue;
+        before[e] += mass[bin[e]];
+        // the first token that top-k leaves out
+        if (bin[e] == k_bin && count[k_bin] + at + e == s.k) cut = before[e];
+    }
+    __syncthreads();
+    double kept = cut;
+    const double bound = s.top_p < 1.0 ? s.top_p * kept : __builtin_inf();
+    double least = kept;
+#pragma unroll
+    for (int h = 0; h < kOwn; ++h)
+        if (end[h] >= bound || own + h == p_bin) least = __builtin_fmin(least, end[h]);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+        if (bin[e] >= 0 && (before[e] >= bound || weight[e] < s.min_p))
+            least = __builtin_fmin(least, before[e]);
+    kept = block_reduce(least, __builtin_inf(), part.d, Min());
+    const double target = s.u * kept;
+    int chosen = kList, last = -1;
+#pragma unroll
+    for (int e = kEach - 1; e >= 0; --e) {
+        if (bin[e] < 0) continue;
+        if (weight[e] > 0.0 && before[e] <= target && last < 0) last = at + e;
+        if (before[e] + weight[e] > target) chosen = at + e;
+    }
+    chosen = block_reduce(chosen, kList, part.i, Min());
+    if (chosen == kList) {  // past them by a rounding: the last
+        last = block_reduce(last, -1, part.i, Max());
+        chosen = max(last, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        if (bin[e] < 0 || at + e != chosen) continue;
+        g.tokens[row] = static_cast<int>(static_cast<uint32_t>(u.list[at + e]));
+        if (g.logprobs) g.logprobs[row] = static_cast<float>(log(weight[e] / kept));
+    }
+}
+
+// Rows of one launch of the split kernels: their grids stay below 2^31 threads, and the
+// workspace is bounded.
+constexpr int kSplitRows = 128;
+
+// One block a row from 64 rows on, and where a row is a few units: one launch and no trip
+// through memory, where the split takes three.
+bool sample_whole(int rows, int units) { return rows >= 64 || units <= 16; }
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+// The workspace's parts for a number of rows; its size.
+size_t sample_layout(int rows, int units, char* base, SampleWork* w) {
+    const size_t n = rows < 1 ? 1 : rows < kSplitRows ? rows : kSplitRows;
+    size_t at = 0;
+    SampleWork none;
+    SampleWork& t = w ? *w : none;
+    auto take = [&](auto*& p, size_t count) {
+        p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(base + at);
+        at += align256(count * sizeof(*p));
+    };
+    take(t.peaks, n * units);
+    take(t.mass, n * kBins);
+    take(t.count, n * kBins);
+    take(t.list, n * kList);
+    take(t.listed, n);
+    take(t.done, n);
+    return at;
+}
+
+// Of any type: float32 has the most units.
+size_t sample_workspace(int rows, int vocab) {
+    return sample_layout(rows, units_of<F32>(vocab), nullptr, nullptr);
+}
 
 int check_rows(const char* fn, int rows, int vocab) {
     if (rows < 0 || vocab < 0) return invalid("%s: negative size", fn);
@@ -345,9 +1089,29 @@ int sample(const char* fn, const void* logits, long stride, const float* uniform
     for (const void* p : four)
         if (!aligned_to(p, 4)) return invalid("%s: a vector is not 4-byte aligned", fn);
     if (int e = check_workspace(fn, ws, size, sample_workspace(rows, vocab))) return e;
-    SampleArgs g{logits, stride, uniforms, tokens, logprobs, rows, vocab, *set};
-    hipLaunchKernelGGL(sample_row_kernel<T>, dim3(rows), dim3(kRow), 0, as_stream(stream), g);
-    return launch_status(fn);
+    SampleArgs g{logits, stride, uniforms, tokens, logprobs, vocab, *set};
+    SampleWork w{};
+    w.units = units_of<T>(vocab);
+    sample_layout(rows, w.units, static_cast<char*>(ws), &w);
+    const hipStream_t st = as_stream(stream);
+    if (sample_whole(rows, w.units)) {
+        w.rows = rows;
+        w.parts = 1;
+        hipLaunchKernelGGL((sample_pick_kernel<T, true>), dim3(rows), dim3(kRow), 0, st, g, w);
+        return launch_status(fn);
+    }
+    const int blocks = (w.units + kSplitBlock / kWave - 1) / (kSplitBlock / kWave);
+    for (w.first = 0; w.first < rows; w.first += w.rows) {
+        w.rows = rows - w.first < kSplitRows ? rows - w.first : kSplitRows;
+        const int most = (w.units + kWaves - 1) / kWaves, fill = (256 + w.rows - 1) / w.rows;
+        w.parts = fill < most ? fill : most;
+        if (w.parts > 16) w.parts = 16;
+        hipLaunchKernelGGL(sample_peaks_kernel<T>, dim3(blocks, w.rows), dim3(kSplitBlock), 0, st, g, w);
+        hipLaunchKernelGGL(sample_bins_kernel<T>, dim3(blocks, w.rows), dim3(kSplitBlock), 0, st, g, w);
+        hipLaunchKernelGGL((sample_pick_kernel<T, false>), dim3(w.parts, w.rows), dim3(kRow), 0, st, g, w);
+        if (int e = launch_status(fn)) return e;
+    }
+    return 0;
 }
 
 // ---- log-probabilities --------------------------------------------------------------
@@ -378,7 +1142,7 @@ __global__ __launch_bounds__(kRow) void logprob_row_kernel(LogprobArgs g) {
     const typename T::Bits* l = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
     float top = -__builtin_inff();
     for (int i = threadIdx.x; i < g.vocab; i += kRow) top = __builtin_fmaxf(top, clean(T::load(l + i)));
-    top = block_reduce(top, part.f, [](float a, float b) { return __builtin_fmaxf(a, b); });
+    top = block_reduce(top, -__builtin_inff(), part.f, Max());
     // the largest ones are counted apart: beside a 1, weights of 1e-11 would lose digits
     double rest = 0.0;
     int largest = 0;
@@ -389,8 +1153,8 @@ __global__ __launch_bounds__(kRow) void logprob_row_kernel(LogprobArgs g) {
         else if (v != -__builtin_inff())
             rest += expf(v - top);
     }
-    rest = block_reduce(rest, part.d, [](double a, double b) { return a + b; });
-    largest = block_reduce(largest, part.i, [](int a, int b) { return a + b; });
+    rest = block_reduce(rest, 0.0, part.d, Add());
+    largest = block_reduce(largest, 0, part.i, Add());
     const double norm = log1p(rest + (largest - 1));
     auto logprob = [&](float v) {
         return v == -__builtin_inff() ? v : static_cast<float>((v == top ? 0.0 : static_cast<double>(v) - top) - norm);
@@ -405,7 +1169,7 @@ __global__ __launch_bounds__(kRow) void logprob_row_kernel(LogprobArgs g) {
                 static_cast<uint32_t>(~i);
             if (c < last && c > best) best = c;
         }
-        last = block_reduce(best, part.u, [](unsigned long long a, unsigned long long b) { return a > b ? a : b; });
+        last = block_reduce(best, 0ull, part.u, Max());
         if (threadIdx.x == 0) {
             g.top_ids[static_cast<long>(row) * g.top + n] = static_cast<int>(~static_cast<uint32_t>(last));
             g.top_logprobs[static_cast<long>(row) * g.top + n] = logprob(from_key(static_cast<uint32_t>(last >> 32)));
