@@ -53,14 +53,12 @@ struct Half {
     }
 };
 
-// A logit with NaN as minus infinity and one zero.
-__device__ __forceinline__ float clean(float v) {
-    return v != v ? -__builtin_inff() : v + 0.0f;
-}
+// A logit with NaN as minus infinity: the maximum of a NaN and a number is the number.
+__device__ __forceinline__ float clean(float v) { return __builtin_fmaxf(v, -__builtin_inff()); }
 
-// Order of the logits as unsigned numbers.
+// Order of the logits as unsigned numbers, with one zero.
 __device__ __forceinline__ uint32_t key_of(float v) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);
     return b >> 31 ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float from_key(uint32_t k) {
@@ -281,10 +279,13 @@ __device__ __forceinline__ double weight_of(float l, float top, double inv_t) {
     return d > -64.0 ? exp_of(d) : 0.0;
 }
 
-// A weight as a whole number of 1 / unit, one = 2^52 / unit.
+// A weight as a whole number of 1 / unit, one = 2^52 / unit: the sum's low bits (those of a
+// power of two are 0).
 __device__ __forceinline__ unsigned long long fixed(double w, double one) {
-    return __builtin_bit_cast(unsigned long long, w + one) -
-           __builtin_bit_cast(unsigned long long, one);
+    const auto b = __builtin_bit_cast(unsigned long long, w + one);
+    const uint32_t hi = static_cast<uint32_t>(b >> 32) -
+                        static_cast<uint32_t>(__builtin_bit_cast(unsigned long long, one) >> 32);
+    return static_cast<unsigned long long>(hi) << 32 | static_cast<uint32_t>(b);
 }
 
 // -- from the row itself, in up to a dozen readings: for rows whose borders fall among
@@ -467,6 +468,7 @@ __device__ void sample_row(const SampleArgs& g, int row, const Settings& s, floa
 constexpr int kBins = 2048;
 constexpr int kOwn = kBins / kRow;  // bins of a thread
 constexpr int kList = 4096;         // tokens of the bins in question
+constexpr int kSplitBins = 64;      // most bins that are split again
 constexpr int kPeaks = 1024;        // units of a row whose largest logit is kept in LDS
 constexpr int kSplitBlock = 256;
 
@@ -480,11 +482,11 @@ struct SampleWork {
     int first, rows, units, parts;  // rows of this launch, blocks of a row in the last kernel
 };
 
-// A wave's part of a row: 4 loads of 16 bytes a lane, from 16-byte boundaries on, so unit u
-// begins up to 7 logits before u * kSize.
+// A wave's part of a row: 16 logits a lane in loads of 16 bytes, from 16-byte boundaries
+// on, so unit u begins up to 7 logits before u * kSize.
 template <class T>
 struct Unit {
-    static constexpr int kLoads = 4, kSize = kLoads * kWave * T::kVec;
+    static constexpr int kLoads = 16 / T::kVec, kSize = 16 * kWave;
     uint4 bits[kLoads];
 
     static __device__ __forceinline__ int start(const typename T::Bits* row, int unit) {
@@ -500,7 +502,7 @@ struct Unit {
                 bits[n] = *reinterpret_cast<const uint4*>(row + i);
         }
     }
-    // f(logit, index) of each loaded logit; minus infinity outside the row.
+    // f(logit, index, number of it) of each loaded logit; minus infinity outside the row.
     template <class F>
     __device__ __forceinline__ void each(const typename T::Bits* row, int vocab, int unit, F f) const {
         const int first = start(row, unit);
@@ -516,7 +518,7 @@ struct Unit {
                     v[e] = i + e >= 0 && i + e < vocab ? T::load(row + i + e) : -__builtin_inff();
             }
 #pragma unroll
-            for (int e = 0; e < T::kVec; ++e) f(clean(v[e]), i + e);
+            for (int e = 0; e < T::kVec; ++e) f(clean(v[e]), i + e, n * T::kVec + e);
         }
     }
 };
@@ -555,7 +557,7 @@ __device__ __forceinline__ int bin_of(float l, float top, float bins) {
 template <class T>
 __device__ __forceinline__ float unit_peak(const Unit<T>& x, const typename T::Bits* row, int vocab, int u) {
     float peak = -__builtin_inff();
-    x.each(row, vocab, u, [&](float l, int) { peak = __builtin_fmaxf(peak, l); });
+    x.each(row, vocab, u, [&](float l, int, int) { peak = __builtin_fmaxf(peak, l); });
     return from_lane(wave_scan(peak, -__builtin_inff(), Max()), kWave - 1);
 }
 
@@ -563,12 +565,13 @@ __device__ __forceinline__ float unit_peak(const Unit<T>& x, const typename T::B
 template <class T>
 __device__ __forceinline__ void add_unit(const Unit<T>& x, const typename T::Bits* row, int vocab, int u,
                                          const Settings& s, float top, unsigned long long* mass, int* count) {
-    x.each(row, vocab, u, [&](float l, int) {
-        if (l == -__builtin_inff()) return;
+    x.each(row, vocab, u, [&](float l, int, int) {
         const int b = bin_of(l, top, s.bins);
-        const unsigned long long m = fixed(weight_of(l, top, s.inv_t), s.one);
+        // below e^-64 it is 0 as a whole number; so is minus infinity's
+        const double d = (static_cast<double>(l) - static_cast<double>(top)) * s.inv_t;
+        const unsigned long long m = fixed(exp_of(__builtin_fmax(d, -64.0)), s.one);
         if (m) atomicAdd(&mass[b], m);
-        if (count) atomicAdd(&count[b], 1);
+        if (count && l != -__builtin_inff()) atomicAdd(&count[b], 1);
     });
 }
 
@@ -610,11 +613,9 @@ __global__ __launch_bounds__(kSplitBlock) void sample_bins_kernel(SampleArgs g, 
     __shared__ unsigned long long mass[kBins];
     __shared__ int count[kBins];
     __shared__ float part[kSplitBlock / kWave];
+    constexpr int kTogether = kSplitBlock / kWave;
     const int r = blockIdx.y, row = w.first + r, tid = threadIdx.x;
-    const int u = blockIdx.x * (kSplitBlock / kWave) + tid / kWave;
     const typename T::Bits* logits = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
-    Unit<T> x;
-    if (u < w.units) x.load(logits, g.vocab, u);
     const Settings s = settings_of(g, row);
     const bool by_count = s.k < g.vocab;
     for (int b = tid; b < kBins; b += kSplitBlock) {
@@ -624,7 +625,10 @@ __global__ __launch_bounds__(kSplitBlock) void sample_bins_kernel(SampleArgs g, 
     const float top = row_peak(w.peaks + static_cast<long>(r) * w.units, w.units, kSplitBlock, part,
                                kSplitBlock / kWave);
     if (__builtin_isinf(top)) return;
-    if (u < w.units) add_unit<T>(x, logits, g.vocab, u, s, top, mass, by_count ? count : nullptr);
+    each_unit<T>(logits, g.vocab, blockIdx.x * kTogether + tid / kWave, gridDim.x * kTogether, w.units,
+                 [](int) { return true; }, [&](const Unit<T>& x, int u) {
+                     add_unit<T>(x, logits, g.vocab, u, s, top, mass, by_count ? count : nullptr);
+                 });
     __syncthreads();
     for (int b = tid; b < kBins; b += kSplitBlock) {
         if (mass[b])
@@ -716,7 +720,10 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
         double mass[kWaves];
         int count[kWaves];
     } sums;
-    __shared__ uint32_t marked[kBins / 32];
+    __shared__ uint32_t marked[kBins / 32], marked_parts[kBins / 32];
+    __shared__ int slots[kBins / 32];  // marked bins before each word
+    __shared__ double gap_mass[2][kSplitBins + 1];  // between marked bins: from, to
+    __shared__ int gap_count[2][kSplitBins + 1];
     __shared__ int listed, found[5], heaviest_bin, base;
     __shared__ double cut;
     const int r = kWhole ? blockIdx.x : blockIdx.y, q = kWhole ? 0 : blockIdx.x;
@@ -729,7 +736,6 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
     if (tid < 5) found[tid] = kBins;
     if (tid == 5) listed = 0;
     if (tid == 6) heaviest_bin = 0;
-    if (tid < kBins / 32) marked[tid] = 0;
     auto all_units = [](int) { return true; };
     float top = -__builtin_inff();
     if constexpr (kWhole) {
@@ -773,14 +779,27 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
         mine[h] = static_cast<double>(kWhole ? masses.fixed[own + h] : w.mass[at]) / s.unit;
         if (by_count) mine_count[h] = kWhole ? count[own + h] : w.count[at];
     }
-    double total, sum = 0.0;
-    int total_count, sum_count = 0;
+    // A bin's place among the marked ones, once they are split.
+    int parts_of_bin = 0;  // 0: bins are not split
+    auto place_of = [&](float y) {  // y: bins below the largest logit
+        const int b = static_cast<int>(__builtin_fminf(y, kBins - 1.0f));
+        if (parts_of_bin == 0) return b;
+        const uint32_t below = marked[b / 32] & ((1u << (b % 32)) - 1);
+        const int slot = slots[b / 32] + __popc(below), first = slot * parts_of_bin;
+        if (!(marked[b / 32] >> (b % 32) & 1)) return first;
+        const int part = static_cast<int>(__builtin_fminf(y - b, 1.0f) * (parts_of_bin - 1));
+        return first + 1 + min(part, parts_of_bin - 2);
+    };
+    double total;
+    int total_count;
+    auto add_up = [&]() {  // mine[], mine_count[] -> mass[], count[]
+        double sum = 0.0;
+        int sum_count = 0;
 #pragma unroll
-    for (int h = 0; h < kOwn; ++h) {
-        sum += mine[h];
-        sum_count += mine_count[h];
-    }
-    {
+        for (int h = 0; h < kOwn; ++h) {
+            sum += mine[h];
+            sum_count += mine_count[h];
+        }
         BlockScan<double> m;
         BlockScan<int> c;
         m.before(sum, sums.mass);
@@ -788,119 +807,143 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
         __syncthreads();
         sum = m.after(sums.mass, &total);
         sum_count = c.after(sums.count, &total_count);
-    }
 #pragma unroll
-    for (int h = 0; h < kOwn; ++h) {
-        mass[own + h] = sum;
-        count[own + h] = sum_count;
-        sum += mine[h];
-        sum_count += mine_count[h];
-    }
-    if (tid == 0) {
-        mass[kBins] = total;
-        count[kBins] = total_count;
-    }
-    __syncthreads();
-    // bins in question.  The bounds of a sum that a bin leaves open give a first and a last
-    // bin, a little widened: sums over bins and over tokens round differently.
-    const double less = 1.0 - 0x1p-36, more = 1.0 + 0x1p-36;
-    double end[kOwn];
-    int heavy = -1;
-    auto find = [&](int which, auto holds) {  // the first bin of which it holds
-        int first = kBins;
-#pragma unroll
-        for (int h = kOwn - 1; h >= 0; --h)
-            if (holds(h)) first = own + h;
-        const unsigned long long set = __ballot(first < kBins);
-        if (set) {
-            first = from_lane(first, __ffsll(set) - 1);
-            if (lane == 0) atomicMin(&found[which], first);
+        for (int h = 0; h < kOwn; ++h) {
+            mass[own + h] = sum;
+            count[own + h] = sum_count;
+            sum += mine[h];
+            sum_count += mine_count[h];
         }
-    };
-#pragma unroll
-    for (int h = 0; h < kOwn; ++h) {
-        end[h] = mass[own + h + 1];
-        if (mine[h] > 0.0) heavy = own + h;
-    }
-    const unsigned long long heavies = __ballot(heavy >= 0);
-    if (heavies) {
-        heavy = from_lane(heavy, 63 - __clzll(heavies));
-        if (lane == 0) atomicMax(&heaviest_bin, heavy);
-    }
-    if (by_count) find(0, [&](int h) { return count[own + h + 1] >= s.k; });
-    __syncthreads();
-    // bins behind the last one with a weight need no order: whatever is kept of them
-    const int heaviest = heaviest_bin;
-    int k_bin = kBins;
-    double low = total, upper = total;  // bounds of what top-k keeps
-    if (by_count && s.k < total_count && found[0] <= heaviest) {
-        k_bin = found[0];
-        low = upper = mass[k_bin + 1];
-        if (count[k_bin + 1] == s.k)
-            k_bin = kBins;  // ends with the bin
-        else
-            low = mass[k_bin];
-    }
-    const double k_mass = upper;  // of top-k, where no bin is in question
-    int first_marked = kBins, last_marked = -1;
-    auto mark = [&](int a, int b) {
-        a = max(a, 0);
-        b = min(b, heaviest);
-        if (a > b) return;
-        first_marked = min(first_marked, a);
-        last_marked = max(last_marked, b);
-        if (tid < kBins / 32 && tid >= a / 32 && tid <= b / 32) {
-            uint32_t bits = ~0u;
-            if (tid == a / 32) bits &= ~0u << (a % 32);
-            if (tid == b / 32) bits &= ~0u >> (31 - b % 32);
-            marked[tid] |= bits;  // its thread's own word
+        if (tid == 0) {
+            mass[kBins] = total;
+            count[kBins] = total_count;
         }
-    };
-    if (k_bin < kBins) mark(k_bin, k_bin);
-    if (s.top_p < 1.0) {
-        find(1, [&](int h) { return end[h] >= s.top_p * low * less; });
-        find(2, [&](int h) { return end[h] >= s.top_p * upper * more; });
         __syncthreads();
-        const int a = min(found[1], heaviest), b = min(found[2], heaviest);
-        mark(a, b);
-        low = __builtin_fmin(low, s.top_p * low * less);
-        upper = __builtin_fmin(upper, mass[b + 1]);
-    }
-    int p_bin = kBins;  // the last bin that min-p may keep a part of
-    if (s.min_p > 0.0) {
-        const double x = -log(s.min_p) / s.inv_t * s.bins;
-        const double off = 1e-6 + 3e-7 * x;  // a logit's place among the bins is float32
-        const double a = x - off, b = x + off;
-        const int first = a > 0.0 ? (a < kBins - 1.0 ? static_cast<int>(a) : kBins - 1) : 0;
-        p_bin = b < kBins - 1.0 ? static_cast<int>(b) : kBins - 1;
-        mark(first, p_bin);
-        low = __builtin_fmin(low, mass[first]);
-        upper = __builtin_fmin(upper, mass[p_bin + 1]);
-    }
-    low = __builtin_fmax(low, 1.0);  // the first token stays
-    find(3, [&](int h) { return end[h] > s.u * low * less; });
-    find(4, [&](int h) { return end[h] > s.u * upper * more; });
+    };
+    // The bins in question.  The bounds of a sum that a bin leaves open give a first and a
+    // last bin, a little widened: sums over bins and over tokens round differently.
+    double end[kOwn], k_mass;
+    int k_bin, p_bin, from, to;
+    uint32_t my_marks;  // word tid of the marks
+    auto decide = [&]() {
+        const double less = 1.0 - 0x1p-36, more = 1.0 + 0x1p-36;
+        int heavy = -1;
+        auto find = [&](int which, auto holds) {  // the first bin of which it holds
+            int first = kBins;
+#pragma unroll
+            for (int h = kOwn - 1; h >= 0; --h)
+                if (holds(h)) first = own + h;
+            const unsigned long long set = __ballot(first < kBins);
+            if (set) {
+                first = from_lane(first, __ffsll(set) - 1);
+                if (lane == 0) atomicMin(&found[which], first);
+            }
+        };
+#pragma unroll
+        for (int h = 0; h < kOwn; ++h) {
+            end[h] = mass[own + h + 1];
+            if (mine[h] > 0.0) heavy = own + h;
+        }
+        const unsigned long long heavies = __ballot(heavy >= 0);
+        if (heavies) {
+            heavy = from_lane(heavy, 63 - __clzll(heavies));
+            if (lane == 0) atomicMax(&heaviest_bin, heavy);
+        }
+        if (by_count) find(0, [&](int h) { return count[own + h + 1] >= s.k; });
+        __syncthreads();
+        // bins behind the last one with a weight need no order: whatever is kept of them
+        const int heaviest = heaviest_bin;
+        k_bin = kBins;
+        double low = total, upper = total;  // bounds of what top-k keeps
+        if (by_count && s.k < total_count && found[0] <= heaviest) {
+            k_bin = found[0];
+            low = upper = mass[k_bin + 1];
+            if (count[k_bin + 1] == s.k)
+                k_bin = kBins;  // ends with the bin
+            else
+                low = mass[k_bin];
+        }
+        k_mass = upper;  // of top-k, where no bin is in question
+        from = kBins;
+        to = -1;
+        my_marks = 0;
+        auto mark = [&](int a, int b) {
+            a = max(a, 0);
+            b = min(b, heaviest);
+            if (a > b) return;
+            from = min(from, a);
+            to = max(to, b);
+            if (tid >= a / 32 && tid <= b / 32) {
+                uint32_t bits = ~0u;
+                if (tid == a / 32) bits &= ~0u << (a % 32);
+                if (tid == b / 32) bits &= ~0u >> (31 - b % 32);
+                my_marks |= bits;
+            }
+        };
+        if (k_bin < kBins) mark(k_bin, k_bin);
+        if (s.top_p < 1.0) {
+            find(1, [&](int h) { return end[h] >= s.top_p * low * less; });
+            find(2, [&](int h) { return end[h] >= s.top_p * upper * more; });
+            __syncthreads();
+            const int a = min(found[1], heaviest), b = min(found[2], heaviest);
+            mark(a, b);
+            low = __builtin_fmin(low, s.top_p * low * less);
+            upper = __builtin_fmin(upper, mass[b + 1]);
+        }
+        p_bin = kBins;  // the last bin that min-p may keep a part of
+        if (s.min_p > 0.0) {
+            const double x = -log(s.min_p) / s.inv_t * s.bins;
+            const double off = 1e-6 + 3e-7 * x;  // a logit's place among the bins is float32
+            const int first = place_of(static_cast<float>(__builtin_fmax(x - off, 0.0)));
+            p_bin = place_of(static_cast<float>(x + off));
+            mark(first, p_bin);
+            low = __builtin_fmin(low, mass[first]);
+            upper = __builtin_fmin(upper, mass[p_bin + 1]);
+        }
+        low = __builtin_fmax(low, 1.0);  // the first token stays
+        find(3, [&](int h) { return end[h] > s.u * low * less; });
+        find(4, [&](int h) { return end[h] > s.u * upper * more; });
+        __syncthreads();
+        mark(min(found[3], heaviest), min(found[4], heaviest));
+    };
+    add_up();
+    decide();
+    if (tid < kBins / 32) marked[tid] = my_marks;
     __syncthreads();
-    mark(min(found[3], heaviest), min(found[4], heaviest));
-    const int from = first_marked, to = last_marked;
-    __syncthreads();
-    // their tokens
+    // their tokens: by bounds of the logits, then by their bins
+    const float above = top - from / s.bins * 0.9999f;
+    const float below = to < kBins - 1 ? top - (to + 1) / s.bins * 1.0001f : -__builtin_inff();
     each_unit<T>(
         logits, g.vocab, q * kWaves + wave, w.parts * kWaves, w.units,
         [&](int u) { return (kWhole && u >= kPeaks) || bin_of(peaks[u], top, s.bins) <= to; },
         [&](const Unit<T>& x, int unit) {
-            x.each(logits, g.vocab, unit, [&](float l, int i) {
-                const int b = bin_of(l, top, s.bins);
-                if (b < from || b > to || l == -__builtin_inff()) return;
-                if (!(marked[b / 32] >> (b % 32) & 1)) return;
-                const int place = atomicAdd(&listed, 1);
-                if (place < kList)
-                    u.list[place] = static_cast<unsigned long long>(~key_of(l)) << 32 |
-                                    static_cast<uint32_t>(i);
+            uint32_t near = 0;
+            x.each(logits, g.vocab, unit, [&](float l, int, int e) {
+                near |= static_cast<uint32_t>(l >= below && l <= above && l != -__builtin_inff()) << e;
+            });
+            if (!__any(near != 0)) return;
+            uint32_t hits = 0;
+            x.each(logits, g.vocab, unit, [&](float l, int, int e) {
+                const int b = max(bin_of(l, top, s.bins), 0);
+                hits |= (marked[b / 32] >> (b % 32) & near >> e & 1) << e;
+            });
+            // one addition for the wave, then each lane writes its own
+            const int own_hits = __popc(hits), upto = wave_scan(own_hits, 0, Add());
+            const int all = from_lane(upto, kWave - 1);
+            if (all == 0) return;
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&listed, all);
+            at = from_lane(at, 0) + upto - own_hits;
+            x.each(logits, g.vocab, unit, [&](float l, int i, int e) {
+                if (!(hits >> e & 1)) return;
+                if (at < kList)
+                    u.list[at] = static_cast<unsigned long long>(~key_of(l)) << 32 |
+                                 static_cast<uint32_t>(i);
+                ++at;
             });
         });
     __syncthreads();
-    int n = listed;
+    int n = __builtin_amdgcn_readfirstlane(listed);
     if (!kWhole && w.parts > 1) {  // the block that is done last has all of them, and goes on
         // Stores and loads past the per-XCD L2s (agent scope), each block's stores done
         // (s_waitcnt) before it counts itself; a fence would write a whole L2 back: 90 us of
@@ -919,7 +962,8 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
             base = __hip_atomic_fetch_add(&w.done[r], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         if (base != w.parts - 1) return;
-        n = __hip_atomic_load(&w.listed[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        n = __builtin_amdgcn_readfirstlane(
+            __hip_atomic_load(&w.listed[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
         for (int i = tid; i < min(n, kList); i += kRow)
             u.list[i] = __hip_atomic_load(&w.list[static_cast<long>(r) * kList + i],
                                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -929,55 +973,113 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
         sample_row<T>(g, row, s, top, u.hist);
         return;
     }
+    if (n > kRow) {
+        // The marked bins again, each split into as many parts as there is room for; what is
+        // between them is a part of its own.  It leaves a token or two of each in question:
+        // sorting 1200 took a fifth of the time of 512 flat rows.
+        const uint32_t word = marked[lane];
+        const int own_bits = __popc(word), words = wave_scan(own_bits, 0, Add());
+        const int many = from_lane(words, kWave - 1);
+        if (many <= kSplitBins) {
+            if (wave == 0) slots[lane] = words - own_bits;
+            __syncthreads();
+            auto slot_of = [&](int b) {
+                return slots[b / 32] + __popc(marked[b / 32] & ((1u << (b % 32)) - 1));
+            };
+            if (tid == 0) {
+                gap_mass[0][0] = 0.0;
+                gap_count[0][0] = 0;
+                gap_mass[1][many] = total;
+                gap_count[1][many] = total_count;
+            }
+#pragma unroll
+            for (int h = 0; h < kOwn; ++h) {
+                const int b = own + h;
+                if (!(marked[b / 32] >> (b % 32) & 1)) continue;
+                const int slot = slot_of(b);
+                gap_mass[1][slot] = mass[b];
+                gap_count[1][slot] = count[b];
+                gap_mass[0][slot + 1] = mass[b + 1];
+                gap_count[0][slot + 1] = count[b + 1];
+            }
+            parts_of_bin = (kBins - 1) / many;
+            __syncthreads();
+            for (int b = tid; b < kBins; b += kRow) {
+                masses.fixed[b] = 0;
+                count[b] = 0;
+            }
+            if (tid < 5) found[tid] = kBins;
+            if (tid == 5) listed = 0;
+            if (tid == 6) heaviest_bin = 0;
+            __syncthreads();
+            uint64_t keep[kList / kRow];
+#pragma unroll
+            for (int e = 0; e < kList / kRow; ++e) {
+                const int i = tid + e * kRow;
+                if (i >= n) continue;
+                keep[e] = u.list[i];
+                const float l = from_key(~static_cast<uint32_t>(keep[e] >> 32));
+                const int b = place_of((top - l) * s.bins);
+                atomicAdd(&masses.fixed[b], fixed(weight_of(l, top, s.inv_t), s.one));
+                atomicAdd(&count[b], 1);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int h = 0; h < kOwn; ++h) {
+                const int b = own + h, slot = b / parts_of_bin;
+                mine[h] = static_cast<double>(masses.fixed[b]) / s.unit;
+                mine_count[h] = count[b];
+                if (slot * parts_of_bin == b && slot <= many) {
+                    mine[h] += gap_mass[1][slot] - gap_mass[0][slot];
+                    mine_count[h] += gap_count[1][slot] - gap_count[0][slot];
+                }
+            }
+            add_up();
+            decide();
+            if (tid < kBins / 32) marked_parts[tid] = my_marks;
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < kList / kRow; ++e) {
+                if (tid + e * kRow >= n) continue;
+                const float l = from_key(~static_cast<uint32_t>(keep[e] >> 32));
+                const int b = place_of((top - l) * s.bins);
+                if (marked_parts[b / 32] >> (b % 32) & 1) u.list[atomicAdd(&listed, 1)] = keep[e];
+            }
+            __syncthreads();
+            n = __builtin_amdgcn_readfirstlane(listed);
+        }
+    }
     if (n <= kRow)
         sort_list<1>(u.list, n);
-    else if (n <= 2 * kRow)
-        sort_list<2>(u.list, n);
     else
         sort_list<kList / kRow>(u.list, n);
-    // a thread's neighbours in the list: their weights, and those before them
-    constexpr int kEach = kList / kRow;
-    const int each = (n + kRow - 1) / kRow, at = tid * each;
-    double weight[kEach], before[kEach];
-    int bin[kEach];
-    sum = 0.0;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-        weight[e] = 0.0;
-        bin[e] = -1;
-        if (e >= each || at + e >= n) continue;
-        const float l = from_key(~static_cast<uint32_t>(u.list[at + e] >> 32));
-        weight[e] = weight_of(l, top, s.inv_t);
-        bin[e] = bin_of(l, top, s.bins);
-        before[e] = sum;
-        sum += weight[e];
-    }
+    // A thread's neighbours in the list, one mostly: f(place, weight, bin, weights before it
+    // in the list).
+    const int each = (n + kRow - 1) / kRow, first = min(tid * each, n), behind = min(first + each, n);
+    auto place_at = [&](int i) {
+        return place_of((top - from_key(~static_cast<uint32_t>(u.list[i] >> 32))) * s.bins);
+    };
+    auto each_listed = [&](double before, auto f) {
+        for (int i = first; i < behind; ++i) {
+            const float l = from_key(~static_cast<uint32_t>(u.list[i] >> 32));
+            const double weight = weight_of(l, top, s.inv_t);
+            f(i, weight, place_of((top - l) * s.bins), before);
+            before += weight;
+        }
+        return before;
+    };
     double list_mass;
-    sum = block_scan(sum, part.d, &list_mass);
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-        if (bin[e] < 0) continue;
-        before[e] += sum;
-        const int i = at + e;
-        int previous = -1;
-        if (i > 0) {
-            const float l = from_key(~static_cast<uint32_t>(u.list[i - 1] >> 32));
-            previous = bin_of(l, top, s.bins);
-        }
-        if (previous != bin[e]) {  // sums before the bin, less those before it in the list
-            mass[bin[e]] -= before[e];
-            count[bin[e]] -= i;
-        }
-    }
+    const double sum = block_scan(each_listed(0.0, [](int, double, int, double) {}), part.d, &list_mass);
+    each_listed(sum, [&](int i, double, int b, double before) {
+        if (i > 0 && place_at(i - 1) == b) return;
+        mass[b] -= before;  // weights before the bin, less those before it in the list
+        count[b] -= i;
+    });
     if (tid == 0) cut = k_mass;
     __syncthreads();
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-        if (bin[e] < 0) continue;
-        before[e] += mass[bin[e]];
-        // the first token that top-k leaves out
-        if (bin[e] == k_bin && count[k_bin] + at + e == s.k) cut = before[e];
-    }
+    each_listed(sum, [&](int i, double, int b, double before) {
+        if (b == k_bin && count[b] + i == s.k) cut = before + mass[b];  // the first that top-k leaves out
+    });
     __syncthreads();
     double kept = cut;
     const double bound = s.top_p < 1.0 ? s.top_p * kept : __builtin_inf();
@@ -985,30 +1087,29 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
 #pragma unroll
     for (int h = 0; h < kOwn; ++h)
         if (end[h] >= bound || own + h == p_bin) least = __builtin_fmin(least, end[h]);
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-        if (bin[e] >= 0 && (before[e] >= bound || weight[e] < s.min_p))
-            least = __builtin_fmin(least, before[e]);
+    each_listed(sum, [&](int, double weight, int b, double before) {
+        before += mass[b];
+        if (before >= bound || weight < s.min_p) least = __builtin_fmin(least, before);
+    });
     kept = block_reduce(least, __builtin_inf(), part.d, Min());
     const double target = s.u * kept;
     int chosen = kList, last = -1;
-#pragma unroll
-    for (int e = kEach - 1; e >= 0; --e) {
-        if (bin[e] < 0) continue;
-        if (weight[e] > 0.0 && before[e] <= target && last < 0) last = at + e;
-        if (before[e] + weight[e] > target) chosen = at + e;
-    }
+    each_listed(sum, [&](int i, double weight, int b, double before) {
+        before += mass[b];
+        if (weight > 0.0 && before <= target) last = i;
+        if (before + weight > target) chosen = min(chosen, i);
+    });
     chosen = block_reduce(chosen, kList, part.i, Min());
     if (chosen == kList) {  // past them by a rounding: the last
         last = block_reduce(last, -1, part.i, Max());
         chosen = max(last, 0);
     }
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-        if (bin[e] < 0 || at + e != chosen) continue;
-        g.tokens[row] = static_cast<int>(static_cast<uint32_t>(u.list[at + e]));
-        if (g.logprobs) g.logprobs[row] = static_cast<float>(log(weight[e] / kept));
-    }
+    if (chosen < first || chosen >= behind) return;
+    const unsigned long long token = u.list[chosen];
+    g.tokens[row] = static_cast<int>(static_cast<uint32_t>(token));
+    if (g.logprobs)
+        g.logprobs[row] = static_cast<float>(
+            log(weight_of(from_key(~static_cast<uint32_t>(token >> 32)), top, s.inv_t) / kept));
 }
 
 // Rows of one launch of the split kernels: their grids stay below 2^31 threads, and the
@@ -1040,9 +1141,9 @@ size_t sample_layout(int rows, int units, char* base, SampleWork* w) {
     return at;
 }
 
-// Of any type: float32 has the most units.
+// Of any type: 16-bit rows may begin 7 logits before a boundary.
 size_t sample_workspace(int rows, int vocab) {
-    return sample_layout(rows, units_of<F32>(vocab), nullptr, nullptr);
+    return sample_layout(rows, units_of<Half<F16>>(vocab), nullptr, nullptr);
 }
 
 int check_rows(const char* fn, int rows, int vocab) {
@@ -1107,7 +1208,10 @@ int sample(const char* fn, const void* logits, long stride, const float* uniform
         w.parts = fill < most ? fill : most;
         if (w.parts > 16) w.parts = 16;
         hipLaunchKernelGGL(sample_peaks_kernel<T>, dim3(blocks, w.rows), dim3(kSplitBlock), 0, st, g, w);
-        hipLaunchKernelGGL(sample_bins_kernel<T>, dim3(blocks, w.rows), dim3(kSplitBlock), 0, st, g, w);
+        // Each block adds its bins to the row's: fewer blocks a row, fewer additions in memory.
+        const int share = (1024 + w.rows - 1) / w.rows;
+        hipLaunchKernelGGL(sample_bins_kernel<T>, dim3(blocks < share ? blocks : share, w.rows),
+                           dim3(kSplitBlock), 0, st, g, w);
         hipLaunchKernelGGL((sample_pick_kernel<T, false>), dim3(w.parts, w.rows), dim3(kRow), 0, st, g, w);
         if (int e = launch_status(fn)) return e;
     }
