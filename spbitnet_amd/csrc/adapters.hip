@@ -4,13 +4,17 @@
 #include "paged.hpp"
 #include "spbitnet_amd.h"
 
+#include <type_traits>
+
 namespace spb {
 namespace {
 
 constexpr int kMaxSections = SPB_MAX_SECTIONS;
 constexpr int kMaxRank = 256;
 constexpr int kMaxSize = 1 << 20;  // tokens, rows and columns: indices and grids in 32 bits
-constexpr int kBlock = 256;
+constexpr int kWindow = kWave;     // tokens of a block: a lane looks at each one's id
+constexpr int kTile = 16;          // rows and columns of a matrix product
+constexpr int kStep = 32;          // and its depth
 
 struct Args {
     const uint16_t* a;
@@ -21,50 +25,478 @@ struct Args {
     const uint16_t* x;
     const uint16_t* base;
     uint16_t* out;
-    float* h;  // [tokens][sections * rank]
+    float* h;  // [splits][tokens][sections * rank]
     long a_adapter, a_row, b_adapter, b_row, xs, bs, os;
-    int num, rank, cols, sections, tokens, rows;
+    int num, rank, cols, sections, tokens, rows, splits;
     int end[kMaxSections];  // first row behind each section
+    bool wide;              // base and output by 16 bytes
+};
+
+using Acc = float __attribute__((ext_vector_type(4)));
+
+// Products of 16 x 32 by 32 x 16: lane l holds 8 numbers of row (column) l % 16 from
+// depth l / 16 * 8 on; of the result rows l / 16 * 4 + 0 ... 3 of column l % 16.
+template <class T>
+struct Matrix;
+template <>
+struct Matrix<F16> {
+    using V = _Float16 __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ Acc mac(uint4 a, uint4 b, Acc c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V, a),
+                                                      __builtin_bit_cast(V, b), c, 0, 0, 0);
+    }
+};
+template <>
+struct Matrix<BF16> {
+    using V = __bf16 __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ Acc mac(uint4 a, uint4 b, Acc c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V, a),
+                                                       __builtin_bit_cast(V, b), c, 0, 0, 0);
+    }
 };
 
 __device__ __forceinline__ int rank_of(const Args& g, int a) {
     return g.ranks ? min(max(g.ranks[a], 0), g.rank) : g.rank;
 }
 
-// h[t][j] = A[a][j] . x[t], one wave each.
-template <class T>
-__global__ __launch_bounds__(kBlock) void shrink_kernel(Args g) {
-    const int t = blockIdx.x, lane = threadIdx.x % kWave;
-    const int j = blockIdx.y * (kBlock / kWave) + threadIdx.x / kWave;
-    const int a = g.ids[t];
-    if (a < 0 || a >= g.num || j >= g.sections * g.rank || j % g.rank >= rank_of(g, a)) return;
-    const uint16_t* w = g.a + a * g.a_adapter + j * g.a_row;
-    const uint16_t* x = g.x + t * g.xs;
-    float s = 0.0f;
-    for (int c = lane; c < g.cols; c += kWave) s += T::to_float(w[c]) * T::to_float(x[c]);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
-    if (lane == 0) g.h[static_cast<long>(t) * (g.sections * g.rank) + j] = s;
+// 16 bytes, or zeros: what must not count is not read, so that a NaN there stays out of the
+// products.
+__device__ __forceinline__ uint4 load8(const uint16_t* p, bool valid) {
+    uint4 v = {0, 0, 0, 0};
+    if (valid) v = *reinterpret_cast<const uint4*>(p);
+    return v;
 }
 
-template <class T>
-__global__ __launch_bounds__(kBlock) void expand_kernel(Args g) {
-    const int t = blockIdx.x, row = blockIdx.y * kBlock + threadIdx.x;
-    if (row >= g.rows) return;
-    const int a = g.ids[t];
-    const uint16_t bits = g.base[t * g.bs + row];
-    if (a < 0 || a >= g.num) {
-        if (g.base != g.out) g.out[t * g.os + row] = bits;
-        return;
+// The first n of 8 numbers.
+__device__ __forceinline__ uint4 first_of(uint4 v, int n) {
+    auto part = [n](uint32_t w, int i) { return n > i + 1 ? w : n > i ? w & 0xffffu : 0u; };
+    return {part(v.x, 0), part(v.y, 2), part(v.z, 4), part(v.w, 6)};
+}
+
+// Place of the n-th set bit (from 0; there are more than n).
+__device__ __forceinline__ int nth_bit(uint64_t m, int n) {
+    int at = 0;
+#pragma unroll
+    for (int w = 32; w > 0; w >>= 1) {
+        const int c = __popcll(m & ((uint64_t{1} << w) - 1));
+        const bool up = n >= c;
+        n -= up ? c : 0;
+        at += up ? w : 0;
+        m >>= up ? w : 0;
     }
-    int sec = 0;
-    while (row >= g.end[sec]) ++sec;
-    const uint16_t* w = g.b + a * g.b_adapter + row * g.b_row;
-    const float* h = g.h + static_cast<long>(t) * (g.sections * g.rank) + sec * g.rank;
-    const int r = rank_of(g, a);
-    float s = 0.0f;
-    for (int j = 0; j < r; ++j) s += T::to_float(w[j]) * h[j];
-    g.out[t * g.os + row] = T::from_float(T::to_float(bits) + g.scales[a] * s);
+    return at;
+}
+
+// A window's adapters: f(adapter, set of its tokens) for the z-th, (z + step)-th, ... of those
+// that occur, in the order of their first tokens.  Returns the tokens that have none.
+template <class F>
+__device__ __forceinline__ uint64_t each_adapter(const Args& g, int window, int z, int step, F f) {
+    const int t = window * kWindow + static_cast<int>(threadIdx.x % kWave);
+    const int id = t < g.tokens ? g.ids[t] : -1;
+    const bool has = id >= 0 && id < g.num;
+    uint64_t left = __ballot(has);
+    const uint64_t idle = __ballot(t < g.tokens) & ~left;
+    for (int i = 0; left; ++i) {
+        const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+        const uint64_t mine = __ballot(id == a) & left;
+        left &= ~mine;
+        if (i % step == z) f(a, mine);
+    }
+    return idle;
+}
+
+// output = base in rows [row, end) of the tokens that have no adapter, a wave each.
+__device__ __forceinline__ void copy_idle(const Args& g, int window, uint64_t idle, int row, int end,
+                                          int wave, int waves) {
+    if (g.base == g.out) return;
+    const int lane = threadIdx.x % kWave;
+    for (int i = 0; idle; ++i, idle &= idle - 1) {
+        if (i % waves != wave) continue;
+        const long t = window * kWindow + __builtin_ctzll(idle);
+        if (g.wide) {
+            for (int r = row + lane * 8; r < end; r += kWave * 8)
+                *reinterpret_cast<uint4*>(g.out + t * g.os + r) =
+                    *reinterpret_cast<const uint4*>(g.base + t * g.bs + r);
+        } else {
+            for (int r = row + lane; r < end; r += kWave) g.out[t * g.os + r] = g.base[t * g.bs + r];
+        }
+    }
+}
+
+// Inner products of 8 depths of one token as two 16-bit numbers each, h = (hi + lo) * unit:
+// their sum is within 2^-16 (bf16) or 2^-22 (fp16) of h, so the second product is as exact as
+// the first.  fp16's range is made up for by a power of two for the token.
+template <class T>
+struct Pair {
+    uint4 hi, lo;
+    __device__ __forceinline__ void set(const float (&h)[8], float by) {
+        uint16_t a[8], b[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float v = h[e] * by;
+            a[e] = T::from_float(v);
+            const float rest = v - T::to_float(a[e]);
+            b[e] = T::from_float(__builtin_isfinite(v) ? rest : 0.0f);
+        }
+        auto two = [](uint16_t x, uint16_t y) { return static_cast<uint32_t>(y) << 16 | x; };
+        hi = {two(a[0], a[1]), two(a[2], a[3]), two(a[4], a[5]), two(a[6], a[7])};
+        lo = {two(b[0], b[1]), two(b[2], b[3]), two(b[4], b[5]), two(b[6], b[7])};
+    }
+};
+
+// The power of two that brings a token's inner products, at most `most`, below 2^14.
+template <class T>
+__device__ __forceinline__ int shift_of(float most) {
+    if constexpr (std::is_same_v<T, BF16>) return 0;
+    if (!(most > 0.0f) || !__builtin_isfinite(most)) return 0;
+    const int exponent = static_cast<int>(__builtin_bit_cast(uint32_t, most) >> 23 & 255) - 126;
+    return min(14 - exponent, 100);
+}
+
+// -- few tokens: both products in one launch.  A block has 128 rows of the output and an
+// -- adapter's tokens of a window, and makes the inner products that it needs by itself: its
+// -- 8 waves split the columns and add up in LDS.
+
+constexpr int kFusedWaves = 8, kFusedRows = kFusedWaves * kTile;
+constexpr int kFusedRank = 64;                 // most ranks
+constexpr int kFusedPad = kFusedRank + 4;      // numbers of a token in LDS
+
+template <class T>
+__global__ __launch_bounds__(kFusedWaves* kWave) void fused_kernel(Args g) {
+    __shared__ float part[kFusedWaves][kTile][kFusedPad];
+    __shared__ float total[kTile][kFusedPad];
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const int col = lane % kTile, quad = lane / kTile;
+    int sec = 0, tile = blockIdx.x, row0 = 0;
+    for (;; ++sec) {  // tiles do not cross sections
+        row0 = sec ? g.end[sec - 1] : 0;
+        const int tiles = (g.end[sec] - row0 + kFusedRows - 1) / kFusedRows;
+        if (tile < tiles) break;
+        tile -= tiles;
+    }
+    const int end = g.end[sec];
+    row0 += tile * kFusedRows;
+    const int window = blockIdx.z, steps = (g.cols + kStep - 1) / kStep;
+    const int step0 = steps * wave / kFusedWaves, step1 = steps * (wave + 1) / kFusedWaves;
+    const int brow = row0 + wave * kTile + col;  // of the outer product's left side
+    const uint64_t idle = each_adapter(g, window, blockIdx.y, gridDim.y, [&](int a, uint64_t tokens) {
+        const int r = rank_of(g, a), many = __popcll(tokens);
+        const uint16_t* left = g.a + a * g.a_adapter + static_cast<long>(sec * g.rank) * g.a_row;
+        const float scale = g.scales[a];
+        uint4 up[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int depth = k * kStep + quad * 8;
+            up[k] = load8(g.b + a * g.b_adapter + brow * g.b_row + depth, brow < end && depth < r);
+            up[k] = first_of(up[k], r - depth);
+        }
+        for (int first = 0; first < many; first += kTile) {
+            const bool live = first + col < many;
+            const int t = window * kWindow + nth_bit(tokens, live ? first + col : first);
+            const uint16_t* x = g.x + t * g.xs;
+            const int row = row0 + wave * kTile + quad * 4;
+            uint16_t old[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                old[e] = live && row + e < end ? g.base[t * g.bs + row + e] : 0;
+            Acc acc[kFusedRank / kTile] = {};
+            auto inner = [&](auto tiles) {
+#pragma unroll 4
+                for (int s = step0; s < step1; ++s) {
+                    const int depth = s * kStep + quad * 8;
+                    const bool in = depth < g.cols;
+                    const uint4 v = load8(x + depth, in);
+#pragma unroll
+                    for (int m = 0; m < decltype(tiles)::value; ++m) {
+                        const int j = m * kTile + col;
+                        const uint4 w = load8(left + j * g.a_row + depth, in && j < r);
+                        acc[m] = Matrix<T>::mac(w, v, acc[m]);
+                    }
+                }
+            };
+            if (r <= kTile)
+                inner(std::integral_constant<int, 1>());
+            else if (r <= 2 * kTile)
+                inner(std::integral_constant<int, 2>());
+            else
+                inner(std::integral_constant<int, 4>());
+            const int tiles = (r + kTile - 1) / kTile;
+#pragma unroll
+            for (int m = 0; m < kFusedRank / kTile; ++m)
+                if (m < tiles)
+                    *reinterpret_cast<Acc*>(&part[wave][col][m * kTile + quad * 4]) = acc[m];
+            __syncthreads();
+            for (int i = tid; i < kTile * tiles * kTile; i += kFusedWaves * kWave) {
+                const int c = i / (tiles * kTile), j = i % (tiles * kTile);
+                float s = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kFusedWaves; ++w) s += part[w][c][j];
+                total[c][j] = s;
+            }
+            __syncthreads();
+            float h[2][8], most = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int j = k * kStep + quad * 8 + e;
+                    h[k][e] = j < r ? total[col][j] : 0.0f;
+                    most = __builtin_fmaxf(most, __builtin_fabsf(h[k][e]));
+                }
+            most = __builtin_fmaxf(most, __shfl_xor(most, 16, kWave));
+            most = __builtin_fmaxf(most, __shfl_xor(most, 32, kWave));
+            const int shift = shift_of<T>(most);
+            const float by = __builtin_ldexpf(1.0f, shift);
+            Acc sum = {};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                if (k * kStep >= r) break;
+                Pair<T> p;
+                p.set(h[k], by);
+                sum = Matrix<T>::mac(up[k], p.hi, sum);
+                sum = Matrix<T>::mac(up[k], p.lo, sum);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (live && row + e < end)
+                    g.out[t * g.os + row + e] = T::from_float(
+                        T::to_float(old[e]) + __builtin_ldexpf(scale * sum[e], -shift));
+        }
+    });
+    if (blockIdx.y == 0)
+        copy_idle(g, window, idle, row0, min(row0 + kFusedRows, end), wave, kFusedWaves);
+}
+
+// -- many tokens or ranks: the inner products first, into memory, then the outer ones.
+
+constexpr int kWaves = 4;
+constexpr int kPart = 64;           // ranks of a block of the first, of a pass of the second
+constexpr int kPad = kPart + 4;     // float32 of a token in LDS
+constexpr int kPadHalf = kPart + 8; // 16-bit numbers of a token in LDS
+constexpr int kRows = kWaves * 64;  // rows of a block of the second
+
+// h of an adapter's tokens of a window and 64 rows of A: 64 x 64 a wave, the waves and
+// g.splits blocks splitting the columns.
+template <class T>
+__global__ __launch_bounds__(kWaves* kWave) void shrink_kernel(Args g) {
+    __shared__ float part[2][kWindow][kPad];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int col = lane % kTile, quad = lane / kTile, all = g.sections * g.rank;
+    const int window = blockIdx.x, split = blockIdx.z % g.splits, j0 = blockIdx.z / g.splits * kPart;
+    const int steps = (g.cols + kStep - 1) / kStep, ways = g.splits * kWaves;
+    const int way = split * kWaves + wave;
+    const int step0 = static_cast<int>(static_cast<long>(steps) * way / ways);
+    const int step1 = static_cast<int>(static_cast<long>(steps) * (way + 1) / ways);
+    each_adapter(g, window, blockIdx.y, gridDim.y, [&](int a, uint64_t tokens) {
+        const int r = rank_of(g, a), many = __popcll(tokens);
+        const uint16_t* x[4];
+        const uint16_t* left[4];
+        bool live[4], some[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int n = i * kTile + col, j = j0 + n;
+            x[i] = g.x + (window * kWindow + nth_bit(tokens, n < many ? n : 0)) * g.xs + quad * 8;
+            left[i] = g.a + a * g.a_adapter + static_cast<long>(j) * g.a_row + quad * 8;
+            live[i] = j < all && j % g.rank < r;
+            some[i] = __any(live[i]);
+        }
+        const int tiles = (many + kTile - 1) / kTile;
+        Acc acc[4][4] = {};
+#pragma unroll 2
+        for (int s = step0; s < step1; ++s) {
+            const int depth = s * kStep;
+            const bool in = depth + quad * 8 < g.cols;
+            uint4 v[4], w[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+                if (n < tiles) v[n] = load8(x[n] + depth, in);
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+                if (some[m]) w[m] = load8(left[m] + depth, in && live[m]);
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+                if (some[m])
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+                        if (n < tiles) acc[m][n] = Matrix<T>::mac(w[m], v[n], acc[m][n]);
+        }
+        // waves 2 and 3 to 0 and 1, then 1 to 0
+        for (int half = 2; half > 0; half /= 2) {
+            if (wave >= half && wave < 2 * half)
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+                        if (n < tiles)
+                            *reinterpret_cast<Acc*>(
+                                &part[wave - half][n * kTile + col][m * kTile + quad * 4]) = acc[m][n];
+            __syncthreads();
+            if (wave < half)
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+                        if (n < tiles)
+                            acc[m][n] += *reinterpret_cast<const Acc*>(
+                                &part[wave][n * kTile + col][m * kTile + quad * 4]);
+            __syncthreads();
+        }
+        if (wave > 0) return;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            if (n * kTile + col >= many) continue;
+            const long t = window * kWindow + nth_bit(tokens, n * kTile + col);
+            float* h = g.h + (static_cast<long>(split) * g.tokens + t) * all + j0;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const int j = m * kTile + quad * 4;
+                if (j0 + j < all) *reinterpret_cast<Acc*>(h + j) = acc[m][n];
+            }
+        }
+    });
+}
+
+// 256 rows of an adapter's tokens of a window, 64 rows a wave.  Left rows are dealt to the
+// products so that a lane's results of four are 16 neighbours: it reads and writes whole
+// 32 bytes of the output, 128 with its neighbours.
+template <class T>
+__global__ __launch_bounds__(kWaves* kWave) void expand_kernel(Args g) {
+    __shared__ uint16_t hi[kWindow][kPadHalf], lo[kWindow][kPadHalf];
+    __shared__ int shifts[kWindow];
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const int col = lane % kTile, quad = lane / kTile, all = g.sections * g.rank;
+    int sec = 0, tile = blockIdx.x, row0 = 0;
+    for (;; ++sec) {
+        row0 = sec ? g.end[sec - 1] : 0;
+        const int tiles = (g.end[sec] - row0 + kRows - 1) / kRows;
+        if (tile < tiles) break;
+        tile -= tiles;
+    }
+    const int end = g.end[sec], window = blockIdx.z;
+    row0 += tile * kRows;
+    const int mine = row0 + wave * 64 + quad * 16;  // first of a lane's 16 rows
+    const uint64_t idle = each_adapter(g, window, blockIdx.y, gridDim.y, [&](int a, uint64_t tokens) {
+        const int r = rank_of(g, a), many = __popcll(tokens), tiles = (many + kTile - 1) / kTile;
+        const bool whole = g.wide && mine + 16 <= end;
+        long t[4];
+        uint4 old[4][2];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const int slot = n * kTile + col;
+            t[n] = slot < many ? window * kWindow + nth_bit(tokens, slot) : -1;
+            if (t[n] >= 0 && whole) {
+                old[n][0] = *reinterpret_cast<const uint4*>(g.base + t[n] * g.bs + mine);
+                old[n][1] = *reinterpret_cast<const uint4*>(g.base + t[n] * g.bs + mine + 8);
+            }
+        }
+        // inner products: token tid / 4, 16 of 64 ranks
+        const int slot = tid / 4, k0 = tid % 4 * 16;
+        const bool has = slot < many;
+        const float* from = g.h +
+            (window * kWindow + nth_bit(tokens, has ? slot : 0)) * static_cast<long>(all) + sec * g.rank;
+        auto inner = [&](int k, float (&h)[8]) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] = 0.0f;
+            if (!has || k >= r) return;  // ranks are stored by 8, zeros behind the adapter's
+            for (int s = 0; s < g.splits; ++s) {
+                const float* p = from + static_cast<long>(s) * g.tokens * all + k;
+                const Acc u = *reinterpret_cast<const Acc*>(p), v = *reinterpret_cast<const Acc*>(p + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    h[e] += u[e];
+                    h[4 + e] += v[e];
+                }
+            }
+        };
+        float h[2][8];
+        int shift = 0;
+        if (std::is_same_v<T, F16>) {
+            float most = 0.0f;
+            for (int k = k0; k < r; k += kPart) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    inner(k + 8 * i, h[i]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) most = __builtin_fmaxf(most, __builtin_fabsf(h[i][e]));
+                }
+            }
+            most = __builtin_fmaxf(most, __shfl_xor(most, 1, kWave));
+            most = __builtin_fmaxf(most, __shfl_xor(most, 2, kWave));
+            shift = shift_of<T>(most);
+        }
+        Acc acc[4][4] = {};
+        for (int first = 0; first < r; first += kPart) {
+            uint4 up[2][4];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int depth = first + k * kStep + quad * 8;
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const int row = row0 + wave * 64 + col / 4 * 16 + m * 4 + col % 4;
+                    up[k][m] = load8(g.b + a * g.b_adapter + row * g.b_row + depth,
+                                     row < end && depth < r);
+                    up[k][m] = first_of(up[k][m], r - depth);
+                }
+            }
+            __syncthreads();  // the last pass's numbers are read
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int k = k0 + 8 * i;
+                inner(first + k, h[i]);
+                Pair<T> p;
+                p.set(h[i], __builtin_ldexpf(1.0f, shift));
+                *reinterpret_cast<uint4*>(&hi[slot][k]) = p.hi;
+                *reinterpret_cast<uint4*>(&lo[slot][k]) = p.lo;
+            }
+            if (k0 == 0) shifts[slot] = shift;
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                if (first + k * kStep >= r) break;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    if (n >= tiles) break;
+                    const uint4 u = *reinterpret_cast<const uint4*>(&hi[n * kTile + col][k * kStep + quad * 8]);
+                    const uint4 v = *reinterpret_cast<const uint4*>(&lo[n * kTile + col][k * kStep + quad * 8]);
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) {
+                        acc[m][n] = Matrix<T>::mac(up[k][m], u, acc[m][n]);
+                        acc[m][n] = Matrix<T>::mac(up[k][m], v, acc[m][n]);
+                    }
+                }
+            }
+        }
+        const float scale = g.scales[a];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            if (t[n] < 0) continue;
+            const int back = r > 0 ? -shifts[n * kTile + col] : 0;
+            auto add = [&](uint16_t was, int i) {
+                return T::from_float(T::to_float(was) + __builtin_ldexpf(scale * acc[i / 4][n][i % 4], back));
+            };
+            const uint16_t* base = g.base + t[n] * g.bs + mine;
+            uint16_t* out = g.out + t[n] * g.os + mine;
+            if (whole) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    uint32_t w[4] = {old[n][q].x, old[n][q].y, old[n][q].z, old[n][q].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint16_t l = add(static_cast<uint16_t>(w[e]), q * 8 + 2 * e);
+                        const uint16_t h2 = add(static_cast<uint16_t>(w[e] >> 16), q * 8 + 2 * e + 1);
+                        w[e] = static_cast<uint32_t>(h2) << 16 | l;
+                    }
+                    *reinterpret_cast<uint4*>(out + q * 8) = uint4{w[0], w[1], w[2], w[3]};
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (mine + i < end) out[i] = add(base[i], i);
+            }
+        }
+        __syncthreads();  // shifts are read
+    });
+    if (blockIdx.y == 0) copy_idle(g, window, idle, row0, min(row0 + kRows, end), wave, kWaves);
 }
 
 int check(const char* fn, const spb_adapters* d) {
@@ -102,8 +534,21 @@ int check_tokens(const char* fn, int tokens) {
     return 0;
 }
 
+// Blocks that split the columns of the inner products: a few windows do not fill the GPU.
+int splits_of(int tokens) {
+    const int windows = (tokens + kWindow - 1) / kWindow;
+    return windows <= 16 ? 8 : windows < 128 ? 128 / windows : 1;
+}
+
+// What splits_of(n) * n comes to for no n up to `tokens` is more than this.
 size_t workspace_size(const spb_adapters& d, int tokens) {
-    return sizeof(float) * d.num_sections * d.rank * static_cast<size_t>(tokens);
+    const size_t n = tokens, rows = n * 8 < 8192 ? n * 8 : n > 8192 ? n : 8192;
+    return sizeof(float) * d.num_sections * d.rank * rows;
+}
+
+// One launch for up to a window's tokens and few weights; its blocks read A once each.
+bool fused(const Args& g, int tokens) {
+    return tokens <= kWindow && g.rank <= kFusedRank && g.rank * static_cast<long>(g.cols) <= 64 * 1024;
 }
 
 template <class T>
@@ -152,12 +597,29 @@ int run(const char* fn, const spb_adapters* d, const int* ids, const uint16_t* x
         return invalid("%s: a 16-byte aligned workspace of %zu bytes is needed", fn,
                        workspace_size(*d, tokens));
     const hipStream_t st = as_stream(stream);
-    const int waves = kBlock / kWave;
-    hipLaunchKernelGGL(shrink_kernel<T>, dim3(tokens, (g.sections * g.rank + waves - 1) / waves),
-                       dim3(kBlock), 0, st, g);
-    if (int e = launch_status(fn)) return e;
-    hipLaunchKernelGGL(expand_kernel<T>, dim3(tokens, (g.rows + kBlock - 1) / kBlock),
-                       dim3(kBlock), 0, st, g);
+    g.wide = aligned_to(base, 16) && aligned_to(output, 16) && bs % 8 == 0 && os % 8 == 0;
+    for (int s = 0; s + 1 < d->num_sections; ++s) g.wide = g.wide && g.end[s] % 8 == 0;
+    const int windows = (tokens + kWindow - 1) / kWindow;
+    const int distinct = tokens < kWindow ? tokens : kWindow;  // most adapters of a window
+    const int most = distinct < g.num ? distinct : g.num;
+    auto tiles = [&](int size) {
+        int n = 0;
+        for (int s = 0; s < d->num_sections; ++s) n += (d->section_rows[s] + size - 1) / size;
+        return n;
+    };
+    if (fused(g, tokens)) {
+        hipLaunchKernelGGL(fused_kernel<T>, dim3(tiles(kFusedRows), most, windows),
+                           dim3(kFusedWaves * kWave), 0, st, g);
+        return launch_status(fn);
+    }
+    // blocks for a window's adapters: as many as can occur, as long as the grid is small
+    auto ways = [&](int blocks) { return blocks >= 4096 ? 1 : 4096 / blocks < most ? 4096 / blocks : most; };
+    g.splits = splits_of(tokens);
+    const int parts = (g.sections * g.rank + kPart - 1) / kPart;
+    hipLaunchKernelGGL(shrink_kernel<T>, dim3(windows, ways(windows * parts * g.splits), parts * g.splits),
+                       dim3(kWaves * kWave), 0, st, g);
+    hipLaunchKernelGGL(expand_kernel<T>, dim3(tiles(kRows), ways(windows * tiles(kRows)), windows),
+                       dim3(kWaves * kWave), 0, st, g);
     return launch_status(fn);
 }
 
