@@ -162,7 +162,7 @@ constexpr int kFusedRank = 64;                 // most ranks
 constexpr int kFusedPad = kFusedRank + 4;      // numbers of a token in LDS
 
 template <class T>
-__global__ __launch_bounds__(kFusedWaves* kWave) void fused_kernel(Args g) {
+__global__ __launch_bounds__(kFusedWaves* kWave, 4) void fused_kernel(Args g) {
     __shared__ float part[kFusedWaves][kTile][kFusedPad];
     __shared__ float total[kTile][kFusedPad];
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
@@ -178,11 +178,13 @@ __global__ __launch_bounds__(kFusedWaves* kWave) void fused_kernel(Args g) {
     row0 += tile * kFusedRows;
     const int window = blockIdx.z, steps = (g.cols + kStep - 1) / kStep;
     const int step0 = steps * wave / kFusedWaves, step1 = steps * (wave + 1) / kFusedWaves;
+    const int full1 = min(step1, g.cols / kStep);  // of them whole
     const int brow = row0 + wave * kTile + col;  // of the outer product's left side
     const uint64_t idle = each_adapter(g, window, blockIdx.y, gridDim.y, [&](int a, uint64_t tokens) {
         const int r = rank_of(g, a), many = __popcll(tokens);
         const uint16_t* left = g.a + a * g.a_adapter + static_cast<long>(sec * g.rank) * g.a_row;
         const float scale = g.scales[a];
+        const int last = max(r - 1, 0);
         uint4 up[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -193,25 +195,46 @@ __global__ __launch_bounds__(kFusedWaves* kWave) void fused_kernel(Args g) {
         for (int first = 0; first < many; first += kTile) {
             const bool live = first + col < many;
             const int t = window * kWindow + nth_bit(tokens, live ? first + col : first);
-            const uint16_t* x = g.x + t * g.xs;
+            const uint16_t* x = g.x + t * g.xs + quad * 8;
             const int row = row0 + wave * kTile + quad * 4;
             uint16_t old[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 old[e] = live && row + e < end ? g.base[t * g.bs + row + e] : 0;
             Acc acc[kFusedRank / kTile] = {};
+            // rows of A from the adapter's rank on give numbers that are not used
             auto inner = [&](auto tiles) {
-#pragma unroll 4
-                for (int s = step0; s < step1; ++s) {
-                    const int depth = s * kStep + quad * 8;
-                    const bool in = depth < g.cols;
-                    const uint4 v = load8(x + depth, in);
+                constexpr int kTiles = decltype(tiles)::value;
+                const uint16_t* w[kTiles];
 #pragma unroll
-                    for (int m = 0; m < decltype(tiles)::value; ++m) {
-                        const int j = m * kTile + col;
-                        const uint4 w = load8(left + j * g.a_row + depth, in && j < r);
-                        acc[m] = Matrix<T>::mac(w, v, acc[m]);
+                for (int m = 0; m < kTiles; ++m)
+                    w[m] = left + min(m * kTile + col, last) * g.a_row + quad * 8;
+                auto steps = [&](auto many, int s) {  // their loads in flight together
+                    constexpr int kMany = decltype(many)::value;
+                    uint4 v[kMany], q[kMany][kTiles];
+#pragma unroll
+                    for (int i = 0; i < kMany; ++i) {
+                        v[i] = *reinterpret_cast<const uint4*>(x + (s + i) * kStep);
+#pragma unroll
+                        for (int m = 0; m < kTiles; ++m)
+                            q[i][m] = *reinterpret_cast<const uint4*>(w[m] + (s + i) * kStep);
                     }
+#pragma unroll
+                    for (int i = 0; i < kMany; ++i)
+#pragma unroll
+                        for (int m = 0; m < kTiles; ++m) acc[m] = Matrix<T>::mac(q[i][m], v[i], acc[m]);
+                };
+                constexpr int kAhead = kTiles == 1 ? 5 : 4;
+                int s = step0;
+                for (; s + kAhead <= full1; s += kAhead) steps(std::integral_constant<int, kAhead>(), s);
+                for (; s + 2 <= full1; s += 2) steps(std::integral_constant<int, 2>(), s);
+                if (s < full1) steps(std::integral_constant<int, 1>(), s);
+                if (full1 < step1) {  // columns that end inside a step
+                    const bool in = full1 * kStep + quad * 8 < g.cols;
+                    const uint4 v = load8(x + full1 * kStep, in);
+#pragma unroll
+                    for (int m = 0; m < kTiles; ++m)
+                        acc[m] = Matrix<T>::mac(load8(w[m] + full1 * kStep, in), v, acc[m]);
                 }
             };
             if (r <= kTile)
@@ -275,90 +298,99 @@ constexpr int kPad = kPart + 4;     // float32 of a token in LDS
 constexpr int kPadHalf = kPart + 8; // 16-bit numbers of a token in LDS
 constexpr int kRows = kWaves * 64;  // rows of a block of the second
 
-// h of an adapter's tokens of a window and 64 rows of A: 64 x 64 a wave, the waves and
-// g.splits blocks splitting the columns.
+// h of an adapter's tokens of a window and 64 rows of A; g.splits blocks split the columns.
+// Up to 16 tokens: the waves split the block's columns again and add up in LDS.  More: a
+// wave has 16 tokens, and the waves share the rows of A in the cache.
 template <class T>
 __global__ __launch_bounds__(kWaves* kWave) void shrink_kernel(Args g) {
-    __shared__ float part[2][kWindow][kPad];
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    __shared__ float part[kWaves][kTile][kPad];
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const int col = lane % kTile, quad = lane / kTile, all = g.sections * g.rank;
     const int window = blockIdx.x, split = blockIdx.z % g.splits, j0 = blockIdx.z / g.splits * kPart;
-    const int steps = (g.cols + kStep - 1) / kStep, ways = g.splits * kWaves;
-    const int way = split * kWaves + wave;
-    const int step0 = static_cast<int>(static_cast<long>(steps) * way / ways);
-    const int step1 = static_cast<int>(static_cast<long>(steps) * (way + 1) / ways);
+    const long steps = (g.cols + kStep - 1) / kStep;
     each_adapter(g, window, blockIdx.y, gridDim.y, [&](int a, uint64_t tokens) {
         const int r = rank_of(g, a), many = __popcll(tokens);
-        const uint16_t* x[4];
-        const uint16_t* left[4];
-        bool live[4], some[4];
+        const bool few = many <= kTile;
+        const int way = few ? split * kWaves + wave : split, ways = few ? g.splits * kWaves : g.splits;
+        const int step0 = static_cast<int>(steps * way / ways), step1 = static_cast<int>(steps * (way + 1) / ways);
+        const int slot = few ? col : wave * kTile + col;
+        const uint64_t live = __ballot(j0 + lane < all && (j0 + lane) % g.rank < r);
+        const int ranks = live ? kWave - __builtin_clzll(live) : 0;
+        const uint16_t* x = g.x + (window * kWindow + nth_bit(tokens, slot < many ? slot : 0)) * g.xs + quad * 8;
+        Acc acc[4] = {};
+        auto inner = [&](auto tiles) {
+            constexpr int kM = decltype(tiles)::value;
+            const uint16_t* left[kM];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int n = i * kTile + col, j = j0 + n;
-            x[i] = g.x + (window * kWindow + nth_bit(tokens, n < many ? n : 0)) * g.xs + quad * 8;
-            left[i] = g.a + a * g.a_adapter + static_cast<long>(j) * g.a_row + quad * 8;
-            live[i] = j < all && j % g.rank < r;
-            some[i] = __any(live[i]);
-        }
-        const int tiles = (many + kTile - 1) / kTile;
-        Acc acc[4][4] = {};
-#pragma unroll 2
-        for (int s = step0; s < step1; ++s) {
-            const int depth = s * kStep;
-            const bool in = depth + quad * 8 < g.cols;
-            uint4 v[4], w[4];
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-                if (n < tiles) v[n] = load8(x[n] + depth, in);
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-                if (some[m]) w[m] = load8(left[m] + depth, in && live[m]);
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-                if (some[m])
-#pragma unroll
-                    for (int n = 0; n < 4; ++n)
-                        if (n < tiles) acc[m][n] = Matrix<T>::mac(w[m], v[n], acc[m][n]);
-        }
-        // waves 2 and 3 to 0 and 1, then 1 to 0
-        for (int half = 2; half > 0; half /= 2) {
-            if (wave >= half && wave < 2 * half)
-#pragma unroll
-                for (int m = 0; m < 4; ++m)
-#pragma unroll
-                    for (int n = 0; n < 4; ++n)
-                        if (n < tiles)
-                            *reinterpret_cast<Acc*>(
-                                &part[wave - half][n * kTile + col][m * kTile + quad * 4]) = acc[m][n];
-            __syncthreads();
-            if (wave < half)
-#pragma unroll
-                for (int m = 0; m < 4; ++m)
-#pragma unroll
-                    for (int n = 0; n < 4; ++n)
-                        if (n < tiles)
-                            acc[m][n] += *reinterpret_cast<const Acc*>(
-                                &part[wave][n * kTile + col][m * kTile + quad * 4]);
-            __syncthreads();
-        }
-        if (wave > 0) return;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            if (n * kTile + col >= many) continue;
-            const long t = window * kWindow + nth_bit(tokens, n * kTile + col);
-            float* h = g.h + (static_cast<long>(split) * g.tokens + t) * all + j0;
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const int j = m * kTile + quad * 4;
-                if (j0 + j < all) *reinterpret_cast<Acc*>(h + j) = acc[m][n];
+            for (int m = 0; m < kM; ++m) {
+                // the others' rows are a live one's: what they give is not used
+                const int n = m * kTile + col, j = j0 + (live >> n & 1 ? n : __builtin_ctzll(live));
+                left[m] = g.a + a * g.a_adapter + static_cast<long>(j) * g.a_row + quad * 8;
             }
+            auto steps_at = [&](auto some, auto load, int s) {  // their loads in flight together
+                constexpr int kSome = decltype(some)::value;
+                uint4 v[kSome], w[kSome][kM];
+#pragma unroll
+                for (int i = 0; i < kSome; ++i) {
+                    v[i] = load(x + (s + i) * kStep);
+#pragma unroll
+                    for (int m = 0; m < kM; ++m) w[i][m] = load(left[m] + (s + i) * kStep);
+                }
+#pragma unroll
+                for (int i = 0; i < kSome; ++i)
+#pragma unroll
+                    for (int m = 0; m < kM; ++m) acc[m] = Matrix<T>::mac(w[i][m], v[i], acc[m]);
+            };
+            const int full1 = min(step1, g.cols / kStep);
+            auto plain = [](const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); };
+            constexpr int kAhead = 4;
+            int s = step0;
+            for (; s + kAhead <= full1; s += kAhead) steps_at(std::integral_constant<int, kAhead>(), plain, s);
+            if (s + 2 <= full1) {
+                steps_at(std::integral_constant<int, 2>(), plain, s);
+                s += 2;
+            }
+            if (s < full1) steps_at(std::integral_constant<int, 1>(), plain, s);
+            if (full1 < step1) {  // columns that end inside a step
+                const bool in = full1 * kStep + quad * 8 < g.cols;
+                steps_at(std::integral_constant<int, 1>(), [in](const uint16_t* p) { return load8(p, in); }, full1);
+            }
+        };
+        if (few || wave * kTile < many) {
+            if (ranks > 2 * kTile)
+                inner(std::integral_constant<int, 4>());
+            else if (ranks > kTile)
+                inner(std::integral_constant<int, 2>());
+            else if (ranks > 0)
+                inner(std::integral_constant<int, 1>());
         }
+        auto store = [&](int n, int j, Acc v) {  // 4 ranks of the n-th token
+            if (n >= many || j0 + j >= all) return;
+            const long t = window * kWindow + nth_bit(tokens, n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (!(live >> (j + e) & 1)) v[e] = 0.0f;
+            *reinterpret_cast<Acc*>(g.h + (static_cast<long>(split) * g.tokens + t) * all + j0 + j) = v;
+        };
+        if (!few) {
+#pragma unroll
+            for (int m = 0; m < 4; ++m) store(slot, m * kTile + quad * 4, acc[m]);
+            return;
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) *reinterpret_cast<Acc*>(&part[wave][col][m * kTile + quad * 4]) = acc[m];
+        __syncthreads();
+        Acc sum = *reinterpret_cast<const Acc*>(&part[0][tid / 16][tid % 16 * 4]);
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) sum += *reinterpret_cast<const Acc*>(&part[w][tid / 16][tid % 16 * 4]);
+        store(tid / 16, tid % 16 * 4, sum);
+        __syncthreads();
     });
 }
 
 // 256 rows of an adapter's tokens of a window, 64 rows a wave.  Left rows are dealt to the
-// products so that a lane's results of four are 16 neighbours: it reads and writes whole
-// 32 bytes of the output, 128 with its neighbours.
+// products so that a lane's results of two are 8 neighbours, and with its three neighbours'
+// 64 bytes of a token's output.
 template <class T>
 __global__ __launch_bounds__(kWaves* kWave) void expand_kernel(Args g) {
     __shared__ uint16_t hi[kWindow][kPadHalf], lo[kWindow][kPadHalf];
@@ -374,10 +406,10 @@ __global__ __launch_bounds__(kWaves* kWave) void expand_kernel(Args g) {
     }
     const int end = g.end[sec], window = blockIdx.z;
     row0 += tile * kRows;
-    const int mine = row0 + wave * 64 + quad * 16;  // first of a lane's 16 rows
+    const int mine = row0 + wave * 64 + quad * 8;  // a lane's rows: 8 from here on, and 8 from 32 on
     const uint64_t idle = each_adapter(g, window, blockIdx.y, gridDim.y, [&](int a, uint64_t tokens) {
         const int r = rank_of(g, a), many = __popcll(tokens), tiles = (many + kTile - 1) / kTile;
-        const bool whole = g.wide && mine + 16 <= end;
+        const bool whole = g.wide && mine + 40 <= end;
         long t[4];
         uint4 old[4][2];
 #pragma unroll
@@ -386,7 +418,7 @@ __global__ __launch_bounds__(kWaves* kWave) void expand_kernel(Args g) {
             t[n] = slot < many ? window * kWindow + nth_bit(tokens, slot) : -1;
             if (t[n] >= 0 && whole) {
                 old[n][0] = *reinterpret_cast<const uint4*>(g.base + t[n] * g.bs + mine);
-                old[n][1] = *reinterpret_cast<const uint4*>(g.base + t[n] * g.bs + mine + 8);
+                old[n][1] = *reinterpret_cast<const uint4*>(g.base + t[n] * g.bs + mine + 32);
             }
         }
         // inner products: token tid / 4, 16 of 64 ranks
@@ -432,7 +464,7 @@ __global__ __launch_bounds__(kWaves* kWave) void expand_kernel(Args g) {
                 const int depth = first + k * kStep + quad * 8;
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
-                    const int row = row0 + wave * 64 + col / 4 * 16 + m * 4 + col % 4;
+                    const int row = row0 + wave * 64 + m / 2 * 32 + col / 4 * 8 + m % 2 * 4 + col % 4;
                     up[k][m] = load8(g.b + a * g.b_adapter + row * g.b_row + depth,
                                      row < end && depth < r);
                     up[k][m] = first_of(up[k][m], r - depth);
@@ -486,12 +518,14 @@ __global__ __launch_bounds__(kWaves* kWave) void expand_kernel(Args g) {
                         const uint16_t h2 = add(static_cast<uint16_t>(w[e] >> 16), q * 8 + 2 * e + 1);
                         w[e] = static_cast<uint32_t>(h2) << 16 | l;
                     }
-                    *reinterpret_cast<uint4*>(out + q * 8) = uint4{w[0], w[1], w[2], w[3]};
+                    *reinterpret_cast<uint4*>(out + q * 32) = uint4{w[0], w[1], w[2], w[3]};
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (mine + i < end) out[i] = add(base[i], i);
+                for (int i = 0; i < 16; ++i) {
+                    const int at = i / 8 * 32 + i % 8;
+                    if (mine + at < end) out[at] = add(base[at], i);
+                }
             }
         }
         __syncthreads();  // shifts are read

@@ -1227,61 +1227,252 @@ struct LogprobArgs {
     float* logprobs;
     int* top_ids;
     float* top_logprobs;
-    int rows, vocab, top;
+    int vocab, top;
 };
 
-// One block a row.  log(sum of exp(l - max)) = log1p(the weights of all but one token of
-// the largest logit), so that a token with nearly all of the mass keeps its digits.
+constexpr int kGroups = kRow;      // groups of a row's units whose largest logits are compared
+constexpr int kCandidates = 4096;  // = kMaxTop lanes' largest logits
+
+// A sum of exponentials: the largest logit, how many there are of it, and the exponentials of
+// the others less it.  The largest are counted apart: beside a 1, weights of 1e-11 would lose
+// digits, and a token with nearly all of the mass is told from them.
+struct Sum {
+    float top;
+    int count;
+    double rest;
+
+    static __device__ __forceinline__ double less(float low, float high) {
+        return __builtin_amdgcn_exp2f((low - high) * 0x1.715476p+0f);
+    }
+};
+
+struct LogprobWork {
+    Sum* sums;  // [rows][units]
+    int first, rows, units;
+};
+
+// Adds a unit to a wave's sum: top and count are the wave's, rest is each lane's.  Float32
+// exponentials of float32 differences are off by (|difference| + 1) * 2^-23; 16 of them are
+// added in float32, by pairs, and those in float64.
 template <class T>
-__global__ __launch_bounds__(kRow) void logprob_row_kernel(LogprobArgs g) {
+__device__ __forceinline__ float sum_unit(Sum& s, const Unit<T>& x, const typename T::Bits* row, int vocab,
+                                          int u) {
+    float peak = -__builtin_inff();
+    x.each(row, vocab, u, [&](float l, int, int) { peak = __builtin_fmaxf(peak, l); });
+    peak = from_lane(wave_scan(peak, -__builtin_inff(), Max()), kWave - 1);
+    if (peak == -__builtin_inff()) return peak;
+    if (peak > s.top) {
+        s.rest = (s.rest + (threadIdx.x % kWave == 0 ? s.count : 0)) * Sum::less(s.top, peak);
+        s.top = peak;
+        s.count = 0;
+    }
+    const bool has = peak == s.top;
+    float w[16];
+    int equal = 0;
+    x.each(row, vocab, u, [&](float l, int, int e) {
+        w[e] = __builtin_amdgcn_exp2f((l - s.top) * 0x1.715476p+0f);
+        if (has) {
+            w[e] = l == s.top ? 0.0f : w[e];
+            equal += l == s.top;
+        }
+    });
+#pragma unroll
+    for (int d = 8; d > 0; d /= 2)
+#pragma unroll
+        for (int e = 0; e < d; ++e) w[e] += w[e + d];
+    s.rest += w[0];
+    if (has) s.count += from_lane(wave_scan(equal, 0, Add()), kWave - 1);
+    return peak;
+}
+
+__device__ __forceinline__ unsigned long long rank_key(float l, int index) {
+    return static_cast<unsigned long long>(~key_of(l)) << 32 | static_cast<uint32_t>(index);
+}
+
+// Few rows: a wave has a unit, and another kernel adds up.
+template <class T>
+__global__ __launch_bounds__(kSplitBlock) void logprob_units_kernel(LogprobArgs g, LogprobWork w) {
+    const int r = blockIdx.y, row = w.first + r;
+    const int u = blockIdx.x * (kSplitBlock / kWave) + static_cast<int>(threadIdx.x / kWave);
+    if (u >= w.units) return;
+    const typename T::Bits* logits = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
+    Unit<T> x;
+    x.load(logits, g.vocab, u);
+    Sum s{-__builtin_inff(), 0, 0.0};
+    sum_unit<T>(s, x, logits, g.vocab, u);
+    s.rest = from_lane(wave_scan(s.rest, 0.0, Add()), kWave - 1);
+    if (threadIdx.x % kWave == 0) w.sums[static_cast<long>(r) * w.units + u] = s;
+}
+
+// A row's log-probabilities, and its `top` likeliest tokens.  kWhole: all of it by this block;
+// else from the units' sums.
+//
+// The likeliest are in the `top` groups of units with the largest logits (equal ones: the
+// first), for any other group has `top` tokens before its own.  These groups are read again,
+// and their tokens from the last of those logits on are sorted: a few more than `top`, mostly.
+// Where they are many (a row in rising order), the same is done with lanes for groups: at
+// most 16 of each of `top` lanes are left.
+template <class T, bool kWhole>
+__global__ __launch_bounds__(kRow) void logprob_kernel(LogprobArgs g, LogprobWork w) {
+    __shared__ uint32_t peaks[kGroups];
+    __shared__ unsigned long long list[kCandidates];
     __shared__ union {
         float f[kWaves];
-        double d[kWaves];
         int i[kWaves];
+        double d[kWaves];
         unsigned long long u[kWaves];
     } part;
-    const int row = blockIdx.x;
+    __shared__ int chosen[kMaxTop], listed;
+    const int r = blockIdx.x, row = w.first + r, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const int token = g.tokens ? g.tokens[row] : 0;
     if (token < 0 || token >= g.vocab) return;
-    const typename T::Bits* l = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
-    float top = -__builtin_inff();
-    for (int i = threadIdx.x; i < g.vocab; i += kRow) top = __builtin_fmaxf(top, clean(T::load(l + i)));
-    top = block_reduce(top, -__builtin_inff(), part.f, Max());
-    // the largest ones are counted apart: beside a 1, weights of 1e-11 would lose digits
-    double rest = 0.0;
-    int largest = 0;
-    for (int i = threadIdx.x; i < g.vocab; i += kRow) {
-        const float v = clean(T::load(l + i));
-        if (v == top)
-            ++largest;
-        else if (v != -__builtin_inff())
-            rest += expf(v - top);
-    }
-    rest = block_reduce(rest, 0.0, part.d, Add());
-    largest = block_reduce(largest, 0, part.i, Add());
-    const double norm = log1p(rest + (largest - 1));
-    auto logprob = [&](float v) {
-        return v == -__builtin_inff() ? v : static_cast<float>((v == top ? 0.0 : static_cast<double>(v) - top) - norm);
+    const typename T::Bits* logits = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
+    const float mine = clean(T::load(logits + token));
+    const int size = (w.units + kGroups - 1) / kGroups, groups = (w.units + size - 1) / size;
+    if (tid < groups) peaks[tid] = 0;
+    if (tid == 0) listed = 0;
+    __syncthreads();
+    // a thread's part of the sum: in kWhole each wave's by its first lane, else some units'
+    Sum s{-__builtin_inff(), 0, 0.0};
+    auto peak_of = [&](int u, float peak) {
+        if (!g.top) return;
+        if (size == 1)
+            peaks[u] = key_of(peak);
+        else
+            atomicMax(&peaks[u / size], key_of(peak));
     };
-    if (threadIdx.x == 0 && g.tokens) g.logprobs[row] = logprob(clean(T::load(l + token)));
-    unsigned long long last = ~0ull;  // key, then the lowest index
-    for (int n = 0; n < g.top; ++n) {
-        unsigned long long best = 0;
-        for (int i = threadIdx.x; i < g.vocab; i += kRow) {
-            const unsigned long long c =
-                static_cast<unsigned long long>(key_of(clean(T::load(l + i)))) << 32 |
-                static_cast<uint32_t>(~i);
-            if (c < last && c > best) best = c;
+    if constexpr (kWhole) {
+        each_unit<T>(logits, g.vocab, wave, kWaves, w.units, [](int) { return true; },
+                     [&](const Unit<T>& x, int u) {
+                         const float peak = sum_unit<T>(s, x, logits, g.vocab, u);
+                         if (lane == 0) peak_of(u, peak);
+                     });
+        if (lane > 0) s.count = 0;
+    } else {
+        for (int u = tid; u < w.units; u += kRow) {
+            const Sum o = w.sums[static_cast<long>(r) * w.units + u];
+            peak_of(u, o.top);
+            if (o.top == -__builtin_inff()) continue;
+            if (o.top > s.top) {
+                s.rest = (s.rest + s.count) * Sum::less(s.top, o.top);
+                s.top = o.top;
+                s.count = 0;
+            }
+            s.rest += o.top == s.top ? o.rest : (o.rest + o.count) * Sum::less(o.top, s.top);
+            s.count += o.top == s.top ? o.count : 0;
         }
-        last = block_reduce(best, 0ull, part.u, Max());
-        if (threadIdx.x == 0) {
-            g.top_ids[static_cast<long>(row) * g.top + n] = static_cast<int>(~static_cast<uint32_t>(last));
-            g.top_logprobs[static_cast<long>(row) * g.top + n] = logprob(from_key(static_cast<uint32_t>(last >> 32)));
+    }
+    const float top = block_reduce(s.top, -__builtin_inff(), part.f, Max());
+    double rest = 0.0;
+    if (s.top != -__builtin_inff()) rest = s.top == top ? s.rest : (s.rest + s.count) * Sum::less(s.top, top);
+    rest = block_reduce(rest, 0.0, part.d, Add());
+    const int equal = block_reduce(s.top == top ? s.count : 0, 0, part.i, Add());
+    auto logprob = [&](float l) {
+        if (l == -__builtin_inff()) return l;
+        return static_cast<float>((l == top ? 0.0 : static_cast<double>(l) - top) - log1p(rest + (equal - 1)));
+    };
+    if (tid == 0 && g.tokens) g.logprobs[row] = logprob(mine);
+    if (g.top == 0) return;
+    // the groups: a group's rank is the number of better ones
+    const int many = min(g.top, groups);
+    if (tid < groups) {
+        const uint32_t key = peaks[tid];
+        int rank = 0;
+        for (int i = 0; i < groups; ++i) rank += peaks[i] > key || (peaks[i] == key && i < tid);
+        if (rank < many) chosen[rank] = tid;
+    }
+    __syncthreads();
+    const float bound = many < g.top ? -__builtin_inff() : from_key(peaks[chosen[many - 1]]);
+    // f(unit's logits, index) for the units of the groups, a wave each
+    auto each_chosen = [&](auto f) {
+        for (int i = wave; i < many * size; i += kWaves) {
+            const int u = chosen[i / size] * size + i % size;
+            if (u >= w.units) continue;
+            Unit<T> x;
+            x.load(logits, g.vocab, u);
+            f(x, u, i / size);
         }
+    };
+    auto gather = [&](float least, unsigned long long last) {
+        each_chosen([&](const Unit<T>& x, int u, int) {
+            uint32_t hits = 0;
+            x.each(logits, g.vocab, u, [&](float l, int i, int e) {
+                const bool in = l >= least && i >= 0 && i < g.vocab && rank_key(l, i) <= last;
+                hits |= static_cast<uint32_t>(in) << e;
+            });
+            const int own = __popc(hits), upto = wave_scan(own, 0, Add()), all = from_lane(upto, kWave - 1);
+            if (all == 0) return;
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&listed, all);
+            at = from_lane(at, 0) + upto - own;
+            x.each(logits, g.vocab, u, [&](float l, int i, int e) {
+                if (!(hits >> e & 1)) return;
+                if (at < kCandidates) list[at] = rank_key(l, i);
+                ++at;
+            });
+        });
+        __syncthreads();
+        return __builtin_amdgcn_readfirstlane(listed);
+    };
+    int n = gather(bound, ~0ull);
+    if (n > kRow) {
+        // the best of each of the groups' lanes, and of those the last that can be wanted
+        __syncthreads();
+        if (tid == 0) listed = 0;
+        for (int i = tid; i < kMaxTop * kWave; i += kRow) list[i] = ~0ull;
+        __syncthreads();
+        each_chosen([&](const Unit<T>& x, int u, int c) {
+            unsigned long long best = ~0ull;
+            x.each(logits, g.vocab, u, [&](float l, int i, int) {
+                if (i < 0 || i >= g.vocab) return;
+                const unsigned long long k = rank_key(l, i);
+                best = k < best ? k : best;
+            });
+            atomicMin(&list[c * kWave + lane], best);
+        });
+        __syncthreads();
+        sort_list<kCandidates / kRow>(list, many * kWave);
+        const unsigned long long last = list[g.top - 1];
+        __syncthreads();
+        n = gather(-__builtin_inff(), last);
+    }
+    if (n > kCandidates) {
+        // groups of many units (vocabularies of millions) in rising order: one after the other
+        unsigned long long last = 0;
+        for (int i = 0; i < g.top; ++i) {
+            unsigned long long best = ~0ull;
+            for (int j = tid; j < g.vocab; j += kRow) {
+                const unsigned long long k = rank_key(clean(T::load(logits + j)), j);
+                if ((i == 0 || k > last) && k < best) best = k;
+            }
+            last = block_reduce(best, ~0ull, part.u, Min());
+            if (tid == 0) list[i] = last;
+        }
+        __syncthreads();
+    } else if (n <= kRow) {
+        sort_list<1>(list, n);
+    } else {
+        sort_list<kCandidates / kRow>(list, n);
+    }
+    if (tid < g.top) {
+        const unsigned long long k = list[tid];
+        g.top_ids[static_cast<long>(row) * g.top + tid] = static_cast<int>(static_cast<uint32_t>(k));
+        g.top_logprobs[static_cast<long>(row) * g.top + tid] = logprob(from_key(~static_cast<uint32_t>(k >> 32)));
     }
 }
 
-size_t logprobs_workspace(int rows, int vocab, int top) { return 256; }
+// Rows of one launch of the split kernels.
+size_t logprobs_layout(int rows, int units, char* base, LogprobWork* w) {
+    const size_t n = rows < 1 ? 1 : rows < kSplitRows ? rows : kSplitRows;
+    if (w) w->sums = reinterpret_cast<Sum*>(base);
+    return align256(n * units * sizeof(Sum));
+}
+
+size_t logprobs_workspace(int rows, int vocab) {
+    return logprobs_layout(rows, units_of<Half<F16>>(vocab), nullptr, nullptr);
+}
+
+bool logprobs_whole(int rows, int units) { return rows >= 128 || units <= 16; }
 
 int check_top(const char* fn, int top) {
     if (top < 0 || top > kMaxTop) return invalid("%s: top %d must be in [0, %d]", fn, top, kMaxTop);
@@ -1305,10 +1496,24 @@ int token_logprobs(const char* fn, const void* logits, long stride, const int* t
     const void* four[] = {tokens, logprobs, top_ids, top_logprobs};
     for (const void* p : four)
         if (!aligned_to(p, 4)) return invalid("%s: a vector is not 4-byte aligned", fn);
-    if (int e = check_workspace(fn, ws, size, logprobs_workspace(rows, vocab, top))) return e;
-    LogprobArgs g{logits, stride, tokens, logprobs, top_ids, top_logprobs, rows, vocab, top};
-    hipLaunchKernelGGL(logprob_row_kernel<T>, dim3(rows), dim3(kRow), 0, as_stream(stream), g);
-    return launch_status(fn);
+    if (int e = check_workspace(fn, ws, size, logprobs_workspace(rows, vocab))) return e;
+    LogprobArgs g{logits, stride, tokens, logprobs, top_ids, top_logprobs, vocab, top};
+    LogprobWork w{};
+    w.units = units_of<T>(vocab);
+    logprobs_layout(rows, w.units, static_cast<char*>(ws), &w);
+    const hipStream_t st = as_stream(stream);
+    if (logprobs_whole(rows, w.units)) {
+        hipLaunchKernelGGL((logprob_kernel<T, true>), dim3(rows), dim3(kRow), 0, st, g, w);
+        return launch_status(fn);
+    }
+    const int blocks = (w.units + kSplitBlock / kWave - 1) / (kSplitBlock / kWave);
+    for (w.first = 0; w.first < rows; w.first += w.rows) {
+        w.rows = rows - w.first < kSplitRows ? rows - w.first : kSplitRows;
+        hipLaunchKernelGGL(logprob_units_kernel<T>, dim3(blocks, w.rows), dim3(kSplitBlock), 0, st, g, w);
+        hipLaunchKernelGGL((logprob_kernel<T, false>), dim3(w.rows), dim3(kRow), 0, st, g, w);
+        if (int e = launch_status(fn)) return e;
+    }
+    return 0;
 }
 
 }  // namespace
@@ -1344,7 +1549,7 @@ int spb_sample_bf16(const uint16_t* logits, long logits_stride, const float* uni
 size_t spb_token_logprobs_workspace_size(int rows, int vocab, int top) {
     clear_error();
     const char* fn = "spb_token_logprobs_workspace_size";
-    return check_rows(fn, rows, vocab) || check_top(fn, top) ? 0 : logprobs_workspace(rows, vocab, top);
+    return check_rows(fn, rows, vocab) || check_top(fn, top) ? 0 : logprobs_workspace(rows, vocab);
 }
 int spb_token_logprobs_f32(const float* logits, long logits_stride, const int* tokens,
                            float* logprobs, int* top_ids, float* top_logprobs, int rows,
