@@ -27,7 +27,9 @@ struct Args {
     uint16_t* out;
     float* h;  // [splits][tokens][sections * rank]
     long a_adapter, a_row, b_adapter, b_row, xs, bs, os;
-    int num, rank, cols, sections, tokens, rows, splits;
+    int num, rank, cols, sections, tokens, rows;
+    int id_bits;     // ids are below 2^id_bits
+    int split_bits;  // 2^split_bits blocks split the columns of the inner products
     int end[kMaxSections];  // first row behind each section
     bool wide;              // base and output by 16 bytes
 };
@@ -87,22 +89,48 @@ __device__ __forceinline__ int nth_bit(uint64_t m, int n) {
     return at;
 }
 
-// A window's adapters: f(adapter, set of its tokens) for the z-th, (z + step)-th, ... of those
-// that occur, in the order of their first tokens.  Returns the tokens that have none.
+// An adapter's tokens in a window.
+struct Group {
+    int adapter, many;
+    int listed;  // lane n: the n-th one's place in the window (lanes from `many` on: the first's)
+    // The n-th one's token.
+    __device__ __forceinline__ long token(int window, int n) const {
+        return window * kWindow + __shfl(listed, n, kWave);
+    }
+};
+
+// A window's adapters: f(group) for the z-th, (z + step)-th, ... of those that occur, in the
+// order of their first tokens.  Returns the tokens that have none.  A lane finds the tokens
+// of its own adapter bit by bit of the ids; going through the adapters one after the other
+// took 5 us of the 20 that 24 adapters' inner products did.
 template <class F>
 __device__ __forceinline__ uint64_t each_adapter(const Args& g, int window, int z, int step, F f) {
-    const int t = window * kWindow + static_cast<int>(threadIdx.x % kWave);
+    const int lane = threadIdx.x % kWave, t = window * kWindow + lane;
     const int id = t < g.tokens ? g.ids[t] : -1;
     const bool has = id >= 0 && id < g.num;
-    uint64_t left = __ballot(has);
-    const uint64_t idle = __ballot(t < g.tokens) & ~left;
-    for (int i = 0; left; ++i) {
-        const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-        const uint64_t mine = __ballot(id == a) & left;
-        left &= ~mine;
-        if (i % step == z) f(a, mine);
+    const uint64_t valid = __ballot(has);
+    uint64_t same = valid;
+    for (int b = 0; b < g.id_bits; ++b) {
+        const bool one = id >> b & 1;
+        const uint64_t ones = __ballot(one);
+        same &= one ? ones : ~ones;
     }
-    return idle;
+    const uint64_t before = same & ((uint64_t{1} << lane) - 1);
+    const uint64_t firsts = __ballot(has && before == 0);
+    const int groups = __popcll(firsts);
+    for (int i = z; i < groups; i += step) {
+        const int first = __builtin_amdgcn_readfirstlane(nth_bit(firsts, i));
+        Group q;
+        q.adapter = __builtin_amdgcn_readlane(id, first);
+        const bool mine = has && id == q.adapter;
+        q.many = __popcll(__ballot(mine));
+        // each of its lanes to the lane of its place in the group, the others to the last
+        const int place = mine ? __popcll(before) : kWave - 1;
+        const int got = __builtin_amdgcn_ds_permute(place * 4, lane);
+        q.listed = lane < q.many ? got : first;
+        f(q);
+    }
+    return __ballot(t < g.tokens) & ~valid;
 }
 
 // output = base in rows [row, end) of the tokens that have no adapter, a wave each.
@@ -180,8 +208,8 @@ __global__ __launch_bounds__(kFusedWaves* kWave, 4) void fused_kernel(Args g) {
     const int step0 = steps * wave / kFusedWaves, step1 = steps * (wave + 1) / kFusedWaves;
     const int full1 = min(step1, g.cols / kStep);  // of them whole
     const int brow = row0 + wave * kTile + col;  // of the outer product's left side
-    const uint64_t idle = each_adapter(g, window, blockIdx.y, gridDim.y, [&](int a, uint64_t tokens) {
-        const int r = rank_of(g, a), many = __popcll(tokens);
+    const uint64_t idle = each_adapter(g, window, blockIdx.y, gridDim.y, [&](const Group& q) {
+        const int a = q.adapter, r = rank_of(g, a), many = q.many;
         const uint16_t* left = g.a + a * g.a_adapter + static_cast<long>(sec * g.rank) * g.a_row;
         const float scale = g.scales[a];
         const int last = max(r - 1, 0);
@@ -194,7 +222,7 @@ __global__ __launch_bounds__(kFusedWaves* kWave, 4) void fused_kernel(Args g) {
         }
         for (int first = 0; first < many; first += kTile) {
             const bool live = first + col < many;
-            const int t = window * kWindow + nth_bit(tokens, live ? first + col : first);
+            const long t = q.token(window, live ? first + col : first);
             const uint16_t* x = g.x + t * g.xs + quad * 8;
             const int row = row0 + wave * kTile + quad * 4;
             uint16_t old[4];
@@ -306,17 +334,20 @@ __global__ __launch_bounds__(kWaves* kWave) void shrink_kernel(Args g) {
     __shared__ float part[kWaves][kTile][kPad];
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const int col = lane % kTile, quad = lane / kTile, all = g.sections * g.rank;
-    const int window = blockIdx.x, split = blockIdx.z % g.splits, j0 = blockIdx.z / g.splits * kPart;
-    const long steps = (g.cols + kStep - 1) / kStep;
-    each_adapter(g, window, blockIdx.y, gridDim.y, [&](int a, uint64_t tokens) {
-        const int r = rank_of(g, a), many = __popcll(tokens);
+    const int window = blockIdx.x, split = blockIdx.z & ((1 << g.split_bits) - 1);
+    const int j0 = (blockIdx.z >> g.split_bits) * kPart, steps = (g.cols + kStep - 1) / kStep;
+    int of_section = j0 + lane;  // the row's number in its section
+#pragma unroll
+    for (int s = 1; s < kMaxSections; ++s) of_section -= of_section >= g.rank ? g.rank : 0;
+    each_adapter(g, window, blockIdx.y, gridDim.y, [&](const Group& q) {
+        const int a = q.adapter, r = rank_of(g, a), many = q.many;
         const bool few = many <= kTile;
-        const int way = few ? split * kWaves + wave : split, ways = few ? g.splits * kWaves : g.splits;
-        const int step0 = static_cast<int>(steps * way / ways), step1 = static_cast<int>(steps * (way + 1) / ways);
+        const int way = few ? split * kWaves + wave : split, way_bits = g.split_bits + (few ? 2 : 0);
+        const int step0 = steps * way >> way_bits, step1 = steps * (way + 1) >> way_bits;
         const int slot = few ? col : wave * kTile + col;
-        const uint64_t live = __ballot(j0 + lane < all && (j0 + lane) % g.rank < r);
+        const uint64_t live = __ballot(j0 + lane < all && of_section < r);
         const int ranks = live ? kWave - __builtin_clzll(live) : 0;
-        const uint16_t* x = g.x + (window * kWindow + nth_bit(tokens, slot < many ? slot : 0)) * g.xs + quad * 8;
+        const uint16_t* x = g.x + q.token(window, slot < many ? slot : 0) * g.xs + quad * 8;
         Acc acc[4] = {};
         auto inner = [&](auto tiles) {
             constexpr int kM = decltype(tiles)::value;
@@ -365,8 +396,8 @@ __global__ __launch_bounds__(kWaves* kWave) void shrink_kernel(Args g) {
                 inner(std::integral_constant<int, 1>());
         }
         auto store = [&](int n, int j, Acc v) {  // 4 ranks of the n-th token
+            const long t = q.token(window, n);
             if (n >= many || j0 + j >= all) return;
-            const long t = window * kWindow + nth_bit(tokens, n);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (!(live >> (j + e) & 1)) v[e] = 0.0f;
@@ -407,15 +438,16 @@ __global__ __launch_bounds__(kWaves* kWave) void expand_kernel(Args g) {
     const int end = g.end[sec], window = blockIdx.z;
     row0 += tile * kRows;
     const int mine = row0 + wave * 64 + quad * 8;  // a lane's rows: 8 from here on, and 8 from 32 on
-    const uint64_t idle = each_adapter(g, window, blockIdx.y, gridDim.y, [&](int a, uint64_t tokens) {
-        const int r = rank_of(g, a), many = __popcll(tokens), tiles = (many + kTile - 1) / kTile;
+    const uint64_t idle = each_adapter(g, window, blockIdx.y, gridDim.y, [&](const Group& q) {
+        const int a = q.adapter, r = rank_of(g, a), many = q.many, tiles = (many + kTile - 1) / kTile;
         const bool whole = g.wide && mine + 40 <= end;
         long t[4];
         uint4 old[4][2];
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             const int slot = n * kTile + col;
-            t[n] = slot < many ? window * kWindow + nth_bit(tokens, slot) : -1;
+            t[n] = q.token(window, slot);
+            if (slot >= many) t[n] = -1;
             if (t[n] >= 0 && whole) {
                 old[n][0] = *reinterpret_cast<const uint4*>(g.base + t[n] * g.bs + mine);
                 old[n][1] = *reinterpret_cast<const uint4*>(g.base + t[n] * g.bs + mine + 32);
@@ -424,13 +456,12 @@ __global__ __launch_bounds__(kWaves* kWave) void expand_kernel(Args g) {
         // inner products: token tid / 4, 16 of 64 ranks
         const int slot = tid / 4, k0 = tid % 4 * 16;
         const bool has = slot < many;
-        const float* from = g.h +
-            (window * kWindow + nth_bit(tokens, has ? slot : 0)) * static_cast<long>(all) + sec * g.rank;
+        const float* from = g.h + q.token(window, slot) * all + sec * g.rank;
         auto inner = [&](int k, float (&h)[8]) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) h[e] = 0.0f;
             if (!has || k >= r) return;  // ranks are stored by 8, zeros behind the adapter's
-            for (int s = 0; s < g.splits; ++s) {
+            for (int s = 0; s < 1 << g.split_bits; ++s) {
                 const float* p = from + static_cast<long>(s) * g.tokens * all + k;
                 const Acc u = *reinterpret_cast<const Acc*>(p), v = *reinterpret_cast<const Acc*>(p + 4);
 #pragma unroll
@@ -568,13 +599,13 @@ int check_tokens(const char* fn, int tokens) {
     return 0;
 }
 
-// Blocks that split the columns of the inner products: a few windows do not fill the GPU.
-int splits_of(int tokens) {
+// 2^n blocks split the columns of the inner products: a few windows do not fill the GPU.
+int split_bits_of(int tokens) {
     const int windows = (tokens + kWindow - 1) / kWindow;
-    return windows <= 16 ? 8 : windows < 128 ? 128 / windows : 1;
+    return windows <= 16 ? 3 : windows <= 32 ? 2 : windows <= 64 ? 1 : 0;
 }
 
-// What splits_of(n) * n comes to for no n up to `tokens` is more than this.
+// What the splits of n tokens times n come to for no n up to `tokens` is more than this.
 size_t workspace_size(const spb_adapters& d, int tokens) {
     const size_t n = tokens, rows = n * 8 < 8192 ? n * 8 : n > 8192 ? n : 8192;
     return sizeof(float) * d.num_sections * d.rank * rows;
@@ -619,6 +650,7 @@ int run(const char* fn, const spb_adapters* d, const int* ids, const uint16_t* x
     g.cols = d->cols;
     g.sections = d->num_sections;
     g.tokens = tokens;
+    while (g.id_bits < 31 && d->num_adapters > 1 << g.id_bits) ++g.id_bits;
     for (int s = 0; s < kMaxSections; ++s) {
         if (s < d->num_sections) g.rows += d->section_rows[s];
         g.end[s] = g.rows;
@@ -648,9 +680,10 @@ int run(const char* fn, const spb_adapters* d, const int* ids, const uint16_t* x
     }
     // blocks for a window's adapters: as many as can occur, as long as the grid is small
     auto ways = [&](int blocks) { return blocks >= 4096 ? 1 : 4096 / blocks < most ? 4096 / blocks : most; };
-    g.splits = splits_of(tokens);
+    g.split_bits = split_bits_of(tokens);
     const int parts = (g.sections * g.rank + kPart - 1) / kPart;
-    hipLaunchKernelGGL(shrink_kernel<T>, dim3(windows, ways(windows * parts * g.splits), parts * g.splits),
+    const int blocks = parts << g.split_bits;
+    hipLaunchKernelGGL(shrink_kernel<T>, dim3(windows, ways(windows * blocks), blocks),
                        dim3(kWaves * kWave), 0, st, g);
     hipLaunchKernelGGL(expand_kernel<T>, dim3(tiles(kRows), ways(windows * tiles(kRows)), windows),
                        dim3(kWaves * kWave), 0, st, g);
