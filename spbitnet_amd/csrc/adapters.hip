@@ -69,6 +69,10 @@ __device__ __forceinline__ uint4 load8(const uint16_t* p, bool valid) {
     return v;
 }
 
+__device__ __forceinline__ uint4 zero_unless(bool in, uint4 v) {
+    return {in ? v.x : 0u, in ? v.y : 0u, in ? v.z : 0u, in ? v.w : 0u};
+}
+
 // The first n of 8 numbers.
 __device__ __forceinline__ uint4 first_of(uint4 v, int n) {
     auto part = [n](uint32_t w, int i) { return n > i + 1 ? w : n > i ? w & 0xffffu : 0u; };
@@ -323,109 +327,87 @@ __global__ __launch_bounds__(kFusedWaves* kWave, 4) void fused_kernel(Args g) {
 constexpr int kWaves = 4;
 constexpr int kPart = 64;           // ranks of a block of the first, of a pass of the second
 constexpr int kPad = kPart + 4;     // float32 of a token in LDS
-constexpr int kPadHalf = kPart + 8; // 16-bit numbers of a token in LDS
 constexpr int kRows = kWaves * 64;  // rows of a block of the second
 
-// h of an adapter's tokens of a window and 64 rows of A; g.splits blocks split the columns.
-// Up to 16 tokens: the waves split the block's columns again and add up in LDS.  More: a
-// wave has 16 tokens, and the waves share the rows of A in the cache.
+// h of 16 of an adapter's tokens of a window and 64 rows of A: g.split_bits blocks and their
+// waves split the columns, the waves add up in LDS.  Most of a block's time is fetching its
+// code, which a launch finds in no cache of its CU: one loop, two bodies.
 template <class T>
 __global__ __launch_bounds__(kWaves* kWave) void shrink_kernel(Args g) {
     __shared__ float part[kWaves][kTile][kPad];
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const int col = lane % kTile, quad = lane / kTile, all = g.sections * g.rank;
     const int window = blockIdx.x, split = blockIdx.z & ((1 << g.split_bits) - 1);
-    const int j0 = (blockIdx.z >> g.split_bits) * kPart, steps = (g.cols + kStep - 1) / kStep;
-    int of_section = j0 + lane;  // the row's number in its section
-#pragma unroll
-    for (int s = 1; s < kMaxSections; ++s) of_section -= of_section >= g.rank ? g.rank : 0;
+    const int first = (blockIdx.z >> g.split_bits & 3) * kTile;  // of the adapter's tokens
+    const int j0 = (blockIdx.z >> g.split_bits >> 2) * kPart;
     each_adapter(g, window, blockIdx.y, gridDim.y, [&](const Group& q) {
-        const int a = q.adapter, r = rank_of(g, a), many = q.many;
-        const bool few = many <= kTile;
-        const int way = few ? split * kWaves + wave : split, way_bits = g.split_bits + (few ? 2 : 0);
-        const int step0 = steps * way >> way_bits, step1 = steps * (way + 1) >> way_bits;
-        const int slot = few ? col : wave * kTile + col;
+        if (first >= q.many) return;
+        const int r = rank_of(g, q.adapter);
+        int of_section = j0 + lane;  // the row's number in its section
+        while (of_section >= g.rank) of_section -= g.rank;
         const uint64_t live = __ballot(j0 + lane < all && of_section < r);
         const int ranks = live ? kWave - __builtin_clzll(live) : 0;
-        const uint16_t* x = g.x + q.token(window, slot < many ? slot : 0) * g.xs + quad * 8;
+        const int steps = (g.cols + kStep - 1) / kStep, way = split * kWaves + wave;
+        const int bits = g.split_bits + 2, step0 = steps * way >> bits, step1 = steps * (way + 1) >> bits;
+        const uint16_t* x = g.x + q.token(window, first + col < q.many ? first + col : first) * g.xs + quad * 8;
+        const uint16_t* a = g.a + q.adapter * g.a_adapter + j0 * g.a_row + quad * 8;
         Acc acc[4] = {};
         auto inner = [&](auto tiles) {
-            constexpr int kM = decltype(tiles)::value;
-            const uint16_t* left[kM];
+            constexpr int kM = decltype(tiles)::value, kAhead = kM == 1 ? 4 : 2;
+            const uint16_t* row[kM];
 #pragma unroll
             for (int m = 0; m < kM; ++m) {
                 // the others' rows are a live one's: what they give is not used
-                const int n = m * kTile + col, j = j0 + (live >> n & 1 ? n : __builtin_ctzll(live));
-                left[m] = g.a + a * g.a_adapter + static_cast<long>(j) * g.a_row + quad * 8;
+                const int n = m * kTile + col;
+                row[m] = a + (live >> n & 1 ? n : __builtin_ctzll(live)) * g.a_row;
             }
-            auto steps_at = [&](auto some, auto load, int s) {  // their loads in flight together
-                constexpr int kSome = decltype(some)::value;
-                uint4 v[kSome], w[kSome][kM];
+            for (int s = step0; s < step1; s += kAhead) {  // kAhead steps' loads in flight together
+                uint4 v[kAhead], w[kAhead][kM];
 #pragma unroll
-                for (int i = 0; i < kSome; ++i) {
-                    v[i] = load(x + (s + i) * kStep);
+                for (int i = 0; i < kAhead; ++i) {
+                    const int depth = (s + i) * kStep;
+                    const bool in = s + i < step1 && depth + quad * 8 < g.cols;
+                    v[i] = zero_unless(in, *reinterpret_cast<const uint4*>(x + (in ? depth : 0)));
 #pragma unroll
-                    for (int m = 0; m < kM; ++m) w[i][m] = load(left[m] + (s + i) * kStep);
+                    for (int m = 0; m < kM; ++m)
+                        w[i][m] = zero_unless(in, *reinterpret_cast<const uint4*>(row[m] + (in ? depth : 0)));
                 }
 #pragma unroll
-                for (int i = 0; i < kSome; ++i)
+                for (int i = 0; i < kAhead; ++i)
 #pragma unroll
                     for (int m = 0; m < kM; ++m) acc[m] = Matrix<T>::mac(w[i][m], v[i], acc[m]);
-            };
-            const int full1 = min(step1, g.cols / kStep);
-            auto plain = [](const uint16_t* p) { return *reinterpret_cast<const uint4*>(p); };
-            constexpr int kAhead = 4;
-            int s = step0;
-            for (; s + kAhead <= full1; s += kAhead) steps_at(std::integral_constant<int, kAhead>(), plain, s);
-            if (s + 2 <= full1) {
-                steps_at(std::integral_constant<int, 2>(), plain, s);
-                s += 2;
-            }
-            if (s < full1) steps_at(std::integral_constant<int, 1>(), plain, s);
-            if (full1 < step1) {  // columns that end inside a step
-                const bool in = full1 * kStep + quad * 8 < g.cols;
-                steps_at(std::integral_constant<int, 1>(), [in](const uint16_t* p) { return load8(p, in); }, full1);
             }
         };
-        if (few || wave * kTile < many) {
-            if (ranks > 2 * kTile)
-                inner(std::integral_constant<int, 4>());
-            else if (ranks > kTile)
-                inner(std::integral_constant<int, 2>());
-            else if (ranks > 0)
-                inner(std::integral_constant<int, 1>());
-        }
-        auto store = [&](int n, int j, Acc v) {  // 4 ranks of the n-th token
-            const long t = q.token(window, n);
-            if (n >= many || j0 + j >= all) return;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (!(live >> (j + e) & 1)) v[e] = 0.0f;
-            *reinterpret_cast<Acc*>(g.h + (static_cast<long>(split) * g.tokens + t) * all + j0 + j) = v;
-        };
-        if (!few) {
-#pragma unroll
-            for (int m = 0; m < 4; ++m) store(slot, m * kTile + quad * 4, acc[m]);
-            return;
-        }
+        if (ranks > kTile)
+            inner(std::integral_constant<int, 4>());
+        else if (ranks > 0)
+            inner(std::integral_constant<int, 1>());
+        __syncthreads();  // the last group's sums are read
 #pragma unroll
         for (int m = 0; m < 4; ++m) *reinterpret_cast<Acc*>(&part[wave][col][m * kTile + quad * 4]) = acc[m];
         __syncthreads();
-        Acc sum = *reinterpret_cast<const Acc*>(&part[0][tid / 16][tid % 16 * 4]);
+        const int n = tid / 16, j = tid % 16 * 4;  // 4 ranks of a token
+        Acc sum = {};
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) sum += *reinterpret_cast<const Acc*>(&part[w][tid / 16][tid % 16 * 4]);
-        store(tid / 16, tid % 16 * 4, sum);
-        __syncthreads();
+        for (int w = 0; w < kWaves; ++w) sum += *reinterpret_cast<const Acc*>(&part[w][n][j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = live >> (j + e) & 1 ? sum[e] : 0.0f;
+        const long t = q.token(window, first + n);
+        if (first + n < q.many && j0 + j < all)
+            *reinterpret_cast<Acc*>(g.h + (static_cast<long>(split) * g.tokens + t) * all + j0 + j) = sum;
     });
 }
 
 // 256 rows of an adapter's tokens of a window, 64 rows a wave.  Left rows are dealt to the
 // products so that a lane's results of two are 8 neighbours, and with its three neighbours'
-// 64 bytes of a token's output.
-template <class T>
+// 64 bytes of a token's output.  The adapter's part of B stays in registers, up to 64 ranks;
+// more go in passes for every 16 tokens.
+template <class T, bool kPasses>
 __global__ __launch_bounds__(kWaves* kWave) void expand_kernel(Args g) {
-    __shared__ uint16_t hi[kWindow][kPadHalf], lo[kWindow][kPadHalf];
-    __shared__ int shifts[kWindow];
+    constexpr int kHeld = kPasses ? 32 : kWindow;  // tokens in LDS
+    constexpr int kWidth = kPasses ? kMaxRank + 8 : kPart + 8;
+    __shared__ uint16_t hi[kHeld][kWidth], lo[kHeld][kWidth];
+    __shared__ int shifts[kHeld];
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const int col = lane % kTile, quad = lane / kTile, all = g.sections * g.rank;
     int sec = 0, tile = blockIdx.x, row0 = 0;
@@ -438,128 +420,131 @@ __global__ __launch_bounds__(kWaves* kWave) void expand_kernel(Args g) {
     const int end = g.end[sec], window = blockIdx.z;
     row0 += tile * kRows;
     const int mine = row0 + wave * 64 + quad * 8;  // a lane's rows: 8 from here on, and 8 from 32 on
+    const bool whole = g.wide && mine + 40 <= end;
     const uint64_t idle = each_adapter(g, window, blockIdx.y, gridDim.y, [&](const Group& q) {
-        const int a = q.adapter, r = rank_of(g, a), many = q.many, tiles = (many + kTile - 1) / kTile;
-        const bool whole = g.wide && mine + 40 <= end;
-        long t[4];
-        uint4 old[4][2];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            const int slot = n * kTile + col;
-            t[n] = q.token(window, slot);
-            if (slot >= many) t[n] = -1;
-            if (t[n] >= 0 && whole) {
-                old[n][0] = *reinterpret_cast<const uint4*>(g.base + t[n] * g.bs + mine);
-                old[n][1] = *reinterpret_cast<const uint4*>(g.base + t[n] * g.bs + mine + 32);
-            }
-        }
-        // inner products: token tid / 4, 16 of 64 ranks
-        const int slot = tid / 4, k0 = tid % 4 * 16;
-        const bool has = slot < many;
-        const float* from = g.h + q.token(window, slot) * all + sec * g.rank;
-        auto inner = [&](int k, float (&h)[8]) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[e] = 0.0f;
-            if (!has || k >= r) return;  // ranks are stored by 8, zeros behind the adapter's
-            for (int s = 0; s < 1 << g.split_bits; ++s) {
-                const float* p = from + static_cast<long>(s) * g.tokens * all + k;
-                const Acc u = *reinterpret_cast<const Acc*>(p), v = *reinterpret_cast<const Acc*>(p + 4);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    h[e] += u[e];
-                    h[4 + e] += v[e];
-                }
-            }
-        };
-        float h[2][8];
-        int shift = 0;
-        if (std::is_same_v<T, F16>) {
-            float most = 0.0f;
-            for (int k = k0; k < r; k += kPart) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    inner(k + 8 * i, h[i]);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) most = __builtin_fmaxf(most, __builtin_fabsf(h[i][e]));
-                }
-            }
-            most = __builtin_fmaxf(most, __shfl_xor(most, 1, kWave));
-            most = __builtin_fmaxf(most, __shfl_xor(most, 2, kWave));
-            shift = shift_of<T>(most);
-        }
-        Acc acc[4][4] = {};
-        for (int first = 0; first < r; first += kPart) {
-            uint4 up[2][4];
+        const int r = rank_of(g, q.adapter);
+        const float scale = g.scales[q.adapter];
+        uint4 up[2][4];
+        auto load_up = [&](int first) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int depth = first + k * kStep + quad * 8;
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
                     const int row = row0 + wave * 64 + m / 2 * 32 + col / 4 * 8 + m % 2 * 4 + col % 4;
-                    up[k][m] = load8(g.b + a * g.b_adapter + row * g.b_row + depth,
-                                     row < end && depth < r);
-                    up[k][m] = first_of(up[k][m], r - depth);
+                    const bool in = row < end && depth < r;
+                    up[k][m] = *reinterpret_cast<const uint4*>(g.b + q.adapter * g.b_adapter +
+                                                               (in ? row * g.b_row + depth : row0 * g.b_row));
+                    up[k][m] = first_of(up[k][m], in ? r - depth : 0);
                 }
             }
-            __syncthreads();  // the last pass's numbers are read
+        };
+        if (!kPasses) load_up(0);
+        for (int held = 0; held < q.many; held += kHeld) {
+            uint4 old[2];
+            auto load_old = [&](int slot) {
+                const long t = q.token(window, slot < q.many ? slot : held);
+                if (!whole) return;
+                old[0] = *reinterpret_cast<const uint4*>(g.base + t * g.bs + mine);
+                old[1] = *reinterpret_cast<const uint4*>(g.base + t * g.bs + mine + 32);
+            };
+            load_old(held + col);
+            // inner products, 8 threads a token in passes and 4 else, 16 ranks at a time
+            constexpr int kThreads = kWaves * kWave / kHeld;
+            const int slot = tid / kThreads;
+            const bool has = held + slot < q.many;
+            const float* from = g.h + q.token(window, has ? held + slot : held) * all + sec * g.rank;
+            constexpr int kTurns = (kPasses ? kMaxRank : kPart) / (kThreads * 8);
+            float h[kTurns][8], most = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int k = k0 + 8 * i;
-                inner(first + k, h[i]);
+            for (int i = 0; i < kTurns; ++i) {
+                const int k = (i * kThreads + tid % kThreads) * 8;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[i][e] = 0.0f;
+                if (!has || k >= r) continue;  // ranks are stored by 8, zeros behind the adapter's
+                for (int s = 0; s < 1 << g.split_bits; ++s) {
+                    const float* p = from + static_cast<long>(s) * g.tokens * all + k;
+                    const Acc u = *reinterpret_cast<const Acc*>(p), v = *reinterpret_cast<const Acc*>(p + 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        h[i][e] += u[e];
+                        h[i][4 + e] += v[e];
+                    }
+                }
+                if (std::is_same_v<T, F16>)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) most = __builtin_fmaxf(most, __builtin_fabsf(h[i][e]));
+            }
+            int shift = 0;
+            if (std::is_same_v<T, F16>) {
+#pragma unroll
+                for (int d = 1; d < kThreads; d *= 2) most = __builtin_fmaxf(most, __shfl_xor(most, d, kWave));
+                shift = shift_of<T>(most);
+            }
+            __syncthreads();  // the last tokens' numbers are read
+#pragma unroll
+            for (int i = 0; i < kTurns; ++i) {
+                const int k = (i * kThreads + tid % kThreads) * 8;
+                if (k >= (r + kStep - 1) / kStep * kStep) continue;
                 Pair<T> p;
                 p.set(h[i], __builtin_ldexpf(1.0f, shift));
                 *reinterpret_cast<uint4*>(&hi[slot][k]) = p.hi;
                 *reinterpret_cast<uint4*>(&lo[slot][k]) = p.lo;
             }
-            if (k0 == 0) shifts[slot] = shift;
+            if (tid % kThreads == 0) shifts[slot] = shift;
             __syncthreads();
+            const int count = min(q.many - held, kHeld);
+#pragma unroll 1
+            for (int n = 0; n < count; n += kTile) {
+                Acc acc[4] = {};
+                for (int first = 0; first < r; first += kPart) {
+                    if (kPasses) load_up(first);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                if (first + k * kStep >= r) break;
+                    for (int k = 0; k < 2; ++k) {
+                        if (first + k * kStep >= r) break;
+                        const int depth = first + k * kStep + quad * 8;
+                        const uint4 u = *reinterpret_cast<const uint4*>(&hi[n + col][depth]);
+                        const uint4 v = *reinterpret_cast<const uint4*>(&lo[n + col][depth]);
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    if (n >= tiles) break;
-                    const uint4 u = *reinterpret_cast<const uint4*>(&hi[n * kTile + col][k * kStep + quad * 8]);
-                    const uint4 v = *reinterpret_cast<const uint4*>(&lo[n * kTile + col][k * kStep + quad * 8]);
+                        for (int m = 0; m < 4; ++m) {
+                            acc[m] = Matrix<T>::mac(up[k][m], u, acc[m]);
+                            acc[m] = Matrix<T>::mac(up[k][m], v, acc[m]);
+                        }
+                    }
+                    if (!kPasses) break;
+                }
+                const uint4 was[2] = {old[0], old[1]};
+                const long t = q.token(window, n + col < count ? held + n + col : held);
+                load_old(held + n + kTile + col);
+                if (n + col >= count) continue;
+                const int back = -shifts[n + col];
+                auto add = [&](uint32_t half, int i) {
+                    float v = scale * acc[i / 4][i % 4];
+                    if (std::is_same_v<T, F16>) v = __builtin_ldexpf(v, back);
+                    return T::from_float(T::to_float(static_cast<uint16_t>(half)) + v);
+                };
+                uint16_t* out = g.out + t * g.os + mine;
+                if (whole) {
 #pragma unroll
-                    for (int m = 0; m < 4; ++m) {
-                        acc[m][n] = Matrix<T>::mac(up[k][m], u, acc[m][n]);
-                        acc[m][n] = Matrix<T>::mac(up[k][m], v, acc[m][n]);
+                    for (int h2 = 0; h2 < 2; ++h2) {
+                        uint32_t w[4] = {was[h2].x, was[h2].y, was[h2].z, was[h2].w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint16_t low = add(w[e], h2 * 8 + 2 * e);
+                            w[e] = static_cast<uint32_t>(add(w[e] >> 16, h2 * 8 + 2 * e + 1)) << 16 | low;
+                        }
+                        *reinterpret_cast<uint4*>(out + h2 * 32) = uint4{w[0], w[1], w[2], w[3]};
+                    }
+                } else {
+                    const uint16_t* base = g.base + t * g.bs + mine;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int at = i / 8 * 32 + i % 8;
+                        if (mine + at < end) out[at] = add(base[at], i);
                     }
                 }
             }
         }
-        const float scale = g.scales[a];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            if (t[n] < 0) continue;
-            const int back = r > 0 ? -shifts[n * kTile + col] : 0;
-            auto add = [&](uint16_t was, int i) {
-                return T::from_float(T::to_float(was) + __builtin_ldexpf(scale * acc[i / 4][n][i % 4], back));
-            };
-            const uint16_t* base = g.base + t[n] * g.bs + mine;
-            uint16_t* out = g.out + t[n] * g.os + mine;
-            if (whole) {
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    uint32_t w[4] = {old[n][q].x, old[n][q].y, old[n][q].z, old[n][q].w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint16_t l = add(static_cast<uint16_t>(w[e]), q * 8 + 2 * e);
-                        const uint16_t h2 = add(static_cast<uint16_t>(w[e] >> 16), q * 8 + 2 * e + 1);
-                        w[e] = static_cast<uint32_t>(h2) << 16 | l;
-                    }
-                    *reinterpret_cast<uint4*>(out + q * 32) = uint4{w[0], w[1], w[2], w[3]};
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int at = i / 8 * 32 + i % 8;
-                    if (mine + at < end) out[at] = add(base[at], i);
-                }
-            }
-        }
-        __syncthreads();  // shifts are read
     });
     if (blockIdx.y == 0) copy_idle(g, window, idle, row0, min(row0 + kRows, end), wave, kWaves);
 }
@@ -682,11 +667,14 @@ int run(const char* fn, const spb_adapters* d, const int* ids, const uint16_t* x
     auto ways = [&](int blocks) { return blocks >= 4096 ? 1 : 4096 / blocks < most ? 4096 / blocks : most; };
     g.split_bits = split_bits_of(tokens);
     const int parts = (g.sections * g.rank + kPart - 1) / kPart;
-    const int blocks = parts << g.split_bits;
+    const int blocks = parts * (kWindow / kTile) << g.split_bits;
     hipLaunchKernelGGL(shrink_kernel<T>, dim3(windows, ways(windows * blocks), blocks),
                        dim3(kWaves * kWave), 0, st, g);
-    hipLaunchKernelGGL(expand_kernel<T>, dim3(tiles(kRows), ways(windows * tiles(kRows)), windows),
-                       dim3(kWaves * kWave), 0, st, g);
+    const dim3 grid(tiles(kRows), ways(windows * tiles(kRows)), windows);
+    if (g.rank <= kPart)
+        hipLaunchKernelGGL((expand_kernel<T, false>), grid, dim3(kWaves * kWave), 0, st, g);
+    else
+        hipLaunchKernelGGL((expand_kernel<T, true>), grid, dim3(kWaves * kWave), 0, st, g);
     return launch_status(fn);
 }
 
