@@ -596,9 +596,12 @@ size_t workspace_size(const spb_adapters& d, int tokens) {
     return sizeof(float) * d.num_sections * d.rank * rows;
 }
 
-// One launch for up to a window's tokens and few weights; its blocks read A once each.
-bool fused(const Args& g, int tokens) {
-    return tokens <= kWindow && g.rank <= kFusedRank && g.rank * static_cast<long>(g.cols) <= 64 * 1024;
+// One launch where every CU has a block at most, and A is small: each block reads its section's
+// A.  Rank 16 on q|k|v of 2560 columns: 8 tokens of 8 adapters 7.7 us in one launch (240
+// blocks), 11.3 in two; 32 tokens of 16 (480) 15.9 and 11.5.  One token, rank 32 on 2560
+// columns 9.6 and 11.0, rank 16 on 6912 11.9 and 10.4.
+bool fused(const Args& g, int blocks) {
+    return blocks <= device_cu_count() && g.rank <= kFusedRank && g.rank * g.cols <= 96 * 1024;
 }
 
 template <class T>
@@ -658,7 +661,7 @@ int run(const char* fn, const spb_adapters* d, const int* ids, const uint16_t* x
         for (int s = 0; s < d->num_sections; ++s) n += (d->section_rows[s] + size - 1) / size;
         return n;
     };
-    if (fused(g, tokens)) {
+    if (fused(g, tiles(kFusedRows) * most * windows)) {
         hipLaunchKernelGGL(fused_kernel<T>, dim3(tiles(kFusedRows), most, windows),
                            dim3(kFusedWaves * kWave), 0, st, g);
         return launch_status(fn);

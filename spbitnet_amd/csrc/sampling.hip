@@ -250,33 +250,37 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs& g, int row) {
     return s;
 }
 
-// exp(d) for d in (-64, 0]: 2^n times the exponential of the rest, at most ln(2) / 2, by its
-// series up to the 11th power: off by at most 7e-15 of itself (the 12th: 0.347^12 / 12!).
-// 18 instructions and no table: float64 runs at float32's rate here, and LDS is what the
-// histogram waits for.
-__device__ __forceinline__ double exp_of(double d) {
-    const double n = __builtin_rint(d * 0x1.71547652b82fep+0);      // 1 / ln 2
-    const double r = __builtin_fma(n, -0x1.62e42fefa39efp-1, d);    // ln 2
-    double p = __builtin_fma(r, 1.0 / 39916800, 1.0 / 3628800);
-    p = __builtin_fma(r, p, 1.0 / 362880);
-    p = __builtin_fma(r, p, 1.0 / 40320);
-    p = __builtin_fma(r, p, 1.0 / 5040);
-    p = __builtin_fma(r, p, 1.0 / 720);
-    p = __builtin_fma(r, p, 1.0 / 120);
-    p = __builtin_fma(r, p, 1.0 / 24);
-    p = __builtin_fma(r, p, 1.0 / 6);
-    p = __builtin_fma(r, p, 0.5);
-    p = __builtin_fma(r, p, 1.0);
-    p = __builtin_fma(r, p, 1.0);
-    return __builtin_ldexp(p, static_cast<int>(n));
+// exp(d) for d in [-64, 0]: d in 1/64 octaves is a whole number k and a rest; 2^(k / 64) from a
+// table of 64 in LDS and the exponent, the rest's exponential by its series, of which float64
+// needs to hold the first term only: the others are below 2^-15 and in float32 off by 2^-39
+// of the result.  A float64 instruction takes twice a float32 one's time (8 cycles a wave, as
+// measured): 12 of them here, where a series for a whole octave takes 20.
+__device__ __forceinline__ void fill_powers(double* powers) {
+    if (threadIdx.x < 64) powers[threadIdx.x] = exp2(threadIdx.x / 64.0);
+}
+__device__ __forceinline__ double exp_of(double d, const double* powers) {
+    constexpr double kStep = 0x1.62e42fefa39efp-7;  // ln 2 / 64
+    const double y = d * 0x1.71547652b82fep+6;      // 64 / ln 2
+    const double z = y + 0x1.8p52;                  // its low word is y rounded
+    const int k = static_cast<int>(__builtin_bit_cast(uint64_t, z));
+    const double r = y - (z - 0x1.8p52);
+    const float f = static_cast<float>(r);
+    constexpr float c2 = kStep * kStep / 2, c3 = kStep * kStep * kStep / 6,
+                    c4 = kStep * kStep * kStep * kStep / 24;
+    const float rest = f * f * __builtin_fmaf(f, __builtin_fmaf(f, c4, c3), c2);
+    const double p = __builtin_fma(r, kStep, static_cast<double>(rest));
+    const double t = powers[k & 63];
+    const auto w = __builtin_bit_cast(uint64_t, __builtin_fma(t, p, t));
+    const uint32_t hi = static_cast<uint32_t>(w >> 32) + (static_cast<uint32_t>(k >> 6) << 20);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | static_cast<uint32_t>(w));
 }
 
 // Weight of a logit (not minus infinity) at or below `top`.
-__device__ __forceinline__ double weight_of(float l, float top, double inv_t) {
+__device__ __forceinline__ double weight_of(float l, float top, double inv_t, const double* powers) {
     const double d = (static_cast<double>(l) - static_cast<double>(top)) * inv_t;
     if (l == top) return 1.0;
     // 2^24 weights below e^-64 are nothing beside the first, 1
-    return d > -64.0 ? exp_of(d) : 0.0;
+    return d > -64.0 ? exp_of(d, powers) : 0.0;
 }
 
 // A weight as a whole number of 1 / unit, one = 2^52 / unit: the sum's low bits (those of a
@@ -302,11 +306,12 @@ struct Hist {
 template <class T>
 struct Row {
     const typename T::Bits* l;
+    const double* powers;
     int vocab;
     float top;
     double inv_t, one, unit;
 
-    __device__ __forceinline__ double weight(float v) const { return weight_of(v, top, inv_t); }
+    __device__ __forceinline__ double weight(float v) const { return weight_of(v, top, inv_t, powers); }
 };
 
 // A place in the order: the logit there, how many of that logit stand before it, and the
@@ -401,13 +406,15 @@ __device__ Place select(const Row<T>& r, int rank, double bound, Hist& h) {
 }
 
 template <class T>
-__device__ void sample_row(const SampleArgs& g, int row, const Settings& s, float top, Hist& h) {
+__device__ void sample_row(const SampleArgs& g, int row, const Settings& s, float top, const double* powers,
+                           Hist& h) {
     __shared__ union {
         int i[kWaves];
         unsigned long long u[kWaves];
     } part;
     Row<T> r;
     r.l = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
+    r.powers = powers;
     r.vocab = g.vocab;
     r.inv_t = s.inv_t;
     r.top = top;
@@ -502,7 +509,7 @@ struct Unit {
                 bits[n] = *reinterpret_cast<const uint4*>(row + i);
         }
     }
-    // f(logit, index, number of it) of each loaded logit; minus infinity outside the row.
+    // f(logit as it is, index, number of it) of each loaded one; minus infinity outside the row.
     template <class F>
     __device__ __forceinline__ void each(const typename T::Bits* row, int vocab, int unit, F f) const {
         const int first = start(row, unit);
@@ -518,7 +525,7 @@ struct Unit {
                     v[e] = i + e >= 0 && i + e < vocab ? T::load(row + i + e) : -__builtin_inff();
             }
 #pragma unroll
-            for (int e = 0; e < T::kVec; ++e) f(clean(v[e]), i + e, n * T::kVec + e);
+            for (int e = 0; e < T::kVec; ++e) f(v[e], i + e, n * T::kVec + e);
         }
     }
 };
@@ -561,18 +568,24 @@ __device__ __forceinline__ float unit_peak(const Unit<T>& x, const typename T::B
     return from_lane(wave_scan(peak, -__builtin_inff(), Max()), kWave - 1);
 }
 
-// Adds a unit to a histogram in LDS.
-template <class T>
+// Adds a unit to a histogram in LDS; `cut`: below it (and for a NaN) a weight is 0 as a whole
+// number.
+template <class T, bool kCount>
 __device__ __forceinline__ void add_unit(const Unit<T>& x, const typename T::Bits* row, int vocab, int u,
-                                         const Settings& s, float top, unsigned long long* mass, int* count) {
+                                         const Settings& s, float top, float cut, const double* powers,
+                                         unsigned long long* mass, int* count) {
     x.each(row, vocab, u, [&](float l, int, int) {
-        const int b = bin_of(l, top, s.bins);
-        // below e^-64 it is 0 as a whole number; so is minus infinity's
         const double d = (static_cast<double>(l) - static_cast<double>(top)) * s.inv_t;
-        const unsigned long long m = fixed(exp_of(__builtin_fmax(d, -64.0)), s.one);
-        if (m) atomicAdd(&mass[b], m);
-        if (count && l != -__builtin_inff()) atomicAdd(&count[b], 1);
+        const unsigned long long m = fixed(exp_of(d, powers), s.one);
+        const int b = bin_of(l, top, s.bins);
+        if (l >= cut) atomicAdd(&mass[b], m);
+        if (kCount && l > -__builtin_inff()) atomicAdd(&count[b], 1);
     });
+}
+
+// The least logit whose weight is not below e^-64, and no infinite one.
+__device__ __forceinline__ float cut_of(float top, double inv_t) {
+    return __builtin_fmaxf(static_cast<float>(top - 64.0 / inv_t), -0x1.fffffep127f);
 }
 
 // Few rows: units over blocks.  First their largest logits ...
@@ -612,12 +625,14 @@ template <class T>
 __global__ __launch_bounds__(kSplitBlock) void sample_bins_kernel(SampleArgs g, SampleWork w) {
     __shared__ unsigned long long mass[kBins];
     __shared__ int count[kBins];
+    __shared__ double powers[64];
     __shared__ float part[kSplitBlock / kWave];
     constexpr int kTogether = kSplitBlock / kWave;
     const int r = blockIdx.y, row = w.first + r, tid = threadIdx.x;
     const typename T::Bits* logits = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
     const Settings s = settings_of(g, row);
     const bool by_count = s.k < g.vocab;
+    fill_powers(powers);
     for (int b = tid; b < kBins; b += kSplitBlock) {
         mass[b] = 0;
         if (by_count) count[b] = 0;
@@ -625,9 +640,13 @@ __global__ __launch_bounds__(kSplitBlock) void sample_bins_kernel(SampleArgs g, 
     const float top = row_peak(w.peaks + static_cast<long>(r) * w.units, w.units, kSplitBlock, part,
                                kSplitBlock / kWave);
     if (__builtin_isinf(top)) return;
+    const float cut = cut_of(top, s.inv_t);
     each_unit<T>(logits, g.vocab, blockIdx.x * kTogether + tid / kWave, gridDim.x * kTogether, w.units,
                  [](int) { return true; }, [&](const Unit<T>& x, int u) {
-                     add_unit<T>(x, logits, g.vocab, u, s, top, mass, by_count ? count : nullptr);
+                     if (by_count)
+                         add_unit<T, true>(x, logits, g.vocab, u, s, top, cut, powers, mass, count);
+                     else
+                         add_unit<T, false>(x, logits, g.vocab, u, s, top, cut, powers, mass, count);
                  });
     __syncthreads();
     for (int b = tid; b < kBins; b += kSplitBlock) {
@@ -711,6 +730,7 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
         Hist hist;
     } u;
     __shared__ float own_peaks[kWhole ? kPeaks : 1];
+    __shared__ double powers[64];
     __shared__ union {
         float f[kWaves];
         int i[kWaves];
@@ -725,7 +745,8 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
     __shared__ double gap_mass[2][kSplitBins + 1];  // between marked bins: from, to
     __shared__ int gap_count[2][kSplitBins + 1];
     __shared__ int listed, found[5], heaviest_bin, base;
-    __shared__ double cut;
+    __shared__ double cut_mass;
+    __shared__ float spans[4][2];
     const int r = kWhole ? blockIdx.x : blockIdx.y, q = kWhole ? 0 : blockIdx.x;
     const int row = w.first + r, tid = threadIdx.x;
     const int lane = tid % kWave, wave = tid / kWave, own = tid * kOwn;
@@ -733,6 +754,7 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
     const float* peaks = kWhole ? own_peaks : w.peaks + static_cast<long>(r) * w.units;
     const Settings s = settings_of(g, row);
     const bool by_count = s.k < g.vocab;
+    fill_powers(powers);
     if (tid < 5) found[tid] = kBins;
     if (tid == 5) listed = 0;
     if (tid == 6) heaviest_bin = 0;
@@ -756,7 +778,7 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
         return;
     }
     if (top == __builtin_inff()) {  // bins below an infinite logit have no width
-        if (q == 0) sample_row<T>(g, row, s, top, u.hist);
+        if (q == 0) sample_row<T>(g, row, s, top, powers, u.hist);
         return;
     }
     // kOwn neighbouring bins a thread
@@ -768,8 +790,12 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
             if (by_count) count[b] = 0;
         }
         __syncthreads();
+        const float cut = cut_of(top, s.inv_t);
         each_unit<T>(logits, g.vocab, wave, kWaves, w.units, all_units, [&](const Unit<T>& x, int u) {
-            add_unit<T>(x, logits, g.vocab, u, s, top, masses.fixed, by_count ? count : nullptr);
+            if (by_count)
+                add_unit<T, true>(x, logits, g.vocab, u, s, top, cut, powers, masses.fixed, count);
+            else
+                add_unit<T, false>(x, logits, g.vocab, u, s, top, cut, powers, masses.fixed, count);
         });
         __syncthreads();
     }
@@ -823,7 +849,8 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
     // The bins in question.  The bounds of a sum that a bin leaves open give a first and a
     // last bin, a little widened: sums over bins and over tokens round differently.
     double end[kOwn], k_mass;
-    int k_bin, p_bin, from, to;
+    int k_bin, p_bin, marks, to;  // marks: spans of bins in question; to: the last one
+    constexpr float kLowest = -0x1.fffffep127f;
     uint32_t my_marks;  // word tid of the marks
     auto decide = [&]() {
         const double less = 1.0 - 0x1p-36, more = 1.0 + 0x1p-36;
@@ -864,14 +891,19 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
                 low = mass[k_bin];
         }
         k_mass = upper;  // of top-k, where no bin is in question
-        from = kBins;
+        marks = 0;
         to = -1;
         my_marks = 0;
         auto mark = [&](int a, int b) {
             a = max(a, 0);
             b = min(b, heaviest);
             if (a > b) return;
-            from = min(from, a);
+            // as bounds of the logits, a little widened; minus infinity is in none
+            if (tid == 0) {
+                spans[marks][0] = top - a / s.bins * 0.9999f;
+                spans[marks][1] = b < kBins - 1 ? __builtin_fmaxf(top - (b + 1) / s.bins * 1.0001f, kLowest) : kLowest;
+            }
+            ++marks;
             to = max(to, b);
             if (tid >= a / 32 && tid <= b / 32) {
                 uint32_t bits = ~0u;
@@ -911,36 +943,36 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
     if (tid < kBins / 32) marked[tid] = my_marks;
     __syncthreads();
     // their tokens: by bounds of the logits, then by their bins
-    const float above = top - from / s.bins * 0.9999f;
-    const float below = to < kBins - 1 ? top - (to + 1) / s.bins * 1.0001f : -__builtin_inff();
     each_unit<T>(
         logits, g.vocab, q * kWaves + wave, w.parts * kWaves, w.units,
         [&](int u) { return (kWhole && u >= kPeaks) || bin_of(peaks[u], top, s.bins) <= to; },
         [&](const Unit<T>& x, int unit) {
             uint32_t near = 0;
-            x.each(logits, g.vocab, unit, [&](float l, int, int e) {
-                near |= static_cast<uint32_t>(l >= below && l <= above && l != -__builtin_inff()) << e;
-            });
-            if (!__any(near != 0)) return;
-            uint32_t hits = 0;
-            x.each(logits, g.vocab, unit, [&](float l, int, int e) {
-                const int b = max(bin_of(l, top, s.bins), 0);
-                hits |= (marked[b / 32] >> (b % 32) & near >> e & 1) << e;
-            });
-            // one addition for the wave, then each lane writes its own
-            const int own_hits = __popc(hits), upto = wave_scan(own_hits, 0, Add());
-            const int all = from_lane(upto, kWave - 1);
-            if (all == 0) return;
-            int at = 0;
-            if (lane == 0) at = atomicAdd(&listed, all);
-            at = from_lane(at, 0) + upto - own_hits;
-            x.each(logits, g.vocab, unit, [&](float l, int i, int e) {
-                if (!(hits >> e & 1)) return;
-                if (at < kList)
-                    u.list[at] = static_cast<unsigned long long>(~key_of(l)) << 32 |
-                                 static_cast<uint32_t>(i);
-                ++at;
-            });
+            for (int m = 0; m < marks; ++m) {
+                const float above = spans[m][0], below = spans[m][1];
+                x.each(logits, g.vocab, unit, [&](float l, int, int e) {
+                    near |= static_cast<uint32_t>(l >= below && l <= above) << e;
+                });
+            }
+            const int start = Unit<T>::start(logits, unit);
+            while (__any(near != 0)) {  // a logit of each lane that has one, read again
+                const int e = __ffs(near) - 1, i = start + e / T::kVec * (kWave * T::kVec) + e % T::kVec;
+                float l = 0.0f;
+                bool hit = near != 0;
+                if (hit) {
+                    l = clean(T::load(logits + i));
+                    const int b = bin_of(l, top, s.bins);
+                    hit = marked[b / 32] >> (b % 32) & 1;
+                }
+                near &= near - 1;
+                const unsigned long long hits = __ballot(hit);
+                if (hits == 0) continue;
+                int at = 0;
+                if (lane == 0) at = atomicAdd(&listed, static_cast<int>(__popcll(hits)));
+                at = from_lane(at, 0) + __popcll(hits & ((1ull << lane) - 1));
+                if (hit && at < kList)
+                    u.list[at] = static_cast<unsigned long long>(~key_of(l)) << 32 | static_cast<uint32_t>(i);
+            }
         });
     __syncthreads();
     int n = __builtin_amdgcn_readfirstlane(listed);
@@ -970,7 +1002,7 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
         __syncthreads();
     }
     if (n > kList) {
-        sample_row<T>(g, row, s, top, u.hist);
+        sample_row<T>(g, row, s, top, powers, u.hist);
         return;
     }
     if (n > kRow) {
@@ -1020,7 +1052,7 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
                 keep[e] = u.list[i];
                 const float l = from_key(~static_cast<uint32_t>(keep[e] >> 32));
                 const int b = place_of((top - l) * s.bins);
-                atomicAdd(&masses.fixed[b], fixed(weight_of(l, top, s.inv_t), s.one));
+                atomicAdd(&masses.fixed[b], fixed(weight_of(l, top, s.inv_t, powers), s.one));
                 atomicAdd(&count[b], 1);
             }
             __syncthreads();
@@ -1062,7 +1094,7 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
     auto each_listed = [&](double before, auto f) {
         for (int i = first; i < behind; ++i) {
             const float l = from_key(~static_cast<uint32_t>(u.list[i] >> 32));
-            const double weight = weight_of(l, top, s.inv_t);
+            const double weight = weight_of(l, top, s.inv_t, powers);
             f(i, weight, place_of((top - l) * s.bins), before);
             before += weight;
         }
@@ -1075,13 +1107,13 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
         mass[b] -= before;  // weights before the bin, less those before it in the list
         count[b] -= i;
     });
-    if (tid == 0) cut = k_mass;
+    if (tid == 0) cut_mass = k_mass;
     __syncthreads();
     each_listed(sum, [&](int i, double, int b, double before) {
-        if (b == k_bin && count[b] + i == s.k) cut = before + mass[b];  // the first that top-k leaves out
+        if (b == k_bin && count[b] + i == s.k) cut_mass = before + mass[b];  // the first that top-k leaves out
     });
     __syncthreads();
-    double kept = cut;
+    double kept = cut_mass;
     const double bound = s.top_p < 1.0 ? s.top_p * kept : __builtin_inf();
     double least = kept;
 #pragma unroll
@@ -1109,16 +1141,18 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
     g.tokens[row] = static_cast<int>(static_cast<uint32_t>(token));
     if (g.logprobs)
         g.logprobs[row] = static_cast<float>(
-            log(weight_of(from_key(~static_cast<uint32_t>(token >> 32)), top, s.inv_t) / kept));
+            log(weight_of(from_key(~static_cast<uint32_t>(token >> 32)), top, s.inv_t, powers) / kept));
 }
 
 // Rows of one launch of the split kernels: their grids stay below 2^31 threads, and the
 // workspace is bounded.
 constexpr int kSplitRows = 128;
 
-// One block a row from 64 rows on, and where a row is a few units: one launch and no trip
-// through memory, where the split takes three.
-bool sample_whole(int rows, int units) { return rows >= 64 || units <= 16; }
+// One block a row where rows fill the GPU, or are a few units: one launch and no trip through
+// memory, where the split takes three.  Rows of 8000: 16.3 us for one and 17.4 for 128,
+// split 20.2 and 24.9; 32003: 28 and 34, split 20 and 39 (30 for 64); 128256: 72 and 92,
+// split 21 and 63 (256 rows 100 and 125).
+bool sample_whole(int rows, int units) { return units <= 16 || rows > (units > 64 ? 128 : 64); }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -1270,6 +1304,7 @@ __device__ __forceinline__ float sum_unit(Sum& s, const Unit<T>& x, const typena
     float w[16];
     int equal = 0;
     x.each(row, vocab, u, [&](float l, int, int e) {
+        l = clean(l);
         w[e] = __builtin_amdgcn_exp2f((l - s.top) * 0x1.715476p+0f);
         if (has) {
             w[e] = l == s.top ? 0.0f : w[e];
@@ -1397,6 +1432,7 @@ __global__ __launch_bounds__(kRow) void logprob_kernel(LogprobArgs g, LogprobWor
         each_chosen([&](const Unit<T>& x, int u, int) {
             uint32_t hits = 0;
             x.each(logits, g.vocab, u, [&](float l, int i, int e) {
+                l = clean(l);
                 const bool in = l >= least && i >= 0 && i < g.vocab && rank_key(l, i) <= last;
                 hits |= static_cast<uint32_t>(in) << e;
             });
@@ -1407,7 +1443,7 @@ __global__ __launch_bounds__(kRow) void logprob_kernel(LogprobArgs g, LogprobWor
             at = from_lane(at, 0) + upto - own;
             x.each(logits, g.vocab, u, [&](float l, int i, int e) {
                 if (!(hits >> e & 1)) return;
-                if (at < kCandidates) list[at] = rank_key(l, i);
+                if (at < kCandidates) list[at] = rank_key(clean(l), i);
                 ++at;
             });
         });
@@ -1425,7 +1461,7 @@ __global__ __launch_bounds__(kRow) void logprob_kernel(LogprobArgs g, LogprobWor
             unsigned long long best = ~0ull;
             x.each(logits, g.vocab, u, [&](float l, int i, int) {
                 if (i < 0 || i >= g.vocab) return;
-                const unsigned long long k = rank_key(l, i);
+                const unsigned long long k = rank_key(clean(l), i);
                 best = k < best ? k : best;
             });
             atomicMin(&list[c * kWave + lane], best);
@@ -1472,7 +1508,9 @@ size_t logprobs_workspace(int rows, int vocab) {
     return logprobs_layout(rows, units_of<Half<F16>>(vocab), nullptr, nullptr);
 }
 
-bool logprobs_whole(int rows, int units) { return rows >= 128 || units <= 16; }
+// The same for log-probabilities: 32003 14.2 us for 128 rows, split 13.0; 128256 35 and 23
+// (256 rows 37 and 47).
+bool logprobs_whole(int rows, int units) { return units <= 16 || rows > kSplitRows; }
 
 int check_top(const char* fn, int top) {
     if (top < 0 || top > kMaxTop) return invalid("%s: top %d must be in [0, %d]", fn, top, kMaxTop);
