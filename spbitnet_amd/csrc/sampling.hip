@@ -1144,15 +1144,14 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
             log(weight_of(from_key(~static_cast<uint32_t>(token >> 32)), top, s.inv_t, powers) / kept));
 }
 
-// Rows of one launch of the split kernels: their grids stay below 2^31 threads, and the
-// workspace is bounded.
-constexpr int kSplitRows = 128;
+// Rows of one launch of the split kernels: the workspace is bounded.
+constexpr int kSplitRows = 192;
 
 // One block a row where rows fill the GPU, or are a few units: one launch and no trip through
-// memory, where the split takes three.  Rows of 8000: 16.3 us for one and 17.4 for 128,
-// split 20.2 and 24.9; 32003: 28 and 34, split 20 and 39 (30 for 64); 128256: 72 and 92,
-// split 21 and 63 (256 rows 100 and 125).
-bool sample_whole(int rows, int units) { return units <= 16 || rows > (units > 64 ? 128 : 64); }
+// memory, where the split takes three.  top-k 50 and top-p 0.95, one block a row / split: rows
+// of 16500 23 / 24 us for 32, 24 / 28 for 64; 32003 31 / 26 for 32, 31 / 37 for 96; 64000
+// 49 / 46 for 128, 52 / 59 for 192; 128256 62 / 21 for 1, 82 / 66 for 128, 85 / 85 for 192.
+bool sample_whole(int rows, int units) { return units <= 16 || rows > 2 * units || rows > kSplitRows; }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -1243,7 +1242,7 @@ int sample(const char* fn, const void* logits, long stride, const float* uniform
         if (w.parts > 16) w.parts = 16;
         hipLaunchKernelGGL(sample_peaks_kernel<T>, dim3(blocks, w.rows), dim3(kSplitBlock), 0, st, g, w);
         // Each block adds its bins to the row's: fewer blocks a row, fewer additions in memory.
-        const int share = (1024 + w.rows - 1) / w.rows;
+        const int share = (512 + w.rows - 1) / w.rows;
         hipLaunchKernelGGL(sample_bins_kernel<T>, dim3(blocks < share ? blocks : share, w.rows),
                            dim3(kSplitBlock), 0, st, g, w);
         hipLaunchKernelGGL((sample_pick_kernel<T, false>), dim3(w.parts, w.rows), dim3(kRow), 0, st, g, w);
@@ -1508,8 +1507,8 @@ size_t logprobs_workspace(int rows, int vocab) {
     return logprobs_layout(rows, units_of<Half<F16>>(vocab), nullptr, nullptr);
 }
 
-// The same for log-probabilities: 32003 14.2 us for 128 rows, split 13.0; 128256 35 and 23
-// (256 rows 37 and 47).
+// The same for log-probabilities: 32003 14.0 / 12.3 us for 96 rows, 14.3 / 14.5 for 192; 128256
+// 30 / 14 for 1, 35 / 28 for 192.
 bool logprobs_whole(int rows, int units) { return units <= 16 || rows > kSplitRows; }
 
 int check_top(const char* fn, int top) {
