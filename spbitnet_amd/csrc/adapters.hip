@@ -145,13 +145,14 @@ __device__ __forceinline__ void copy_idle(const Args& g, int window, uint64_t id
     for (int i = 0; idle; ++i, idle &= idle - 1) {
         if (i % waves != wave) continue;
         const long t = window * kWindow + __builtin_ctzll(idle);
+        int rest = row;  // rows that do not go by 8
         if (g.wide) {
-            for (int r = row + lane * 8; r < end; r += kWave * 8)
+            rest = row + (end - row) / 8 * 8;
+            for (int r = row + lane * 8; r < rest; r += kWave * 8)
                 *reinterpret_cast<uint4*>(g.out + t * g.os + r) =
                     *reinterpret_cast<const uint4*>(g.base + t * g.bs + r);
-        } else {
-            for (int r = row + lane; r < end; r += kWave) g.out[t * g.os + r] = g.base[t * g.bs + r];
         }
+        for (int r = rest + lane; r < end; r += kWave) g.out[t * g.os + r] = g.base[t * g.bs + r];
     }
 }
 
@@ -349,8 +350,8 @@ __global__ __launch_bounds__(kWaves* kWave) void shrink_kernel(Args g) {
         const int ranks = live ? kWave - __builtin_clzll(live) : 0;
         const int steps = (g.cols + kStep - 1) / kStep, way = split * kWaves + wave;
         const int bits = g.split_bits + 2, step0 = steps * way >> bits, step1 = steps * (way + 1) >> bits;
-        const uint16_t* x = g.x + q.token(window, first + col < q.many ? first + col : first) * g.xs + quad * 8;
-        const uint16_t* a = g.a + q.adapter * g.a_adapter + j0 * g.a_row + quad * 8;
+        const uint16_t* x = g.x + q.token(window, first + col < q.many ? first + col : first) * g.xs;
+        const uint16_t* a = g.a + q.adapter * g.a_adapter + j0 * g.a_row;
         Acc acc[4] = {};
         auto inner = [&](auto tiles) {
             constexpr int kM = decltype(tiles)::value, kAhead = kM == 1 ? 4 : 2;
@@ -365,8 +366,8 @@ __global__ __launch_bounds__(kWaves* kWave) void shrink_kernel(Args g) {
                 uint4 v[kAhead], w[kAhead][kM];
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i) {
-                    const int depth = (s + i) * kStep;
-                    const bool in = s + i < step1 && depth + quad * 8 < g.cols;
+                    const int depth = (s + i) * kStep + quad * 8;
+                    const bool in = s + i < step1 && depth < g.cols;
                     v[i] = zero_unless(in, *reinterpret_cast<const uint4*>(x + (in ? depth : 0)));
 #pragma unroll
                     for (int m = 0; m < kM; ++m)
@@ -600,7 +601,7 @@ size_t workspace_size(const spb_adapters& d, int tokens) {
 // A.  Rank 16 on q|k|v of 2560 columns: 8 tokens of 8 adapters 7.7 us in one launch (240
 // blocks), 11.3 in two; 32 tokens of 16 (480) 15.9 and 11.5.  One token, rank 32 on 2560
 // columns 9.6 and 11.0, rank 16 on 6912 11.9 and 10.4.
-bool fused(const Args& g, int blocks) {
+bool fused(const Args& g, long blocks) {
     return blocks <= device_cu_count() && g.rank <= kFusedRank && g.rank * g.cols <= 96 * 1024;
 }
 
@@ -661,7 +662,7 @@ int run(const char* fn, const spb_adapters* d, const int* ids, const uint16_t* x
         for (int s = 0; s < d->num_sections; ++s) n += (d->section_rows[s] + size - 1) / size;
         return n;
     };
-    if (fused(g, tiles(kFusedRows) * most * windows)) {
+    if (fused(g, static_cast<long>(tiles(kFusedRows)) * most * windows)) {
         hipLaunchKernelGGL(fused_kernel<T>, dim3(tiles(kFusedRows), most, windows),
                            dim3(kFusedWaves * kWave), 0, st, g);
         return launch_status(fn);

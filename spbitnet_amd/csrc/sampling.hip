@@ -486,7 +486,7 @@ struct SampleWork {
     unsigned long long* list;  // [rows][kList]
     int* listed;               // [rows]: tokens in the list, and blocks that are done
     int* done;
-    int first, rows, units, parts;  // rows of this launch, blocks of a row in the last kernel
+    int units, parts;  // units of a row, blocks of a row in the last kernel
 };
 
 // A wave's part of a row: 16 logits a lane in loads of 16 bytes, from 16-byte boundaries
@@ -591,22 +591,22 @@ __device__ __forceinline__ float cut_of(float top, double inv_t) {
 // Few rows: units over blocks.  First their largest logits ...
 template <class T>
 __global__ __launch_bounds__(kSplitBlock) void sample_peaks_kernel(SampleArgs g, SampleWork w) {
-    const int r = blockIdx.y, row = w.first + r, tid = threadIdx.x;
+    const int row = blockIdx.y, tid = threadIdx.x;
     const int u = blockIdx.x * (kSplitBlock / kWave) + tid / kWave;
     const typename T::Bits* logits = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
     Unit<T> x;
     if (u < w.units) x.load(logits, g.vocab, u);
     for (int b = blockIdx.x * kSplitBlock + tid; b < kBins; b += gridDim.x * kSplitBlock) {
-        w.mass[static_cast<long>(r) * kBins + b] = 0;
-        w.count[static_cast<long>(r) * kBins + b] = 0;
+        w.mass[static_cast<long>(row) * kBins + b] = 0;
+        w.count[static_cast<long>(row) * kBins + b] = 0;
     }
     if (blockIdx.x == 0 && tid == 0) {
-        w.listed[r] = 0;
-        w.done[r] = 0;
+        w.listed[row] = 0;
+        w.done[row] = 0;
     }
     if (u >= w.units) return;
     const float peak = unit_peak<T>(x, logits, g.vocab, u);
-    if (tid % kWave == 0) w.peaks[static_cast<long>(r) * w.units + u] = peak;
+    if (tid % kWave == 0) w.peaks[static_cast<long>(row) * w.units + u] = peak;
 }
 
 __device__ __forceinline__ float row_peak(const float* peaks, int units, int block, float* part, int parts) {
@@ -628,7 +628,7 @@ __global__ __launch_bounds__(kSplitBlock) void sample_bins_kernel(SampleArgs g, 
     __shared__ double powers[64];
     __shared__ float part[kSplitBlock / kWave];
     constexpr int kTogether = kSplitBlock / kWave;
-    const int r = blockIdx.y, row = w.first + r, tid = threadIdx.x;
+    const int row = blockIdx.y, tid = threadIdx.x;
     const typename T::Bits* logits = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
     const Settings s = settings_of(g, row);
     const bool by_count = s.k < g.vocab;
@@ -637,7 +637,7 @@ __global__ __launch_bounds__(kSplitBlock) void sample_bins_kernel(SampleArgs g, 
         mass[b] = 0;
         if (by_count) count[b] = 0;
     }
-    const float top = row_peak(w.peaks + static_cast<long>(r) * w.units, w.units, kSplitBlock, part,
+    const float top = row_peak(w.peaks + static_cast<long>(row) * w.units, w.units, kSplitBlock, part,
                                kSplitBlock / kWave);
     if (__builtin_isinf(top)) return;
     const float cut = cut_of(top, s.inv_t);
@@ -651,10 +651,10 @@ __global__ __launch_bounds__(kSplitBlock) void sample_bins_kernel(SampleArgs g, 
     __syncthreads();
     for (int b = tid; b < kBins; b += kSplitBlock) {
         if (mass[b])
-            __hip_atomic_fetch_add(&w.mass[static_cast<long>(r) * kBins + b], mass[b], __ATOMIC_RELAXED,
+            __hip_atomic_fetch_add(&w.mass[static_cast<long>(row) * kBins + b], mass[b], __ATOMIC_RELAXED,
                                    __HIP_MEMORY_SCOPE_AGENT);
         if (by_count && count[b])
-            __hip_atomic_fetch_add(&w.count[static_cast<long>(r) * kBins + b], count[b], __ATOMIC_RELAXED,
+            __hip_atomic_fetch_add(&w.count[static_cast<long>(row) * kBins + b], count[b], __ATOMIC_RELAXED,
                                    __HIP_MEMORY_SCOPE_AGENT);
     }
 }
@@ -747,11 +747,11 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
     __shared__ int listed, found[5], heaviest_bin, base;
     __shared__ double cut_mass;
     __shared__ float spans[4][2];
-    const int r = kWhole ? blockIdx.x : blockIdx.y, q = kWhole ? 0 : blockIdx.x;
-    const int row = w.first + r, tid = threadIdx.x;
+    const int row = kWhole ? blockIdx.x : blockIdx.y, q = kWhole ? 0 : blockIdx.x;
+    const int tid = threadIdx.x;
     const int lane = tid % kWave, wave = tid / kWave, own = tid * kOwn;
     const typename T::Bits* logits = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
-    const float* peaks = kWhole ? own_peaks : w.peaks + static_cast<long>(r) * w.units;
+    const float* peaks = kWhole ? own_peaks : w.peaks + static_cast<long>(row) * w.units;
     const Settings s = settings_of(g, row);
     const bool by_count = s.k < g.vocab;
     fill_powers(powers);
@@ -801,7 +801,7 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
     }
 #pragma unroll
     for (int h = 0; h < kOwn; ++h) {
-        const long at = static_cast<long>(r) * kBins + own + h;
+        const long at = static_cast<long>(row) * kBins + own + h;
         mine[h] = static_cast<double>(kWhole ? masses.fixed[own + h] : w.mass[at]) / s.unit;
         if (by_count) mine_count[h] = kWhole ? count[own + h] : w.count[at];
     }
@@ -848,8 +848,8 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
     };
     // The bins in question.  The bounds of a sum that a bin leaves open give a first and a
     // last bin, a little widened: sums over bins and over tokens round differently.
-    double end[kOwn], k_mass;
-    int k_bin, p_bin, marks, to;  // marks: spans of bins in question; to: the last one
+    double end[kOwn], k_mass = 0.0;
+    int k_bin = 0, p_bin, marks, to;  // marks: spans of bins in question; to: the last one
     constexpr float kLowest = -0x1.fffffep127f;
     uint32_t my_marks;  // word tid of the marks
     auto decide = [&]() {
@@ -880,9 +880,11 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
         __syncthreads();
         // bins behind the last one with a weight need no order: whatever is kept of them
         const int heaviest = heaviest_bin;
-        k_bin = kBins;
         double low = total, upper = total;  // bounds of what top-k keeps
-        if (by_count && s.k < total_count && found[0] <= heaviest) {
+        if (parts_of_bin && k_bin == kBins) {
+            // where top-k ends with a bin that is not marked, the parts do not show it
+            low = upper = k_mass;
+        } else if (k_bin = kBins; by_count && s.k < total_count && found[0] <= heaviest) {
             k_bin = found[0];
             low = upper = mass[k_bin + 1];
             if (count[k_bin + 1] == s.k)
@@ -981,23 +983,23 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
         // (s_waitcnt) before it counts itself; a fence would write a whole L2 back: 90 us of
         // 150 at 32 rows of 128256.
         if (tid == 0)
-            base = __hip_atomic_fetch_add(&w.listed[r], n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            base = __hip_atomic_fetch_add(&w.listed[row], n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         const int to = base;
         for (int i = tid; i < min(n, kList); i += kRow)
             if (to + i < kList)
-                __hip_atomic_store(&w.list[static_cast<long>(r) * kList + to + i], u.list[i],
+                __hip_atomic_store(&w.list[static_cast<long>(row) * kList + to + i], u.list[i],
                                    __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
         if (tid == 0)
-            base = __hip_atomic_fetch_add(&w.done[r], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            base = __hip_atomic_fetch_add(&w.done[row], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         if (base != w.parts - 1) return;
         n = __builtin_amdgcn_readfirstlane(
-            __hip_atomic_load(&w.listed[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+            __hip_atomic_load(&w.listed[row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
         for (int i = tid; i < min(n, kList); i += kRow)
-            u.list[i] = __hip_atomic_load(&w.list[static_cast<long>(r) * kList + i],
+            u.list[i] = __hip_atomic_load(&w.list[static_cast<long>(row) * kList + i],
                                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
     }
@@ -1144,7 +1146,7 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
             log(weight_of(from_key(~static_cast<uint32_t>(token >> 32)), top, s.inv_t, powers) / kept));
 }
 
-// Rows of one launch of the split kernels: the workspace is bounded.
+// Most rows that are split: the workspace is bounded.
 constexpr int kSplitRows = 192;
 
 // One block a row where rows fill the GPU, or are a few units: one launch and no trip through
@@ -1229,26 +1231,21 @@ int sample(const char* fn, const void* logits, long stride, const float* uniform
     sample_layout(rows, w.units, static_cast<char*>(ws), &w);
     const hipStream_t st = as_stream(stream);
     if (sample_whole(rows, w.units)) {
-        w.rows = rows;
         w.parts = 1;
         hipLaunchKernelGGL((sample_pick_kernel<T, true>), dim3(rows), dim3(kRow), 0, st, g, w);
         return launch_status(fn);
     }
     const int blocks = (w.units + kSplitBlock / kWave - 1) / (kSplitBlock / kWave);
-    for (w.first = 0; w.first < rows; w.first += w.rows) {
-        w.rows = rows - w.first < kSplitRows ? rows - w.first : kSplitRows;
-        const int most = (w.units + kWaves - 1) / kWaves, fill = (256 + w.rows - 1) / w.rows;
-        w.parts = fill < most ? fill : most;
-        if (w.parts > 16) w.parts = 16;
-        hipLaunchKernelGGL(sample_peaks_kernel<T>, dim3(blocks, w.rows), dim3(kSplitBlock), 0, st, g, w);
-        // Each block adds its bins to the row's: fewer blocks a row, fewer additions in memory.
-        const int share = (512 + w.rows - 1) / w.rows;
-        hipLaunchKernelGGL(sample_bins_kernel<T>, dim3(blocks < share ? blocks : share, w.rows),
-                           dim3(kSplitBlock), 0, st, g, w);
-        hipLaunchKernelGGL((sample_pick_kernel<T, false>), dim3(w.parts, w.rows), dim3(kRow), 0, st, g, w);
-        if (int e = launch_status(fn)) return e;
-    }
-    return 0;
+    const int most = (w.units + kWaves - 1) / kWaves, fill = (256 + rows - 1) / rows;
+    w.parts = fill < most ? fill : most;
+    if (w.parts > 16) w.parts = 16;
+    hipLaunchKernelGGL(sample_peaks_kernel<T>, dim3(blocks, rows), dim3(kSplitBlock), 0, st, g, w);
+    // Each block adds its bins to the row's: fewer blocks a row, fewer additions in memory.
+    const int share = (512 + rows - 1) / rows;
+    hipLaunchKernelGGL(sample_bins_kernel<T>, dim3(blocks < share ? blocks : share, rows),
+                       dim3(kSplitBlock), 0, st, g, w);
+    hipLaunchKernelGGL((sample_pick_kernel<T, false>), dim3(w.parts, rows), dim3(kRow), 0, st, g, w);
+    return launch_status(fn);
 }
 
 // ---- log-probabilities --------------------------------------------------------------
@@ -1281,7 +1278,7 @@ struct Sum {
 
 struct LogprobWork {
     Sum* sums;  // [rows][units]
-    int first, rows, units;
+    int units;
 };
 
 // Adds a unit to a wave's sum: top and count are the wave's, rest is each lane's.  Float32
@@ -1326,7 +1323,7 @@ __device__ __forceinline__ unsigned long long rank_key(float l, int index) {
 // Few rows: a wave has a unit, and another kernel adds up.
 template <class T>
 __global__ __launch_bounds__(kSplitBlock) void logprob_units_kernel(LogprobArgs g, LogprobWork w) {
-    const int r = blockIdx.y, row = w.first + r;
+    const int row = blockIdx.y;
     const int u = blockIdx.x * (kSplitBlock / kWave) + static_cast<int>(threadIdx.x / kWave);
     if (u >= w.units) return;
     const typename T::Bits* logits = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
@@ -1335,7 +1332,7 @@ __global__ __launch_bounds__(kSplitBlock) void logprob_units_kernel(LogprobArgs 
     Sum s{-__builtin_inff(), 0, 0.0};
     sum_unit<T>(s, x, logits, g.vocab, u);
     s.rest = from_lane(wave_scan(s.rest, 0.0, Add()), kWave - 1);
-    if (threadIdx.x % kWave == 0) w.sums[static_cast<long>(r) * w.units + u] = s;
+    if (threadIdx.x % kWave == 0) w.sums[static_cast<long>(row) * w.units + u] = s;
 }
 
 // A row's log-probabilities, and its `top` likeliest tokens.  kWhole: all of it by this block;
@@ -1357,7 +1354,7 @@ __global__ __launch_bounds__(kRow) void logprob_kernel(LogprobArgs g, LogprobWor
         unsigned long long u[kWaves];
     } part;
     __shared__ int chosen[kMaxTop], listed;
-    const int r = blockIdx.x, row = w.first + r, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const int token = g.tokens ? g.tokens[row] : 0;
     if (token < 0 || token >= g.vocab) return;
     const typename T::Bits* logits = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
@@ -1384,7 +1381,7 @@ __global__ __launch_bounds__(kRow) void logprob_kernel(LogprobArgs g, LogprobWor
         if (lane > 0) s.count = 0;
     } else {
         for (int u = tid; u < w.units; u += kRow) {
-            const Sum o = w.sums[static_cast<long>(r) * w.units + u];
+            const Sum o = w.sums[static_cast<long>(row) * w.units + u];
             peak_of(u, o.top);
             if (o.top == -__builtin_inff()) continue;
             if (o.top > s.top) {
@@ -1496,7 +1493,6 @@ __global__ __launch_bounds__(kRow) void logprob_kernel(LogprobArgs g, LogprobWor
     }
 }
 
-// Rows of one launch of the split kernels.
 size_t logprobs_layout(int rows, int units, char* base, LogprobWork* w) {
     const size_t n = rows < 1 ? 1 : rows < kSplitRows ? rows : kSplitRows;
     if (w) w->sums = reinterpret_cast<Sum*>(base);
@@ -1544,13 +1540,9 @@ int token_logprobs(const char* fn, const void* logits, long stride, const int* t
         return launch_status(fn);
     }
     const int blocks = (w.units + kSplitBlock / kWave - 1) / (kSplitBlock / kWave);
-    for (w.first = 0; w.first < rows; w.first += w.rows) {
-        w.rows = rows - w.first < kSplitRows ? rows - w.first : kSplitRows;
-        hipLaunchKernelGGL(logprob_units_kernel<T>, dim3(blocks, w.rows), dim3(kSplitBlock), 0, st, g, w);
-        hipLaunchKernelGGL((logprob_kernel<T, false>), dim3(w.rows), dim3(kRow), 0, st, g, w);
-        if (int e = launch_status(fn)) return e;
-    }
-    return 0;
+    hipLaunchKernelGGL(logprob_units_kernel<T>, dim3(blocks, rows), dim3(kSplitBlock), 0, st, g, w);
+    hipLaunchKernelGGL((logprob_kernel<T, false>), dim3(rows), dim3(kRow), 0, st, g, w);
+    return launch_status(fn);
 }
 
 }  // namespace

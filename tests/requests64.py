@@ -66,7 +66,8 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     l = l[~np.isneginf(l)]
     if not temperature > 0 or top_p <= 0:
         return int(order[0]), 0.0, 1
-    w = _weights(l, temperature)
+    # 64 bits of mantissa: sums of thousands of weights beside which one of 1e-14 counts
+    w = _weights(l, temperature).astype(np.longdouble)
     n = len(w) if top_k <= 0 else min(top_k, len(w))
     first = n
     if top_p < 1:
@@ -78,7 +79,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     total = w[:n].cumsum()
     u = min(max(u, 0.0), 1 - 2.0 ** -24) if u == u else 0.0
     at = int(np.argmax(total > u * total[-1]))
-    return int(order[at]), math.log(w[at] / total[-1]), n
+    return int(order[at]), math.log(float(w[at] / total[-1])), n
 
 
 def logprobs(logits, top):

@@ -174,6 +174,27 @@ def test_rows_behind_and_workspace_ends_stay(gpu):
     assert (out[70:] == 7).all() and (ws[size:] == 0x5A).all()
 
 
+@pytest.mark.parametrize("tokens", [2, 70, 600])
+@pytest.mark.parametrize("sections", [(13,), (256, 131), (264, 70)])
+def test_ragged_last_rows_leave_the_padding(gpu, tokens, sections):
+    """Padded rows whose last section is no multiple of 8: tokens with and without an adapter."""
+    d = make("bf16", tokens, 96, sections, 8, 3, [t % 5 - 1 for t in range(tokens)], seed=tokens)
+    rows, wide = sum(sections), sum(sections) // 8 * 8 + 16
+    base = torch.full((tokens, wide), 7.0, dtype=torch.bfloat16, device="cuda")
+    base[:, :rows] = d["base"]
+    out = torch.full((tokens, wide), 3.0, dtype=torch.bfloat16, device="cuda")
+    run(d, out=out[:, :rows], base=base[:, :rows])
+    assert bool((out[:, rows:] == 3.0).all())
+    close(out[:, :rows], d)
+
+
+@pytest.mark.parametrize("cols", [8, 16, 24, 40])
+@pytest.mark.parametrize("tokens", [70, 1500])
+def test_few_columns(gpu, cols, tokens):
+    d = make("f16", tokens, cols, (300, 9), 24, 80, None, seed=cols)
+    close(run(d), d)
+
+
 def test_smaller_batches_in_a_workspace_of_a_larger_one(gpu):
     d = make("bf16", 1000, 512, (64, 64), 64, 5, None, seed=4)
     ad = handle(d)

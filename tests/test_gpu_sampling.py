@@ -164,6 +164,23 @@ def test_flat_and_steep_rows(gpu, std, zipf, temperature, vocab):
         check(x, u, sample(x, u, **s), s)
 
 
+@pytest.mark.parametrize("rows", [1, 400])
+def test_top_k_ends_between_logits_of_which_thousands_decide(gpu, rows):
+    """min-p's border is among 2000 nearly equal logits, top-k's before them between two."""
+    vocab = 20000
+    g = torch.Generator().manual_seed(rows)
+    x = torch.full((rows, vocab), -60.0)
+    at = torch.randperm(vocab, generator=g)
+    x[:, at[:2000]] = -20.0 + torch.rand(rows, 2000, generator=g) * 0.01
+    x[:, at[2000:2010]] = torch.arange(10).float() * -0.4
+    u = uniforms_of(rows, rows)
+    for k in (1, 2, 5, 9, 10, 0):
+        for p in (1.0, 0.1, 0.6):
+            s = dict(temperature=50.0, top_k=k, top_p=p, min_p=math.exp(-19.995 / 50))
+            got = sample(x, u, **s)
+            check(x[:5], u[:5], [v[:5] for v in got], s)
+
+
 def test_temperatures_and_settings_out_of_range(gpu):
     rows = 14
     x = logits_of("f32", rows, 3000, 2)
