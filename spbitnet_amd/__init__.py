@@ -5,6 +5,8 @@ sparse-ternary linear-layer hot path.
 * ``spbitnet_amd/csrc/*.hip``       hand-written gfx950 kernels behind it
 * ``spbitnet_amd.kernels``          the reference's kernel API, in Python, over the C ABI, and
                                     the operators of a token batch over a paged cache
+                                    and of what its requests bring of their own
+                                    (adapters, sampling, log-probabilities)
 * ``spbitnet_amd.model``            Model / InferenceEngine: loader, random-init
                                     models and the decode engines over the C ABI
 * ``spbitnet_amd.weights``          host-side format: generation and packing

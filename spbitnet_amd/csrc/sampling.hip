@@ -7,11 +7,12 @@
 // three filters keeps a first part of that order, so the kept tokens are the first n,
 // and the token taken is the first whose weight with those before it passes u times
 // their sum M.  All that is looked for is a place in one order where a sum of counts
-// or weights passes a bound: a selection by digits of the logits' bits, without a sort.
+// or weights passes a bound: a histogram of the logits says in which bins, and only
+// those bins' tokens are sorted.
 //
-// Sums of weights decide between neighbours among up to 2^24 tokens, so they are held
-// to ~2^-46 of the largest weight and do not depend on the order of adding: weights are
-// computed in float64 and added as 64-bit whole numbers.
+// Sums of weights decide between neighbours among up to 2^24 tokens, and must not depend
+// on the order of adding: weights are computed in float64, to 2^-38 of their values, and
+// added as 64-bit whole numbers of 2^-38 (2^24 tokens) to 2^-49 of the largest weight.
 #include "common.hpp"
 #include "paged.hpp"
 #include "spbitnet_amd.h"
@@ -252,9 +253,10 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs& g, int row) {
 
 // exp(d) for d in [-64, 0]: d in 1/64 octaves is a whole number k and a rest; 2^(k / 64) from a
 // table of 64 in LDS and the exponent, the rest's exponential by its series, of which float64
-// needs to hold the first term only: the others are below 2^-15 and in float32 off by 2^-39
-// of the result.  A float64 instruction takes twice a float32 one's time (8 cycles a wave, as
-// measured): 12 of them here, where a series for a whole octave takes 20.
+// needs to hold the first term only: the others are below 2^-15 and in float32 off by 2^-38.7
+// of the result at most (20 million d compared with long double).  A float64 instruction takes
+// twice a float32 one's time (8 cycles a wave, as measured): 12 of them here, where a series
+// for a whole octave takes 20.
 __device__ __forceinline__ void fill_powers(double* powers) {
     if (threadIdx.x < 64) powers[threadIdx.x] = exp2(threadIdx.x / 64.0);
 }

@@ -97,7 +97,9 @@ def logprobs(logits, top):
     else:
         far = np.where(np.isneginf(l), 0.0, best - np.where(np.isneginf(l), best, l))
         out = np.where(np.isneginf(l), -math.inf, l - best - math.log1p(rest))
-    # the others' weights: float32 differences (2^-24 of them) and exponentials (2 steps)
+    # the others' weights: float32 differences (2^-24 of them) and exponentials (2 steps),
+    # and those that float32 has no normal number for (2^-126) may count as nothing, each
     lost = float((np.where(w < 1, w, 0.0) * (far + 4) * 2.0 ** -23).sum()) + 2.0 ** -126
+    lost += float(np.where(w < 2.0 ** -125, w, 0.0).sum())
     err = lost / (1 + rest) + 2.0 ** -24 * np.where(np.isfinite(out), np.abs(out), 0.0) + 2.0 ** -149
     return out, err * 1.001, order[:top]

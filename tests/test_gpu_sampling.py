@@ -395,6 +395,26 @@ def test_logprobs_in_sorted_and_equal_rows(gpu, kind):
         logprob_check(x, tokens, logprobs(x, tokens, top), top, note=top)
 
 
+@pytest.mark.parametrize("kind,vocab", [("f32", 700001), ("bf16", 3000001), ("f32", 3000001)])
+def test_logprobs_of_vocabularies_of_millions(gpu, kind, vocab):
+    """Groups of many units; in rising order more than the list holds are left of them."""
+    up = torch.linspace(-9, 9, vocab)
+    for x in (up[None], logits_of("f32", 1, vocab, vocab)):
+        x = x.to(TYPES[kind])
+        tokens = torch.tensor([vocab - 9], dtype=torch.int32)
+        for top in (3, 64):
+            logprob_check(x, tokens, logprobs(x, tokens, top), top, note=top)
+
+
+def test_the_largest_vocabulary(gpu):
+    vocab = 1 << 24
+    x = logits_of("f16", 1, vocab, 1)
+    s = dict(temperature=1.1, top_k=3000, top_p=0.9)
+    check(x, [0.7], sample(x, [0.7], **s), s)
+    tokens = torch.tensor([vocab - 1], dtype=torch.int32)
+    logprob_check(x, tokens, logprobs(x, tokens, 20), 20)
+
+
 def test_logprobs_masked_infinite_and_padded(gpu):
     v = 5000
     x = logits_of("f32", 9, v, 3)
