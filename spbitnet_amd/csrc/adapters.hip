@@ -332,8 +332,11 @@ constexpr int kRows = kWaves * 64;  // rows of a block of the second
 
 // h of 16 of an adapter's tokens of a window and 64 rows of A: g.split_bits blocks and their
 // waves split the columns, the waves add up in LDS.  Most of a block's time is fetching its
-// code, which a launch finds in no cache of its CU: one loop, two bodies.
-template <class T>
+// code, which a launch finds in no cache of its CU: one loop, two bodies.  kDeep products'
+// loads are in flight together: 2 where windows are few, and the code's fetch counts (32
+// tokens of 18 adapters, rank 16, q|k|v of 2560: 5.3 us, with 5 6.5), 5 else (2049 tokens,
+// rank 32: 14.5 us, with 2 18.0; x is 10 MB, A 1.6).
+template <class T, int kDeep>
 __global__ __launch_bounds__(kWaves* kWave) void shrink_kernel(Args g) {
     __shared__ float part[kWaves][kTile][kPad];
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
@@ -354,7 +357,7 @@ __global__ __launch_bounds__(kWaves* kWave) void shrink_kernel(Args g) {
         const uint16_t* a = g.a + q.adapter * g.a_adapter + j0 * g.a_row;
         Acc acc[4] = {};
         auto inner = [&](auto tiles) {
-            constexpr int kM = decltype(tiles)::value, kAhead = kM == 1 ? 4 : 2;
+            constexpr int kM = decltype(tiles)::value, kAhead = kM == 1 ? 4 : kDeep;
             const uint16_t* row[kM];
 #pragma unroll
             for (int m = 0; m < kM; ++m) {
@@ -585,15 +588,20 @@ int check_tokens(const char* fn, int tokens) {
     return 0;
 }
 
-// 2^n blocks split the columns of the inner products: a few windows do not fill the GPU.
+constexpr int kFewWindows = 16;
+
+// 2^n blocks split the columns of the inner products: 512 blocks and more, two a CU, while the
+// outer products' reading of the parts does not cost more.  gate|up of 2560 columns, rank 32:
+// 2049 tokens 46.9 us by 4, 50.9 by 2, 57.9 by 8; 4096 86.6 by 4, 79.4 by 2; 1100 34.2 by 4,
+// 40.0 by 8.
 int split_bits_of(int tokens) {
     const int windows = (tokens + kWindow - 1) / kWindow;
-    return windows <= 16 ? 3 : windows <= 32 ? 2 : windows <= 64 ? 1 : 0;
+    return windows <= kFewWindows ? 3 : windows < 64 ? 2 : windows < 128 ? 1 : 0;
 }
 
 // What the splits of n tokens times n come to for no n up to `tokens` is more than this.
 size_t workspace_size(const spb_adapters& d, int tokens) {
-    const size_t n = tokens, rows = n * 8 < 8192 ? n * 8 : n > 8192 ? n : 8192;
+    const size_t n = tokens, rows = n * 8 < 16384 ? n * 8 : n > 16384 ? n : 16384;
     return sizeof(float) * d.num_sections * d.rank * rows;
 }
 
@@ -672,8 +680,11 @@ int run(const char* fn, const spb_adapters* d, const int* ids, const uint16_t* x
     g.split_bits = split_bits_of(tokens);
     const int parts = (g.sections * g.rank + kPart - 1) / kPart;
     const int blocks = parts * (kWindow / kTile) << g.split_bits;
-    hipLaunchKernelGGL(shrink_kernel<T>, dim3(windows, ways(windows * blocks), blocks),
-                       dim3(kWaves * kWave), 0, st, g);
+    const dim3 inner(windows, ways(windows * blocks), blocks);
+    if (windows <= kFewWindows)
+        hipLaunchKernelGGL((shrink_kernel<T, 2>), inner, dim3(kWaves * kWave), 0, st, g);
+    else
+        hipLaunchKernelGGL((shrink_kernel<T, 5>), inner, dim3(kWaves * kWave), 0, st, g);
     const dim3 grid(tiles(kRows), ways(windows * tiles(kRows)), windows);
     if (g.rank <= kPart)
         hipLaunchKernelGGL((expand_kernel<T, false>), grid, dim3(kWaves * kWave), 0, st, g);
