@@ -481,6 +481,11 @@ __device__ void sample_row(const SampleArgs& g, int row, const Settings& s, floa
 // -- sorted, and decide.  Between the bins nothing needs an order.  So a row is read three
 // -- times: for its largest logit, for the bins, and for those tokens; parts whose largest
 // -- logit is below the bins in question are left out the third time.
+// --
+// -- 512 rows of 128256 float32 logits, top-p 0.95, a block a row: 170 us, of them 33 for the
+// -- largest logits (memory, 8 TB/s: the rows fit the last cache mostly), 65 for the bins (issue
+// -- of the weights' float64), 36 for the tokens in question (memory), 11 for sorting them and
+// -- the end.  The two blocks of a CU go through them in step.
 
 constexpr int kBins = 2048;
 constexpr int kOwn = kBins / kRow;  // bins of a thread
@@ -609,7 +614,8 @@ __device__ __forceinline__ float cut_of(float top, double inv_t) {
     return __builtin_fmaxf(static_cast<float>(top - 64.0 / inv_t), -0x1.fffffep127f);
 }
 
-// Few rows: units over blocks.  First their largest logits ...
+// Few rows: units over blocks.  First their largest logits (1 row of 128256 1.9 us, 32 rows
+// 4.3) ...
 template <class T>
 __global__ __launch_bounds__(kSplitBlock) void sample_peaks_kernel(SampleArgs g, SampleWork w) {
     const int row = blockIdx.y, tid = threadIdx.x;
@@ -635,7 +641,8 @@ __global__ __launch_bounds__(kSplitBlock) void sample_peaks_kernel(SampleArgs g,
     }
 }
 
-// ... then the histogram, added up in LDS and from there in memory.
+// ... then the histogram, added up in LDS and from there in memory (6.5 and 14.6 us: clearing,
+// the float64 weights, and additions in memory past L2) ...
 template <class T>
 __global__ __launch_bounds__(kSplitBlock) void sample_bins_kernel(SampleArgs g, SampleWork w) {
     __shared__ unsigned long long mass[kBins];
@@ -747,8 +754,9 @@ __device__ __forceinline__ void sort_list(unsigned long long* list, int n) {
     __syncthreads();
 }
 
-// The token of a row.  kWhole: all of it by this block; else from the histogram in memory, the
-// tokens in question gathered by w.parts blocks.
+// ... and the token of a row (12.6 and 26.5 us: a chain of dependent steps, a barrier each, and
+// the fetch of their code).  kWhole: all of it by this block; else from the histogram in memory,
+// the tokens in question gathered by w.parts blocks.
 template <class T, bool kWhole>
 __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, SampleWork w) {
     __shared__ union {
@@ -1358,7 +1366,8 @@ __device__ __forceinline__ unsigned long long rank_key(float l, int index) {
     return static_cast<unsigned long long>(~key_of(l)) << 32 | static_cast<uint32_t>(index);
 }
 
-// Few rows: a wave has a unit, and another kernel adds up.
+// Few rows: a wave has a unit, and another kernel adds up.  1 row of 128256 2.4 us and 14.5 in
+// the other (20 alternatives), 32 rows 4.0 and 10.4 (5).
 template <class T>
 __global__ __launch_bounds__(kSplitBlock) void logprob_units_kernel(LogprobArgs g, LogprobWork w) {
     const int row = blockIdx.y;
@@ -1381,6 +1390,10 @@ __global__ __launch_bounds__(kSplitBlock) void logprob_units_kernel(LogprobArgs 
 // and their tokens from the last of those logits on are sorted: a few more than `top`, mostly.
 // Where they are many (a row in rising order), the same is done with lanes for groups: at
 // most 16 of each of `top` lanes are left.
+//
+// 2048 rows of 128256 float32 logits, 5 alternatives: 207 us for 1.05 GB, 5.1 TB/s, what a copy
+// reaches; the row's few groups are read again from the caches.  1023 rows of 32003 bf16: 22 us,
+// 3.0 TB/s: rows of 64 KB, whose start and end (launch, sums over the block) show.
 template <class T, bool kWhole>
 __global__ __launch_bounds__(kRow) void logprob_kernel(LogprobArgs g, LogprobWork w) {
     __shared__ uint32_t peaks[kGroups];
