@@ -342,7 +342,7 @@ constexpr int kRows = kWaves * 64;  // rows of a block of the second
 // waves split the columns, the waves add up in LDS.  Most of a block's time is fetching its
 // code, which a launch finds in no cache of its CU: one loop, two bodies.  kDeep products'
 // loads are in flight together: 2 where windows are few, and the code's fetch counts (32
-// tokens of 18 adapters, rank 16, q|k|v of 2560: 5.3 us, with 5 6.5), 5 else (2049 tokens,
+// tokens of up to 20 adapters, rank 16, q|k|v of 2560: 5.3 us, with 5 6.5), 5 else (2049 tokens,
 // rank 32: 14.5 us, with 2 18.0; x is 10 MB, A 1.6).
 template <class T, int kDeep>
 __global__ __launch_bounds__(kWaves* kWave) void shrink_kernel(Args g) {
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(kWaves* kWave) void shrink_kernel(Args g) {
 // products so that a lane's results of two are 8 neighbours, and with its three neighbours'
 // 64 bytes of a token's output.  The adapter's part of B stays in registers, up to 64 ranks;
 // more go in passes for every 16 tokens.  2049 tokens, rank 32 on gate|up of 6912 rows each:
-// 33.9 us for 113 MB of base and output and the 4 parts of the inner products, 3.4 TB/s; 18
+// 33.9 us for 113 MB of base and output and the 4 parts of the inner products, 3.4 TB/s; up to 20
 // adapters over 32 tokens, rank 16 on q|k|v: 7.4 us, bound as the kernel above.
 template <class T, bool kPasses>
 __global__ __launch_bounds__(kWaves* kWave) void expand_kernel(Args g) {

@@ -43,7 +43,7 @@ def check(logits, uniforms, got, settings, note=""):
         assert got[0][i] == token, (where, got[0][i], token)
         if math.isinf(lp):
             assert got[1][i] == lp, where
-        else:  # one rounding to float32, and sums held to 2^-38 of the largest weight or better
+        else:  # one rounding to float32; sums of these weights are held to 2^-38 of the largest
             assert abs(got[1][i] - lp) <= 2.0 ** -24 * abs(lp) + 2.0 ** -36, (where, got[1][i], lp)
 
 
@@ -413,6 +413,24 @@ def test_the_largest_vocabulary(gpu):
     check(x, [0.7], sample(x, [0.7], **s), s)
     tokens = torch.tensor([vocab - 1], dtype=torch.int32)
     logprob_check(x, tokens, logprobs(x, tokens, 20), 20)
+
+
+def test_many_rows_of_a_vocabulary_of_a_million(gpu):
+    """A block a row, with more units than it keeps the largest logits of."""
+    vocab, rows = 1100003, 194
+    two = logits_of("f16", 2, vocab, 7)
+    two[1] = two[1].sort().values
+    x = two.cuda().repeat(rows // 2, 1)
+    u = [0.1, 0.93] * (rows // 2)
+    for s in (dict(temperature=1.3, top_p=0.9), dict(top_k=900, min_p=0.001)):
+        tokens, lp = sample(x, u, logits_gpu=x, **s)
+        assert tokens == tokens[:2] * (rows // 2) and lp == lp[:2] * (rows // 2)
+        check(two, u[:2], [tokens[:2], lp[:2]], s)
+    t = torch.tensor([5, vocab - 1] * (rows // 2), dtype=torch.int32)
+    got = logprobs(x, t, 20, logits_gpu=x)
+    logprob_check(two, t[:2], [v[:2] for v in got], 20)
+    for v in got:
+        assert torch.equal(v, v[:2].repeat(rows // 2, *[1] * (v.dim() - 1)))
 
 
 def test_logprobs_masked_infinite_and_padded(gpu):
