@@ -589,10 +589,10 @@ typedef struct spb_sampling {
  * NaN logits count as minus infinity, which is never taken; of infinite ones the
  * others have no weight.  A row of minus infinities gives token -1 and log-probability
  * minus infinity.  Weights are computed to 2^-38 of their values and added as whole
- * numbers of 2^-b of the largest weight, b = 49 or, for a vocabulary of 2^14 tokens or
- * more, 62 - floor(log2(vocab)) (46 for 128256): sums do not depend on the order of
- * execution, and a border that is nearer to a token's place than that may fall on
- * either side of it.  vocab <= 2^24, rows <= 2^20. */
+ * numbers, of steps that follow the weights' size: sums do not depend on the order of
+ * execution, and are off by 2^-37 of the weights besides the largest and 2^-50 of all, also
+ * where millions of tokens far below the largest decide.  A border that is nearer to a
+ * token's place than that may fall on either side of it.  vocab <= 2^24, rows <= 2^20. */
 size_t spb_sample_workspace_size(int rows, int vocab);
 int spb_sample_f32(const float* logits, long logits_stride, const float* uniforms, int* tokens,
                    float* logprobs, int rows, int vocab, const spb_sampling* sampling,

@@ -12,7 +12,9 @@
 //
 // Sums of weights decide between neighbours among up to 2^24 tokens, and must not depend
 // on the order of adding: weights are computed in float64, to 2^-38 of their values, and
-// added as 64-bit whole numbers of 2^-38 (2^24 tokens) to 2^-49 of the largest weight.
+// added as 64-bit whole numbers.  A step relative to a row's largest weight, 1, would lose what
+// many far tokens weigh together (2^24 of them at e^-27 have 3e-5 of a row, each is below half
+// a step of 2^-38): each bin has a step of its own, 2^-38 (2^24 tokens) to 2^-49 of its weights.
 #include "common.hpp"
 #include "paged.hpp"
 #include "spbitnet_amd.h"
@@ -217,52 +219,55 @@ struct SampleArgs {
     spb_sampling set;
 };
 
+constexpr double kPerUnit = 0x1.71547652b82fep+6;  // 64 / ln 2
+
 // A row's settings, with what is off or out of range taken care of.
 struct Settings {
-    double inv_t, u;
+    double t, u;
     double top_p, min_p;  // 1 and 0: off
     int k;                // vocab: off
+    double per;           // 1/64 octaves of a weight per unit of a logit
     float bins;           // bins per unit of a logit
-    double unit, one;     // weights are added as whole numbers of 1 / unit, one = 2^52 / unit
+    uint32_t octaves;     // a bin's width in 2^-20 octaves of a weight, at most 2^20 / 64 / ln 2
+    int bits;             // a bin's weights, as numbers of up to 1, are added as whole numbers
+    double one;           // of 2^-bits; one = 2^(52 - bits)
 };
 
 __device__ __forceinline__ Settings settings_of(const SampleArgs& g, int row) {
     Settings s;
-    float t = g.set.temperatures ? g.set.temperatures[row] : g.set.temperature;
+    float heat = g.set.temperatures ? g.set.temperatures[row] : g.set.temperature;
     int k = g.set.top_ks ? g.set.top_ks[row] : g.set.top_k;
     const float p = g.set.top_ps ? g.set.top_ps[row] : g.set.top_p;
     const float m = g.set.min_ps ? g.set.min_ps[row] : g.set.min_p;
     const float u = g.uniforms[row];
     if (k <= 0 || k > g.vocab) k = g.vocab;
-    if (!(t > 0.0f)) {  // greedy: the first token of the order
-        t = 1.0f;
+    if (!(heat > 0.0f)) {  // greedy: the first token of the order
+        heat = 1.0f;
         k = 1;
     }
     if (p <= 0.0f) k = 1;
     s.top_p = p < 1.0f && p > 0.0f ? p : 1.0;
     s.min_p = m > 0.0f ? (m < 1.0f ? m : 1.0) : 0.0;
     s.k = k;
-    s.inv_t = 1.0 / static_cast<double>(t);
+    s.t = heat;
+    s.per = kPerUnit / s.t;
     s.u = u > 0.0f ? (u < 1.0f ? u : 0x1.fffffep-1) : 0.0;
-    s.bins = static_cast<float>(__builtin_fmin(64.0 * __builtin_fmax(s.inv_t, 1.0), 0x1p40));
-    const int bits = 32 - __clz(g.vocab);  // vocab < 2^bits: a row of ones stays below 2^63
-    s.unit = __builtin_ldexp(1.0, min(49, 63 - bits));
-    s.one = __builtin_ldexp(1.0, max(3, bits - 11));
+    s.bits = min(49, 31 + __clz(g.vocab));  // a row of ones stays below 2^63
+    s.one = __builtin_ldexp(1.0, 52 - s.bits);
     return s;
 }
 
-// exp(d) for d in [-64, 0]: d in 1/64 octaves is a whole number k and a rest; 2^(k / 64) from a
-// table of 64 in LDS and the exponent, the rest's exponential by its series, of which float64
-// needs to hold the first term only: the others are below 2^-15 and in float32 off by 2^-38.7
-// of the result at most (20 million d compared with long double).  A float64 instruction takes
-// twice a float32 one's time (8 cycles a wave, as measured): 12 of them here, where a series
-// for a whole octave takes 20.
+// 2^(y / 64) for y in [-64, 0] times 64 / ln 2, times 2^(up / 2^20), up a multiple of 2^20: y is
+// a whole number k and a rest; 2^(k / 64) from a table of 64 in LDS and the exponent, the rest's
+// exponential by its series, of which float64 needs to hold the first term only: the others
+// are below 2^-15 and in float32 off by 2^-38.7 of the result at most (20 million y compared with
+// long double).  A float64 instruction takes twice a float32 one's time (8 cycles a wave, as
+// measured): 11 of them here with y's own, where a series for a whole octave takes 19.
 __device__ __forceinline__ void fill_powers(double* powers) {
     if (threadIdx.x < 64) powers[threadIdx.x] = exp2(threadIdx.x / 64.0);
 }
-__device__ __forceinline__ double exp_of(double d, const double* powers) {
+__device__ __forceinline__ double power_of(double y, uint32_t up, const double* powers) {
     constexpr double kStep = 0x1.62e42fefa39efp-7;  // ln 2 / 64
-    const double y = d * 0x1.71547652b82fep+6;      // 64 / ln 2
     const double z = y + 0x1.8p52;                  // its low word is y rounded
     const int k = static_cast<int>(__builtin_bit_cast(uint64_t, z));
     const double r = y - (z - 0x1.8p52);
@@ -273,20 +278,19 @@ __device__ __forceinline__ double exp_of(double d, const double* powers) {
     const double p = __builtin_fma(r, kStep, static_cast<double>(rest));
     const double t = powers[k & 63];
     const auto w = __builtin_bit_cast(uint64_t, __builtin_fma(t, p, t));
-    const uint32_t hi = static_cast<uint32_t>(w >> 32) + (static_cast<uint32_t>(k >> 6) << 20);
+    const uint32_t hi = static_cast<uint32_t>(w >> 32) + (static_cast<uint32_t>(k) << 14 & 0xfff00000u) + up;
     return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | static_cast<uint32_t>(w));
 }
 
 // Weight of a logit (not minus infinity) at or below `top`.
-__device__ __forceinline__ double weight_of(float l, float top, double inv_t, const double* powers) {
-    const double d = (static_cast<double>(l) - static_cast<double>(top)) * inv_t;
+__device__ __forceinline__ double weight_of(float l, float top, double per, const double* powers) {
+    const double y = (static_cast<double>(l) - static_cast<double>(top)) * per;
     if (l == top) return 1.0;
     // 2^24 weights below e^-64 are nothing beside the first, 1
-    return d > -64.0 ? exp_of(d, powers) : 0.0;
+    return y > -64.0 * kPerUnit ? power_of(y, 0, powers) : 0.0;
 }
 
-// A weight as a whole number of 1 / unit, one = 2^52 / unit: the sum's low bits (those of a
-// power of two are 0).
+// A weight as a whole number of 2^-52 * one: the sum's low bits (those of a power of two are 0).
 __device__ __forceinline__ unsigned long long fixed(double w, double one) {
     const auto b = __builtin_bit_cast(unsigned long long, w + one);
     const uint32_t hi = static_cast<uint32_t>(b >> 32) -
@@ -294,15 +298,34 @@ __device__ __forceinline__ unsigned long long fixed(double w, double one) {
     return static_cast<unsigned long long>(hi) << 32 | static_cast<uint32_t>(b);
 }
 
-// -- from the row itself, in up to a dozen readings: for rows whose borders fall among
-// -- thousands of nearly equal logits
+// -- from the row itself, in up to 15 readings (its sums, four digits for each of the three
+// -- places, twice for the token's index): for rows whose borders fall among thousands of
+// -- nearly equal logits, and those that bins do not fit
 
+// A sum of weights of all sizes up to 1: whole numbers of 2^-38, and what that leaves of each
+// (2^-39 at most, of either sign) as whole numbers of 2^-76.  2^24 weights are off by 2^-53.
+struct Mass {
+    unsigned long long coarse, fine;
+
+    static __device__ __forceinline__ Mass of(double w) {
+        const double z = w + 0x1p14, rest = w - (z - 0x1p14);
+        return {fixed(w, 0x1p14), __builtin_bit_cast(unsigned long long, rest + 0x1.8p-24) -
+                                      __builtin_bit_cast(unsigned long long, 0x1.8p-24)};
+    }
+    __device__ __forceinline__ double value() const {
+        return __builtin_fma(static_cast<double>(static_cast<long long>(fine)), 0x1p-76,
+                             static_cast<double>(coarse) * 0x1p-38);
+    }
+};
+
+// Four of each digit side by side, a lane adds to one of them: most lanes have the same digit.
 struct Hist {
-    unsigned long long mass[256];
-    int count[256];
+    static constexpr int kSides = 4;
+    unsigned long long coarse[256][kSides], fine[256][kSides];
+    int count[256][kSides];
     int digit;
     int before_count;
-    unsigned long long before_mass;
+    Mass before_mass;
 };
 
 template <class T>
@@ -311,9 +334,29 @@ struct Row {
     const double* powers;
     int vocab;
     float top;
-    double inv_t, one, unit;
+    double per;
 
-    __device__ __forceinline__ double weight(float v) const { return weight_of(v, top, inv_t, powers); }
+    __device__ __forceinline__ double weight(float v) const { return weight_of(v, top, per, powers); }
+
+    // f(logit) of this thread's, minus infinities apart; the loads of the next four are in flight.
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+        constexpr int kAhead = 4;
+        float v[kAhead];
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) {
+            const int i = threadIdx.x + n * kRow;
+            v[n] = i < vocab ? T::load(l + i) : 0.0f;
+        }
+#pragma unroll 1
+        for (int i = threadIdx.x; i < vocab; i += kRow) {
+            const float now = clean(v[0]);
+#pragma unroll
+            for (int n = 1; n < kAhead; ++n) v[n - 1] = v[n];
+            if (i + kAhead * kRow < vocab) v[kAhead - 1] = T::load(l + i + kAhead * kRow);
+            if (now != -__builtin_inff()) f(now);
+        }
+    }
 };
 
 // A place in the order: the logit there, how many of that logit stand before it, and the
@@ -328,63 +371,71 @@ struct Place {
 // before it is above bound (at the end of all of them the last with a weight).  Four
 // digits of the key, each a histogram of the tokens that share the digits before it.
 template <bool kMass, class T>
-__device__ Place select(const Row<T>& r, int rank, double bound, Hist& h) {
+__device__ __forceinline__ Place select(const Row<T>& r, int rank, double bound, Hist& h) {
     uint32_t prefix = 0;
     int count = 0;
-    unsigned long long mass = 0;
+    Mass mass = {0, 0};
     for (int shift = 24; shift >= 0; shift -= 8) {
         __syncthreads();
-        if (threadIdx.x < 256) {
-            h.mass[threadIdx.x] = 0;
-            h.count[threadIdx.x] = 0;
+        for (int i = threadIdx.x; i < 256 * Hist::kSides; i += kRow) {
+            (&h.coarse[0][0])[i] = 0;
+            (&h.fine[0][0])[i] = 0;
+            (&h.count[0][0])[i] = 0;
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < r.vocab; i += kRow) {
-            const float l = clean(T::load(r.l + i));
-            if (l == -__builtin_inff()) continue;
+        r.each([&](float l) {
             const uint32_t key = key_of(l);
-            if (shift < 24 && (key >> (shift + 8)) != (prefix >> (shift + 8))) continue;
+            if (shift < 24 && (key >> (shift + 8)) != (prefix >> (shift + 8))) return;
             const int d = key >> shift & 255;
             // equal logits are added by one lane: a row of 128256 times one value took 1000 us
             // with each lane adding its own, 450 so
             const bool led = key == __builtin_amdgcn_readfirstlane(key);
             const unsigned long long same = __ballot(led);
             const int times = led ? __popcll(same) : 1;
-            if (led && threadIdx.x % kWave != __ffsll(same) - 1) continue;
-            atomicAdd(&h.count[d], times);
-            atomicAdd(&h.mass[d], times * fixed(r.weight(l), r.one));
-        }
+            if (led && threadIdx.x % kWave != __ffsll(same) - 1) return;
+            const Mass m = Mass::of(r.weight(l));
+            const int side = threadIdx.x % Hist::kSides;
+            atomicAdd(&h.count[d][side], times);
+            atomicAdd(&h.coarse[d][side], times * m.coarse);
+            atomicAdd(&h.fine[d][side], times * m.fine);
+        });
         __syncthreads();
         if (threadIdx.x < kWave) {  // a wave takes the digits from the highest on, 4 a lane
             const int lane = threadIdx.x;
             int c[4], sum_c = 0;
-            unsigned long long m[4], sum_m = 0;
+            Mass m[4], sum_m = {0, 0};
+#pragma unroll
             for (int i = 0; i < 4; ++i) {
-                sum_c += c[i] = h.count[255 - 4 * lane - i];
-                sum_m += m[i] = h.mass[255 - 4 * lane - i];
-            }
-            int upto_c = sum_c;
-            unsigned long long upto_m = sum_m;
-            for (int off = 1; off < kWave; off <<= 1) {
-                const int oc = __shfl_up(upto_c, off, kWave);
-                const unsigned long long om = __shfl_up(upto_m, off, kWave);
-                if (lane >= off) {
-                    upto_c += oc;
-                    upto_m += om;
+                const int d = 255 - 4 * lane - i;
+                c[i] = 0;
+                m[i] = {0, 0};
+#pragma unroll
+                for (int side = 0; side < Hist::kSides; ++side) {
+                    c[i] += h.count[d][side];
+                    m[i].coarse += h.coarse[d][side];
+                    m[i].fine += h.fine[d][side];
                 }
+                sum_c += c[i];
+                sum_m.coarse += m[i].coarse;
+                sum_m.fine += m[i].fine;
             }
+            const int upto_c = wave_scan(sum_c, 0, Add());
             int bc = count + upto_c - sum_c, at_c = 0, first = -1, last = -1;
-            unsigned long long bm = mass + upto_m - sum_m, at_m = 0;
-            for (int i = 0; i < 4 && first < 0; ++i) {
-                if (kMass ? m[i] != 0 : c[i] != 0) {
+            Mass bm = {mass.coarse + wave_scan(sum_m.coarse, 0ull, Add()) - sum_m.coarse,
+                       mass.fine + wave_scan(sum_m.fine, 0ull, Add()) - sum_m.fine},
+                 at_m = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (first >= 0) continue;
+                if (kMass ? (m[i].coarse | m[i].fine) != 0 : c[i] != 0) {
                     last = i;
                     at_c = bc;
                     at_m = bm;
                 }
                 bc += c[i];
-                bm += m[i];
-                if (last == i && (kMass ? static_cast<double>(bm) > bound * r.unit : bc > rank))
-                    first = i;
+                bm.coarse += m[i].coarse;
+                bm.fine += m[i].fine;
+                if (last == i && (kMass ? bm.value() > bound : bc > rank)) first = i;
             }
             // the first digit that passes, or the last that has tokens
             const unsigned long long passed = __ballot(first >= 0), some = __ballot(last >= 0);
@@ -403,9 +454,10 @@ __device__ Place select(const Row<T>& r, int rank, double bound, Hist& h) {
     }
     Place p;
     p.key = prefix;
-    const int ties = h.count[prefix & 255];
+    int ties = 0;
+    for (int side = 0; side < Hist::kSides; ++side) ties += h.count[prefix & 255][side];
     const double w = r.weight(from_key(prefix));
-    p.mass = static_cast<double>(mass) / r.unit;
+    p.mass = mass.value();
     double in = kMass ? (bound - p.mass) / w : rank - count;
     in = in < ties - 1 ? in : ties - 1;
     p.before_ties = in > 0 ? static_cast<int>(in) : 0;
@@ -414,7 +466,7 @@ __device__ Place select(const Row<T>& r, int rank, double bound, Hist& h) {
 }
 
 template <class T>
-__device__ void sample_row(const SampleArgs& g, int row, const Settings& s, float top, const double* powers,
+__device__ __forceinline__ void sample_row(const SampleArgs& g, int row, const Settings& s, float top, const double* powers,
                            Hist& h) {
     __shared__ union {
         int i[kWaves];
@@ -424,24 +476,29 @@ __device__ void sample_row(const SampleArgs& g, int row, const Settings& s, floa
     r.l = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
     r.powers = powers;
     r.vocab = g.vocab;
-    r.inv_t = s.inv_t;
+    r.per = s.per;
     r.top = top;
-    r.unit = s.unit;
-    r.one = s.one;
     // the kept mass: the least of what each filter keeps
-    unsigned long long all = 0, high = 0;
+    Mass all = {0, 0}, high = {0, 0};
     int live = 0;
-    for (int i = threadIdx.x; i < g.vocab; i += kRow) {
-        const float l = clean(T::load(r.l + i));
-        if (l == -__builtin_inff()) continue;
+    r.each([&](float l) {
         ++live;
         const double w = r.weight(l);
-        all += fixed(w, r.one);
-        if (w >= s.min_p) high += fixed(w, r.one);
-    }
+        const Mass m = Mass::of(w);
+        all.coarse += m.coarse;
+        all.fine += m.fine;
+        if (w >= s.min_p) {
+            high.coarse += m.coarse;
+            high.fine += m.fine;
+        }
+    });
     live = block_reduce(live, 0, part.i, Add());
-    double kept = static_cast<double>(block_reduce(all, 0ull, part.u, Add())) / r.unit;
-    const double over = static_cast<double>(block_reduce(high, 0ull, part.u, Add())) / r.unit;
+    auto sum = [](const Mass& m) {
+        return Mass{block_reduce(m.coarse, 0ull, part.u, Add()), block_reduce(m.fine, 0ull, part.u, Add())}
+            .value();
+    };
+    double kept = sum(all);
+    const double over = sum(high);
     if (s.k < live) kept = select<false>(r, s.k, 0.0, h).mass;
     if (s.top_p < 1.0) {
         // the token at the place passes the bound: it is the last that stays, unless the
@@ -473,12 +530,14 @@ __device__ void sample_row(const SampleArgs& g, int row, const Settings& s, floa
 }
 
 // -- with a histogram: of 2048 bins of the logits, from the row's largest down, the weights
-// -- and, where top-k is on, the tokens.  Bins are 1/64 of the temperature wide, at most 1/64,
-// -- or where that reaches below the row's least logit, 1/2048 of the row's range: rows of
-// -- nearly equal logits (128256 within 0.2) took 1.3 ms of 0.13 with the fixed width, their
-// -- bins' tokens being more than the list holds.  What is below the last bin is in the last.  The sums say which bins hold a border of a
-// -- filter or the place of u: their tokens (some hundreds, mostly) are taken from the row,
-// -- sorted, and decide.  Between the bins nothing needs an order.  So a row is read three
+// -- and, where top-k is on, the tokens.  Bins are 1/64 of the temperature wide, or where that
+// -- reaches below the row's least logit, 1/2047 of the row's range: 256 rows of nearly equal
+// -- logits (128256 within 0.2) took 1290 us with the fixed width, their bins' tokens being more
+// -- than the list holds, and 112 so.  What is below the last bin is in the last.  A bin's weights
+// -- are within a factor of 1.02 of each other and are added as multiples of a power of two of
+// -- their own; those in the last bin go on down from 2^-46 (where bins go by the range, they end
+// -- with it).  The sums say which bins hold a border of a filter or the place of u: their tokens
+// -- (some hundreds, mostly) are taken from the row, sorted, and decide.  Between the bins nothing needs an order.  So a row is read three
 // -- times: for its largest logit, for the bins, and for those tokens; parts whose largest
 // -- logit is below the bins in question are left out the third time.
 // --
@@ -493,10 +552,11 @@ constexpr int kList = 4096;         // tokens of the bins in question
 constexpr int kSplitBins = 64;      // most bins that are split again
 constexpr int kPeaks = 1024;        // units of a row whose largest logit is kept in LDS
 constexpr int kSplitBlock = 256;
+constexpr float kMask = -4096.0f;   // no model's logit: below it a mask's finite stand-in
 
 struct SampleWork {
     float* peaks;              // [rows][units]: the largest logit of each
-    float* lows;               // [rows][units]: the least one that is not minus infinity
+    float* lows;               // [rows][units]: the least one from kMask on
     unsigned long long* mass;  // [rows][kBins]
     int* count;                // [rows][kBins], where top-k is on
     unsigned long long* list;  // [rows][kList]
@@ -584,34 +644,59 @@ __device__ __forceinline__ float unit_peak(const Unit<T>& x, const typename T::B
     float peak = -__builtin_inff();
     x.each(row, vocab, u, [&](float l, int, int) {
         peak = __builtin_fmaxf(peak, l);
-        low = __builtin_fminf(low, l == -__builtin_inff() ? __builtin_inff() : l);
+        low = __builtin_fminf(low, l < kMask ? __builtin_inff() : l);
     });
     return from_lane(wave_scan(peak, -__builtin_inff(), Max()), kWave - 1);
 }
 
-// Bins per unit of a logit, for a row whose logits are in [low, top].
-__device__ __forceinline__ float bins_of(float wide, float top, float low) {
-    return __builtin_fmaxf(wide, __builtin_fminf((kBins - 1) / (top - low), 0x1p40f));
+// The least logit whose weight is not below e^-64, and no infinite one.
+__device__ __forceinline__ float cut_of(float top, double t) {
+    return __builtin_fmaxf(static_cast<float>(top - 64.0 * t), -0x1.fffffep127f);
 }
 
-// Adds a unit to a histogram in LDS; `cut`: below it (and for a NaN) a weight is 0 as a whole
-// number.
+// The bins of a row whose largest logit is `top`; false if bins do not fit it.  What is below
+// kMask has no part in the range: masks of -1e9 would leave the bins' width as wide as it gets.
+__device__ __forceinline__ bool fit_bins(Settings& s, float top, float low) {
+    // bins below an infinite logit have no width
+    if (__builtin_isinf(top)) return false;
+    // differences of logits that have weights must not overflow
+    if (__builtin_isinf(top - cut_of(top, s.t))) return false;
+    // nor the bins.  A logit of 2^-80 or more is 2^-104 and more from any other: below a
+    // temperature of 2^-114 the others have no weight.
+    if (s.t < 0x1p-114) {
+        if (__builtin_fabsf(top) < 0x1p-80f) return false;
+        s.t = 0x1p-114;
+        s.per = 0x1p114 * kPerUnit;
+    }
+    const float per = static_cast<float>(s.per);
+    s.bins = __builtin_fmaxf(per * 0x1.62e42ep-1f, 0x1p-110f);  // ln 2: 64 a temperature
+    s.bins = __builtin_fmaxf(s.bins, __builtin_fminf((kBins - 1) / (top - low), 0x1p40f));
+    s.octaves = static_cast<uint32_t>(per / s.bins * 0x1p14f);
+    return true;
+}
+
+// The power of two that brings a bin's weights to [0.49, 1.0001].
+__device__ __forceinline__ uint32_t octaves_of(int bin, const Settings& s) {
+    return __umul24(static_cast<uint32_t>(bin), s.octaves);  // 2^-20 of one
+}
+
+// A bin's sum of whole numbers as a weight.
+__device__ __forceinline__ double mass_of(unsigned long long sum, int bin, const Settings& s) {
+    return __builtin_ldexp(static_cast<double>(sum), -s.bits - static_cast<int>(octaves_of(bin, s) >> 20));
+}
+
+// Adds a unit to a histogram in LDS; `cut`: below it (and for a NaN) a weight counts as 0.
 template <class T, bool kCount>
 __device__ __forceinline__ void add_unit(const Unit<T>& x, const typename T::Bits* row, int vocab, int u,
                                          const Settings& s, float top, float cut, const double* powers,
                                          unsigned long long* mass, int* count) {
     x.each(row, vocab, u, [&](float l, int, int) {
-        const double d = (static_cast<double>(l) - static_cast<double>(top)) * s.inv_t;
-        const unsigned long long m = fixed(exp_of(d, powers), s.one);
+        const double y = (static_cast<double>(l) - static_cast<double>(top)) * s.per;
         const int b = bin_of(l, top, s.bins);
+        const unsigned long long m = fixed(power_of(y, octaves_of(b, s) & 0xfff00000u, powers), s.one);
         if (l >= cut) atomicAdd(&mass[b], m);
         if (kCount && l > -__builtin_inff()) atomicAdd(&count[b], 1);
     });
-}
-
-// The least logit whose weight is not below e^-64, and no infinite one.
-__device__ __forceinline__ float cut_of(float top, double inv_t) {
-    return __builtin_fmaxf(static_cast<float>(top - 64.0 / inv_t), -0x1.fffffep127f);
 }
 
 // Few rows: units over blocks.  First their largest logits (1 row of 128256 1.9 us, 32 rows
@@ -677,9 +762,8 @@ __global__ __launch_bounds__(kSplitBlock) void sample_bins_kernel(SampleArgs g, 
         top = __builtin_fmaxf(top, part[0][i]);
         low = __builtin_fminf(low, part[1][i]);
     }
-    if (__builtin_isinf(top)) return;
-    s.bins = bins_of(s.bins, top, low);
-    const float cut = cut_of(top, s.inv_t);
+    if (!fit_bins(s, top, low)) return;
+    const float cut = cut_of(top, s.t);
     each_unit<T>(logits, g.vocab, blockIdx.x * kTogether + tid / kWave, gridDim.x * kTogether, w.units,
                  [](int) { return true; }, [&](const Unit<T>& x, int u) {
                      if (by_count)
@@ -782,6 +866,7 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
     } sums;
     __shared__ uint32_t marked[kBins / 32], marked_parts[kBins / 32];
     __shared__ int slots[kBins / 32];  // marked bins before each word
+    __shared__ int bin_at[kSplitBins + 1];  // and the bin of each
     __shared__ double gap_mass[2][kSplitBins + 1];  // between marked bins: from, to
     __shared__ int gap_count[2][kSplitBins + 1];
     __shared__ int listed, found[5], heaviest_bin, base;
@@ -821,11 +906,10 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
         }
         return;
     }
-    if (top == __builtin_inff()) {  // bins below an infinite logit have no width
+    if (!fit_bins(s, top, low)) {
         if (q == 0) sample_row<T>(g, row, s, top, powers, u.hist);
         return;
     }
-    s.bins = bins_of(s.bins, top, low);
     // kOwn neighbouring bins a thread
     double mine[kOwn];
     int mine_count[kOwn] = {};
@@ -835,7 +919,7 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
             if (by_count) count[b] = 0;
         }
         __syncthreads();
-        const float cut = cut_of(top, s.inv_t);
+        const float cut = cut_of(top, s.t);
         each_unit<T>(logits, g.vocab, wave, kWaves, w.units, all_units, [&](const Unit<T>& x, int u) {
             if (by_count)
                 add_unit<T, true>(x, logits, g.vocab, u, s, top, cut, powers, masses.fixed, count);
@@ -847,7 +931,7 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
 #pragma unroll
     for (int h = 0; h < kOwn; ++h) {
         const long at = static_cast<long>(row) * kBins + own + h;
-        mine[h] = static_cast<double>(kWhole ? masses.fixed[own + h] : w.mass[at]) / s.unit;
+        mine[h] = mass_of(kWhole ? masses.fixed[own + h] : w.mass[at], own + h, s);
         if (by_count) mine_count[h] = kWhole ? count[own + h] : w.count[at];
     }
     // A bin's place among the marked ones, once they are split.
@@ -971,7 +1055,7 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
         }
         p_bin = kBins;  // the last bin that min-p may keep a part of
         if (s.min_p > 0.0) {
-            const double x = -log(s.min_p) / s.inv_t * s.bins;
+            const double x = -log(s.min_p) * s.t * s.bins;
             const double off = 1e-6 + 3e-7 * x;  // a logit's place among the bins is float32
             const int first = place_of(static_cast<float>(__builtin_fmax(x - off, 0.0)));
             p_bin = place_of(static_cast<float>(x + off));
@@ -1076,6 +1160,7 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
                 const int b = own + h;
                 if (!(marked[b / 32] >> (b % 32) & 1)) continue;
                 const int slot = slot_of(b);
+                bin_at[slot] = b;
                 gap_mass[1][slot] = mass[b];
                 gap_count[1][slot] = count[b];
                 gap_mass[0][slot + 1] = mass[b + 1];
@@ -1099,14 +1184,16 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
                 keep[e] = u.list[i];
                 const float l = from_key(~static_cast<uint32_t>(keep[e] >> 32));
                 const int b = place_of((top - l) * s.bins);
-                atomicAdd(&masses.fixed[b], fixed(weight_of(l, top, s.inv_t, powers), s.one));
+                const int up = octaves_of(bin_of(l, top, s.bins), s) >> 20;
+                const double weight = __builtin_ldexp(weight_of(l, top, s.per, powers), up);
+                atomicAdd(&masses.fixed[b], fixed(weight, s.one));
                 atomicAdd(&count[b], 1);
             }
             __syncthreads();
 #pragma unroll
             for (int h = 0; h < kOwn; ++h) {
                 const int b = own + h, slot = b / parts_of_bin;
-                mine[h] = static_cast<double>(masses.fixed[b]) / s.unit;
+                mine[h] = slot < many ? mass_of(masses.fixed[b], bin_at[slot], s) : 0.0;
                 mine_count[h] = count[b];
                 if (slot * parts_of_bin == b && slot <= many) {
                     mine[h] += gap_mass[1][slot] - gap_mass[0][slot];
@@ -1141,7 +1228,7 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
     auto each_listed = [&](double before, auto f) {
         for (int i = first; i < behind; ++i) {
             const float l = from_key(~static_cast<uint32_t>(u.list[i] >> 32));
-            const double weight = weight_of(l, top, s.inv_t, powers);
+            const double weight = weight_of(l, top, s.per, powers);
             f(i, weight, place_of((top - l) * s.bins), before);
             before += weight;
         }
@@ -1188,7 +1275,7 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
     g.tokens[row] = static_cast<int>(static_cast<uint32_t>(token));
     if (g.logprobs)
         g.logprobs[row] = static_cast<float>(
-            log(weight_of(from_key(~static_cast<uint32_t>(token >> 32)), top, s.inv_t, powers) / kept));
+            log(weight_of(from_key(~static_cast<uint32_t>(token >> 32)), top, s.per, powers) / kept));
 }
 
 // Most rows that are split: the workspace is bounded.
