@@ -1407,6 +1407,15 @@ struct Sum {
     static __device__ __forceinline__ double less(float low, float high) {
         return __builtin_amdgcn_exp2f((low - high) * 0x1.715476p+0f);
     }
+    // Before a unit with the largest logit `peak`.  In float64: a row that rises slowly comes here
+    // for each unit, with the same difference each time, and 2048 float32 roundings to the same
+    // side (2^24 tokens rising by 0.2) put a log-probability off by 6e-6.
+    __device__ __forceinline__ void raise(float peak, int own) {
+        if (!(peak > top)) return;
+        if (top != -__builtin_inff()) rest = (rest + own) * exp(static_cast<double>(top) - peak);
+        top = peak;
+        count = 0;
+    }
 };
 
 struct LogprobWork {
@@ -1424,11 +1433,7 @@ __device__ __forceinline__ float sum_unit(Sum& s, const Unit<T>& x, const typena
     x.each(row, vocab, u, [&](float l, int, int) { peak = __builtin_fmaxf(peak, l); });
     peak = from_lane(wave_scan(peak, -__builtin_inff(), Max()), kWave - 1);
     if (peak == -__builtin_inff()) return peak;
-    if (peak > s.top) {
-        s.rest = (s.rest + (threadIdx.x % kWave == 0 ? s.count : 0)) * Sum::less(s.top, peak);
-        s.top = peak;
-        s.count = 0;
-    }
+    s.raise(peak, threadIdx.x % kWave == 0 ? s.count : 0);
     const bool has = peak == s.top;
     float w[16];
     int equal = 0;
@@ -1522,11 +1527,7 @@ __global__ __launch_bounds__(kRow) void logprob_kernel(LogprobArgs g, LogprobWor
             const Sum o = w.sums[static_cast<long>(row) * w.units + u];
             peak_of(u, o.top);
             if (o.top == -__builtin_inff()) continue;
-            if (o.top > s.top) {
-                s.rest = (s.rest + s.count) * Sum::less(s.top, o.top);
-                s.top = o.top;
-                s.count = 0;
-            }
+            s.raise(o.top, s.count);
             s.rest += o.top == s.top ? o.rest : (o.rest + o.count) * Sum::less(o.top, s.top);
             s.count += o.top == s.top ? o.count : 0;
         }

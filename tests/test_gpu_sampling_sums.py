@@ -187,3 +187,23 @@ def test_logits_and_temperatures_at_the_ends_of_the_range(gpu, rows, vocab):
         token, lp = run(x.cuda().repeat(rows, 1), [u] * rows, temperature=t)
         assert token == token[:1] * rows and lp == lp[:1] * rows
         Row(R.f64(x), t).check(u, token[0], lp[0], note=(t, vocab))
+
+
+@pytest.mark.parametrize("vocab,rise", [(128256, 0.5), (1100003, 0.01), (1100003, 0.1), (1100003, 0.3),
+                                        (1100003, 0.7), (1100003, 20.0), (1 << 24, 0.2)])
+@pytest.mark.parametrize("rows", [3, 194])
+def test_logprobs_in_slowly_rising_rows(gpu, rows, vocab, rise):
+    """The largest logit so far changes with every 1024 of a row, in one block or in several."""
+    x = torch.linspace(0.0, rise, vocab)
+    tokens = torch.tensor([0, vocab // 2, vocab - 1] * rows, dtype=torch.int32)[:rows]
+    got = S.logprobs(x, tokens, 2, logits_gpu=x.cuda().repeat(rows, 1))
+    for v in got:  # alike in all rows of a token
+        assert torch.equal(v[3:], v[:-3])
+    want, err, best = R.logprobs(R.f64(x), 2)
+    lp, ids, values = (v.cpu() for v in got)
+    for i in range(3):
+        t = int(tokens[i])
+        assert abs(float(lp[i]) - want[t]) <= err[t], (t, float(lp[i]), want[t], err[t])
+        assert ids[i].tolist() == best.tolist()
+        for j, b in enumerate(best):
+            assert abs(float(values[i, j]) - want[b]) <= err[b], (j, float(values[i, j]), want[b], err[b])
