@@ -545,8 +545,8 @@ typedef struct spb_adapters {
 /* output[t] = base[t] + scales[i] * B_i (A_i x[t]) with i = ids[t] (device int32):
  * base is what the shared projection gave for x.  A token whose id is outside
  * [0, num_adapters) has no adapter: its output is base.  Both products accumulate in
- * float32; the inner one is kept in float32 or as two 16-bit numbers, and the output
- * is rounded once.  base == output adds in place (same stride); other overlaps of
+ * float32; the inner one is kept as its float32 sum, in fp16 to 2^-22 of that (2^-38 of
+ * the token's largest, if that is more), and the output is rounded once.  base == output adds in place (same stride); other overlaps of
  * output are not allowed.  x 16-byte aligned, x_stride a multiple of 8.
  * num_tokens <= 2^20; the workspace of more tokens serves fewer. */
 size_t spb_adapters_workspace_size(const spb_adapters* adapters, int num_tokens);

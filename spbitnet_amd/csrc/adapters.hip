@@ -162,24 +162,38 @@ __device__ __forceinline__ void copy_idle(const Args& g, int window, uint64_t id
     }
 }
 
-// Inner products of 8 depths of one token as two 16-bit numbers each, h = (hi + lo) * unit:
-// their sum is within 2^-16 (bf16) or 2^-22 (fp16) of h, so the second product is as exact as
-// the first.  fp16's range is made up for by a power of two for the token.
+// Inner products of 8 depths of one token as 16-bit numbers, h = (the parts' sum) * unit.  bf16:
+// three, each the first 8 bits of what those before it leave, so they are the float32 number; two
+// were off by 2^-18, as much as shows where two of them nearly cancel, and took 0.1 us of 7.6
+// less (one token) and 0.5 of 59.6 (2049).  fp16: two, which are within 2^-22 of h, or 2^-38 of
+// the token's largest where that is more; its range is made up for by a power of two for the token.
 template <class T>
-struct Pair {
-    uint4 hi, lo;
+struct Parts {
+    static constexpr int kMany = std::is_same_v<T, BF16> ? 3 : 2;
+    uint4 v[kMany];
     __device__ __forceinline__ void set(const float (&h)[8], float by) {
-        uint16_t a[8], b[8];
+        uint16_t a[kMany][8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float v = h[e] * by;
-            a[e] = T::from_float(v);
-            const float rest = v - T::to_float(a[e]);
-            b[e] = T::from_float(__builtin_isfinite(v) ? rest : 0.0f);
+            if constexpr (std::is_same_v<T, BF16>) {
+                float rest = h[e];
+#pragma unroll
+                for (int n = 0; n < kMany; ++n) {
+                    const uint32_t first = __builtin_bit_cast(uint32_t, rest) & 0xffff0000u;
+                    a[n][e] = static_cast<uint16_t>(first >> 16);
+                    rest = __builtin_isfinite(h[e]) ? rest - __builtin_bit_cast(float, first) : 0.0f;
+                }
+            } else {
+                const float v = h[e] * by;
+                a[0][e] = T::from_float(v);
+                const float rest = v - T::to_float(a[0][e]);
+                a[1][e] = T::from_float(__builtin_isfinite(v) ? rest : 0.0f);
+            }
         }
         auto two = [](uint16_t x, uint16_t y) { return static_cast<uint32_t>(y) << 16 | x; };
-        hi = {two(a[0], a[1]), two(a[2], a[3]), two(a[4], a[5]), two(a[6], a[7])};
-        lo = {two(b[0], b[1]), two(b[2], b[3]), two(b[4], b[5]), two(b[6], b[7])};
+#pragma unroll
+        for (int n = 0; n < kMany; ++n)
+            v[n] = {two(a[n][0], a[n][1]), two(a[n][2], a[n][3]), two(a[n][4], a[n][5]), two(a[n][6], a[n][7])};
     }
 };
 
@@ -315,10 +329,10 @@ __global__ __launch_bounds__(kFusedWaves* kWave, 4) void fused_kernel(Args g) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 if (k * kStep >= r) break;
-                Pair<T> p;
+                Parts<T> p;
                 p.set(h[k], by);
-                sum = Matrix<T>::mac(up[k], p.hi, sum);
-                sum = Matrix<T>::mac(up[k], p.lo, sum);
+#pragma unroll
+                for (int n = 0; n < Parts<T>::kMany; ++n) sum = Matrix<T>::mac(up[k], p.v[n], sum);
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -420,7 +434,8 @@ template <class T, bool kPasses>
 __global__ __launch_bounds__(kWaves* kWave) void expand_kernel(Args g) {
     constexpr int kHeld = kPasses ? 32 : kWindow;  // tokens in LDS
     constexpr int kWidth = kPasses ? kMaxRank + 8 : kPart + 8;
-    __shared__ uint16_t hi[kHeld][kWidth], lo[kHeld][kWidth];
+    constexpr int kMany = Parts<T>::kMany;
+    __shared__ uint16_t inner[kMany][kHeld][kWidth];
     __shared__ int shifts[kHeld];
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const int col = lane % kTile, quad = lane / kTile, all = g.sections * g.rank;
@@ -500,10 +515,10 @@ __global__ __launch_bounds__(kWaves* kWave) void expand_kernel(Args g) {
             for (int i = 0; i < kTurns; ++i) {
                 const int k = (i * kThreads + tid % kThreads) * 8;
                 if (k >= (r + kStep - 1) / kStep * kStep) continue;
-                Pair<T> p;
+                Parts<T> p;
                 p.set(h[i], __builtin_ldexpf(1.0f, shift));
-                *reinterpret_cast<uint4*>(&hi[slot][k]) = p.hi;
-                *reinterpret_cast<uint4*>(&lo[slot][k]) = p.lo;
+#pragma unroll
+                for (int n = 0; n < kMany; ++n) *reinterpret_cast<uint4*>(&inner[n][slot][k]) = p.v[n];
             }
             if (tid % kThreads == 0) shifts[slot] = shift;
             __syncthreads();
@@ -517,13 +532,14 @@ __global__ __launch_bounds__(kWaves* kWave) void expand_kernel(Args g) {
                     for (int k = 0; k < 2; ++k) {
                         if (first + k * kStep >= r) break;
                         const int depth = first + k * kStep + quad * 8;
-                        const uint4 u = *reinterpret_cast<const uint4*>(&hi[n + col][depth]);
-                        const uint4 v = *reinterpret_cast<const uint4*>(&lo[n + col][depth]);
+                        uint4 u[kMany];
 #pragma unroll
-                        for (int m = 0; m < 4; ++m) {
-                            acc[m] = Matrix<T>::mac(up[k][m], u, acc[m]);
-                            acc[m] = Matrix<T>::mac(up[k][m], v, acc[m]);
-                        }
+                        for (int i = 0; i < kMany; ++i)
+                            u[i] = *reinterpret_cast<const uint4*>(&inner[i][n + col][depth]);
+#pragma unroll
+                        for (int m = 0; m < 4; ++m)
+#pragma unroll
+                            for (int i = 0; i < kMany; ++i) acc[m] = Matrix<T>::mac(up[k][m], u[i], acc[m]);
                     }
                     if (!kPasses) break;
                 }

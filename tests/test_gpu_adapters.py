@@ -300,3 +300,41 @@ def test_own_stream(gpu):
     K.adapters_gpu(ad, d["ids"], d["x"], d["base"], out, ws, stream=s)
     s.synchronize()
     close(out, d)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("tokens,rank", [(1, 8), (5, 16), (40, 64), (90, 40), (300, 200), (1100, 16)])
+def test_differences_of_near_inner_products(gpu, kind, tokens, rank):
+    """Inner products of 24 bits whose last ones differ, each exact in float32, and a B that
+    subtracts two of them, exact in float32 too.  fp16 holds them to 2^-22, bf16 as they are,
+    and the output is rounded once."""
+    dt, num, rows, cols = HALF[kind], 3, rank + 7, 64
+    g = torch.Generator().manual_seed(tokens)
+
+    def odd(*shape):  # odd numbers of 7 and 8 bits
+        return (torch.randint(32, 112, shape, generator=g) * 2 + 1).double()
+    a, x = torch.zeros(num, rank, cols, dtype=torch.float64), torch.zeros(tokens, cols, dtype=torch.float64)
+    a[:, :, 3] = odd(num, 1)
+    a[:, :, 50] = (odd(num, 1) + 2 * torch.randint(0, 15, (num, rank), generator=g)) / 256
+    x[:, 3], x[:, 50] = odd(tokens), odd(tokens) * (torch.randint(0, 2, (tokens,), generator=g) * 2 - 1)
+    b = torch.zeros(num, rows, rank, dtype=torch.float64)
+    one, two = torch.arange(rows) % rank, (torch.arange(rows) + 1) % rank
+    b[:, torch.arange(rows), one] = 1.0 / 256
+    b[:, torch.arange(rows), two] = -1.0 / 256
+    ids = [t % (num + 1) - 1 if tokens > 1 else 1 for t in range(tokens)]
+    h = torch.matmul(a, x.t()).transpose(1, 2) / 256  # [adapter][token][rank]
+    at = torch.tensor(ids).clamp_min(0), torch.arange(tokens)
+    live = torch.tensor([[float(i >= 0)] for i in ids])
+    h1, h2 = h[at][:, one] * live, h[at][:, two] * live
+    assert torch.equal(h.float().double(), h) and torch.equal((h1 - h2).float().double(), h1 - h2)
+    d = dict(a=a.to(dt).cuda(), b=b.to(dt).cuda(), scales=torch.ones(num).cuda(), ranks=None, sections=(rows,),
+             ids=torch.tensor(ids, dtype=torch.int32).cuda(), x=x.to(dt).cuda(),
+             base=torch.zeros(tokens, rows, dtype=dt, device="cuda"))
+    for name, v in (("a", a), ("b", b), ("x", x)):
+        assert torch.equal(d[name].cpu().double(), v), name  # all of it is exact in the type
+    want = (h1 - h2).numpy()
+    held = (h1.abs() + h2.abs()).numpy() * (2.0 ** -22 if kind == "f16" else 0.0)
+    err = held * (1 + R.HALF_STEP[dt]) + R.HALF_STEP[dt] * np.abs(want) + R.SMALLEST[dt]
+    got = R.f64(run(d))
+    assert (np.abs(got - want) <= err).all(), np.abs(got - want).max()
+    assert np.abs(want).max() > 0
