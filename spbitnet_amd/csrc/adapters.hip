@@ -197,11 +197,17 @@ struct Parts {
     }
 };
 
+// The larger of `most` and a finite h: beside an infinite one the others must stay finite too.
+__device__ __forceinline__ float larger(float most, float h) {
+    const float size = __builtin_fabsf(h);
+    return size < __builtin_inff() ? __builtin_fmaxf(most, size) : most;
+}
+
 // The power of two that brings a token's inner products, at most `most`, below 2^14.
 template <class T>
 __device__ __forceinline__ int shift_of(float most) {
     if constexpr (std::is_same_v<T, BF16>) return 0;
-    if (!(most > 0.0f) || !__builtin_isfinite(most)) return 0;
+    if (!(most > 0.0f)) return 0;
     const int exponent = static_cast<int>(__builtin_bit_cast(uint32_t, most) >> 23 & 255) - 126;
     return min(14 - exponent, 100);
 }
@@ -319,7 +325,7 @@ __global__ __launch_bounds__(kFusedWaves* kWave, 4) void fused_kernel(Args g) {
                 for (int e = 0; e < 8; ++e) {
                     const int j = k * kStep + quad * 8 + e;
                     h[k][e] = j < r ? total[col][j] : 0.0f;
-                    most = __builtin_fmaxf(most, __builtin_fabsf(h[k][e]));
+                    most = larger(most, h[k][e]);
                 }
             most = __builtin_fmaxf(most, __shfl_xor(most, 16, kWave));
             most = __builtin_fmaxf(most, __shfl_xor(most, 32, kWave));
@@ -502,7 +508,7 @@ __global__ __launch_bounds__(kWaves* kWave) void expand_kernel(Args g) {
                 }
                 if (std::is_same_v<T, F16>)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) most = __builtin_fmaxf(most, __builtin_fabsf(h[i][e]));
+                    for (int e = 0; e < 8; ++e) most = larger(most, h[i][e]);
             }
             int shift = 0;
             if (std::is_same_v<T, F16>) {

@@ -338,3 +338,22 @@ def test_differences_of_near_inner_products(gpu, kind, tokens, rank):
     got = R.f64(run(d))
     assert (np.abs(got - want) <= err).all(), np.abs(got - want).max()
     assert np.abs(want).max() > 0
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("tokens,rank", [(2, 16), (90, 16), (90, 128)])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_an_infinite_inner_product_beside_large_ones(gpu, kind, tokens, rank, bad):
+    """The others are past fp16's range and of the other sign: the output is still infinite."""
+    d = make(kind, tokens, 64, (40,), rank, 2, [t % 2 for t in range(tokens)], seed=1)
+    d["scales"].fill_(1.0)
+    d["x"].fill_(1.0)
+    d["b"].fill_(0.5)
+    d["a"].fill_(-3e4)  # inner products of -1.9e6
+    if bad < 0:
+        d["a"].fill_(3e4)
+    d["a"][1, 5, 9] = bad
+    got = run(d)
+    other = run(dict(d, ids=torch.zeros_like(d["ids"])))
+    assert torch.equal(got[0::2].view(torch.int16), other[0::2].view(torch.int16))
+    assert torch.isnan(got[1::2]).all() if bad != bad else bool((got[1::2] == bad).all()), got[1, :4]
