@@ -622,19 +622,29 @@ int check_tokens(const char* fn, int tokens) {
 
 constexpr int kFewWindows = 16;
 
-// 2^n blocks split the columns of the inner products: 512 blocks and more, two a CU, while the
-// outer products' reading of the parts does not cost more.  gate|up of 2560 columns, rank 32:
-// 2049 tokens 46.9 us by 4, 50.9 by 2, 57.9 by 8; 4096 86.6 by 4, 79.4 by 2; 1100 34.2 by 4,
-// 40.0 by 8.
+// 2^n blocks split the columns of the inner products of up to kSplitWindows[n] windows, the
+// largest such n: 512 blocks and more, two a CU, while the outer products' reading of the parts
+// does not cost more.  gate|up of 2560 columns, rank 32: 2049 tokens 46.9 us by 4, 50.9 by 2, 57.9
+// by 8; 4096 86.6 by 4, 79.4 by 2; 1100 34.2 by 4, 40.0 by 8.
+constexpr int kSplitWindows[] = {kMaxSize / kWindow, 127, 63, kFewWindows};
+constexpr int kMostSplitBits = 3;
+
 int split_bits_of(int tokens) {
     const int windows = (tokens + kWindow - 1) / kWindow;
-    return windows <= kFewWindows ? 3 : windows < 64 ? 2 : windows < 128 ? 1 : 0;
+    int bits = kMostSplitBits;
+    while (bits > 0 && windows > kSplitWindows[bits]) --bits;
+    return bits;
 }
 
-// What the splits of n tokens times n come to for no n up to `tokens` is more than this.
+// Of the most parts that up to `tokens` tokens have, for a workspace serves fewer too.
 size_t workspace_size(const spb_adapters& d, int tokens) {
-    const size_t n = tokens, rows = n * 8 < 16384 ? n * 8 : n > 16384 ? n : 16384;
-    return sizeof(float) * d.num_sections * d.rank * rows;
+    size_t most = 0;
+    for (int bits = 0; bits <= kMostSplitBits; ++bits) {
+        const int end = kSplitWindows[bits] * kWindow;
+        const size_t parts = static_cast<size_t>(tokens < end ? tokens : end) << bits;
+        most = parts > most ? parts : most;
+    }
+    return sizeof(float) * d.num_sections * d.rank * most;
 }
 
 // One launch where every CU has a block at most, and A is small: each block reads its section's

@@ -357,3 +357,21 @@ def test_an_infinite_inner_product_beside_large_ones(gpu, kind, tokens, rank, ba
     other = run(dict(d, ids=torch.zeros_like(d["ids"])))
     assert torch.equal(got[0::2].view(torch.int16), other[0::2].view(torch.int16))
     assert torch.isnan(got[1::2]).all() if bad != bad else bool((got[1::2] == bad).all()), got[1, :4]
+
+
+@pytest.mark.parametrize("kind,rank", [("bf16", 8), ("f16", 72)])
+@pytest.mark.parametrize("tokens", [1024, 1025, 4032, 4033, 8128, 8129, 16384, 16385])
+def test_ends_of_the_workspace_where_the_split_changes(gpu, tokens, kind, rank):
+    """Tokens of one window more or less than go by 8, 4, 2 and 1 parts, a workspace of just
+    the size that is asked for, and the same workspace for fewer of them."""
+    d = make(kind, tokens, 16, (24, 9), rank, 3, None, seed=tokens)
+    ad = handle(d)
+    size, guard = K.adapters_workspace_size(ad, tokens), 1 << 20
+    ws = torch.full((size + guard,), 0x5A, dtype=torch.uint8, device="cuda")
+    for n in (tokens, 1024, 1000):
+        out = torch.full_like(d["base"][:n], float("nan"))
+        assert K.adapters_workspace_size(ad, n) <= size
+        K.adapters_gpu(ad, d["ids"][:n], d["x"][:n], d["base"][:n], out, ws[:size])
+        torch.cuda.synchronize()
+        assert bool((ws[size:] == 0x5A).all())
+        close(out, dict(d, ids=d["ids"][:n], x=d["x"][:n], base=d["base"][:n]), note=n)
