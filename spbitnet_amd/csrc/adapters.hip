@@ -215,7 +215,7 @@ __device__ __forceinline__ int shift_of(float most) {
 // -- few tokens: both products in one launch.  A block has 128 rows of the output and an
 // -- adapter's tokens of a window, and makes the inner products that it needs by itself: its
 // -- 8 waves split the columns and add up in LDS.  One token, rank 16 on q|k|v of 2560 columns:
-// -- 6.8 us of the kernel, 7.5 a call, for 0.4 MB: bound by dependent steps (ids, A and x, B)
+// -- 6.9 us of the kernel, 7.6 a call, for 0.4 MB: bound by dependent steps (ids, A and x, B)
 // -- and the fetch of the code.
 
 constexpr int kFusedWaves = 8, kFusedRows = kFusedWaves * kTile;
@@ -363,7 +363,7 @@ constexpr int kRows = kWaves * 64;  // rows of a block of the second
 // code, which a launch finds in no cache of its CU: one loop, two bodies.  kDeep products'
 // loads are in flight together: 2 where windows are few, and the code's fetch counts (32
 // tokens of up to 20 adapters, rank 16, q|k|v of 2560: 5.3 us, with 5 6.5), 5 else (2049 tokens,
-// rank 32: 14.5 us, with 2 18.0; x is 10 MB, A 1.6).
+// rank 32: 14.4 us, with 2 18.0, with x (10 MB) and A (1.6 MB) in the last cache; 16.7 without).
 template <class T, int kDeep>
 __global__ __launch_bounds__(kWaves* kWave) void shrink_kernel(Args g) {
     __shared__ float part[kWaves][kTile][kPad];
@@ -434,8 +434,9 @@ __global__ __launch_bounds__(kWaves* kWave) void shrink_kernel(Args g) {
 // products so that a lane's results of two are 8 neighbours, and with its three neighbours'
 // 64 bytes of a token's output.  The adapter's part of B stays in registers, up to 64 ranks;
 // more go in passes for every 16 tokens.  2049 tokens, rank 32 on gate|up of 6912 rows each:
-// 33.9 us for 113 MB of base and output and the 4 parts of the inner products, 3.4 TB/s; up to 20
-// adapters over 32 tokens, rank 16 on q|k|v: 7.4 us, bound as the kernel above.
+// 44.5 us for 113 MB of base and output and the 4 parts of the inner products, 2.5 TB/s, or 35.0
+// with all of it in the last cache; up to 20 adapters over 32 tokens, rank 16 on q|k|v: 7.3 us,
+// bound as the kernel above.
 template <class T, bool kPasses>
 __global__ __launch_bounds__(kWaves* kWave) void expand_kernel(Args g) {
     constexpr int kHeld = kPasses ? 32 : kWindow;  // tokens in LDS
@@ -624,8 +625,9 @@ constexpr int kFewWindows = 16;
 
 // 2^n blocks split the columns of the inner products of up to kSplitWindows[n] windows, the
 // largest such n: 512 blocks and more, two a CU, while the outer products' reading of the parts
-// does not cost more.  gate|up of 2560 columns, rank 32: 2049 tokens 46.9 us by 4, 50.9 by 2, 57.9
-// by 8; 4096 86.6 by 4, 79.4 by 2; 1100 34.2 by 4, 40.0 by 8.
+// does not cost more.  gate|up of 2560 columns, rank 32, the same inputs again and again (they
+// fit the last cache; others take 59.6 of the first 46.9): 2049 tokens 46.9 us by 4, 50.9 by 2,
+// 57.9 by 8; 4096 86.6 by 4, 79.4 by 2; 1100 34.2 by 4, 40.0 by 8.
 constexpr int kSplitWindows[] = {kMaxSize / kWindow, 127, 63, kFewWindows};
 constexpr int kMostSplitBits = 3;
 

@@ -388,7 +388,7 @@ __device__ __forceinline__ Place select(const Row<T>& r, int rank, double bound,
             if (shift < 24 && (key >> (shift + 8)) != (prefix >> (shift + 8))) return;
             const int d = key >> shift & 255;
             // equal logits are added by one lane: a row of 128256 times one value took 1000 us
-            // with each lane adding its own, 450 so
+            // with each lane adding its own, 440 so
             const bool led = key == __builtin_amdgcn_readfirstlane(key);
             const unsigned long long same = __ballot(led);
             const int times = led ? __popcll(same) : 1;
@@ -541,10 +541,15 @@ __device__ __forceinline__ void sample_row(const SampleArgs& g, int row, const S
 // -- times: for its largest logit, for the bins, and for those tokens; parts whose largest
 // -- logit is below the bins in question are left out the third time.
 // --
-// -- 512 rows of 128256 float32 logits, top-p 0.95, a block a row: 170 us, of them 33 for the
-// -- largest logits (memory, 8 TB/s: the rows fit the last cache mostly), 65 for the bins (issue
-// -- of the weights' float64), 36 for the tokens in question (memory), 11 for sorting them and
-// -- the end.  The two blocks of a CU go through them in step.
+// -- 512 rows of 128256 float32 logits, top-p 0.95, a block a row: 168 us.  Mean of the blocks: 42
+// -- for the largest logits (memory, 6 TB/s), 63 for the bins (issue of the weights' float64), 3 for
+// -- their sums and borders, 34 for the tokens in question (memory), 11 for sorting them and the end,
+// -- 152 in all; the slowest one's bins take 80.  The two blocks of a CU go through them in step.
+// --
+// -- A bin of thousands of equal logits overflows the list and leaves the row to the selection
+// -- above.  16-bit logits have such bins in flat rows: bfloat16 ones between 8 and 16 are 1/16
+// -- apart.  512 flat bfloat16 rows of 128256 take 1.1 ms (float32 0.17, fp16 0.17), of 200000 at a
+// -- temperature of 1.5 2.3 ms (float32 0.28).
 
 constexpr int kBins = 2048;
 constexpr int kOwn = kBins / kRow;  // bins of a thread
@@ -699,8 +704,8 @@ __device__ __forceinline__ void add_unit(const Unit<T>& x, const typename T::Bit
     });
 }
 
-// Few rows: units over blocks.  First their largest logits (1 row of 128256 1.9 us, 32 rows
-// 4.3) ...
+// Few rows: units over blocks.  First their largest logits (1 row of 128256 2.0 us, 32 rows
+// 4.2) ...
 template <class T>
 __global__ __launch_bounds__(kSplitBlock) void sample_peaks_kernel(SampleArgs g, SampleWork w) {
     const int row = blockIdx.y, tid = threadIdx.x;
@@ -726,7 +731,7 @@ __global__ __launch_bounds__(kSplitBlock) void sample_peaks_kernel(SampleArgs g,
     }
 }
 
-// ... then the histogram, added up in LDS and from there in memory (6.5 and 14.6 us: clearing,
+// ... then the histogram, added up in LDS and from there in memory (5.9 and 14.5 us: clearing,
 // the float64 weights, and additions in memory past L2) ...
 template <class T>
 __global__ __launch_bounds__(kSplitBlock) void sample_bins_kernel(SampleArgs g, SampleWork w) {
@@ -838,7 +843,7 @@ __device__ __forceinline__ void sort_list(unsigned long long* list, int n) {
     __syncthreads();
 }
 
-// ... and the token of a row (12.6 and 26.5 us: a chain of dependent steps, a barrier each, and
+// ... and the token of a row (11.8 and 25.4 us: a chain of dependent steps, a barrier each, and
 // the fetch of their code).  kWhole: all of it by this block; else from the histogram in memory,
 // the tokens in question gathered by w.parts blocks.
 template <class T, bool kWhole>
@@ -1458,8 +1463,8 @@ __device__ __forceinline__ unsigned long long rank_key(float l, int index) {
     return static_cast<unsigned long long>(~key_of(l)) << 32 | static_cast<uint32_t>(index);
 }
 
-// Few rows: a wave has a unit, and another kernel adds up.  1 row of 128256 2.4 us and 14.5 in
-// the other (20 alternatives), 32 rows 4.0 and 10.4 (5).
+// Few rows: a wave has a unit, and another kernel adds up.  1 row of 128256 2.2 us and 14.5 in
+// the other (20 alternatives), 32 rows 3.8 and 10.6 (5).
 template <class T>
 __global__ __launch_bounds__(kSplitBlock) void logprob_units_kernel(LogprobArgs g, LogprobWork w) {
     const int row = blockIdx.y;
@@ -1480,12 +1485,14 @@ __global__ __launch_bounds__(kSplitBlock) void logprob_units_kernel(LogprobArgs 
 // The likeliest are in the `top` groups of units with the largest logits (equal ones: the
 // first), for any other group has `top` tokens before its own.  These groups are read again,
 // and their tokens from the last of those logits on are sorted: a few more than `top`, mostly.
-// Where they are many (a row in rising order), the same is done with lanes for groups: at
-// most 16 of each of `top` lanes are left.
+// Where they are many, the same is done with lanes for groups: at most 16 of each of `top` lanes
+// are left.  They are many in a row in rising order, and wherever a row has fewer groups than
+// alternatives are asked for (vocabularies up to 1024 (top - 1)), for then the groups say nothing:
+// 20 of 16384 tokens take 67 us for 1 row, 70 for 256, of 20480 18 and 23; 64 of 32003 76 and 86.
 //
-// 2048 rows of 128256 float32 logits, 5 alternatives: 207 us for 1.05 GB, 5.1 TB/s, what a copy
-// reaches; the row's few groups are read again from the caches.  1023 rows of 32003 bf16: 22 us,
-// 3.0 TB/s: rows of 64 KB, whose start and end (launch, sums over the block) show.
+// 2048 rows of 128256 float32 logits, 5 alternatives: 209 us for 1.05 GB, 5.0 TB/s, what a copy
+// reaches; the row's few groups are read again from the caches.  1023 rows of 32003 bf16: 22.5 us,
+// 2.9 TB/s: rows of 64 KB, whose start and end (launch, sums over the block) show.
 template <class T, bool kWhole>
 __global__ __launch_bounds__(kRow) void logprob_kernel(LogprobArgs g, LogprobWork w) {
     __shared__ uint32_t peaks[kGroups];
