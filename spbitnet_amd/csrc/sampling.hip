@@ -561,7 +561,7 @@ constexpr float kMask = -4096.0f;   // no model's logit: below it a mask's finit
 
 struct SampleWork {
     float* peaks;              // [rows][units]: the largest logit of each
-    float* lows;               // [rows][units]: the least one from kMask on
+    float* lows;               // [rows][units]: the least one (Lows)
     unsigned long long* mass;  // [rows][kBins]
     int* count;                // [rows][kBins], where top-k is on
     unsigned long long* list;  // [rows][kList]
@@ -642,16 +642,33 @@ __device__ __forceinline__ int bin_of(float l, float top, float bins) {
     return static_cast<int>(__builtin_fminf((top - l) * bins, kBins - 1.0f));
 }
 
+// A row's least logits but minus infinity: of those from kMask on, and of the parts that have
+// none of these.
+struct Lows {
+    float near = __builtin_inff(), deep = __builtin_inff();
+
+    __device__ __forceinline__ void add(float low) {  // a part's
+        near = __builtin_fminf(near, low < kMask ? __builtin_inff() : low);
+        deep = __builtin_fminf(deep, low);
+    }
+    __device__ __forceinline__ float of(float top) const { return top < kMask ? deep : near; }
+};
+
 // The largest logit of a unit, the same for all, and to a lane's `low` the least of its own.
 template <class T>
 __device__ __forceinline__ float unit_peak(const Unit<T>& x, const typename T::Bits* row, int vocab, int u,
-                                           float& low) {
+                                           Lows& low) {
     float peak = -__builtin_inff();
     x.each(row, vocab, u, [&](float l, int, int) {
         peak = __builtin_fmaxf(peak, l);
-        low = __builtin_fminf(low, l < kMask ? __builtin_inff() : l);
+        low.near = __builtin_fminf(low.near, l < kMask ? __builtin_inff() : l);
     });
-    return from_lane(wave_scan(peak, -__builtin_inff(), Max()), kWave - 1);
+    peak = from_lane(wave_scan(peak, -__builtin_inff(), Max()), kWave - 1);
+    if (peak < kMask)
+        x.each(row, vocab, u, [&](float l, int, int) {
+            low.deep = __builtin_fminf(low.deep, l == -__builtin_inff() ? __builtin_inff() : l);
+        });
+    return peak;
 }
 
 // The least logit whose weight is not below e^-64, and no infinite one.
@@ -660,7 +677,8 @@ __device__ __forceinline__ float cut_of(float top, double t) {
 }
 
 // The bins of a row whose largest logit is `top`; false if bins do not fit it.  What is below
-// kMask has no part in the range: masks of -1e9 would leave the bins' width as wide as it gets.
+// kMask has no part in the range, unless all of the row is: masks of -1e9 would leave bins as wide
+// as they get.
 __device__ __forceinline__ bool fit_bins(Settings& s, float top, float low) {
     // bins below an infinite logit have no width
     if (__builtin_isinf(top)) return false;
@@ -722,9 +740,9 @@ __global__ __launch_bounds__(kSplitBlock) void sample_peaks_kernel(SampleArgs g,
         w.done[row] = 0;
     }
     if (u >= w.units) return;
-    float low = __builtin_inff();
-    const float peak = unit_peak<T>(x, logits, g.vocab, u, low);
-    low = from_lane(wave_scan(low, __builtin_inff(), Min()), kWave - 1);
+    Lows lows;
+    const float peak = unit_peak<T>(x, logits, g.vocab, u, lows);
+    const float low = from_lane(wave_scan(lows.of(peak), __builtin_inff(), Min()), kWave - 1);
     if (tid % kWave == 0) {
         w.peaks[static_cast<long>(row) * w.units + u] = peak;
         w.lows[static_cast<long>(row) * w.units + u] = low;
@@ -738,7 +756,7 @@ __global__ __launch_bounds__(kSplitBlock) void sample_bins_kernel(SampleArgs g, 
     __shared__ unsigned long long mass[kBins];
     __shared__ int count[kBins];
     __shared__ double powers[64];
-    __shared__ float part[2][kSplitBlock / kWave];
+    __shared__ float part[3][kSplitBlock / kWave];
     constexpr int kTogether = kSplitBlock / kWave;
     const int row = blockIdx.y, tid = threadIdx.x;
     const typename T::Bits* logits = static_cast<const typename T::Bits*>(g.logits) + row * g.stride;
@@ -749,24 +767,29 @@ __global__ __launch_bounds__(kSplitBlock) void sample_bins_kernel(SampleArgs g, 
         mass[b] = 0;
         if (by_count) count[b] = 0;
     }
-    float top = -__builtin_inff(), low = __builtin_inff();
+    float top = -__builtin_inff();
+    Lows lows;
     for (int i = tid; i < w.units; i += kSplitBlock) {
         top = __builtin_fmaxf(top, w.peaks[static_cast<long>(row) * w.units + i]);
-        low = __builtin_fminf(low, w.lows[static_cast<long>(row) * w.units + i]);
+        lows.add(w.lows[static_cast<long>(row) * w.units + i]);
     }
     top = wave_scan(top, -__builtin_inff(), Max());
-    low = wave_scan(low, __builtin_inff(), Min());
+    lows.near = wave_scan(lows.near, __builtin_inff(), Min());
+    lows.deep = wave_scan(lows.deep, __builtin_inff(), Min());
     if (tid % kWave == kWave - 1) {
         part[0][tid / kWave] = top;
-        part[1][tid / kWave] = low;
+        part[1][tid / kWave] = lows.near;
+        part[2][tid / kWave] = lows.deep;
     }
     __syncthreads();
     top = part[0][0];
-    low = part[1][0];
+    lows = {part[1][0], part[2][0]};
     for (int i = 1; i < kTogether; ++i) {
         top = __builtin_fmaxf(top, part[0][i]);
-        low = __builtin_fminf(low, part[1][i]);
+        lows.near = __builtin_fminf(lows.near, part[1][i]);
+        lows.deep = __builtin_fminf(lows.deep, part[2][i]);
     }
+    const float low = lows.of(top);
     if (!fit_bins(s, top, low)) return;
     const float cut = cut_of(top, s.t);
     each_unit<T>(logits, g.vocab, blockIdx.x * kTogether + tid / kWave, gridDim.x * kTogether, w.units,
@@ -889,21 +912,22 @@ __global__ __launch_bounds__(kRow, 4) void sample_pick_kernel(SampleArgs g, Samp
     if (tid == 5) listed = 0;
     if (tid == 6) heaviest_bin = 0;
     auto all_units = [](int) { return true; };
-    float top = -__builtin_inff(), low = __builtin_inff();
+    float top = -__builtin_inff();
+    Lows lows;
     if constexpr (kWhole) {
         each_unit<T>(logits, g.vocab, wave, kWaves, w.units, all_units, [&](const Unit<T>& x, int u) {
-            const float peak = unit_peak<T>(x, logits, g.vocab, u, low);
+            const float peak = unit_peak<T>(x, logits, g.vocab, u, lows);
             if (lane == 0 && u < kPeaks) own_peaks[u] = peak;
             top = __builtin_fmaxf(top, peak);
         });
     } else {
         for (int i = tid; i < w.units; i += kRow) {
             top = __builtin_fmaxf(top, peaks[i]);
-            low = __builtin_fminf(low, w.lows[static_cast<long>(row) * w.units + i]);
+            lows.add(w.lows[static_cast<long>(row) * w.units + i]);
         }
     }
     top = block_reduce(top, -__builtin_inff(), part.f, Max());
-    low = block_reduce(low, __builtin_inff(), part.f, Min());
+    const float low = block_reduce(lows.of(top), __builtin_inff(), part.f, Min());
     if (top == -__builtin_inff()) {
         if (q == 0 && tid == 0) {
             g.tokens[row] = -1;

@@ -207,3 +207,27 @@ def test_logprobs_in_slowly_rising_rows(gpu, rows, vocab, rise):
         assert ids[i].tolist() == best.tolist()
         for j, b in enumerate(best):
             assert abs(float(values[i, j]) - want[b]) <= err[b], (j, float(values[i, j]), want[b], err[b])
+
+
+@pytest.mark.parametrize("rows", [2, 200])
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_rows_wholly_below_the_masks_bound(gpu, rows, kind):
+    """Logits around -5000 and -3e4, some parts of a row without any other, some of the row's
+    parts wholly masked: the bins' width comes from them where no logit is above."""
+    vocab = 9000
+    g = torch.Generator().manual_seed(rows)
+    u = [0.2, 0.9]
+    for low, wide, mask in ((-5000.0, 0.2, None), (-3e4, 900.0, -65504.0), (-4096.0, 3.0, -1e4),
+                            (-4100.0, 9.0, -math.inf)):
+        x = low + wide * torch.rand(2, vocab, generator=g)
+        if mask is not None:
+            x[:, 2000:5000] = mask
+        x[1, 17] = math.nan
+        x = x.to(S.TYPES[kind])
+        for s in (dict(), dict(top_p=0.7, temperature=2.0), dict(top_k=900)):
+            got = run(x.cuda().repeat(rows // 2, 1), u * (rows // 2), **s)
+            assert [v[:2] * (rows // 2) for v in got] == [list(v) for v in got]
+            for i in range(2):
+                one = R.f64(x[i])
+                one[np.isnan(one)] = -math.inf
+                Row(one, **s).check(u[i], got[0][i], got[1][i], note=(low, kind, s))
