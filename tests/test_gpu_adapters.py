@@ -375,3 +375,19 @@ def test_ends_of_the_workspace_where_the_split_changes(gpu, tokens, kind, rank):
         torch.cuda.synchronize()
         assert bool((ws[size:] == 0x5A).all())
         close(out, dict(d, ids=d["ids"][:n], x=d["x"][:n], base=d["base"][:n]), note=n)
+
+
+@pytest.mark.parametrize("tokens,rank", [(1, 8), (70, 16), (70, 136)])
+def test_inner_products_next_to_the_largest_float32(gpu, tokens, rank):
+    """Beyond the largest bf16 number and its half step: still finite, and so is the output."""
+    d = make("bf16", tokens, 64, (24,), rank, 2, [t % 2 for t in range(tokens)], seed=1)
+    d["scales"].fill_(1.0)
+    d["base"].zero_()
+    d["a"].zero_()
+    d["x"].zero_()
+    d["a"][:, :, 7], d["x"][:, 7] = 255 / 128 * 2.0 ** 63, 2.0 ** 64
+    d["a"][:, :, 40], d["x"][:, 40] = 127 / 64 * 2.0 ** 56, 2.0 ** 63
+    d["b"].zero_()
+    d["b"][:, :, 3] = 2.0 ** -120
+    assert float(R.f64(d["a"])[0, 3] @ R.f64(d["x"])[0]) > 1.998 * 2.0 ** 127
+    close(run(d), d)
